@@ -49,6 +49,10 @@ extern "C" {
 /* KV planes (KVST sub field, sw/sim/include/tsr_ref_at.h:56-57) */
 #define TSR_HIP_KV_K        0u
 #define TSR_HIP_KV_V        1u
+/* KV cache types: llama.cpp's cache types of the same names */
+#define TSR_HIP_KV_Q8_0     0u
+#define TSR_HIP_KV_Q4_0     1u   /* 32 values: f16 d, 16 bytes; value d (n - 8), n of 4 bits */
+#define TSR_HIP_KV_Q4_1     2u   /* 32 values: f16 d, f16 m, 16 bytes; value d n + m */
 /* tsr_hip_mul_mat flags (the MUL_MAT record's FLAGS word, sw/ctrl/ref/mulmat_ref.hpp:14-16) */
 #define TSR_HIP_MM_ACC_DST  0x1u  /* y = FA(y_old, W.x) */
 /* The weight's rows 2j and 2j + 1 are the gate and up rows of output j, and y[j] = SWIGLU(gate . x,
@@ -166,6 +170,14 @@ int tsr_hip_mul_mat_isums(tsr_hip_ctx * ctx, const tsr_hip_weight * w, const flo
  * the library's own; get / set bytes convert to and from the ggml q8_0 image exactly
  * (tsr_kv_set_bytes / tsr_kv_get_bytes, sw/sim/tsr_ref_at.c:178-212). E % 64 == 0. */
 int tsr_hip_kv_create(tsr_hip_ctx * ctx, uint32_t E, uint32_t kv_size, tsr_hip_kv ** out);
+/* The same for a cache of `type` (TSR_HIP_KV_*; no counterpart in the reference, whose caches are q8_0):
+ * tsr_hip_kv_create is type TSR_HIP_KV_Q8_0. The 4-bit types hold a cell in 18 (q4_0) or 20 (q4_1) bytes
+ * a block of 32 values against q8_0's 34; kv_size < 2^31. get / set bytes are those of the type's ggml
+ * image (E/32 blocks of 18 or 20 bytes a cell), tsr_hip_kv_set_rows and tsr_hip_rope_kv write every type,
+ * tsr_hip_kv_get_rows reads every type. FLASH_ATTN_EXT over a 4-bit cache is tsr_hip_flash_attn_kv4; the
+ * entry points that are the reference's q8_0 attention refuse it (TSR_HIP_E_FMT). A cache is created with
+ * every value 0 (q4_0: d 0). One handle is a K or a V plane, as `which` says, from its first write on. */
+int tsr_hip_kv_create_type(tsr_hip_ctx * ctx, uint32_t type, uint32_t E, uint32_t kv_size, tsr_hip_kv ** out);
 int tsr_hip_kv_free(tsr_hip_ctx * ctx, tsr_hip_kv * kv);
 /* Bytes [off, off + bytes) of the ggml image of plane `which` (row j = cell j, E/32 * 34 bytes). */
 int tsr_hip_kv_set_bytes(tsr_hip_ctx * ctx, tsr_hip_kv * kv, uint32_t which, size_t off, const void * src, size_t bytes);
@@ -176,6 +188,20 @@ int tsr_hip_kv_get_bytes(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t whic
  * out-of-range index stores nothing and sets *bad_dev if bad_dev is not NULL). */
 int tsr_hip_kv_set_rows(tsr_hip_ctx * ctx, tsr_hip_kv * kv, uint32_t which, const float * src_dev, uint32_t n_rows,
                         uint64_t src_stride, const int64_t * idx_dev, int32_t * bad_dev, void * stream);
+/* Into a 4-bit cache the rows are quantized by ggml's rule for a block, every step one f32 operation:
+ *   q4_0  d = M / -8, M the first value of the largest magnitude; n = min(15, trunc(x (1/d) + 8.5))
+ *   q4_1  m = min x, d = (max x - m) / 15;                        n = min(15, trunc((x - m) (1/d) + 0.5))
+ * (1/d is 0 where d is 0; d and m are then rounded to f16.) A NaN is stored as 0; a block with an infinity,
+ * or one whose d is beyond f16, stands for infinities and NaNs. The indices of one call are distinct for
+ * every type: a cell that two rows of a call name holds a mixture of both. */
+
+/* Cells back as f32 rows: dst_dev[i * dst_stride + e] = value e of cell idx_dev[i] (int64, device), i < n_rows,
+ * what the stored block stands for (q4_1: d n + m rounded once). The reverse of tsr_hip_kv_set_rows, with
+ * its rules of alignment, strides (n_rows <= 65535) and out-of-range indices (such a row of dst is left as
+ * it was). The GGML_OP_GET_ROWS / CPY to f32 that llama.cpp's context shift makes of a quantized cache (no
+ * counterpart in the reference). */
+int tsr_hip_kv_get_rows(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t which, const int64_t * idx_dev,
+                        uint32_t n_rows, float * dst_dev, uint64_t dst_stride, int32_t * bad_dev, void * stream);
 
 /* The decoder layer's ROPE of q and k followed by SET_ROWS_KV of k and v (the ROPE, SET_ROWS_KV records
  * of sw/ctrl/tests/test_fw_m7_layer.cpp:646-686) in one launch, bit-identical to tsr_hip_rope over the
@@ -183,7 +209,8 @@ int tsr_hip_kv_set_rows(tsr_hip_ctx * ctx, tsr_hip_kv * kv, uint32_t which, cons
  * the rotated k into kc and of v into vc. Token t's row at qkv_dev + t * stride holds n_head q heads,
  * n_head_kv k heads and n_head_kv v heads of head_dim floats (head_dim % 32 == 0; the row at most 16384
  * floats); its position is pos_dev[t] (int32) and its cell cell_dev[t] (int64), both on the device. A
- * cell outside either cache stores nothing and sets *bad_dev (nullable). */
+ * cell outside either cache stores nothing and sets *bad_dev (nullable). Caches of every type, and of two
+ * types; with a 4-bit one among them it is those three calls (three launches, T <= 65535). */
 int tsr_hip_rope_kv(tsr_hip_ctx * ctx, float * qkv_dev, uint32_t T, uint64_t stride, uint32_t head_dim, uint32_t n_head,
                     uint32_t n_head_kv, uint32_t n_dims, int mode, const int32_t * pos_dev, float freq_base,
                     float attn_factor, tsr_hip_kv * kc, tsr_hip_kv * vc, const int64_t * cell_dev, int32_t * bad_dev,
@@ -324,6 +351,34 @@ int tsr_hip_flash_attn_noalloc(tsr_hip_ctx * ctx, const float * q_dev, uint32_t 
                                uint32_t n_head_kv, float scale, const uint32_t * msum, const float * mask_f32_dev,
                                const uint32_t (*new_runs)[2], uint32_t n_new, float * out_dev, uint64_t out_stride,
                                void * stream);
+
+/* FLASH_ATTN_EXT over a 4-bit cache (TSR_HIP_KV_Q4_0 / _Q4_1; no counterpart in the reference, whose cache is
+ * q8_0): out = softmax(scale q K^T + mask) V on the values that the blocks stand for, f32 queries and
+ * results, in f32 arithmetic (q and the weights p enter the matrix cores as two f16 pieces of 22 bits).
+ *   q_dev, out_dev  as tsr_hip_flash_attn; 16-byte aligned, strides multiples of 4
+ *   kc, vc          caches of one 4-bit type, E = n_head_kv * D
+ *   n_kv            cells of the caches that the call may touch, <= kv_size (0: every row is empty)
+ *   runs_dev        (nullable) [T][4] uint32 in device memory, 16-byte aligned: token t sees the cells
+ *                   [lo0, hi0) and [lo1, hi1), ends beyond n_kv cut to n_kv, lo >= hi none: an MSUM's row words
+ *                   (words 8 + 4 t .. of tsr_hip_msum_build_f16, not GENERAL). NULL: all n_kv cells.
+ *   mask_f16_dev    (nullable) f16 mask rows in device memory, mask_stride values apart, mask[t][c] added to the scaled
+ *                   score of cell c < n_kv; -inf hides the cell. With runs_dev a cell is seen where both allow it.
+ *   ws_dev          a workspace of ws_bytes >= tsr_hip_flash_attn_kv4_ws(...) for the same arguments, 16-byte
+ *                   aligned; NULL: the context's scratch. Calls that share a workspace run one after another. Under
+ *                   graph capture a call whose workspace is not of 0 bytes needs one here (else
+ *                   TSR_HIP_E_ARG): graphs that may run at once take one each.
+ * A row that sees no cell (or whose scores are all -inf) is 0. What a cell holds that a row does not see
+ * (infinities and NaN too) does not reach the row. The masks and runs are read when the kernels run: a captured
+ * call replays over what they hold then, within its n_kv. D in {64, 128, 256, 512}, n_head % n_head_kv == 0,
+ * n_head / n_head_kv <= 64, n_head D <= 32768, T <= 65535; scale finite, normal and > 0. Results do not depend
+ * on the order in which workgroups run. */
+int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const tsr_hip_kv * kc,
+                           const tsr_hip_kv * vc, uint32_t D, uint32_t n_head, uint32_t n_head_kv, float scale,
+                           uint32_t n_kv, const uint32_t * runs_dev, const uint16_t * mask_f16_dev, uint64_t mask_stride,
+                           float * out_dev, uint64_t out_stride, void * ws_dev, size_t ws_bytes, void * stream);
+/* The workspace that such a call needs, in bytes (0: none, and for arguments that it refuses). */
+size_t tsr_hip_flash_attn_kv4_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv,
+                                 uint32_t n_kv);
 
 /* ---- decode-layer glue ops ----------------------------------------------------------------------
  * The f32 ops around MUL_MAT and FLASH_ATTN in a decoder layer, on the vector unit's f32 rules

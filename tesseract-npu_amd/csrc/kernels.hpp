@@ -92,6 +92,29 @@ struct KvArgs {
     uint32_t E, kv_size;
 };
 
+// KV cache types (TSR_HIP_KV_Q8_0 ..) and a plane of a 4-bit cache (kv4.hpp has the layout).
+constexpr uint32_t kKvQ8_0 = 0u, kKvQ4_0 = 1u, kKvQ4_1 = 2u;
+struct Kv4Args {
+    uint8_t * base;
+    uint32_t type, E, kv_size, n_tiles;
+};
+
+// Attention over a 4-bit cache (k_attn4.hip).
+struct Attn4Args {
+    const float * q;         // [T][n_head][D], token t at q + t * q_stride
+    uint64_t q_stride;
+    const uint8_t * k, * v;  // the planes
+    const uint32_t * runs;   // nullable: [T][4] the cells [lo0, hi0) and [lo1, hi1) that a token sees
+    const uint16_t * mask;   // nullable: f16 [T], rows of mask_stride
+    uint64_t mask_stride;
+    float * out;             // [T][n_head][D], token t at out + t * out_stride
+    uint64_t out_stride;
+    float * part;            // S > 1: [split][T n_head] (maximum, sum), then [split][T n_head][D] unnormalised rows
+    uint32_t type, D, T, G, n_head_kv, n_kv, n_tiles;
+    uint32_t S;              // splits of the cells
+    float scale;
+};
+
 // The work list of one call. Small lists (decode) travel inline in the kernel arguments; larger ones
 // are copied to device memory once per call and the kernels read them there (FaArgs::items != 0).
 struct FaPlan {
@@ -230,6 +253,17 @@ int tsr_launch_kv_bytes(const tsr::KvArgs & a, uint32_t which, uint64_t off, uin
                         hipStream_t s);
 int tsr_launch_kv_set_rows(const tsr::KvArgs & a, uint32_t which, const float * src, uint32_t n_rows,
                            uint64_t src_stride, const int64_t * idx, int32_t * bad, hipStream_t s);
+// 4-bit caches (k_kv4.hip): the ggml image's bytes, SET_ROWS, cells back as f32 rows; q8_0 cells as f32 rows
+int tsr_launch_kv4_bytes(const tsr::Kv4Args & a, uint32_t which, uint64_t off, uint64_t n, uint8_t * stage, int to_dev,
+                         hipStream_t s);
+int tsr_launch_kv4_set_rows(const tsr::Kv4Args & a, uint32_t which, const float * src, uint32_t n_rows,
+                            uint64_t src_stride, const int64_t * idx, int32_t * bad, hipStream_t s);
+int tsr_launch_kv4_get_rows(const tsr::Kv4Args & a, uint32_t which, const int64_t * idx, uint32_t n_rows, float * dst,
+                            uint64_t dst_stride, int32_t * bad, hipStream_t s);
+int tsr_launch_kv_get_rows(const tsr::KvArgs & a, uint32_t which, const int64_t * idx, uint32_t n_rows, float * dst,
+                           uint64_t dst_stride, int32_t * bad, hipStream_t s);
+// attention over a 4-bit cache, its waves' rows and splits by attn4_plan.hpp (k_attn4.hip)
+int tsr_launch_attn4(const tsr::Attn4Args & a, bool split_waves, hipStream_t s);
 int tsr_launch_fa(const tsr::FaArgs & a, const tsr::FaPlan & p, uint32_t T, uint32_t n_cu, hipStream_t s);
 int tsr_launch_fa_dec(const tsr::FaDecArgs & a, hipStream_t s);
 int tsr_launch_xcd_probe(uint32_t * out64, hipStream_t s);

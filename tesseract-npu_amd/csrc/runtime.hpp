@@ -208,9 +208,10 @@ struct tsr_hip_weight {
     size_t bytes = 0;
 };
 
-// A q8_0 KV cache plane in the device layout of k_kv.hip: cells in groups of 16; the fp16 block
-// scales ("meta") and the int8 quants in separate regions.
+// A KV cache plane: q8_0 in the device layout of k_kv.hip (cells in groups of 16; the fp16 block
+// scales ("meta") and the int8 quants in separate regions), or 4-bit blocks in the layout of kv4.hpp.
 struct tsr_hip_kv {
+    uint32_t type = TSR_HIP_KV_Q8_0;
     uint32_t E = 0, kv_size = 0;
     uint8_t * dev = nullptr;
     size_t meta_row = 0;         // bytes per cell of the meta region

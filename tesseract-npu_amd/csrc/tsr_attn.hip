@@ -13,6 +13,7 @@
 
 #include "fa_plan.hpp"
 #include "kernels.hpp"
+#include "kv4.hpp"
 #include "runtime.hpp"
 #include "tsr_hip.h"
 
@@ -27,18 +28,33 @@ static tsr::KvArgs kv_args(const tsr_hip_kv * kv) {
     return a;
 }
 
+static tsr::Kv4Args kv4_args(const tsr_hip_kv * kv) {
+    return tsr::Kv4Args{ kv->dev, kv->type, kv->E, kv->kv_size, tsr::kv4_tiles(kv->kv_size) };
+}
+
 int tsr_hip_kv_create(tsr_hip_ctx * ctx, uint32_t E, uint32_t kv_size, tsr_hip_kv ** out) {
+    return tsr_hip_kv_create_type(ctx, TSR_HIP_KV_Q8_0, E, kv_size, out);
+}
+
+int tsr_hip_kv_create_type(tsr_hip_ctx * ctx, uint32_t type, uint32_t E, uint32_t kv_size, tsr_hip_kv ** out) {
     if (ctx == nullptr || out == nullptr) return TSR_HIP_E_ARG;
     *out = nullptr;
+    if (type > TSR_HIP_KV_Q4_1) return TSR_HIP_E_FMT;
     if (E == 0u || E % 64u != 0u || E > 32768u || kv_size == 0u) return TSR_HIP_E_SHAPE;
+    if (type != TSR_HIP_KV_Q8_0 && kv_size > 0x7FFFFFFFu) return TSR_HIP_E_SHAPE;   // (tiles' cells stay below 2^32)
     auto * kv = new (std::nothrow) tsr_hip_kv();
     if (kv == nullptr) return TSR_HIP_E_NOMEM;
     const size_t ng = (kv_size + 15u) / 16u;
+    kv->type = type;
     kv->E = E;
     kv->kv_size = kv_size;
-    kv->meta_row = (size_t)E / 32u * 2u;
-    kv->quant_off = (ng * 16u * kv->meta_row + 255u) & ~(size_t)255u;
-    kv->bytes = kv->quant_off + ng * 16u * E;
+    if (type == TSR_HIP_KV_Q8_0) {
+        kv->meta_row = (size_t)E / 32u * 2u;
+        kv->quant_off = (ng * 16u * kv->meta_row + 255u) & ~(size_t)255u;
+        kv->bytes = kv->quant_off + ng * 16u * E;
+    } else {
+        kv->bytes = tsr::kKv4Header + (size_t)(E / 64u) * tsr::kv4_tiles(kv_size) * tsr::kv4_tile_bytes(type);
+    }
     std::lock_guard<std::mutex> lk(ctx->mtx);
     (void)hipSetDevice(ctx->device);
     int rc = hip_err(hipMalloc((void **)&kv->dev, kv->bytes), "hipMalloc kv");
@@ -68,7 +84,8 @@ static int kv_bytes(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t which, si
                     int to_dev) {
     if (ctx == nullptr || kv == nullptr || (bytes && host == nullptr)) return TSR_HIP_E_ARG;
     if (which > 1u) return TSR_HIP_E_ARG;
-    const uint64_t total = (uint64_t)kv->kv_size * (kv->E / 32u) * 34u;
+    const uint64_t block = kv->type == TSR_HIP_KV_Q8_0 ? 34u : tsr::kv4_block_bytes(kv->type);
+    const uint64_t total = (uint64_t)kv->kv_size * (kv->E / 32u) * block;
     if ((uint64_t)off > total || (uint64_t)bytes > total - off) return TSR_HIP_E_RANGE;
     if (bytes == 0) return TSR_HIP_OK;
     std::lock_guard<std::mutex> lk(ctx->mtx);
@@ -77,7 +94,12 @@ static int kv_bytes(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t which, si
     if (rc) return rc;
     uint8_t * stage = (uint8_t *)ctx->scratch.ptr;
     if (to_dev) rc = hip_err(hipMemcpyAsync(stage, host, bytes, hipMemcpyHostToDevice, ctx->stream), "kv H2D");
-    if (rc == 0) rc = tsr_launch_kv_bytes(kv_args(kv), which, off, bytes, stage, to_dev, ctx->stream) ? TSR_HIP_E_HIP : 0;
+    if (rc == 0) {
+        const int k = kv->type == TSR_HIP_KV_Q8_0
+                          ? tsr_launch_kv_bytes(kv_args(kv), which, off, bytes, stage, to_dev, ctx->stream)
+                          : tsr_launch_kv4_bytes(kv4_args(kv), which, off, bytes, stage, to_dev, ctx->stream);
+        rc = k ? TSR_HIP_E_HIP : 0;
+    }
     if (rc == 0 && !to_dev) rc = hip_err(hipMemcpyAsync(host, stage, bytes, hipMemcpyDeviceToHost, ctx->stream), "kv D2H");
     if (rc == 0) rc = hip_err(hipStreamSynchronize(ctx->stream), "hipStreamSynchronize");
     return rc;
@@ -101,9 +123,29 @@ int tsr_hip_kv_set_rows(tsr_hip_ctx * ctx, tsr_hip_kv * kv, uint32_t which, cons
     std::lock_guard<std::mutex> lk(ctx->mtx);
     (void)hipSetDevice(ctx->device);
     ctx->ctr.set_rows_calls++;
-    return tsr_launch_kv_set_rows(kv_args(kv), which, src_dev, n_rows, src_stride, idx_dev, ctx->flag(bad_dev), ctx->pick(stream))
-               ? TSR_HIP_E_HIP
-               : TSR_HIP_OK;
+    const int rc = kv->type == TSR_HIP_KV_Q8_0
+                       ? tsr_launch_kv_set_rows(kv_args(kv), which, src_dev, n_rows, src_stride, idx_dev,
+                                                ctx->flag(bad_dev), ctx->pick(stream))
+                       : tsr_launch_kv4_set_rows(kv4_args(kv), which, src_dev, n_rows, src_stride, idx_dev,
+                                                 ctx->flag(bad_dev), ctx->pick(stream));
+    return rc ? TSR_HIP_E_HIP : TSR_HIP_OK;
+}
+
+int tsr_hip_kv_get_rows(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t which, const int64_t * idx_dev,
+                        uint32_t n_rows, float * dst_dev, uint64_t dst_stride, int32_t * bad_dev, void * stream) {
+    if (ctx == nullptr || kv == nullptr || dst_dev == nullptr || idx_dev == nullptr || which > 1u) return TSR_HIP_E_ARG;
+    if (n_rows == 0u) return TSR_HIP_OK;
+    if (((uintptr_t)dst_dev & 15u) != 0u || (n_rows > 1u && (dst_stride % 4u != 0u || dst_stride < kv->E)) ||
+        n_rows > 65535u)
+        return TSR_HIP_E_ARG;
+    std::lock_guard<std::mutex> lk(ctx->mtx);
+    (void)hipSetDevice(ctx->device);
+    const int rc = kv->type == TSR_HIP_KV_Q8_0
+                       ? tsr_launch_kv_get_rows(kv_args(kv), which, idx_dev, n_rows, dst_dev, dst_stride,
+                                                ctx->flag(bad_dev), ctx->pick(stream))
+                       : tsr_launch_kv4_get_rows(kv4_args(kv), which, idx_dev, n_rows, dst_dev, dst_stride,
+                                                 ctx->flag(bad_dev), ctx->pick(stream));
+    return rc ? TSR_HIP_E_HIP : TSR_HIP_OK;
 }
 
 int tsr_hip_rope_kv(tsr_hip_ctx * ctx, float * qkv_dev, uint32_t T, uint64_t stride, uint32_t head_dim, uint32_t n_head,
@@ -121,6 +163,15 @@ int tsr_hip_rope_kv(tsr_hip_ctx * ctx, float * qkv_dev, uint32_t T, uint64_t str
     if (kc->E != E || vc->E != E) return TSR_HIP_E_SHAPE;
     if (((uintptr_t)qkv_dev & 15u) != 0u || (T > 1u && (stride % 4u != 0u || stride < nrow))) return TSR_HIP_E_ARG;
     if (!(freq_base > 0.0f) || !std::isfinite(freq_base)) return TSR_HIP_E_ARG;
+    if (kc->type != TSR_HIP_KV_Q8_0 || vc->type != TSR_HIP_KV_Q8_0) {   // 4-bit blocks: the three ops it stands for
+        if (T > 65535u) return TSR_HIP_E_ARG;
+        int rc = tsr_hip_rope(ctx, qkv_dev, T, stride, head_dim, n_head + n_head_kv, n_dims, mode, pos_dev, freq_base, 1.0f,
+                              attn_factor, nullptr, qkv_dev, stride, stream);
+        const float * k = qkv_dev + (size_t)n_head * head_dim;
+        if (rc == 0) rc = tsr_hip_kv_set_rows(ctx, kc, TSR_HIP_KV_K, k, T, stride, cell_dev, bad_dev, stream);
+        if (rc == 0) rc = tsr_hip_kv_set_rows(ctx, vc, TSR_HIP_KV_V, k + E, T, stride, cell_dev, bad_dev, stream);
+        return rc;
+    }
     tsr::RopeKvArgs a{};
     a.qkv = qkv_dev;
     a.stride = stride;
@@ -295,6 +346,7 @@ static int fa_unplanned(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint
     int rc = fa_check_shape(D, n_head, n_head_kv, scale);
     if (rc) return rc;
     const uint32_t E = n_head_kv * D, K = n_head * D;
+    if (kc->type != TSR_HIP_KV_Q8_0 || vc->type != TSR_HIP_KV_Q8_0) return TSR_HIP_E_FMT;
     if (kc->E != E || vc->E != E || kc->kv_size != vc->kv_size) return TSR_HIP_E_SHAPE;
     if (msum[0] != 0x4D55534Du || msum[1] != T || msum[2] > kc->kv_size) return TSR_HIP_E_MASK;
     if (((uintptr_t)q_dev & 15u) != 0u || (T > 1u && (q_stride % 4u != 0u || q_stride < K)) ||
@@ -598,6 +650,7 @@ static int fa_plan_launch(tsr_hip_ctx * ctx, const tsr_hip_fa_plan * plan, const
     int rc = fa_check_shape(plan->D, plan->n_head, plan->n_head_kv, scale);
     if (rc) return rc;
     const uint32_t E = plan->n_head_kv * plan->D, K = plan->n_head * plan->D, T = plan->T;
+    if (kc->type != TSR_HIP_KV_Q8_0 || vc->type != TSR_HIP_KV_Q8_0) return TSR_HIP_E_FMT;
     if (kc->E != E || vc->E != E || kc->kv_size != vc->kv_size || kc->kv_size < plan->kv_size) return TSR_HIP_E_SHAPE;
     if (((uintptr_t)q_dev & 15u) != 0u || (T > 1u && (q_stride % 4u != 0u || q_stride < K)) || (T > 1u && out_stride < K))
         return TSR_HIP_E_ARG;
@@ -766,6 +819,8 @@ int tsr_hip_attn_qkv_plan_rope_tab(tsr_hip_ctx * ctx, const tsr_hip_fa_plan * pl
     if (ctx == nullptr || plan == nullptr || w_qkv == nullptr || x_dev == nullptr || qkv_dev == nullptr ||
         tab_dev == nullptr || ((uintptr_t)tab_dev & 7u) != 0u)
         return TSR_HIP_E_ARG;
+    if ((kc != nullptr && kc->type != TSR_HIP_KV_Q8_0) || (vc != nullptr && vc->type != TSR_HIP_KV_Q8_0))
+        return TSR_HIP_E_FMT;
     const uint32_t D = plan->D, nkv = plan->n_head_kv, G = nkv ? plan->n_head / nkv : 0u;
     if (w_qkv->N != (plan->n_head + 2u * nkv) * D) return TSR_HIP_E_SHAPE;
     tsr::FaArgs r;

@@ -21,6 +21,8 @@ LIB_PATH = os.path.join(HERE, "libtsr_hip.so")
 FMT_Q8_0, FMT_Q4_K = 0, 1
 QA_A32, QA_A256 = 0, 1
 KV_K, KV_V = 0, 1
+KV_Q8_0, KV_Q4_0, KV_Q4_1 = 0, 1, 2
+KV_BLOCK_BYTES = {KV_Q8_0: 34, KV_Q4_0: 18, KV_Q4_1: 20}     # of 32 values in the ggml image
 MM_ACC_DST, MM_GLU, MM_SCALE, MM_SOFTCAP = 1, 2, 4, 8
 ROPE_NORMAL, ROPE_NEOX, ROPE_IMROPE = 0, 2, 40
 
@@ -39,6 +41,7 @@ EXPORTS = (
     "tsr_hip_flash_attn_plan_rope_tab", "tsr_hip_mul_mat_epi", "tsr_hip_set_fa_wait_limit",
     "tsr_hip_flash_attn_noalloc", "tsr_hip_get_flags", "tsr_hip_msum_mask_f32", "tsr_hip_attn_qkv_plan_rope_tab",
     "tsr_hip_fa_plan_set_epoch",
+    "tsr_hip_kv_create_type", "tsr_hip_kv_get_rows", "tsr_hip_flash_attn_kv4", "tsr_hip_flash_attn_kv4_ws",
 )
 
 
@@ -123,6 +126,11 @@ def load(path: str = LIB_PATH) -> C.CDLL:
                                              C.c_int),
         "tsr_hip_attn_qkv_plan_rope_tab": ([vp, vp, vp, vp, C.c_float, vp, vp, vp, vp, C.c_float, u32, C.c_int, vp, vp,
                                             vp, vp, vp, u64, vp], C.c_int),
+        "tsr_hip_kv_create_type": ([vp, u32, u32, u32, C.POINTER(vp)], C.c_int),
+        "tsr_hip_kv_get_rows": ([vp, vp, u32, vp, u32, vp, u64, vp, vp], C.c_int),
+        "tsr_hip_flash_attn_kv4": ([vp, vp, u32, u64, vp, vp, u32, u32, u32, C.c_float, u32, vp, vp, u64, vp, u64, vp, sz,
+                                    vp], C.c_int),
+        "tsr_hip_flash_attn_kv4_ws": ([vp, u32, u32, u32, u32, u32], sz),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -250,15 +258,15 @@ class Weight:
 
 
 class KvCache:
-    def __init__(self, dev: "Device", E: int, kv_size: int):
-        self.dev, self.E, self.kv_size = dev, E, kv_size
+    def __init__(self, dev: "Device", E: int, kv_size: int, type: int = KV_Q8_0):
+        self.dev, self.E, self.kv_size, self.type = dev, E, kv_size, type
         h = C.c_void_p()
-        _check(dev.L.tsr_hip_kv_create(dev.ctx, E, kv_size, C.byref(h)), "kv_create")
+        _check(dev.L.tsr_hip_kv_create_type(dev.ctx, type, E, kv_size, C.byref(h)), "kv_create")
         self.h = h.value
 
     @property
     def row_bytes(self) -> int:
-        return self.E // 32 * 34
+        return self.E // 32 * KV_BLOCK_BYTES[self.type]
 
     def set_bytes(self, which: int, data, off: int = 0) -> None:
         a = np.ascontiguousarray(data, np.uint8)
@@ -391,8 +399,8 @@ class Device:
     def weight(self, fmt: int, blocks, N: int, K: int) -> Weight:
         return Weight(self, fmt, blocks, N, K)
 
-    def kv(self, E: int, kv_size: int) -> KvCache:
-        return KvCache(self, E, kv_size)
+    def kv(self, E: int, kv_size: int, type: int = KV_Q8_0) -> KvCache:
+        return KvCache(self, E, kv_size, type)
 
     # -- ops (device pointers are ints or Buffers) -----------------------------------------------
     @staticmethod
@@ -438,6 +446,24 @@ class Device:
                     stream=None) -> None:
         _check(self.L.tsr_hip_kv_set_rows(self.ctx, kv.h, which, self._p(src), n_rows, src_stride, self._p(idx),
                                           self._p(bad), stream), "kv_set_rows")
+
+    def kv_get_rows(self, kv: KvCache, which: int, idx, n_rows: int, dst, dst_stride: int, bad=None, stream=None) -> None:
+        """Cells idx (int64) of a cache of any type back as f32 rows."""
+        _check(self.L.tsr_hip_kv_get_rows(self.ctx, kv.h, which, self._p(idx), n_rows, self._p(dst), dst_stride,
+                                          self._p(bad), stream), "kv_get_rows")
+
+    def flash_attn_kv4_ws(self, T: int, D: int, n_head: int, n_head_kv: int, n_kv: int) -> int:
+        """Bytes of workspace that flash_attn_kv4 needs (0: none)."""
+        return int(self.L.tsr_hip_flash_attn_kv4_ws(self.ctx, T, D, n_head, n_head_kv, n_kv))
+
+    def flash_attn_kv4(self, q, T: int, q_stride: int, kc: KvCache, vc: KvCache, D: int, n_head: int, n_head_kv: int,
+                       scale: float, n_kv: int, out, out_stride: int, runs=None, mask=None, mask_stride: int = 0,
+                       ws: "Buffer | None" = None, stream=None) -> None:
+        """Attention over 4-bit caches: token t sees the cells of its two runs (runs: device uint32 [T, 4]) under an
+        f16 mask (device), either of them None; ws: the workspace Buffer of a captured call."""
+        _check(self.L.tsr_hip_flash_attn_kv4(self.ctx, self._p(q), T, q_stride, kc.h, vc.h, D, n_head, n_head_kv, scale,
+                                             n_kv, self._p(runs), self._p(mask), mask_stride, self._p(out), out_stride,
+                                             self._p(ws), 0 if ws is None else ws.nbytes, stream), "flash_attn_kv4")
 
     def flash_attn(self, q, T: int, q_stride: int, kc: KvCache, vc: KvCache, D: int, n_head: int, n_head_kv: int,
                    scale: float, msum, out, out_stride: int, mask_f32=None, new_runs=None, stream=None) -> None:
