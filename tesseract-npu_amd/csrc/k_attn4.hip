@@ -3,17 +3,16 @@
 // A wave takes 16 NT query rows of one KV head (row r of a KV head is token r / G, query head r % G of the head's G) and
 // tiles of 32 cells, one pass with a running maximum and sum; everything stays in registers.
 //   scores   S^T[cell][row] = sum over blocks of d[cell] (sum of n q): the matrix instruction f32 <- f16 16x16x32, one a
-//            block and piece of q. The operand n is not converted: four bits in the low mantissa bits of an f16 are the
-//            subnormal n 2^-24 (2^-20 in the next four), which the instruction multiplies exactly, so that a word of eight
-//            codes is unpacked by four ANDs and one shift. q is scaled to [2^13, 2^14) by a power of two a row and split
-//            into two f16 pieces (22 bits). The zero point of q4_0 (n - 8) is the instruction's starting value
-//            -8 sum(q), that of q4_1 (d n + m) one product m sum(q) a block.
+//            block and piece of q. The first operand are n - 8 (q4_1: n), made of a word of eight codes by an AND with an OR
+//            and one packed f16 operation a pair. q is scaled to [2^13, 2^14) by a power of two a row and split into two f16
+//            pieces (22 bits). q4_1 (d n + m) adds m sum(q) a block.
 //   softmax  in base 2, f32: a lane holds the scores of one row for four cells of every 16, which is, cells
 //            permuted, the second operand of the next product: P stays where it is.
-//   P V      O^T[value][row]: the first operand are codes as they are again, the second p d[cell] of a block in two f16
-//            pieces (one instruction makes each: f16(p d), f16(p d - hi)). p carries 2^k with 2^k max|d| in [2^14, 2^15)
-//            from the plane's header, so that no piece overflows and the pieces keep 2^-39 of the largest. The zero
-//            point -8 sum(p d) (q4_1: + sum(p m)) is summed aside in f32.
+//   P V      O^T[value][row]: the first operand are n - 8 again, the second p d[cell] of a block in two f16 pieces (one instruction makes each: f16(p d),
+//            f16(p d - hi)). Sums of raw codes would be large and nearly cancel: an error that grows with the root of the
+//            cells. p carries 2^k with 2^k max|d| in [2^8, 2^9) from the plane's header and is at most 2^6 (the maximum
+//            follows when it is passed by that), so that no piece overflows and the pieces keep 2^-33 of the largest.
+//            q4_1: sum p (m + 8 d) is summed aside in f32.
 // The scales meet the f32 sums only, where a cell that its row does not see is replaced by nothing: an infinity or a
 // NaN in a masked cell reaches no result. Sums, maxima and results are f32; both splits keep 22 bits of f32's 24.
 #include "kernels.hpp"
@@ -30,11 +29,26 @@ __device__ __forceinline__ float half_of(uint32_t w, int i) {     // f16 half i 
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> (16 * i)));
 }
 __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-// The eight codes of two words whose nibbles sit at bits 0 and 16 (times 16: at bits 4 and 20) of the word and of the
-// word shifted by 8.
-__device__ __forceinline__ h8 codes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __builtin_bit_cast(h8, make_uint4(a, b, c, d));
+// n - zero of the nibbles at bits 0 and 16 of a word ((1024 + n) - (1024 + zero)) and at bits 4 and 20 ((1024 + 16 n) / 16 -
+// (64 + zero)), exact. (The bits alone, as subnormals n 2^-24, would save the packed operation; but the instruction aligns
+// subnormal operands by their nominal exponent and loses four bits of every product.)
+__device__ __forceinline__ h2 codes_lo(uint32_t w, float zero) {
+    const _Float16 z = (_Float16)(-1024.0f - zero);
+    return __builtin_bit_cast(h2, (w & 0x000F000Fu) | 0x64006400u) + h2{ z, z };
 }
+__device__ __forceinline__ h2 codes_hi(uint32_t w, float zero) {
+    const _Float16 z = (_Float16)(-64.0f - zero), f = (_Float16)0.0625f;
+    return __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00F000F0u) | 0x64006400u), h2{ f, f }, h2{ z, z });
+}
+// Two f32 as f16. The word is made once: left to itself the compiler rounds an operand of the matrix instruction and the
+// same value in the residual that follows it by different instructions, once and twice, which differ in rare ties.
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+    uint32_t w = __builtin_bit_cast(uint32_t, h2{ (_Float16)a, (_Float16)b });
+    asm("" : "+v"(w));
+    return w;
+}
+__device__ __forceinline__ h8 of_words(const uint32_t (&w)[4]) { return __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3])); }
+__device__ __forceinline__ h8 four(h2 a, h2 b, h2 c, h2 d) { return h8{ a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1] }; }
 // max / sum over the four lanes that hold one row (l, l ^ 16, l ^ 32, l ^ 48)
 __device__ __forceinline__ float rows_max(float x) {
     auto a = __builtin_amdgcn_permlane16_swap(fb(x), fb(x), false, false);
@@ -51,17 +65,13 @@ __device__ __forceinline__ float rows_sum(float x) {
 
 constexpr uint32_t kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 6.0f;                  // weights are at most 2^6: a maximum is followed when it is passed by more
 
-// One tile's operands of a plane as a lane holds them.
-template <int D, uint32_t TYPE>
-struct KTile {
-    uint2 w[D / 64][2];                         // codes of 16 cells x 64 values
-    uint4 sc[D / 64][2][TYPE == kKvQ4_1 ? 2 : 1];
-};
-template <int D, uint32_t TYPE>
-struct VTile {
-    uint4 w[D / 64];
-    uint4 sc[D / 64][2][TYPE == kKvQ4_1 ? 2 : 1];
+// A chunk of a tile: 64 NP values of its 32 cells as a lane holds them, codes and scales.
+template <int NP, uint32_t TYPE>
+struct Chunk {
+    uint4 w[NP];                                // K: two groups of 16 cells x two blocks; V: two blocks x two groups
+    uint4 sc[NP][2][TYPE == kKvQ4_1 ? 2 : 1];   // [group of 16 cells] the lane's four cells
 };
 
 // The word {d of block 0, d of block 1} of cell i (of the lane's four) and, q4_1, {m, m}.
@@ -75,35 +85,29 @@ __device__ __forceinline__ uint32_t scale_m(const T & sc, int i) {
     return i == 0 ? sc[0].y : i == 1 ? sc[0].w : i == 2 ? sc[1].y : sc[1].w;
 }
 
-template <int D, uint32_t TYPE>
-__device__ __forceinline__ void load_scales(uint4 (&sc)[2][TYPE == kKvQ4_1 ? 2 : 1], const uint8_t * t, uint32_t g) {
-    constexpr uint32_t n = TYPE == kKvQ4_1 ? 2u : 1u;
-#pragma unroll
-    for (uint32_t s = 0; s < 2; ++s)
-#pragma unroll
-        for (uint32_t j = 0; j < n; ++j) sc[s][j] = *(const uint4 *)(t + 1024u + 4u * n * (16u * s + 4u * g) + 16u * j);
-}
-
 // SPLIT: the four waves of a workgroup have the same rows and take different tiles; else each has rows of its own.
 template <int D, int NT, uint32_t TYPE, bool SPLIT>
 struct Attn4 {
-    static constexpr int NB = D / 32, NP = D / 64;
-    struct Row {                                // of the lane's query row in each group of 16
+    static constexpr int NB = D / 32;                              // blocks of a head
+    static constexpr int DC = D < 128 ? D : 128, NC = D / DC, NPC = DC / 64, NBC = DC / 32;   // a chunk's values; chunks
+    static constexpr int BUF = NC > 1 ? 2 : 1;
+    using Ch = Chunk<NPC, TYPE>;
+    struct Row {                                                   // of the lane's query row in each group of 16
         uint32_t lo0, hi0, lo1, hi1, t;
     };
     Row row[NT];
-    h8 qh[NT][NB], ql[NT][NB];
-    float qs[NT][NB];                           // sum of the block's q, times 2^-24
-    float csc[NT];                              // scores' unit, base 2
+    float qs[NT][TYPE == kKvQ4_1 ? NB : 1];                        // q4_1: sum of the block's q
+    float csc[NT];                                                 // the scores' unit, base 2
     f4 o[NT][2 * NB];
-    float bias[NT][NB];
+    float bias[NT][TYPE == kKvQ4_1 ? NB : 1];                      // q4_1: sum p (m + 8 d)
     float m[NT], l[NT];
 
     __device__ __forceinline__ bool sees(int n, uint32_t c) const {
         return (c >= row[n].lo0 && c < row[n].hi0) || (c >= row[n].lo1 && c < row[n].hi1);
     }
 
-    __device__ __forceinline__ void load_rows(const Attn4Args & a, uint32_t h, uint32_t r0, uint32_t lane) {
+    // The rows' runs and queries; put: this wave writes the queries' pieces to `lds` (the caller's barrier follows).
+    __device__ __forceinline__ void load_rows(const Attn4Args & a, uint32_t h, uint32_t r0, uint32_t lane, h8 * lds, bool put) {
         const uint32_t g = lane >> 4;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -122,38 +126,43 @@ struct Attn4 {
                 w.hi0 = a.n_kv;
             }
             const float * q = a.q + (size_t)t * a.q_stride + (size_t)hq * D + 4u * g;
-            float x[NB][8], top = 0.0f;
+            float top = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const float4 u = *(const float4 *)(q + 32 * b), v = *(const float4 *)(q + 32 * b + 16);
-                x[b][0] = u.x; x[b][1] = u.y; x[b][2] = u.z; x[b][3] = u.w;
-                x[b][4] = v.x; x[b][5] = v.y; x[b][6] = v.z; x[b][7] = v.w;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[b][i]));
+                top = fmaxf(fmaxf(fmaxf(top, fabsf(u.x)), fmaxf(fabsf(u.y), fabsf(u.z))), fabsf(u.w));
+                top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
             }
             top = rows_max(top);
+            asm volatile("" : "+v"(q));                            // (read again rather than kept: D 512 has no registers for it)
             const int e = 140 - (int)(fb(top) >> 23);              // 2^e top in [2^13, 2^14)
-            csc[n] = __builtin_ldexpf(a.scale * kLog2e, 24 - e);
+            csc[n] = __builtin_ldexpf(a.scale * kLog2e, -e);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                const float4 u = *(const float4 *)(q + 32 * b), v = *(const float4 *)(q + 32 * b + 16);
+                const float x[8] = { u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w };
                 float sum = 0.0f;
                 float y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    y[i] = __builtin_ldexpf(x[b][i], e);
+                    y[i] = __builtin_ldexpf(x[i], e);
                     sum += y[i];
-                    if (i >= 4) y[i] *= 0.0625f;                   // these meet codes times 16
                 }
-                qs[n][b] = rows_sum(sum) * 0x1p-24f;
-                const float z[8] = { y[0], y[2], y[4], y[6], y[1], y[3], y[5], y[7] };
+                if constexpr (TYPE == kKvQ4_1) qs[n][b] = rows_sum(sum);
+                if (put) {
+                    const float z[8] = { y[0], y[2], y[4], y[6], y[1], y[3], y[5], y[7] };
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const _Float16 hi = (_Float16)z[i];
-                    qh[n][b][i] = hi;
-                    ql[n][b][i] = (_Float16)(z[i] - (float)hi);
+                    for (int i = 0; i < 4; ++i) {
+                        hi[i] = pair_of(z[2 * i], z[2 * i + 1]);
+                        lo[i] = pair_of(z[2 * i] - half_of(hi[i], 0), z[2 * i + 1] - half_of(hi[i], 1));
+                    }
+                    lds[((n * NB + b) * 2 + 0) * 64 + lane] = of_words(hi);
+                    lds[((n * NB + b) * 2 + 1) * 64 + lane] = of_words(lo);
                 }
-                bias[n][b] = 0.0f;
             }
+#pragma unroll
+            for (int b = 0; b < (TYPE == kKvQ4_1 ? NB : 1); ++b) bias[n][b] = 0.0f;
 #pragma unroll
             for (int j = 0; j < 2 * NB; ++j) o[n][j] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
             m[n] = -__builtin_inff();
@@ -161,42 +170,41 @@ struct Attn4 {
         }
     }
 
-    __device__ __forceinline__ void load_k(KTile<D, TYPE> & k, const uint8_t * p, size_t pair, uint32_t lane) const {
+    template <bool V>
+    static __device__ __forceinline__ void load(Ch & k, const uint8_t * p, size_t pair, uint32_t lane) {
+        constexpr uint32_t n = TYPE == kKvQ4_1 ? 2u : 1u;
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
+        for (int j = 0; j < NPC; ++j) {
             const uint8_t * t = p + j * pair;
+            if constexpr (V) {
+                k.w[j] = *(const uint4 *)(t + 16u * lane);
+            } else {
+                const uint2 x = *(const uint2 *)(t + 8u * lane), y = *(const uint2 *)(t + 512u + 8u * lane);
+                k.w[j] = make_uint4(x.x, x.y, y.x, y.y);
+            }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) k.w[j][s] = *(const uint2 *)(t + 512u * s + 8u * lane);
-            load_scales<D, TYPE>(k.sc[j], t, lane >> 4);
-        }
-    }
-    __device__ __forceinline__ void load_v(VTile<D, TYPE> & v, const uint8_t * p, size_t pair, uint32_t lane) const {
+            for (uint32_t s = 0; s < 2; ++s)
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            const uint8_t * t = p + j * pair;
-            v.w[j] = *(const uint4 *)(t + 16u * lane);
-            load_scales<D, TYPE>(v.sc[j], t, lane >> 4);
+                for (uint32_t i = 0; i < n; ++i)
+                    k.sc[j][s][i] = *(const uint4 *)(t + 1024u + 4u * n * (16u * s + 4u * (lane >> 4)) + 16u * i);
         }
     }
 
-    __device__ __forceinline__ void scores(const KTile<D, TYPE> & k, f4 (&s)[NT][2]) const {
-        constexpr uint32_t L = 0x000F000Fu, H = 0x00F000F0u;
+    __device__ __forceinline__ void scores(const Ch & k, int c, const h8 * q, f4 (&s)[NT][2]) const {
+        constexpr float zero = TYPE == kKvQ4_0 ? 8.0f : 0.0f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+        for (int j = 0; j < NPC; ++j)
 #pragma unroll
-        for (int j = 0; j < NP; ++j)
+            for (int bb = 0; bb < 2; ++bb) {
+                const int b = NBC * c + 2 * j + bb;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int bb = 0; bb < 2; ++bb) {
-                    const int b = 2 * j + bb;
-                    const uint32_t w = bb ? k.w[j][u].y : k.w[j][u].x, w8 = w >> 8;
-                    const h8 c = codes(w & L, w & H, w8 & L, w8 & H);
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t w = u ? (bb ? k.w[j].w : k.w[j].z) : (bb ? k.w[j].y : k.w[j].x);
+                    const h8 n8 = four(codes_lo(w, zero), codes_hi(w, zero), codes_lo(w >> 8, zero), codes_hi(w >> 8, zero));
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const float z = TYPE == kKvQ4_0 ? -8.0f * qs[n][b] : 0.0f;
-                        f4 x = mfma(c, qh[n][b], f4{ z, z, z, z });
-                        x = mfma(c, ql[n][b], x);
+                        f4 x = mfma(n8, q[((n * NB + b) * 2 + 0) * 64], f4{ 0.0f, 0.0f, 0.0f, 0.0f });
+                        x = mfma(n8, q[((n * NB + b) * 2 + 1) * 64], x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             s[n][u][i] = __builtin_fmaf(half_of(scale_d<TYPE>(k.sc[j][u], i), bb), x[i], s[n][u][i]);
@@ -205,15 +213,15 @@ struct Attn4 {
                         }
                     }
                 }
+            }
     }
 
-    // One tile: MASKED when some row does not see all of it (or a mask is given); c0 its first cell.
+    // The weights of a tile from its scores: s becomes p 2^k. MASKED when some row does not see all of it (or a mask is
+    // given): vis gets the cells that the lane's row sees (bit 4 u + i: its cell i of group u). c0: the first cell.
     template <bool MASKED>
-    __device__ __forceinline__ void tile(const Attn4Args & a, f4 (&s)[NT][2], const VTile<D, TYPE> & v, uint32_t c0,
-                                         uint32_t lane, float kexp) {
-        constexpr uint32_t L = 0x000F000Fu, H = 0x00F000F0u;
+    __device__ __forceinline__ void weights(const Attn4Args & a, f4 (&s)[NT][2], uint32_t (&vis)[NT], uint32_t c0, uint32_t lane,
+                                            float kexp) {
         const uint32_t g = lane >> 4;
-        uint32_t vis[NT];                                          // bit 4 u + i: the lane's cell i of group u
         bool grow = false;
         float top[NT];
 #pragma unroll
@@ -236,91 +244,92 @@ struct Attn4 {
                         vis[n] |= in ? 1u << (4 * u + i) : 0u;
                         s[n][u][i] = in ? x : -__builtin_inff();
                     }
-            } else {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[n][u][i] *= csc[n];
             }
             float x = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3]));
             x = fmaxf(x, fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
-            top[n] = rows_max(x);
-            grow |= top[n] > m[n];
+            top[n] = MASKED ? x : x * csc[n];
+            grow |= top[n] > m[n] + kSlack;
         }
-        if (__ballot(grow)) {                                      // a new maximum: what is summed so far shrinks
+        if (__ballot(grow)) {                                      // a larger maximum: what is summed so far shrinks
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float mn = fmaxf(m[n], top[n]);
+                const float mn = fmaxf(m[n], rows_max(top[n]));
                 const float f = mn == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
                 m[n] = mn;
                 l[n] *= f;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) bias[n][b] *= f;
+                for (int b = 0; b < (TYPE == kKvQ4_1 ? NB : 1); ++b) bias[n][b] *= f;
 #pragma unroll
                 for (int j = 0; j < 2 * NB; ++j) o[n][j] *= f;
             }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float sub = (m[n] == -__builtin_inff() ? 0.0f : m[n]) - kexp;
+            const float sub = kexp - (m[n] == -__builtin_inff() ? 0.0f : m[n]), unit = MASKED ? 1.0f : csc[n];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[n][u][i] = __builtin_amdgcn_exp2f(s[n][u][i] - sub);
+                    s[n][u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][u][i], unit, sub));
                     l[n] += s[n][u][i];
                 }
         }
+    }
+
+    template <bool MASKED>
+    __device__ __forceinline__ void values(const Ch & v, int c, const f4 (&s)[NT][2], const uint32_t (&vis)[NT]) {
 #pragma unroll
-        for (int j = 0; j < NP; ++j)
+        for (int j = 0; j < NPC; ++j)
 #pragma unroll
             for (int bb = 0; bb < 2; ++bb) {
-                const int b = 2 * j + bb;
-                const uint32_t w0 = bb ? v.w[j].z : v.w[j].x, w1 = bb ? v.w[j].w : v.w[j].y, x0 = w0 >> 8, x1 = w1 >> 8;
-                const h8 clo = codes(w0 & L, x0 & L, w1 & L, x1 & L), chi = codes(w0 & H, x0 & H, w1 & H, x1 & H);
+                const int b = NBC * c + 2 * j + bb;
+                const uint32_t w0 = bb ? v.w[j].z : v.w[j].x, w1 = bb ? v.w[j].w : v.w[j].y;
+                const h8 clo = four(codes_lo(w0, 8.0f), codes_lo(w0 >> 8, 8.0f), codes_lo(w1, 8.0f), codes_lo(w1 >> 8, 8.0f));
+                const h8 chi = four(codes_hi(w0, 8.0f), codes_hi(w0 >> 8, 8.0f), codes_hi(w1, 8.0f), codes_hi(w1 >> 8, 8.0f));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    h8 ph, pl;
+                    uint32_t ph[4], pl[4];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool in = !MASKED || ((vis[n] >> (4 * u + i)) & 1u);
-                            const float d = half_of(in ? scale_d<TYPE>(v.sc[j][u], i) : 0u, bb);
-                            const float p = s[n][u][i];
-                            const _Float16 hi = (_Float16)__builtin_fmaf(p, d, -0.0f);
-                            ph[4 * u + i] = hi;
-                            pl[4 * u + i] = (_Float16)__builtin_fmaf(p, d, -(float)hi);
-                            if constexpr (TYPE == kKvQ4_0) bias[n][b] = __builtin_fmaf(p, d, bias[n][b]);
-                            else bias[n][b] = __builtin_fmaf(p, half_of(in ? scale_m(v.sc[j][u], i) : 0u, bb), bias[n][b]);
+                    for (int x = 0; x < 4; ++x) {                  // cells 2 x, 2 x + 1 of the lane's eight
+                        const int u = x >> 1, i = 2 * (x & 1);
+                        const float p0 = s[n][u][i], p1 = s[n][u][i + 1];
+                        const bool in0 = !MASKED || ((vis[n] >> (2 * x)) & 1u), in1 = !MASKED || ((vis[n] >> (2 * x + 1)) & 1u);
+                        const float d0 = half_of(in0 ? scale_d<TYPE>(v.sc[j][u], i) : 0u, bb);
+                        const float d1 = half_of(in1 ? scale_d<TYPE>(v.sc[j][u], i + 1) : 0u, bb);
+                        ph[x] = pair_of(__builtin_fmaf(p0, d0, -0.0f), __builtin_fmaf(p1, d1, -0.0f));
+                        pl[x] = pair_of(__builtin_fmaf(p0, d0, -half_of(ph[x], 0)), __builtin_fmaf(p1, d1, -half_of(ph[x], 1)));
+                        if constexpr (TYPE == kKvQ4_1) {
+                            const float m0 = half_of(in0 ? scale_m(v.sc[j][u], i) : 0u, bb);
+                            const float m1 = half_of(in1 ? scale_m(v.sc[j][u], i + 1) : 0u, bb);
+                            bias[n][b] = __builtin_fmaf(p0, __builtin_fmaf(d0, 8.0f, m0), bias[n][b]);
+                            bias[n][b] = __builtin_fmaf(p1, __builtin_fmaf(d1, 8.0f, m1), bias[n][b]);
                         }
-                    o[n][2 * b] = mfma(clo, ph, o[n][2 * b]);
-                    o[n][2 * b] = mfma(clo, pl, o[n][2 * b]);
-                    o[n][2 * b + 1] = mfma(chi, ph, o[n][2 * b + 1]);
-                    o[n][2 * b + 1] = mfma(chi, pl, o[n][2 * b + 1]);
+                    }
+                    o[n][2 * b] = mfma(clo, of_words(ph), o[n][2 * b]);
+                    o[n][2 * b + 1] = mfma(chi, of_words(ph), o[n][2 * b + 1]);
+                    o[n][2 * b] = mfma(clo, of_words(pl), o[n][2 * b]);
+                    o[n][2 * b + 1] = mfma(chi, of_words(pl), o[n][2 * b + 1]);
                 }
             }
     }
 
-    // The next tile at or after i (in steps) that a row of the wave sees; t1 when there is none.
-    __device__ __forceinline__ uint32_t next(uint32_t i, uint32_t t1, uint32_t step) const {
+    // The next tile at or after i (in steps) that all rows of the wave see whole (WHOLE; none under a mask), or that a row
+    // sees and not all see whole; t1 when there is none.
+    template <bool WHOLE>
+    __device__ __forceinline__ uint32_t next(const Attn4Args & a, uint32_t i, uint32_t t1, uint32_t step) const {
         for (; i < t1; i += step) {
-            bool any = false;
+            const uint32_t c0 = 32u * i, c1 = c0 + 32u;
+            bool any = false, all = a.mask == nullptr;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                any |= (row[n].lo0 < row[n].hi0 && row[n].lo0 < 32u * i + 32u && row[n].hi0 > 32u * i) ||
-                       (row[n].lo1 < row[n].hi1 && row[n].lo1 < 32u * i + 32u && row[n].hi1 > 32u * i);
-            if (__ballot(any)) break;
+            for (int n = 0; n < NT; ++n) {
+                all = all && ((row[n].lo0 <= c0 && row[n].hi0 >= c1) || (row[n].lo1 <= c0 && row[n].hi1 >= c1));
+                any |= (row[n].lo0 < row[n].hi0 && row[n].lo0 < c1 && row[n].hi0 > c0) ||
+                       (row[n].lo1 < row[n].hi1 && row[n].lo1 < c1 && row[n].hi1 > c0);
+            }
+            const bool whole = __ballot(!all) == 0ull;
+            if (WHOLE ? whole : (!whole && __ballot(any) != 0ull)) break;
         }
         return min(i, t1);
-    }
-    __device__ __forceinline__ bool whole(const Attn4Args & a, uint32_t i) const {
-        bool all = a.mask == nullptr;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            all = all && ((row[n].lo0 <= 32u * i && row[n].hi0 >= 32u * i + 32u) ||
-                          (row[n].lo1 <= 32u * i && row[n].hi1 >= 32u * i + 32u));
-        return __ballot(!all) == 0ull;
     }
     // The tiles that the rows can see: [lo, hi)
     __device__ __forceinline__ void hull(uint32_t & t0, uint32_t & t1) const {
@@ -338,35 +347,58 @@ struct Attn4 {
         lo = __builtin_amdgcn_readfirstlane(lo);
         hi = __builtin_amdgcn_readfirstlane(hi);
         t0 = min(lo, hi) / 32u;
-        t1 = (uint32_t)(((uint64_t)hi + 31u) / 32u);
+        t1 = (hi + 31u) / 32u;                                     // (cells stay below 2^31)
     }
 
-    __device__ __forceinline__ void run(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, uint32_t lane) {
-        const size_t tb = kv4_tile_bytes(TYPE), pair = (size_t)a.n_tiles * tb;
-        const uint8_t * kp = a.k + kKv4Header + (size_t)h * NP * pair, * vp = a.v + kKv4Header + (size_t)h * NP * pair;
-        // 2^k: the largest |d| of the V plane times 2^k in [2^14, 2^15) (an infinite one counts as the largest finite)
-        const uint32_t dm = *(const uint32_t *)a.v;
-        const float top = (float)__builtin_bit_cast(_Float16, (uint16_t)min(dm, 0x7BFFu));
-        const float kexp = top == 0.0f ? 0.0f : (float)(14 - ((int)(fb(top) >> 23) - 127));
-        uint32_t t0, t1;
-        hull(t0, t1);
-        uint32_t i = next(t0 + part, t1, parts);
+    // The tiles t0, t0 + parts, .. below t1 that are (not) whole, the chunks of a tile and the next tile's first one loaded
+    // ahead.
+    template <bool WHOLE>
+    __device__ __forceinline__ void tiles(const Attn4Args & a, const uint8_t * kp, const uint8_t * vp, size_t pair, uint32_t t0,
+                                          uint32_t t1, uint32_t parts, float kexp, const h8 * lds, uint32_t lane) {
+        constexpr size_t tb = kv4_tile_bytes(TYPE);
+        uint32_t i = next<WHOLE>(a, t0, t1, parts);
         if (i >= t1) return;
-        KTile<D, TYPE> k;
-        VTile<D, TYPE> v;
-        load_k(k, kp + i * tb, pair, lane);
-        load_v(v, vp + i * tb, pair, lane);
+        Ch k[BUF], v[BUF];
+        load<false>(k[0], kp + i * tb, pair, lane);
+        load<true>(v[0], vp + i * tb, pair, lane);
         for (;;) {
-            const uint32_t nx = next(i + parts, t1, parts), ld = nx < t1 ? nx : i;
+            const uint32_t nx = next<WHOLE>(a, i + parts, t1, parts), ld = nx < t1 ? nx : i;
+            uint32_t ql = lane;                                    // the pieces of q are read from LDS for every tile: kept in
+            asm volatile("" : "+v"(ql));                           // registers they would spill
             f4 s[NT][2];
-            scores(k, s);
-            load_k(k, kp + ld * tb, pair, lane);
-            if (whole(a, i)) tile<false>(a, s, v, 32u * i, lane, kexp);
-            else tile<true>(a, s, v, 32u * i, lane, kexp);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if constexpr (BUF == 2)
+                    load<false>(k[(c + 1) & 1], kp + (c + 1 < NC ? i : ld) * tb + ((c + 1) % NC) * NPC * pair, pair, lane);
+                scores(k[c & (BUF - 1)], c, lds + ql, s);
+            }
+            if constexpr (BUF == 1) load<false>(k[0], kp + ld * tb, pair, lane);
+            uint32_t vis[NT];
+            weights<!WHOLE>(a, s, vis, 32u * i, lane, kexp);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if constexpr (BUF == 2)
+                    load<true>(v[(c + 1) & 1], vp + (c + 1 < NC ? i : ld) * tb + ((c + 1) % NC) * NPC * pair, pair, lane);
+                values<!WHOLE>(v[c & (BUF - 1)], c, s, vis);
+            }
             if (nx >= t1) break;
-            load_v(v, vp + ld * tb, pair, lane);
+            if constexpr (BUF == 1) load<true>(v[0], vp + ld * tb, pair, lane);
             i = nx;
         }
+    }
+    __device__ __forceinline__ void run(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, const h8 * lds, uint32_t lane) {
+        const size_t pair = (size_t)a.n_tiles * kv4_tile_bytes(TYPE);
+        const uint8_t * kp = a.k + kKv4Header + (size_t)h * (D / 64) * pair, * vp = a.v + kKv4Header + (size_t)h * (D / 64) * pair;
+        // 2^k: the largest |d| of the V plane times 2^k in [2^8, 2^9) (an infinite one counts as the largest finite)
+        const uint32_t dm = *(const uint32_t *)a.v;
+        const float top = (float)__builtin_bit_cast(_Float16, (uint16_t)min(dm, 0x7BFFu));
+        const float kexp = top == 0.0f ? 0.0f : (float)(8 - ((int)(fb(top) >> 23) - 127));
+        uint32_t t0, t1;
+        hull(t0, t1);
+        tiles<true>(a, kp, vp, pair, t0 + part, t1, parts, kexp, lds, lane);
+        tiles<false>(a, kp, vp, pair, t0 + part, t1, parts, kexp, lds, lane);
     }
 
     // Rows summed over their lanes; o becomes sum p v (2^k times), value 32 b + 16 c + 4 g + i in o[2 b + c][i].
@@ -374,32 +406,32 @@ struct Attn4 {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             l[n] = rows_sum(l[n]);
+            if constexpr (TYPE == kKvQ4_1)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const float z = rows_sum(bias[n][b]) * (TYPE == kKvQ4_0 ? -8.0f : 1.0f);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o[n][2 * b][i] = __builtin_fmaf(o[n][2 * b][i], 0x1p24f, z);
-                    o[n][2 * b + 1][i] = __builtin_fmaf(o[n][2 * b + 1][i], 0x1p20f, z);
+                for (int b = 0; b < NB; ++b) {
+                    const float z = rows_sum(bias[n][b]);
+                    o[n][2 * b] += z;
+                    o[n][2 * b + 1] += z;
                 }
-            }
         }
     }
 };
 
 // Workgroup (KV head, split, group of rows), KV heads fastest: with eight of them every XCD's L2 holds one head.
 template <int D, int NT, uint32_t TYPE, bool SPLIT>
-__global__ __launch_bounds__(256, D >= 256 || NT > 1 ? 1 : 2) void k_attn4(Attn4Args a) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : D <= 256 ? 2 : 1) void k_attn4(Attn4Args a) {
     using A = Attn4<D, NT, TYPE, SPLIT>;
     constexpr uint32_t kRows = 16u * NT * (SPLIT ? 1u : kWaves);
     const uint32_t h = blockIdx.x % a.n_head_kv, rest = blockIdx.x / a.n_head_kv, split = rest % a.S;
     const uint32_t n_rg = gridDim.x / a.n_head_kv / a.S, rg = n_rg - 1u - rest / a.S;   // causal: the long rows first
     const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u, g = lane >> 4;
     const uint32_t r0 = rg * kRows + (SPLIT ? 0u : 16u * NT * wave), R = a.T * a.G;
+    __shared__ h8 lq[(SPLIT ? 1 : kWaves) * NT * A::NB * 2 * 64];
     A w;
-    w.load_rows(a, h, r0, lane);
-    if constexpr (SPLIT) w.run(a, h, split * kWaves + wave, a.S * kWaves, lane);
-    else w.run(a, h, split, a.S, lane);
+    w.load_rows(a, h, r0, lane, lq + (SPLIT ? 0u : wave) * NT * A::NB * 2 * 64, !SPLIT || wave == 0u);
+    __syncthreads();
+    if constexpr (SPLIT) w.run(a, h, split * kWaves + wave, a.S * kWaves, lq, lane);
+    else w.run(a, h, split, a.S, lq + wave * NT * A::NB * 2 * 64, lane);
     w.finish();
     if constexpr (SPLIT) {                                         // the waves' sums joined
         constexpr uint32_t DC = D < 128 ? D : 128;                  // values joined at a time
@@ -479,30 +511,56 @@ __global__ __launch_bounds__(256, D >= 256 || NT > 1 ? 1 : 2) void k_attn4(Attn4
     }
 }
 
-// The splits of a row joined, in order: a thread a value.
+// The splits of a row joined: a workgroup a row, 256 / (D / 4) threads of the same four values take splits in turn, then
+// meet in LDS; the order of the additions is fixed.
 template <int D>
-__global__ __launch_bounds__(D) void k_attn4_join(Attn4Args a) {
-    const uint32_t ro = blockIdx.x, nh = a.G * a.n_head_kv, d = threadIdx.x;
+__global__ __launch_bounds__(256) void k_attn4_join(Attn4Args a) {
+    constexpr uint32_t W = D / 4, NG = 256u / W;
+    __shared__ float4 acc[256];
+    __shared__ float wt[64];
+    const uint32_t ro = blockIdx.x, nh = a.G * a.n_head_kv, c = threadIdx.x % W, s0 = threadIdx.x / W;
     const size_t nr = (size_t)a.T * nh;
-    const float2 * ml = (const float2 *)a.part;
-    const float * po = a.part + 2u * a.S * nr + (size_t)ro * D + d;
-    float M = -__builtin_inff();
-    for (uint32_t s = 0; s < a.S; ++s) M = fmaxf(M, ml[s * nr + ro].x);
-    float y = 0.0f, L = 0.0f;
-    for (uint32_t s = 0; s < a.S; ++s) {
-        const float2 e = ml[s * nr + ro];
+    const float4 * po = (const float4 *)(a.part + 2u * a.S * nr + (size_t)ro * D) + c;
+    if (threadIdx.x < 64u) {                                       // S <= 64: a lane a split
+        float2 e = make_float2(-__builtin_inff(), 0.0f);
+        if (threadIdx.x < a.S) e = ((const float2 *)a.part)[threadIdx.x * nr + ro];
+        float M = e.x;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
         const float f = e.x == M ? 1.0f : __builtin_amdgcn_exp2f(e.x - M);
-        L += e.y * f;
-        y += po[s * nr * D] * f;
+        float L = e.y * f;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) L += __shfl_xor(L, d);
+        wt[threadIdx.x] = L == 0.0f ? 0.0f : f / L;
     }
-    a.out[(size_t)(ro / nh) * a.out_stride + (size_t)(ro % nh) * D + d] = L == 0.0f ? 0.0f : y / L;
+    float4 x[64 / NG];
+#pragma unroll
+    for (uint32_t i = 0; i < 64u / NG; ++i)                        // all loads in flight at once
+        x[i] = s0 + NG * i < a.S ? po[(size_t)(s0 + NG * i) * nr * W] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __syncthreads();
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (uint32_t i = 0; i < 64u / NG; ++i) {
+        const float f = wt[s0 + NG * i];
+        if (s0 + NG * i < a.S) { y.x += x[i].x * f; y.y += x[i].y * f; y.z += x[i].z * f; y.w += x[i].w * f; }
+    }
+    acc[threadIdx.x] = y;
+    __syncthreads();
+    if (s0 == 0u) {
+#pragma unroll
+        for (uint32_t i = 1; i < NG; ++i) {
+            const float4 z = acc[i * W + c];
+            y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+        }
+        *((float4 *)(a.out + (size_t)(ro / nh) * a.out_stride + (size_t)(ro % nh) * D) + c) = y;
+    }
 }
 
 template <int D, int NT, uint32_t TYPE, bool SPLIT>
 static int launch(const Attn4Args & a, hipStream_t s) {
     const uint32_t rows = 16u * NT * (SPLIT ? 1u : kWaves), n_rg = (a.T * a.G + rows - 1u) / rows;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4<D, NT, TYPE, SPLIT>), dim3(n_rg * a.S * a.n_head_kv), dim3(256), 0, s, a);
-    if (a.S > 1u) hipLaunchKernelGGL(k_attn4_join<D>, dim3(a.T * a.G * a.n_head_kv), dim3(D), 0, s, a);
+    if (a.S > 1u) hipLaunchKernelGGL(k_attn4_join<D>, dim3(a.T * a.G * a.n_head_kv), dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 

@@ -272,3 +272,35 @@ def test_refusals(dev):
     assert n_ws > 4096
     assert call(kc=big.h, vc=big.h, n_kv=4096, ws=b.ptr, wb=n_ws - 1) == -1
     assert dev.flash_attn_kv4_ws(0, 64, 4, 2, 4096) == 0 and dev.flash_attn_kv4_ws(2, 65, 4, 2, 4096) == 0
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("nh,nkv,D,T,n_kv,kind", [(8, 4, 128, 64, 1000, "causal"), (8, 4, 128, 64, 1000, "mask"),
+                                                  (8, 4, 256, 64, 1000, "mask"), (32, 8, 128, 1, 1000, "mask"),
+                                                  (32, 8, 128, 16, 20000, "batch"), (4, 1, 64, 1, 30000, "causal")])
+def test_precision(dev, typ, nh, nkv, D, T, n_kv, kind):
+    """The error of whole rows, where roundings of either sign add as squares and not as bounds do. On normal values a score
+    of spread 1 (the sum of D products by 1 / sqrt(D)) is off by the pieces of q (2^-23 of it), the rounding of each block's
+    and the running sum (D / 32 of 2^-24 on some four times the score's spread, for the zero point) and of the change of
+    base (2^-24 of at most 6): below 2^-21 altogether; a weight by that, exp2 (2^-24) and its pieces (2^-22), so that a
+    row, a sum of weights times values of either sign, is off by less than 2^-21 of its length on average, and 2^-19 leaves
+    four times that for the worst of a few hundred rows. (One value of one cell that is rounded to 11 bits shows as 2^-16.)"""
+    E, scale = nkv * D, 1.0 / math.sqrt(D)
+    ki, kc, vi, vc = caches(dev, typ, n_kv, E, 1, v_scale=0.5)
+    q = S.normal(9, T * nh * D).reshape(T, nh * D)
+    rng = np.random.default_rng(3)
+    runs = mask = None
+    if kind == "mask":
+        mask = np.zeros((T, n_kv), np.float16)
+        mask[rng.random((T, n_kv)) < 0.2] = -np.inf
+        mask[:, 0] = 0
+    elif kind == "batch":
+        runs = np.zeros((T, 4), np.uint32)
+        runs[:, 1] = np.cumsum(rng.integers(n_kv // T // 8, n_kv // T, T))
+        runs[1:, 0] = runs[:-1, 1]
+    else:
+        runs = causal(T, n_kv - T)
+    want, _ = R.attention(q, ki, vi, typ, D, nh, nkv, scale, runs, mask)
+    got = attend(dev, q, kc, vc, D, nh, nkv, scale, n_kv, runs, mask).astype(np.float64)
+    rel = np.linalg.norm(got - want, axis=-1) / np.linalg.norm(want, axis=-1)
+    assert rel.max() <= 2.0 ** -19, (rel.max(), np.unravel_index(rel.argmax(), rel.shape))
