@@ -32,13 +32,18 @@ __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_m
 // n - zero of the nibbles at bits 0 and 16 of a word ((1024 + n) - (1024 + zero)) and at bits 4 and 20 ((1024 + 16 n) / 16 -
 // (64 + zero)), exact. (The bits alone, as subnormals n 2^-24, would save the packed operation; but the instruction aligns
 // subnormal operands by their nominal exponent and loses four bits of every product.)
-__device__ __forceinline__ h2 codes_lo(uint32_t w, float zero) {
-    const _Float16 z = (_Float16)(-1024.0f - zero);
-    return __builtin_bit_cast(h2, (w & 0x000F000Fu) | 0x64006400u) + h2{ z, z };
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+    uint32_t r;                                 // one operation: of its two constants only one may be a scalar register
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(magic));
+    return r;
 }
-__device__ __forceinline__ h2 codes_hi(uint32_t w, float zero) {
+__device__ __forceinline__ h2 codes_lo(uint32_t w, uint32_t magic, float zero) {
+    const _Float16 z = (_Float16)(-1024.0f - zero);
+    return __builtin_bit_cast(h2, and_or(w, 0x000F000Fu, magic)) + h2{ z, z };
+}
+__device__ __forceinline__ h2 codes_hi(uint32_t w, uint32_t magic, float zero) {
     const _Float16 z = (_Float16)(-64.0f - zero), f = (_Float16)0.0625f;
-    return __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00F000F0u) | 0x64006400u), h2{ f, f }, h2{ z, z });
+    return __builtin_elementwise_fma(__builtin_bit_cast(h2, and_or(w, 0x00F000F0u, magic)), h2{ f, f }, h2{ z, z });
 }
 // Two f32 as f16. The word is made once: left to itself the compiler rounds an operand of the matrix instruction and the
 // same value in the residual that follows it by different instructions, once and twice, which differ in rare ties.
@@ -64,34 +69,38 @@ __device__ __forceinline__ float rows_sum(float x) {
 }
 
 constexpr uint32_t kWaves = 4;
+#ifndef FENCE
+#define FENCE 256
+#endif
+constexpr int kFence = FENCE;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 6.0f;                  // weights are at most 2^6: a maximum is followed when it is passed by more
 
-// A chunk of a tile: 64 NP values of its 32 cells as a lane holds them, codes and scales.
-template <int NP, uint32_t TYPE>
-struct Chunk {
-    uint4 w[NP];                                // K: two groups of 16 cells x two blocks; V: two blocks x two groups
-    uint4 sc[NP][2][TYPE == kKvQ4_1 ? 2 : 1];   // [group of 16 cells] the lane's four cells
+// A tile of one plane as a lane holds it: the codes, and of the scales the words of one cell (the lane's place in its row of
+// 16 lanes says which): the others are fetched from the row's lanes when they are needed.
+template <int D, uint32_t TYPE>
+struct Tile {
+    uint4 w[D / 64];                            // K: two groups of 16 cells x two blocks; V: two blocks x two groups
+    uint32_t d[D / 64];                         // {d, d of the next cell}
+    uint32_t m[TYPE == kKvQ4_1 ? D / 64 : 1];
 };
-
-// The word {d of block 0, d of block 1} of cell i (of the lane's four) and, q4_1, {m, m}.
-template <uint32_t TYPE, class T>
-__device__ __forceinline__ uint32_t scale_d(const T & sc, int i) {
-    if constexpr (TYPE == kKvQ4_1) return i == 0 ? sc[0].x : i == 1 ? sc[0].z : i == 2 ? sc[1].x : sc[1].z;
-    else return i == 0 ? sc[0].x : i == 1 ? sc[0].y : i == 2 ? sc[0].z : sc[0].w;
+// The word that lane I of the row of 16 lanes holds: block I / 4, group of 16 cells I / 2 % 2, cells 4 g + 2 (I % 2) and
+// the next.
+template <int I>
+__device__ __forceinline__ uint32_t from_row(uint32_t w) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0x150 + I, 0xF, 0xF, true);
 }
-template <class T>
-__device__ __forceinline__ uint32_t scale_m(const T & sc, int i) {
-    return i == 0 ? sc[0].y : i == 1 ? sc[0].w : i == 2 ? sc[1].y : sc[1].w;
+__device__ __forceinline__ void all_cells(uint32_t w, uint32_t (&x)[2][4]) {
+    x[0][0] = from_row<0>(w); x[0][1] = from_row<1>(w); x[0][2] = from_row<2>(w); x[0][3] = from_row<3>(w);
+    x[1][0] = from_row<4>(w); x[1][1] = from_row<5>(w); x[1][2] = from_row<6>(w); x[1][3] = from_row<7>(w);
 }
 
 // SPLIT: the four waves of a workgroup have the same rows and take different tiles; else each has rows of its own.
 template <int D, int NT, uint32_t TYPE, bool SPLIT>
 struct Attn4 {
     static constexpr int NB = D / 32;                              // blocks of a head
-    static constexpr int DC = D < 128 ? D : 128, NC = D / DC, NPC = DC / 64, NBC = DC / 32;   // a chunk's values; chunks
-    static constexpr int BUF = NC > 1 ? 2 : 1;
-    using Ch = Chunk<NPC, TYPE>;
+    static constexpr int AHEAD = D >= 512 ? 1 : 2;                 // tiles loaded ahead
+    using Tl = Tile<D, TYPE>;
     struct Row {                                                   // of the lane's query row in each group of 16
         uint32_t lo0, hi0, lo1, hi1, t;
     };
@@ -101,6 +110,7 @@ struct Attn4 {
     f4 o[NT][2 * NB];
     float bias[NT][TYPE == kKvQ4_1 ? NB : 1];                      // q4_1: sum p (m + 8 d)
     float m[NT], l[NT];
+    uint32_t magic;                                                // 0x64006400 (f16 1024) in a vector register
 
     __device__ __forceinline__ bool sees(int n, uint32_t c) const {
         return (c >= row[n].lo0 && c < row[n].hi0) || (c >= row[n].lo1 && c < row[n].hi1);
@@ -109,6 +119,7 @@ struct Attn4 {
     // The rows' runs and queries; put: this wave writes the queries' pieces to `lds` (the caller's barrier follows).
     __device__ __forceinline__ void load_rows(const Attn4Args & a, uint32_t h, uint32_t r0, uint32_t lane, h8 * lds, bool put) {
         const uint32_t g = lane >> 4;
+        asm("v_mov_b32 %0, 0x64006400" : "=v"(magic));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const uint32_t r = r0 + 16u * n + (lane & 15u);
@@ -171,10 +182,10 @@ struct Attn4 {
     }
 
     template <bool V>
-    static __device__ __forceinline__ void load(Ch & k, const uint8_t * p, size_t pair, uint32_t lane) {
-        constexpr uint32_t n = TYPE == kKvQ4_1 ? 2u : 1u;
+    static __device__ __forceinline__ void load(Tl & k, const uint8_t * p, size_t pair, uint32_t lane) {
+        const uint32_t word = 8u * (lane >> 4) + (lane & 7u);
 #pragma unroll
-        for (int j = 0; j < NPC; ++j) {
+        for (int j = 0; j < D / 64; ++j) {
             const uint8_t * t = p + j * pair;
             if constexpr (V) {
                 k.w[j] = *(const uint4 *)(t + 16u * lane);
@@ -182,38 +193,47 @@ struct Attn4 {
                 const uint2 x = *(const uint2 *)(t + 8u * lane), y = *(const uint2 *)(t + 512u + 8u * lane);
                 k.w[j] = make_uint4(x.x, x.y, y.x, y.y);
             }
-#pragma unroll
-            for (uint32_t s = 0; s < 2; ++s)
-#pragma unroll
-                for (uint32_t i = 0; i < n; ++i)
-                    k.sc[j][s][i] = *(const uint4 *)(t + 1024u + 4u * n * (16u * s + 4u * (lane >> 4)) + 16u * i);
+            if constexpr (TYPE == kKvQ4_1) {
+                const uint2 z = *(const uint2 *)(t + 1024u + 8u * word);
+                k.d[j] = z.x;
+                k.m[j] = z.y;
+            } else {
+                k.d[j] = *(const uint32_t *)(t + 1024u + 4u * word);
+            }
         }
     }
 
-    __device__ __forceinline__ void scores(const Ch & k, int c, const h8 * q, f4 (&s)[NT][2]) const {
+    __device__ __forceinline__ void scores(const Tl & k, const h8 * q, f4 (&s)[NT][2]) const {
         constexpr float zero = TYPE == kKvQ4_0 ? 8.0f : 0.0f;
 #pragma unroll
-        for (int j = 0; j < NPC; ++j)
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            uint32_t dw[2][4], mw[2][4];
+            all_cells(k.d[j], dw);
+            if constexpr (TYPE == kKvQ4_1) all_cells(k.m[j], mw);
 #pragma unroll
             for (int bb = 0; bb < 2; ++bb) {
-                const int b = NBC * c + 2 * j + bb;
+                const int b = 2 * j + bb;
+                if constexpr (D >= kFence) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const uint32_t w = u ? (bb ? k.w[j].w : k.w[j].z) : (bb ? k.w[j].y : k.w[j].x);
-                    const h8 n8 = four(codes_lo(w, zero), codes_hi(w, zero), codes_lo(w >> 8, zero), codes_hi(w >> 8, zero));
+                    const h8 n8 = four(codes_lo(w, magic, zero), codes_hi(w, magic, zero), codes_lo(w >> 8, magic, zero), codes_hi(w >> 8, magic, zero));
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         f4 x = mfma(n8, q[((n * NB + b) * 2 + 0) * 64], f4{ 0.0f, 0.0f, 0.0f, 0.0f });
                         x = mfma(n8, q[((n * NB + b) * 2 + 1) * 64], x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            s[n][u][i] = __builtin_fmaf(half_of(scale_d<TYPE>(k.sc[j][u], i), bb), x[i], s[n][u][i]);
-                            if constexpr (TYPE == kKvQ4_1)
-                                s[n][u][i] = __builtin_fmaf(half_of(scale_m(k.sc[j][u], i), bb), qs[n][b], s[n][u][i]);
+                            const int y = 2 * u + (i >> 1);
+                            s[n][u][i] = __builtin_fmaf(half_of(dw[bb][y], i & 1), x[i], s[n][u][i]);
+                            if constexpr (TYPE == kKvQ4_1) s[n][u][i] = __builtin_fmaf(half_of(mw[bb][y], i & 1), qs[n][b], s[n][u][i]);
                         }
                     }
                 }
             }
+        }
     }
 
     // The weights of a tile from its scores: s becomes p 2^k. MASKED when some row does not see all of it (or a mask is
@@ -277,32 +297,41 @@ struct Attn4 {
     }
 
     template <bool MASKED>
-    __device__ __forceinline__ void values(const Ch & v, int c, const f4 (&s)[NT][2], const uint32_t (&vis)[NT]) {
+    __device__ __forceinline__ void values(const Tl & v, const f4 (&s)[NT][2], const uint32_t (&vis)[NT]) {
+        uint32_t p16[NT][4], in[NT][4];                            // of the cells 2 x, 2 x + 1 of the lane's eight
 #pragma unroll
-        for (int j = 0; j < NPC; ++j)
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                p16[n][x] = pair_of(s[n][x >> 1][2 * (x & 1)], s[n][x >> 1][2 * (x & 1) + 1]);
+                in[n][x] = ((vis[n] >> (2 * x)) & 1u ? 0x0000FFFFu : 0u) | ((vis[n] >> (2 * x)) & 2u ? 0xFFFF0000u : 0u);
+            }
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            uint32_t dw[2][4], mw[2][4];
+            all_cells(v.d[j], dw);
+            if constexpr (TYPE == kKvQ4_1) all_cells(v.m[j], mw);
 #pragma unroll
             for (int bb = 0; bb < 2; ++bb) {
-                const int b = NBC * c + 2 * j + bb;
+                const int b = 2 * j + bb;
+                if constexpr (D >= kFence) __builtin_amdgcn_sched_barrier(0);
                 const uint32_t w0 = bb ? v.w[j].z : v.w[j].x, w1 = bb ? v.w[j].w : v.w[j].y;
-                const h8 clo = four(codes_lo(w0, 8.0f), codes_lo(w0 >> 8, 8.0f), codes_lo(w1, 8.0f), codes_lo(w1 >> 8, 8.0f));
-                const h8 chi = four(codes_hi(w0, 8.0f), codes_hi(w0 >> 8, 8.0f), codes_hi(w1, 8.0f), codes_hi(w1 >> 8, 8.0f));
+                const h8 clo = four(codes_lo(w0, magic, 8.0f), codes_lo(w0 >> 8, magic, 8.0f), codes_lo(w1, magic, 8.0f), codes_lo(w1 >> 8, magic, 8.0f));
+                const h8 chi = four(codes_hi(w0, magic, 8.0f), codes_hi(w0 >> 8, magic, 8.0f), codes_hi(w1, magic, 8.0f), codes_hi(w1 >> 8, magic, 8.0f));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     uint32_t ph[4], pl[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {                  // cells 2 x, 2 x + 1 of the lane's eight
-                        const int u = x >> 1, i = 2 * (x & 1);
-                        const float p0 = s[n][u][i], p1 = s[n][u][i + 1];
-                        const bool in0 = !MASKED || ((vis[n] >> (2 * x)) & 1u), in1 = !MASKED || ((vis[n] >> (2 * x + 1)) & 1u);
-                        const float d0 = half_of(in0 ? scale_d<TYPE>(v.sc[j][u], i) : 0u, bb);
-                        const float d1 = half_of(in1 ? scale_d<TYPE>(v.sc[j][u], i + 1) : 0u, bb);
-                        ph[x] = pair_of(__builtin_fmaf(p0, d0, -0.0f), __builtin_fmaf(p1, d1, -0.0f));
-                        pl[x] = pair_of(__builtin_fmaf(p0, d0, -half_of(ph[x], 0)), __builtin_fmaf(p1, d1, -half_of(ph[x], 1)));
+                    for (int x = 0; x < 4; ++x) {
+                        const float p0 = s[n][x >> 1][2 * (x & 1)], p1 = s[n][x >> 1][2 * (x & 1) + 1];
+                        const uint32_t d = MASKED ? dw[bb][x] & in[n][x] : dw[bb][x];
+                        const h2 hi = __builtin_bit_cast(h2, p16[n][x]) * __builtin_bit_cast(h2, d);
+                        ph[x] = __builtin_bit_cast(uint32_t, hi);
+                        pl[x] = pair_of(__builtin_fmaf(p0, half_of(d, 0), -half_of(ph[x], 0)), __builtin_fmaf(p1, half_of(d, 1), -half_of(ph[x], 1)));
                         if constexpr (TYPE == kKvQ4_1) {
-                            const float m0 = half_of(in0 ? scale_m(v.sc[j][u], i) : 0u, bb);
-                            const float m1 = half_of(in1 ? scale_m(v.sc[j][u], i + 1) : 0u, bb);
-                            bias[n][b] = __builtin_fmaf(p0, __builtin_fmaf(d0, 8.0f, m0), bias[n][b]);
-                            bias[n][b] = __builtin_fmaf(p1, __builtin_fmaf(d1, 8.0f, m1), bias[n][b]);
+                            const uint32_t m = MASKED ? mw[bb][x] & in[n][x] : mw[bb][x];
+                            bias[n][b] = __builtin_fmaf(p0, __builtin_fmaf(half_of(d, 0), 8.0f, half_of(m, 0)), bias[n][b]);
+                            bias[n][b] = __builtin_fmaf(p1, __builtin_fmaf(half_of(d, 1), 8.0f, half_of(m, 1)), bias[n][b]);
                         }
                     }
                     o[n][2 * b] = mfma(clo, of_words(ph), o[n][2 * b]);
@@ -311,6 +340,7 @@ struct Attn4 {
                     o[n][2 * b + 1] = mfma(chi, of_words(pl), o[n][2 * b + 1]);
                 }
             }
+        }
     }
 
     // The next tile at or after i (in steps) that all rows of the wave see whole (WHOLE; none under a mask), or that a row
@@ -350,51 +380,60 @@ struct Attn4 {
         t1 = (hi + 31u) / 32u;                                     // (cells stay below 2^31)
     }
 
-    // The tiles t0, t0 + parts, .. below t1 that are (not) whole, the chunks of a tile and the next tile's first one loaded
-    // ahead.
+    // The tiles t0, t0 + parts, .. below t1 that are (not) whole, the next two loaded ahead.
     template <bool WHOLE>
     __device__ __forceinline__ void tiles(const Attn4Args & a, const uint8_t * kp, const uint8_t * vp, size_t pair, uint32_t t0,
                                           uint32_t t1, uint32_t parts, float kexp, const h8 * lds, uint32_t lane) {
         constexpr size_t tb = kv4_tile_bytes(TYPE);
-        uint32_t i = next<WHOLE>(a, t0, t1, parts);
-        if (i >= t1) return;
-        Ch k[BUF], v[BUF];
-        load<false>(k[0], kp + i * tb, pair, lane);
-        load<true>(v[0], vp + i * tb, pair, lane);
-        for (;;) {
-            const uint32_t nx = next<WHOLE>(a, i + parts, t1, parts), ld = nx < t1 ? nx : i;
+        uint32_t i0 = next<WHOLE>(a, t0, t1, parts);
+        if (i0 >= t1) return;
+        uint32_t i1 = next<WHOLE>(a, i0 + parts, t1, parts);
+        Tl k0, v0, k1, v1;
+        load<false>(k0, kp + i0 * tb, pair, lane);
+        load<true>(v0, vp + i0 * tb, pair, lane);
+        if constexpr (AHEAD == 2) {
+            const size_t c1 = (i1 < t1 ? i1 : i0) * tb;            // (past the last tile: the one before again)
+            load<false>(k1, kp + c1, pair, lane);
+            load<true>(v1, vp + c1, pair, lane);
+        }
+        auto one = [&](Tl & k, Tl & v, uint32_t i, uint32_t ahead) {
             uint32_t ql = lane;                                    // the pieces of q are read from LDS for every tile: kept in
             asm volatile("" : "+v"(ql));                           // registers they would spill
             f4 s[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                if constexpr (BUF == 2)
-                    load<false>(k[(c + 1) & 1], kp + (c + 1 < NC ? i : ld) * tb + ((c + 1) % NC) * NPC * pair, pair, lane);
-                scores(k[c & (BUF - 1)], c, lds + ql, s);
-            }
-            if constexpr (BUF == 1) load<false>(k[0], kp + ld * tb, pair, lane);
             uint32_t vis[NT];
+            const size_t c = (ahead < t1 ? ahead : i) * tb;
+            scores(k, lds + ql, s);
+            load<false>(k, kp + c, pair, lane);
             weights<!WHOLE>(a, s, vis, 32u * i, lane, kexp);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                if constexpr (BUF == 2)
-                    load<true>(v[(c + 1) & 1], vp + (c + 1 < NC ? i : ld) * tb + ((c + 1) % NC) * NPC * pair, pair, lane);
-                values<!WHOLE>(v[c & (BUF - 1)], c, s, vis);
+            values<!WHOLE>(v, s, vis);
+            load<true>(v, vp + c, pair, lane);
+        };
+        if constexpr (AHEAD == 1) {
+            for (;;) {
+                one(k0, v0, i0, i1);
+                if (i1 >= t1) return;
+                i0 = i1;
+                i1 = next<WHOLE>(a, i0 + parts, t1, parts);
             }
-            if (nx >= t1) break;
-            if constexpr (BUF == 1) load<true>(v[0], vp + ld * tb, pair, lane);
-            i = nx;
+        }
+        for (;;) {
+            const uint32_t i2 = next<WHOLE>(a, i1 + parts, t1, parts);
+            one(k0, v0, i0, i2);
+            if (i1 >= t1) break;
+            const uint32_t i3 = next<WHOLE>(a, i2 + parts, t1, parts);
+            one(k1, v1, i1, i3);
+            if (i2 >= t1) break;
+            i0 = i2;
+            i1 = i3;
         }
     }
     __device__ __forceinline__ void run(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, const h8 * lds, uint32_t lane) {
         const size_t pair = (size_t)a.n_tiles * kv4_tile_bytes(TYPE);
         const uint8_t * kp = a.k + kKv4Header + (size_t)h * (D / 64) * pair, * vp = a.v + kKv4Header + (size_t)h * (D / 64) * pair;
-        // 2^k: the largest |d| of the V plane times 2^k in [2^8, 2^9) (an infinite one counts as the largest finite)
+        // 2^k: the largest |d| of the V plane times 2^k in [2^8, 2^9) (an infinite one counts as the largest finite), k <= 9
         const uint32_t dm = *(const uint32_t *)a.v;
         const float top = (float)__builtin_bit_cast(_Float16, (uint16_t)min(dm, 0x7BFFu));
-        const float kexp = top == 0.0f ? 0.0f : (float)(8 - ((int)(fb(top) >> 23) - 127));
+        const float kexp = top == 0.0f ? 0.0f : (float)min(8 - ((int)(fb(top) >> 23) - 127), 9);
         uint32_t t0, t1;
         hull(t0, t1);
         tiles<true>(a, kp, vp, pair, t0 + part, t1, parts, kexp, lds, lane);

@@ -10,7 +10,7 @@
 // wave loads them with full-width loads and unpacks them with a mask alone (k_attn4.hip):
 //   K codes  [2 groups of 16 cells][lane 16 g + cell][2 blocks] words: bytes 4 g .. 4 g + 3 of the block
 //   V codes  [lane 16 g + j][2 blocks][2 groups of 16 cells] words: byte j of the block for cells 4 g + 0, 2, 1, 3
-//   scales   [32 cells] {d of block 0, d of block 1} (q4_1: and {m of block 0, m of block 1})
+//   scales   [g][2 blocks][2 groups of 16 cells][2] words {d of cell 4 g + 2 x, of the next one} (q4_1: and {m, m})
 // One cell owns every byte that its row is stored in, so that rows are stored without reading their neighbours'.
 #pragma once
 
@@ -35,7 +35,8 @@ __host__ __device__ inline uint32_t kv4_code(uint32_t which, uint32_t cell, uint
     return 16u * (16u * (c >> 2) + j) + 8u * (b & 1u) + 4u * s + ((i & 1u) << 1 | i >> 1);
 }
 __host__ __device__ inline uint32_t kv4_scale(uint32_t type, uint32_t cell, uint32_t b) {
-    return 1024u + (type == kKvQ4_1 ? 8u : 4u) * (cell & 31u) + 2u * (b & 1u);
+    const uint32_t word = 8u * ((cell >> 2) & 3u) + 4u * (b & 1u) + 2u * ((cell >> 4) & 1u) + ((cell >> 1) & 1u);
+    return 1024u + (type == kKvQ4_1 ? 8u : 4u) * word + 2u * (cell & 1u);
 }
 
 }  // namespace tsr
