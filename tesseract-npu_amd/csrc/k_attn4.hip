@@ -15,6 +15,7 @@
 //            q4_1: sum p (m + 8 d) is summed aside in f32.
 // The scales meet the f32 sums only, where a cell that its row does not see is replaced by nothing: an infinity or a
 // NaN in a masked cell reaches no result. Sums, maxima and results are f32; both splits keep 22 bits of f32's 24.
+#include "attn4_plan.hpp"
 #include "kernels.hpp"
 #include "kv4.hpp"
 #include "tsr_dev.hpp"
@@ -68,21 +69,34 @@ __device__ __forceinline__ float rows_sum(float x) {
     return bf(b[0]) + bf(b[1]);
 }
 
-constexpr uint32_t kWaves = 4;
 #ifndef FENCE
 #define FENCE 256
 #endif
 constexpr int kFence = FENCE;
+constexpr uint32_t kWaves = 4;                  // of a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 6.0f;                  // weights are at most 2^6: a maximum is followed when it is passed by more
 
-// A tile of one plane as a lane holds it: the codes, and of the scales the words of one cell (the lane's place in its row of
-// 16 lanes says which): the others are fetched from the row's lanes when they are needed.
-template <int D, uint32_t TYPE>
+// A tile of one plane as a lane holds it: the codes, and the scales. Where a column of the matrix instruction is a query row
+// (C 1): of each pair of blocks one word {d, d of the next cell} (the lane's place in its row of 16 lanes says which; the
+// others are fetched from the row's lanes when they are needed). Where C columns share a row: the words of the lane's
+// eight cells for the blocks C k + c of its column.
+template <int D, int C, uint32_t TYPE>
 struct Tile {
     uint4 w[D / 64];                            // K: two groups of 16 cells x two blocks; V: two blocks x two groups
-    uint32_t d[D / 64];                         // {d, d of the next cell}
-    uint32_t m[TYPE == kKvQ4_1 ? D / 64 : 1];
+    uint32_t d[C == 1 ? D / 64 : 1];
+    uint32_t m[C == 1 && TYPE == kKvQ4_1 ? D / 64 : 1];
+    uint4 sc[C == 1 ? 1 : D / 32 / C][TYPE == kKvQ4_1 ? 2 : 1];
+    // {d, d of the next cell} of the lane's cells 2 x, 2 x + 1 for its k-th block, and {m, m}
+    __device__ __forceinline__ uint32_t dk(int k, int x) const {
+        const uint4 & u = sc[k][0];
+        if constexpr (TYPE == kKvQ4_1) return x == 0 ? u.x : x == 1 ? u.z : x == 2 ? sc[k][TYPE == kKvQ4_1].x : sc[k][TYPE == kKvQ4_1].z;
+        return x == 0 ? u.x : x == 1 ? u.y : x == 2 ? u.z : u.w;
+    }
+    __device__ __forceinline__ uint32_t mk(int k, int x) const {
+        const uint4 & u = sc[k][0], & v = sc[k][TYPE == kKvQ4_1];
+        return x == 0 ? u.y : x == 1 ? u.w : x == 2 ? v.y : v.w;
+    }
 };
 // The word that lane I of the row of 16 lanes holds: block I / 4, group of 16 cells I / 2 % 2, cells 4 g + 2 (I % 2) and
 // the next.
@@ -95,20 +109,48 @@ __device__ __forceinline__ void all_cells(uint32_t w, uint32_t (&x)[2][4]) {
     x[1][0] = from_row<4>(w); x[1][1] = from_row<5>(w); x[1][2] = from_row<6>(w); x[1][3] = from_row<7>(w);
 }
 
-// SPLIT: the four waves of a workgroup have the same rows and take different tiles; else each has rows of its own.
-template <int D, int NT, uint32_t TYPE, bool SPLIT>
+// The token of row r of a KV head: r / G by a product (r < 2^22, G <= 64: exact).
+__device__ __forceinline__ uint32_t token(const Attn4Args & a, uint32_t r) {
+    return a.T == 1u ? 0u : a.inv_G == 0u ? r : __umulhi(r, a.inv_G);
+}
+// Over the wave, by DPP inside the rows of 16 lanes (the four rows hold the same values).
+__device__ __forceinline__ uint32_t rows16_min(uint32_t v) {
+    v = min(v, (uint32_t)dpp_i<kDppXor1>((int)v));
+    v = min(v, (uint32_t)dpp_i<kDppXor2>((int)v));
+    v = min(v, (uint32_t)dpp_i<kDppRowHalfMirror>((int)v));
+    v = min(v, (uint32_t)dpp_i<kDppRowMirror>((int)v));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+__device__ __forceinline__ uint32_t rows16_max(uint32_t v) { return ~rows16_min(~v); }
+// Sum over the C columns of a row (aligned groups of C lanes).
+template <int C>
+__device__ __forceinline__ float columns_sum(float x) {
+    if constexpr (C >= 2) x += dpp_f<kDppXor1>(x);
+    if constexpr (C >= 4) x += dpp_f<kDppXor2>(x);
+    if constexpr (C >= 8) x += dpp_f<kDppRowHalfMirror>(x);
+    return x;
+}
+
+// SPLIT: the waves of a workgroup have the same rows and take different tiles; else each has rows of its own.
+// C: columns of the matrix instruction a query row. With few rows (a decode token's G query heads) 16 / C rows fill the
+// 16 columns: column C r + c is row r and meets the blocks C k + c alone (its q is zero for the others, and of its results
+// for the values of other blocks nothing is used), so that a lane scales the products and splits the weights of D / 32 / C
+// blocks and not of all D / 32.
+template <int D, int NT, int C, uint32_t TYPE, bool SPLIT>
 struct Attn4 {
-    static constexpr int NB = D / 32;                              // blocks of a head
+    static constexpr int NB = D / 32, NK = NB / C;                 // blocks of a head, of a column
+    static constexpr int RW = 16 / C;                              // query rows of a group of 16 columns
     static constexpr int AHEAD = D >= 512 ? 1 : 2;                 // tiles loaded ahead
-    using Tl = Tile<D, TYPE>;
+    using Tl = Tile<D, C, TYPE>;
     struct Row {                                                   // of the lane's query row in each group of 16
         uint32_t lo0, hi0, lo1, hi1, t;
     };
     Row row[NT];
-    float qs[NT][TYPE == kKvQ4_1 ? NB : 1];                        // q4_1: sum of the block's q
+    const float * qp[NT];
+    float qs[NT][TYPE == kKvQ4_1 ? NK : 1];                        // q4_1: sum of the block's q
     float csc[NT];                                                 // the scores' unit, base 2
     f4 o[NT][2 * NB];
-    float bias[NT][TYPE == kKvQ4_1 ? NB : 1];                      // q4_1: sum p (m + 8 d)
+    float bias[NT][TYPE == kKvQ4_1 ? NK : 1];                      // q4_1: sum p (m + 8 d)
     float m[NT], l[NT];
     uint32_t magic;                                                // 0x64006400 (f16 1024) in a vector register
 
@@ -116,27 +158,35 @@ struct Attn4 {
         return (c >= row[n].lo0 && c < row[n].hi0) || (c >= row[n].lo1 && c < row[n].hi1);
     }
 
-    // The rows' runs and queries; put: this wave writes the queries' pieces to `lds` (the caller's barrier follows).
-    __device__ __forceinline__ void load_rows(const Attn4Args & a, uint32_t h, uint32_t r0, uint32_t lane, h8 * lds, bool put) {
-        const uint32_t g = lane >> 4;
+    // The rows' runs, and where the lane's parts of their queries are.
+    __device__ __forceinline__ void load_runs(const Attn4Args & a, uint32_t h, uint32_t r0, uint32_t lane) {
         asm("v_mov_b32 %0, 0x64006400" : "=v"(magic));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const uint32_t r = r0 + 16u * n + (lane & 15u);
-            const uint32_t ru = min(r, a.T * a.G - 1u), t = ru / a.G, hq = h * a.G + ru % a.G;   // (past the last: its copies)
+            const uint32_t r = r0 + RW * n + (lane & 15u) / C;
+            const uint32_t ru = min(r, a.T * a.G - 1u), t = token(a, ru), hq = h * a.G + ru - t * a.G;   // (past the last: its copies)
             Row & w = row[n];
             w.t = t;
-            if (a.runs != nullptr) {
-                const uint4 u = *(const uint4 *)(a.runs + 4u * (size_t)t);
-                w.lo0 = u.x;
-                w.hi0 = min(u.y, a.n_kv);
-                w.lo1 = u.z;
-                w.hi1 = min(u.w, a.n_kv);
-            } else {
-                w.lo0 = w.lo1 = w.hi1 = 0u;
-                w.hi0 = a.n_kv;
-            }
-            const float * q = a.q + (size_t)t * a.q_stride + (size_t)hq * D + 4u * g;
+            uint4 u = make_uint4(0u, a.n_kv, 0u, 0u);
+            if (a.runs != nullptr) u = *(const uint4 *)(a.runs + (a.T == 1u ? 0u : 4u * (size_t)t));
+            w.lo0 = u.x;
+            w.hi0 = min(u.y, a.n_kv);
+            w.lo1 = u.z;
+            w.hi1 = min(u.w, a.n_kv);
+            qp[n] = a.q + (size_t)t * a.q_stride + (size_t)hq * D + 4u * (lane >> 4);
+#pragma unroll
+            for (int k = 0; k < (TYPE == kKvQ4_1 ? NK : 1); ++k) bias[n][k] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2 * NB; ++j) o[n][j] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+            m[n] = -__builtin_inff();
+            l[n] = 0.0f;
+        }
+    }
+    // The queries; their pieces go to `lds`, [row group][block][piece][lane]. With SPLIT the waves share the blocks out.
+    __device__ __forceinline__ void load_queries(float scale, uint32_t lane, h8 * lds, uint32_t wave) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float * q = qp[n];
             float top = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -145,9 +195,9 @@ struct Attn4 {
                 top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
             }
             top = rows_max(top);
-            asm volatile("" : "+v"(q));                            // (read again rather than kept: D 512 has no registers for it)
+            if constexpr (D > 128) asm volatile("" : "+v"(q));     // (read again rather than kept: no registers for it)
             const int e = 140 - (int)(fb(top) >> 23);              // 2^e top in [2^13, 2^14)
-            csc[n] = __builtin_ldexpf(a.scale * kLog2e, -e);
+            csc[n] = __builtin_ldexpf(scale * kLog2e, -e);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const float4 u = *(const float4 *)(q + 32 * b), v = *(const float4 *)(q + 32 * b + 16);
@@ -159,25 +209,24 @@ struct Attn4 {
                     y[i] = __builtin_ldexpf(x[i], e);
                     sum += y[i];
                 }
-                if constexpr (TYPE == kKvQ4_1) qs[n][b] = rows_sum(sum);
-                if (put) {
+                const bool mine = C == 1 || (lane & (C - 1u)) == b % C;
+                if constexpr (TYPE == kKvQ4_1) {
+                    const float z = rows_sum(sum);
+                    if (mine) qs[n][b / C] = z;
+                }
+                if (!SPLIT || (b % kWaves) == wave) {
                     const float z[8] = { y[0], y[2], y[4], y[6], y[1], y[3], y[5], y[7] };
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         hi[i] = pair_of(z[2 * i], z[2 * i + 1]);
                         lo[i] = pair_of(z[2 * i] - half_of(hi[i], 0), z[2 * i + 1] - half_of(hi[i], 1));
+                        if (!mine) hi[i] = lo[i] = 0u;
                     }
                     lds[((n * NB + b) * 2 + 0) * 64 + lane] = of_words(hi);
                     lds[((n * NB + b) * 2 + 1) * 64 + lane] = of_words(lo);
                 }
             }
-#pragma unroll
-            for (int b = 0; b < (TYPE == kKvQ4_1 ? NB : 1); ++b) bias[n][b] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 2 * NB; ++j) o[n][j] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
-            m[n] = -__builtin_inff();
-            l[n] = 0.0f;
         }
     }
 
@@ -193,20 +242,69 @@ struct Attn4 {
                 const uint2 x = *(const uint2 *)(t + 8u * lane), y = *(const uint2 *)(t + 512u + 8u * lane);
                 k.w[j] = make_uint4(x.x, x.y, y.x, y.y);
             }
-            if constexpr (TYPE == kKvQ4_1) {
+            if constexpr (C == 1 && TYPE == kKvQ4_1) {
                 const uint2 z = *(const uint2 *)(t + 1024u + 8u * word);
                 k.d[j] = z.x;
                 k.m[j] = z.y;
-            } else {
+            } else if constexpr (C == 1) {
                 k.d[j] = *(const uint32_t *)(t + 1024u + 4u * word);
             }
         }
+        if constexpr (C > 1)
+#pragma unroll
+            for (int y = 0; y < NK; ++y) {
+                const uint32_t b = C * y + (lane & (C - 1u));
+                constexpr uint32_t n = TYPE == kKvQ4_1 ? 2u : 1u;
+                const uint8_t * t = p + (b >> 1) * pair + 1024u + 4u * n * (8u * (lane >> 4) + 4u * (b & 1u));
+#pragma unroll
+                for (uint32_t i = 0; i < n; ++i) k.sc[y][i] = *(const uint4 *)(t + 16u * i);
+            }
     }
 
     __device__ __forceinline__ void scores(const Tl & k, const h8 * q, f4 (&s)[NT][2]) const {
         constexpr float zero = TYPE == kKvQ4_0 ? 8.0f : 0.0f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+        if constexpr (C > 1) {
+#pragma unroll
+            for (int y = 0; y < NK; ++y) {
+                f4 x[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const int b = C * y + c;
+                    const uint4 & w4 = k.w[b >> 1];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t w = u ? (b & 1 ? w4.w : w4.z) : (b & 1 ? w4.y : w4.x);
+                        const h8 n8 = four(codes_lo(w, magic, zero), codes_hi(w, magic, zero), codes_lo(w >> 8, magic, zero),
+                                           codes_hi(w >> 8, magic, zero));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            x[n][u] = mfma(n8, q[((n * NB + b) * 2 + 0) * 64], x[n][u]);
+                            x[n][u] = mfma(n8, q[((n * NB + b) * 2 + 1) * 64], x[n][u]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int z = 2 * u + (i >> 1);
+                            s[n][u][i] = __builtin_fmaf(half_of(k.dk(y, z), i & 1), x[n][u][i], s[n][u][i]);
+                            if constexpr (TYPE == kKvQ4_1) s[n][u][i] = __builtin_fmaf(half_of(k.mk(y, z), i & 1), qs[n][y], s[n][u][i]);
+                        }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[n][u][i] = columns_sum<C>(s[n][u][i]);
+        } else
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
             uint32_t dw[2][4], mw[2][4];
@@ -278,7 +376,7 @@ struct Attn4 {
                 m[n] = mn;
                 l[n] *= f;
 #pragma unroll
-                for (int b = 0; b < (TYPE == kKvQ4_1 ? NB : 1); ++b) bias[n][b] *= f;
+                for (int k = 0; k < (TYPE == kKvQ4_1 ? NK : 1); ++k) bias[n][k] *= f;
 #pragma unroll
                 for (int j = 0; j < 2 * NB; ++j) o[n][j] *= f;
             }
@@ -306,138 +404,175 @@ struct Attn4 {
                 p16[n][x] = pair_of(s[n][x >> 1][2 * (x & 1)], s[n][x >> 1][2 * (x & 1) + 1]);
                 in[n][x] = ((vis[n] >> (2 * x)) & 1u ? 0x0000FFFFu : 0u) | ((vis[n] >> (2 * x)) & 2u ? 0xFFFF0000u : 0u);
             }
+        // the pieces of the weights times the scales of a block, {d, d of the next cell} in d and {m, m} in mm
+        auto pieces = [&](int n, int k, const uint32_t (&dd)[4], const uint32_t (&mm)[4], uint32_t (&ph)[4], uint32_t (&pl)[4]) {
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-            uint32_t dw[2][4], mw[2][4];
-            all_cells(v.d[j], dw);
-            if constexpr (TYPE == kKvQ4_1) all_cells(v.m[j], mw);
+            for (int x = 0; x < 4; ++x) {
+                const float p0 = s[n][x >> 1][2 * (x & 1)], p1 = s[n][x >> 1][2 * (x & 1) + 1];
+                const uint32_t d = MASKED ? dd[x] & in[n][x] : dd[x];
+                ph[x] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, p16[n][x]) * __builtin_bit_cast(h2, d));
+                pl[x] = pair_of(__builtin_fmaf(p0, half_of(d, 0), -half_of(ph[x], 0)), __builtin_fmaf(p1, half_of(d, 1), -half_of(ph[x], 1)));
+                if constexpr (TYPE == kKvQ4_1) {
+                    const uint32_t m = MASKED ? mm[x] & in[n][x] : mm[x];
+                    bias[n][k] = __builtin_fmaf(p0, __builtin_fmaf(half_of(d, 0), 8.0f, half_of(m, 0)), bias[n][k]);
+                    bias[n][k] = __builtin_fmaf(p1, __builtin_fmaf(half_of(d, 1), 8.0f, half_of(m, 1)), bias[n][k]);
+                }
+            }
+        };
+        auto add = [&](int b, const uint32_t (&ph)[NT][4], const uint32_t (&pl)[NT][4]) {
+            const uint4 & w = v.w[b >> 1];
+            const uint32_t w0 = b & 1 ? w.z : w.x, w1 = b & 1 ? w.w : w.y;
+            const h8 clo = four(codes_lo(w0, magic, 8.0f), codes_lo(w0 >> 8, magic, 8.0f), codes_lo(w1, magic, 8.0f), codes_lo(w1 >> 8, magic, 8.0f));
+            const h8 chi = four(codes_hi(w0, magic, 8.0f), codes_hi(w0 >> 8, magic, 8.0f), codes_hi(w1, magic, 8.0f), codes_hi(w1 >> 8, magic, 8.0f));
 #pragma unroll
-            for (int bb = 0; bb < 2; ++bb) {
-                const int b = 2 * j + bb;
-                if constexpr (D >= kFence) __builtin_amdgcn_sched_barrier(0);
-                const uint32_t w0 = bb ? v.w[j].z : v.w[j].x, w1 = bb ? v.w[j].w : v.w[j].y;
-                const h8 clo = four(codes_lo(w0, magic, 8.0f), codes_lo(w0 >> 8, magic, 8.0f), codes_lo(w1, magic, 8.0f), codes_lo(w1 >> 8, magic, 8.0f));
-                const h8 chi = four(codes_hi(w0, magic, 8.0f), codes_hi(w0 >> 8, magic, 8.0f), codes_hi(w1, magic, 8.0f), codes_hi(w1 >> 8, magic, 8.0f));
+            for (int n = 0; n < NT; ++n) {
+                o[n][2 * b] = mfma(clo, of_words(ph[n]), o[n][2 * b]);
+                o[n][2 * b + 1] = mfma(chi, of_words(ph[n]), o[n][2 * b + 1]);
+                o[n][2 * b] = mfma(clo, of_words(pl[n]), o[n][2 * b]);
+                o[n][2 * b + 1] = mfma(chi, of_words(pl[n]), o[n][2 * b + 1]);
+            }
+        };
+        uint32_t ph[NT][4], pl[NT][4];
+        if constexpr (C > 1) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint32_t ph[4], pl[4];
+            for (int y = 0; y < NK; ++y) {
+                const uint32_t dd[4] = { v.dk(y, 0), v.dk(y, 1), v.dk(y, 2), v.dk(y, 3) };
+                uint32_t mm[4] = {};
+                if constexpr (TYPE == kKvQ4_1)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float p0 = s[n][x >> 1][2 * (x & 1)], p1 = s[n][x >> 1][2 * (x & 1) + 1];
-                        const uint32_t d = MASKED ? dw[bb][x] & in[n][x] : dw[bb][x];
-                        const h2 hi = __builtin_bit_cast(h2, p16[n][x]) * __builtin_bit_cast(h2, d);
-                        ph[x] = __builtin_bit_cast(uint32_t, hi);
-                        pl[x] = pair_of(__builtin_fmaf(p0, half_of(d, 0), -half_of(ph[x], 0)), __builtin_fmaf(p1, half_of(d, 1), -half_of(ph[x], 1)));
-                        if constexpr (TYPE == kKvQ4_1) {
-                            const uint32_t m = MASKED ? mw[bb][x] & in[n][x] : mw[bb][x];
-                            bias[n][b] = __builtin_fmaf(p0, __builtin_fmaf(half_of(d, 0), 8.0f, half_of(m, 0)), bias[n][b]);
-                            bias[n][b] = __builtin_fmaf(p1, __builtin_fmaf(half_of(d, 1), 8.0f, half_of(m, 1)), bias[n][b]);
-                        }
-                    }
-                    o[n][2 * b] = mfma(clo, of_words(ph), o[n][2 * b]);
-                    o[n][2 * b + 1] = mfma(chi, of_words(ph), o[n][2 * b + 1]);
-                    o[n][2 * b] = mfma(clo, of_words(pl), o[n][2 * b]);
-                    o[n][2 * b + 1] = mfma(chi, of_words(pl), o[n][2 * b + 1]);
+                    for (int x = 0; x < 4; ++x) mm[x] = v.mk(y, x);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) pieces(n, y, dd, mm, ph[n], pl[n]);
+#pragma unroll
+                for (int c = 0; c < C; ++c) add(C * y + c, ph, pl);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+                uint32_t dw[2][4], mw[2][4] = {};
+                all_cells(v.d[j], dw);
+                if constexpr (TYPE == kKvQ4_1) all_cells(v.m[j], mw);
+#pragma unroll
+                for (int bb = 0; bb < 2; ++bb) {
+                    if constexpr (D >= kFence) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) pieces(n, 2 * j + bb, dw[bb], mw[bb], ph[n], pl[n]);
+                    add(2 * j + bb, ph, pl);
                 }
             }
         }
     }
 
-    // The next tile at or after i (in steps) that all rows of the wave see whole (WHOLE; none under a mask), or that a row
-    // sees and not all see whole; t1 when there is none.
-    template <bool WHOLE>
-    __device__ __forceinline__ uint32_t next(const Attn4Args & a, uint32_t i, uint32_t t1, uint32_t step) const {
-        for (; i < t1; i += step) {
-            const uint32_t c0 = 32u * i, c1 = c0 + 32u;
-            bool any = false, all = a.mask == nullptr;
+    // Whether a row of the wave sees a cell of tile i.
+    __device__ __forceinline__ bool any(uint32_t i) const {
+        const uint32_t c0 = 32u * i, c1 = c0 + 32u;
+        bool x = false;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                all = all && ((row[n].lo0 <= c0 && row[n].hi0 >= c1) || (row[n].lo1 <= c0 && row[n].hi1 >= c1));
-                any |= (row[n].lo0 < row[n].hi0 && row[n].lo0 < c1 && row[n].hi0 > c0) ||
-                       (row[n].lo1 < row[n].hi1 && row[n].lo1 < c1 && row[n].hi1 > c0);
-            }
-            const bool whole = __ballot(!all) == 0ull;
-            if (WHOLE ? whole : (!whole && __ballot(any) != 0ull)) break;
-        }
-        return min(i, t1);
+        for (int n = 0; n < NT; ++n)
+            x |= (row[n].lo0 < row[n].hi0 && row[n].lo0 < c1 && row[n].hi0 > c0) ||
+                 (row[n].lo1 < row[n].hi1 && row[n].lo1 < c1 && row[n].hi1 > c0);
+        return __ballot(x) != 0ull;
     }
-    // The tiles that the rows can see: [lo, hi)
-    __device__ __forceinline__ void hull(uint32_t & t0, uint32_t & t1) const {
-        uint32_t lo = 0xFFFFFFFFu, hi = 0u;
+    struct Span {                                                  // tiles [lo, hi)
+        uint32_t lo, hi;
+        __device__ __forceinline__ uint32_t size() const { return hi - lo; }
+    };
+    // The tiles that every row sees whole by its first (second) run; the tiles that hold all cells that any row sees.
+    __device__ __forceinline__ void spans(const Attn4Args & a, Span & w0, Span & w1, Span & all) const {
+        uint32_t l0 = 0u, h0 = 0xFFFFFFFFu, l1 = 0u, h1 = 0xFFFFFFFFu, lo = 0xFFFFFFFFu, hi = 0u;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            if (row[n].lo0 < row[n].hi0) { lo = min(lo, row[n].lo0); hi = max(hi, row[n].hi0); }
-            if (row[n].lo1 < row[n].hi1) { lo = min(lo, row[n].lo1); hi = max(hi, row[n].hi1); }
+            const Row & r = row[n];
+            l0 = max(l0, r.lo0); h0 = min(h0, r.hi0);
+            l1 = max(l1, r.lo1); h1 = min(h1, r.hi1);
+            if (r.lo0 < r.hi0) { lo = min(lo, r.lo0); hi = max(hi, r.hi0); }
+            if (r.lo1 < r.hi1) { lo = min(lo, r.lo1); hi = max(hi, r.hi1); }
         }
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
-            hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
+        if (a.T != 1u) {
+            l0 = rows16_max(l0); h0 = rows16_min(h0);
+            l1 = rows16_max(l1); h1 = rows16_min(h1);
+            lo = rows16_min(lo); hi = rows16_max(hi);
+        } else {                                                   // (the lanes agree)
+            l0 = __builtin_amdgcn_readfirstlane(l0); h0 = __builtin_amdgcn_readfirstlane(h0);
+            l1 = __builtin_amdgcn_readfirstlane(l1); h1 = __builtin_amdgcn_readfirstlane(h1);
+            lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi);
         }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = __builtin_amdgcn_readfirstlane(hi);
-        t0 = min(lo, hi) / 32u;
-        t1 = (hi + 31u) / 32u;                                     // (cells stay below 2^31)
+        all = Span{ min(lo, hi) / 32u, (hi + 31u) / 32u };         // (cells stay below 2^31)
+        w0 = Span{ (min(l0, 0x7FFFFFFFu) + 31u) / 32u, h0 / 32u };
+        w1 = Span{ (min(l1, 0x7FFFFFFFu) + 31u) / 32u, h1 / 32u };
+        if (w0.lo >= w0.hi || a.mask != nullptr) w0 = Span{ all.lo, all.lo };
+        if (w1.lo >= w1.hi || a.mask != nullptr) w1 = Span{ all.hi, all.hi };
+        if (w1.lo < w0.lo) { const Span x = w0; w0 = w1; w1 = x; }
+        w1.lo = max(w1.lo, w0.hi);                                 // (runs that overlap: each tile once)
+        w1.hi = max(w1.hi, w1.lo);
     }
 
-    // The tiles t0, t0 + parts, .. below t1 that are (not) whole, the next two loaded ahead.
+    // The scores and the values of one tile, its registers loaded again from tile `ahead` behind their last use.
     template <bool WHOLE>
-    __device__ __forceinline__ void tiles(const Attn4Args & a, const uint8_t * kp, const uint8_t * vp, size_t pair, uint32_t t0,
-                                          uint32_t t1, uint32_t parts, float kexp, const h8 * lds, uint32_t lane) {
-        constexpr size_t tb = kv4_tile_bytes(TYPE);
-        uint32_t i0 = next<WHOLE>(a, t0, t1, parts);
-        if (i0 >= t1) return;
-        uint32_t i1 = next<WHOLE>(a, i0 + parts, t1, parts);
-        Tl k0, v0, k1, v1;
-        load<false>(k0, kp + i0 * tb, pair, lane);
-        load<true>(v0, vp + i0 * tb, pair, lane);
-        if constexpr (AHEAD == 2) {
-            const size_t c1 = (i1 < t1 ? i1 : i0) * tb;            // (past the last tile: the one before again)
-            load<false>(k1, kp + c1, pair, lane);
-            load<true>(v1, vp + c1, pair, lane);
-        }
-        auto one = [&](Tl & k, Tl & v, uint32_t i, uint32_t ahead) {
-            uint32_t ql = lane;                                    // the pieces of q are read from LDS for every tile: kept in
-            asm volatile("" : "+v"(ql));                           // registers they would spill
-            f4 s[NT][2];
-            uint32_t vis[NT];
-            const size_t c = (ahead < t1 ? ahead : i) * tb;
-            scores(k, lds + ql, s);
-            load<false>(k, kp + c, pair, lane);
-            weights<!WHOLE>(a, s, vis, 32u * i, lane, kexp);
-            values<!WHOLE>(v, s, vis);
-            load<true>(v, vp + c, pair, lane);
-        };
-        if constexpr (AHEAD == 1) {
-            for (;;) {
-                one(k0, v0, i0, i1);
-                if (i1 >= t1) return;
-                i0 = i1;
-                i1 = next<WHOLE>(a, i0 + parts, t1, parts);
-            }
-        }
-        for (;;) {
-            const uint32_t i2 = next<WHOLE>(a, i1 + parts, t1, parts);
-            one(k0, v0, i0, i2);
-            if (i1 >= t1) break;
-            const uint32_t i3 = next<WHOLE>(a, i2 + parts, t1, parts);
-            one(k1, v1, i1, i3);
-            if (i2 >= t1) break;
-            i0 = i2;
-            i1 = i3;
-        }
+    __device__ __forceinline__ void one(const Attn4Args & a, Tl & k, Tl & v, uint32_t i, uint32_t ahead, const uint8_t * kp,
+                                        const uint8_t * vp, size_t pair, float kexp, const h8 * lds, uint32_t lane) {
+        uint32_t ql = lane;                                        // q's pieces: read from LDS for every tile where registers
+        if constexpr (D * NT > 128) asm volatile("" : "+v"(ql));   // would spill, kept where they do not
+        f4 s[NT][2];
+        uint32_t vis[NT];
+        const size_t c = (size_t)ahead * kv4_tile_bytes(TYPE);
+        scores(k, lds + ql, s);
+        load<false>(k, kp + c, pair, lane);
+        weights<!WHOLE>(a, s, vis, 32u * i, lane, kexp);
+        values<!WHOLE>(v, s, vis);
+        load<true>(v, vp + c, pair, lane);
     }
-    __device__ __forceinline__ void run(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, const h8 * lds, uint32_t lane) {
-        const size_t pair = (size_t)a.n_tiles * kv4_tile_bytes(TYPE);
+    // The tiles that the rows see, every parts-th: those that all rows see whole with the next AHEAD tiles loaded ahead,
+    // then the others. `lds`: room for the queries' pieces.
+    __device__ __forceinline__ void run(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, h8 * lds, uint32_t wave,
+                                        uint32_t lane) {
+        constexpr size_t tb = kv4_tile_bytes(TYPE);
+        const size_t pair = (size_t)a.n_tiles * tb;
         const uint8_t * kp = a.k + kKv4Header + (size_t)h * (D / 64) * pair, * vp = a.v + kKv4Header + (size_t)h * (D / 64) * pair;
         // 2^k: the largest |d| of the V plane times 2^k in [2^8, 2^9) (an infinite one counts as the largest finite), k <= 9
         const uint32_t dm = *(const uint32_t *)a.v;
         const float top = (float)__builtin_bit_cast(_Float16, (uint16_t)min(dm, 0x7BFFu));
         const float kexp = top == 0.0f ? 0.0f : (float)min(8 - ((int)(fb(top) >> 23) - 127), 9);
-        uint32_t t0, t1;
-        hull(t0, t1);
-        tiles<true>(a, kp, vp, pair, t0 + part, t1, parts, kexp, lds, lane);
-        tiles<false>(a, kp, vp, pair, t0 + part, t1, parts, kexp, lds, lane);
+        Span w0, w1, all;
+        spans(a, w0, w1, all);
+        const uint32_t n0 = w0.size(), nw = n0 + w1.size();
+        auto whole = [&](uint32_t j) { return j < n0 ? w0.lo + j : w1.lo + (j - n0); };
+        // two tiles ahead: tiles 0, 1 of an even count go to the registers 0, 1; of an odd count tile 0 goes to 1 and is done
+        // first, so that the loop is whole pairs and its waits count the loads behind the ones they wait for
+        Tl k0, v0, k1, v1;
+        const uint32_t cnt = part < nw ? (nw - 1u - part) / parts + 1u : 0u, odd = AHEAD == 2 ? cnt & 1u : 0u;
+        auto nth = [&](uint32_t x) { return whole(part + min(x, cnt - 1u) * parts); };   // (past the last: it again)
+        if (cnt != 0u) {
+            load<false>(k0, kp + nth(odd) * tb, pair, lane);
+            load<true>(v0, vp + nth(odd) * tb, pair, lane);
+            if constexpr (AHEAD == 2) {
+                load<false>(k1, kp + nth(1u - odd) * tb, pair, lane);
+                load<true>(v1, vp + nth(1u - odd) * tb, pair, lane);
+            }
+        }
+        load_queries(a.scale, lane, lds, wave);
+        __syncthreads();
+        if (odd) one<true>(a, k1, v1, nth(0u), nth(2u), kp, vp, pair, kexp, lds, lane);
+        for (uint32_t x = odd; x < cnt; x += AHEAD) {
+            one<true>(a, k0, v0, nth(x), nth(x + AHEAD), kp, vp, pair, kexp, lds, lane);
+            if constexpr (AHEAD == 2) one<true>(a, k1, v1, nth(x + 1u), nth(x + 3u), kp, vp, pair, kexp, lds, lane);
+        }
+        // the others: the hull without w0 and w1, dealt on from the wave after the one that took the last whole tile
+        const uint32_t g0 = w0.lo - all.lo, g1 = g0 + (w1.lo - w0.hi), np = all.size() - nw;
+        uint32_t x = part + parts - nw % parts;
+        x = x >= parts ? x - parts : x;
+        auto other = [&](uint32_t y) { return y < g0 ? all.lo + y : y < g1 ? w0.hi + (y - g0) : w1.hi + (y - g1); };
+        while (x < np && !any(other(x))) x += parts;
+        if (x >= np) return;
+        load<false>(k0, kp + other(x) * tb, pair, lane);
+        load<true>(v0, vp + other(x) * tb, pair, lane);
+        for (;;) {
+            uint32_t nx = x + parts;
+            while (nx < np && !any(other(nx))) nx += parts;
+            one<false>(a, k0, v0, other(x), other(nx < np ? nx : x), kp, vp, pair, kexp, lds, lane);
+            if (nx >= np) break;
+            x = nx;
+        }
     }
 
     // Rows summed over their lanes; o becomes sum p v (2^k times), value 32 b + 16 c + 4 g + i in o[2 b + c][i].
@@ -447,143 +582,145 @@ struct Attn4 {
             l[n] = rows_sum(l[n]);
             if constexpr (TYPE == kKvQ4_1)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const float z = rows_sum(bias[n][b]);
-                    o[n][2 * b] += z;
-                    o[n][2 * b + 1] += z;
+                for (int k = 0; k < NK; ++k) {
+                    const float z = rows_sum(bias[n][k]);          // (used where column and block belong together)
+#pragma unroll
+                    for (int j = 2 * C * k; j < 2 * C * (k + 1); ++j) o[n][j] += z;
                 }
         }
     }
 };
 
 // Workgroup (KV head, split, group of rows), KV heads fastest: with eight of them every XCD's L2 holds one head.
-template <int D, int NT, uint32_t TYPE, bool SPLIT>
-__global__ __launch_bounds__(256, D == 64 ? 4 : D <= 256 ? 2 : 1) void k_attn4(Attn4Args a) {
-    using A = Attn4<D, NT, TYPE, SPLIT>;
-    constexpr uint32_t kRows = 16u * NT * (SPLIT ? 1u : kWaves);
-    const uint32_t h = blockIdx.x % a.n_head_kv, rest = blockIdx.x / a.n_head_kv, split = rest % a.S;
-    const uint32_t n_rg = gridDim.x / a.n_head_kv / a.S, rg = n_rg - 1u - rest / a.S;   // causal: the long rows first
-    const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u, g = lane >> 4;
-    const uint32_t r0 = rg * kRows + (SPLIT ? 0u : 16u * NT * wave), R = a.T * a.G;
+template <int D, int NT, int C, uint32_t TYPE, bool SPLIT>
+__global__ __launch_bounds__(256, D == 64 ? 4 : D == 128 && C == 4 ? 3 : D <= 256 ? 2 : 1) void k_attn4(Attn4Args a) {
+    using A = Attn4<D, NT, C, TYPE, SPLIT>;
+    constexpr uint32_t RT = A::RW * NT, kRows = RT * (SPLIT ? 1u : kWaves);    // rows of a wave, of the workgroup
+    const uint32_t h = blockIdx.x, split = blockIdx.y, rg = gridDim.z - 1u - blockIdx.z;   // causal: the long rows first
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u, g = lane >> 4;
+    const uint32_t c = lane & (C - 1u), rl = (lane & 15u) / C;
+    const uint32_t r0 = rg * kRows + (SPLIT ? 0u : RT * wave), R = a.T * a.G, nh = a.G * a.n_head_kv;
+    const size_t nr = (size_t)a.T * nh;
     __shared__ h8 lq[(SPLIT ? 1 : kWaves) * NT * A::NB * 2 * 64];
     A w;
-    w.load_rows(a, h, r0, lane, lq + (SPLIT ? 0u : wave) * NT * A::NB * 2 * 64, !SPLIT || wave == 0u);
-    __syncthreads();
-    if constexpr (SPLIT) w.run(a, h, split * kWaves + wave, a.S * kWaves, lq, lane);
-    else w.run(a, h, split, a.S, lq + wave * NT * A::NB * 2 * 64, lane);
+    w.load_runs(a, h, r0, lane);
+    if constexpr (SPLIT) w.run(a, h, split * kWaves + wave, a.S * kWaves, lq, wave, lane);
+    else w.run(a, h, split, a.S, lq + wave * NT * A::NB * 2 * 64, wave, lane);
     w.finish();
+    // where row r's result goes: the output, or its place in the split's partial rows
+    auto place = [&](uint32_t r) {
+        const uint32_t t = token(a, r), hq = h * a.G + r - t * a.G;
+        return a.S > 1u ? a.part + 2u * a.S * nr + (split * nr + (size_t)t * nh + hq) * D
+                        : a.out + (size_t)t * a.out_stride + (size_t)hq * D;
+    };
+    auto sums = [&](uint32_t r, float m, float l) {
+        const uint32_t t = token(a, r);
+        *(float2 *)(a.part + 2u * (split * nr + (size_t)t * nh + h * a.G + r - t * a.G)) = make_float2(m, l);
+    };
     if constexpr (SPLIT) {                                         // the waves' sums joined
-        constexpr uint32_t DC = D < 128 ? D : 128;                  // values joined at a time
-        __shared__ float lm[kWaves * 16 * NT], ll[kWaves * 16 * NT];
-        __shared__ __align__(16) float lo[kWaves * 16 * NT * DC];
+        constexpr uint32_t DC = D < 128 ? D : 128;                 // values joined at a time
+        __shared__ float2 ml[kWaves * RT];
+        __shared__ __align__(16) float lo[kWaves * RT * DC];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (g == 0u) {
-                lm[wave * 16 * NT + 16 * n + lane] = w.m[n];
-                ll[wave * 16 * NT + 16 * n + lane] = w.l[n];
-            }
-        __syncthreads();
-        float f[NT];
+        for (uint32_t z = 0; z < D / DC; ++z) {
+            if (z != 0u) __syncthreads();
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const uint32_t r = 16u * n + (lane & 15u);
-            float M = lm[r];
-#pragma unroll
-            for (uint32_t x = 1; x < kWaves; ++x) M = fmaxf(M, lm[x * 16 * NT + r]);
-            f[n] = M == w.m[n] ? 1.0f : __builtin_amdgcn_exp2f(w.m[n] - M);
-        }
-#pragma unroll
-        for (uint32_t c = 0; c < D / DC; ++c) {
-            if (c != 0u) __syncthreads();
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                if (z == 0u && g == 0u && c == 0u) ml[wave * RT + A::RW * n + rl] = make_float2(w.m[n], w.l[n]);
 #pragma unroll
                 for (uint32_t j = 0; j < DC / 16; ++j) {
-                    const f4 x = w.o[n][c * (DC / 16) + j] * f[n];
-                    *(float4 *)(lo + (wave * 16 * NT + 16 * n + (lane & 15u)) * DC + 16 * j + 4 * g) =
-                        make_float4(x[0], x[1], x[2], x[3]);
+                    const f4 x = w.o[n][z * (DC / 16) + j];
+                    if (C == 1 || ((z * (DC / 16) + j) / 2u) % C == c)
+                        *(float4 *)(lo + (wave * RT + A::RW * n + rl) * DC + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
                 }
+            }
             __syncthreads();
-            for (uint32_t e = threadIdx.x; e < 16u * NT * (DC / 4); e += 256u) {
+            for (uint32_t e = threadIdx.x; e < RT * (DC / 4); e += 64u * kWaves) {
                 const uint32_t r = e / (DC / 4), d = 4u * (e % (DC / 4));
                 if (r0 + r >= R) continue;
-                float M = lm[r], L = 0.0f;
+                float2 u[kWaves];
+                float M = -__builtin_inff(), L = 0.0f;
 #pragma unroll
-                for (uint32_t x = 1; x < kWaves; ++x) M = fmaxf(M, lm[x * 16 * NT + r]);
+                for (uint32_t x = 0; x < kWaves; ++x) { u[x] = ml[x * RT + r]; M = fmaxf(M, u[x].x); }
                 float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (uint32_t x = 0; x < kWaves; ++x) {
-                    const float mx = lm[x * 16 * NT + r];
-                    L += ll[x * 16 * NT + r] * (mx == M ? 1.0f : __builtin_amdgcn_exp2f(mx - M));
-                    const float4 z = *(const float4 *)(lo + (x * 16 * NT + r) * DC + d);
-                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+                    const float f = u[x].x == M ? 1.0f : __builtin_amdgcn_exp2f(u[x].x - M);
+                    const float4 v = *(const float4 *)(lo + (x * RT + r) * DC + d);
+                    L += u[x].y * f;
+                    y.x += v.x * f; y.y += v.y * f; y.z += v.z * f; y.w += v.w * f;
                 }
-                const uint32_t t = (r0 + r) / a.G, hq = h * a.G + (r0 + r) % a.G, nh = a.G * a.n_head_kv;
-                const size_t nr = (size_t)a.T * nh, ro = (size_t)t * nh + hq;
-                if (a.S == 1u) {
-                    const float il = L == 0.0f ? 0.0f : 1.0f / L;
-                    *(float4 *)(a.out + (size_t)t * a.out_stride + (size_t)hq * D + c * DC + d) =
-                        make_float4(y.x * il, y.y * il, y.z * il, y.w * il);
-                } else {
-                    *(float4 *)(a.part + 2u * a.S * nr + (split * nr + ro) * D + c * DC + d) = y;
-                    if (c == 0u && d == 0u) *(float2 *)(a.part + 2u * (split * nr + ro)) = make_float2(M, L);
-                }
+                const float il = a.S > 1u ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+                *(float4 *)(place(r0 + r) + z * DC + d) = make_float4(y.x * il, y.y * il, y.z * il, y.w * il);
+                if (a.S > 1u && z == 0u && d == 0u) sums(r0 + r, M, L);
             }
         }
     } else {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const uint32_t r = r0 + 16u * n + (lane & 15u);
+            const uint32_t r = r0 + A::RW * n + rl;
             if (r >= R) continue;
-            const uint32_t t = r / a.G, hq = h * a.G + r % a.G, nh = a.G * a.n_head_kv;
-            const size_t nr = (size_t)a.T * nh, ro = (size_t)t * nh + hq;
             const float f = a.S > 1u ? 1.0f : w.l[n] == 0.0f ? 0.0f : 1.0f / w.l[n];
-            float * y = a.S > 1u ? a.part + 2u * a.S * nr + (split * nr + ro) * D
-                                 : a.out + (size_t)t * a.out_stride + (size_t)hq * D;
+            float * y = place(r);
 #pragma unroll
             for (int j = 0; j < 2 * A::NB; ++j) {
                 const f4 x = w.o[n][j] * f;
-                *(float4 *)(y + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
+                if (C == 1 || (uint32_t)(j / 2) % C == c) *(float4 *)(y + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
             }
-            if (a.S > 1u && g == 0u) *(float2 *)(a.part + 2u * (split * nr + ro)) = make_float2(w.m[n], w.l[n]);
+            if (a.S > 1u && g == 0u && c == 0u) sums(r, w.m[n], w.l[n]);
         }
     }
 }
 
-// The splits of a row joined: a workgroup a row, 256 / (D / 4) threads of the same four values take splits in turn, then
-// meet in LDS; the order of the additions is fixed.
+// The splits of a row joined: a workgroup a row. 256 / (D / 4) groups of threads take splits in turn, then meet in LDS; the
+// order of the additions is fixed.
 template <int D>
 __global__ __launch_bounds__(256) void k_attn4_join(Attn4Args a) {
-    constexpr uint32_t W = D / 4, NG = 256u / W;
+    constexpr uint32_t W = D / 4, NG = 256u / W, N = 8;            // N: loads in flight
     __shared__ float4 acc[256];
-    __shared__ float wt[64];
-    const uint32_t ro = blockIdx.x, nh = a.G * a.n_head_kv, c = threadIdx.x % W, s0 = threadIdx.x / W;
+    __shared__ float wt[kSplitsMax], red[8];
+    const uint32_t ro = blockIdx.x, nh = a.G * a.n_head_kv, tid = threadIdx.x, c = tid % W, s0 = tid / W;
     const size_t nr = (size_t)a.T * nh;
     const float4 * po = (const float4 *)(a.part + 2u * a.S * nr + (size_t)ro * D) + c;
-    if (threadIdx.x < 64u) {                                       // S <= 64: a lane a split
-        float2 e = make_float2(-__builtin_inff(), 0.0f);
-        if (threadIdx.x < a.S) e = ((const float2 *)a.part)[threadIdx.x * nr + ro];
-        float M = e.x;
+    float4 x[N];
+    auto fetch = [&](uint32_t i0) {
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
-        const float f = e.x == M ? 1.0f : __builtin_amdgcn_exp2f(e.x - M);
-        float L = e.y * f;
+        for (uint32_t i = 0; i < N; ++i) {
+            const uint32_t sp = s0 + NG * (i0 + i);
+            x[i] = sp < a.S ? po[(size_t)sp * nr * W] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+    fetch(0u);
+    static_assert(kSplitsMax == 256u, "a thread a split");
+    float2 e = make_float2(-__builtin_inff(), 0.0f);
+    if (tid < a.S) e = ((const float2 *)a.part)[tid * nr + ro];
+    float M = e.x;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) L += __shfl_xor(L, d);
-        wt[threadIdx.x] = L == 0.0f ? 0.0f : f / L;
-    }
-    float4 x[64 / NG];
-#pragma unroll
-    for (uint32_t i = 0; i < 64u / NG; ++i)                        // all loads in flight at once
-        x[i] = s0 + NG * i < a.S ? po[(size_t)(s0 + NG * i) * nr * W] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+    if ((tid & 63u) == 0u) red[tid / 64u] = M;
     __syncthreads();
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float f = e.x == M ? 1.0f : __builtin_amdgcn_exp2f(e.x - M);
+    float L = e.y * f;
 #pragma unroll
-    for (uint32_t i = 0; i < 64u / NG; ++i) {
-        const float f = wt[s0 + NG * i];
-        if (s0 + NG * i < a.S) { y.x += x[i].x * f; y.y += x[i].y * f; y.z += x[i].z * f; y.w += x[i].w * f; }
+    for (int d = 1; d < 64; d <<= 1) L += __shfl_xor(L, d);
+    if ((tid & 63u) == 0u) red[4u + tid / 64u] = L;
+    wt[tid] = f;
+    __syncthreads();
+    L = (red[4] + red[5]) + (red[6] + red[7]);
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t i0 = 0;;) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            const uint32_t sp = s0 + NG * (i0 + i);
+            const float w = sp < a.S ? wt[sp] : 0.0f;
+            y.x += x[i].x * w; y.y += x[i].y * w; y.z += x[i].z * w; y.w += x[i].w * w;
+        }
+        i0 += N;
+        if (i0 * NG >= a.S) break;
+        fetch(i0);
     }
-    acc[threadIdx.x] = y;
+    acc[tid] = y;
     __syncthreads();
     if (s0 == 0u) {
 #pragma unroll
@@ -591,32 +728,44 @@ __global__ __launch_bounds__(256) void k_attn4_join(Attn4Args a) {
             const float4 z = acc[i * W + c];
             y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
         }
-        *((float4 *)(a.out + (size_t)(ro / nh) * a.out_stride + (size_t)(ro % nh) * D) + c) = y;
+        const float il = L == 0.0f ? 0.0f : 1.0f / L;
+        *((float4 *)(a.out + (size_t)(ro / nh) * a.out_stride + (size_t)(ro % nh) * D) + c) =
+            make_float4(y.x * il, y.y * il, y.z * il, y.w * il);
     }
 }
 
-template <int D, int NT, uint32_t TYPE, bool SPLIT>
+template <int D, int NT, int C, uint32_t TYPE, bool SPLIT>
 static int launch(const Attn4Args & a, hipStream_t s) {
-    const uint32_t rows = 16u * NT * (SPLIT ? 1u : kWaves), n_rg = (a.T * a.G + rows - 1u) / rows;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4<D, NT, TYPE, SPLIT>), dim3(n_rg * a.S * a.n_head_kv), dim3(256), 0, s, a);
+    const uint32_t rows = 16u / C * NT * (SPLIT ? 1u : kWaves), n_rg = (a.T * a.G + rows - 1u) / rows;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4<D, NT, C, TYPE, SPLIT>), dim3(a.n_head_kv, a.S, n_rg), dim3(64u * kWaves), 0, s, a);
     if (a.S > 1u) hipLaunchKernelGGL(k_attn4_join<D>, dim3(a.T * a.G * a.n_head_kv), dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
-template <int D>
-static int launch_d(const Attn4Args & a, bool split, hipStream_t s) {
-    if (a.type == kKvQ4_0) return split ? launch<D, 1, kKvQ4_0, true>(a, s) : launch<D, 1, kKvQ4_0, false>(a, s);
-    return split ? launch<D, 1, kKvQ4_1, true>(a, s) : launch<D, 1, kKvQ4_1, false>(a, s);
+template <int D, uint32_t TYPE>
+static int launch_d(const Attn4Args & a, const Attn4Plan & p, hipStream_t s) {
+    if (!p.split_waves) return launch<D, 1, 1, TYPE, false>(a, s);
+    switch (p.C) {
+        case 2: return launch<D, 1, 2, TYPE, true>(a, s);
+        case 4:
+            if constexpr (D >= 128) return launch<D, 1, 4, TYPE, true>(a, s);
+        default: return launch<D, 1, 1, TYPE, true>(a, s);
+    }
+}
+
+template <uint32_t TYPE>
+static int launch_t(const Attn4Args & a, const Attn4Plan & p, hipStream_t s) {
+    switch (a.D) {
+        case 64: return launch_d<64, TYPE>(a, p, s);
+        case 128: return launch_d<128, TYPE>(a, p, s);
+        case 256: return launch_d<256, TYPE>(a, p, s);
+        case 512: return launch_d<512, TYPE>(a, p, s);
+        default: return -2;
+    }
 }
 
 }  // namespace tsr
 
-int tsr_launch_attn4(const tsr::Attn4Args & a, bool split_waves, hipStream_t s) {
-    switch (a.D) {
-        case 64: return tsr::launch_d<64>(a, split_waves, s);
-        case 128: return tsr::launch_d<128>(a, split_waves, s);
-        case 256: return tsr::launch_d<256>(a, split_waves, s);
-        case 512: return tsr::launch_d<512>(a, split_waves, s);
-        default: return -2;
-    }
+int tsr_launch_attn4(const tsr::Attn4Args & a, const tsr::Attn4Plan & p, hipStream_t s) {
+    return a.type == tsr::kKvQ4_0 ? tsr::launch_t<tsr::kKvQ4_0>(a, p, s) : tsr::launch_t<tsr::kKvQ4_1>(a, p, s);
 }

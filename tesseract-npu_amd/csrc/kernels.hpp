@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "attn4_plan.hpp"
 #include "fa_item.hpp"
 
 namespace tsr {
@@ -111,6 +112,7 @@ struct Attn4Args {
     uint64_t out_stride;
     float * part;            // S > 1: [split][T n_head] (maximum, sum), then [split][T n_head][D] unnormalised rows
     uint32_t type, D, T, G, n_head_kv, n_kv, n_tiles;
+    uint32_t inv_G;          // floor(2^32 / G) + 1 (G 1: 0)
     uint32_t S;              // splits of the cells
     float scale;
 };
@@ -262,8 +264,8 @@ int tsr_launch_kv4_get_rows(const tsr::Kv4Args & a, uint32_t which, const int64_
                             uint64_t dst_stride, int32_t * bad, hipStream_t s);
 int tsr_launch_kv_get_rows(const tsr::KvArgs & a, uint32_t which, const int64_t * idx, uint32_t n_rows, float * dst,
                            uint64_t dst_stride, int32_t * bad, hipStream_t s);
-// attention over a 4-bit cache, its waves' rows and splits by attn4_plan.hpp (k_attn4.hip)
-int tsr_launch_attn4(const tsr::Attn4Args & a, bool split_waves, hipStream_t s);
+// attention over a 4-bit cache, cut as attn4_plan.hpp says (k_attn4.hip)
+int tsr_launch_attn4(const tsr::Attn4Args & a, const tsr::Attn4Plan & p, hipStream_t s);
 int tsr_launch_fa(const tsr::FaArgs & a, const tsr::FaPlan & p, uint32_t T, uint32_t n_cu, hipStream_t s);
 int tsr_launch_fa_dec(const tsr::FaDecArgs & a, hipStream_t s);
 int tsr_launch_xcd_probe(uint32_t * out64, hipStream_t s);

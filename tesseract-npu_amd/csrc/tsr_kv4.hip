@@ -53,6 +53,7 @@ int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, u
     a.D = D;
     a.T = T;
     a.G = n_head / n_head_kv;
+    a.inv_G = a.G == 1u ? 0u : (uint32_t)((1ull << 32) / a.G) + 1u;
     a.n_head_kv = n_head_kv;
     a.n_kv = n_kv;
     a.n_tiles = tsr::kv4_tiles(kc->kv_size);
@@ -72,5 +73,5 @@ int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, u
     }
     ctx->ctr.flash_attn_calls++;
     ctx->ctr.flash_attn_kv_bytes += (uint64_t)n_kv * (E / 32u) * tsr::kv4_block_bytes(kc->type) * 2u;
-    return tsr_launch_attn4(a, p.split_waves, s) ? TSR_HIP_E_HIP : TSR_HIP_OK;
+    return tsr_launch_attn4(a, p, s) ? TSR_HIP_E_HIP : TSR_HIP_OK;
 }
