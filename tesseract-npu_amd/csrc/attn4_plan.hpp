@@ -10,24 +10,35 @@ namespace tsr {
 constexpr uint32_t kSplitsMax = 256u;
 
 struct Attn4Plan {
-    bool split_waves;        // the four waves of a workgroup share 16 rows and take different cells; else 64 rows
-    uint32_t C;              // split_waves: columns of the matrix instruction a row (k_attn4.hip)
+    uint32_t C;              // columns of the matrix instruction a row (k_attn4.hip): 16 / C rows a group
+    uint32_t NT;             // groups of rows of a workgroup
     uint32_t S;              // splits of the cells, joined by a second launch
     size_t ws_bytes;         // partial rows of S > 1
 };
 
-// T tokens of G query heads a KV head over at most n_kv cells (tiles of 32).
+// T tokens of n_head query heads over at most n_kv cells (tiles of 32).
 inline Attn4Plan attn4_plan(uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_kv, uint32_t n_cu) {
     Attn4Plan p{};
-    const uint64_t R = (uint64_t)T * (n_head / n_head_kv), tiles = std::max<uint64_t>(1u, ((uint64_t)n_kv + 31u) / 32u);
-    p.split_waves = (R + 63u) / 64u * n_head_kv < n_cu;
-    p.C = !p.split_waves || R > 8u ? 1u : R > 4u || D == 64u ? 2u : 4u;
-    const uint64_t rows = p.split_waves ? 16u / p.C : 64u, wgs = (R + rows - 1u) / rows * n_head_kv;
-    const uint64_t share = p.split_waves ? 4u : 1u, most = (tiles + share - 1u) / share;
-    p.S = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ 2u * (uint64_t)n_cu / wgs, most, kSplitsMax }));
-#ifdef TSR_TUNE
-    if (getenv("TS")) p.S = atoi(getenv("TS"));
-#endif
+    const uint64_t G = n_head / n_head_kv, R = T * G, tiles = std::max<uint64_t>(1u, ((uint64_t)n_kv + 31u) / 32u);
+    auto wgs = [&](uint64_t rows) { return (R + rows - 1u) / rows * n_head_kv; };
+    // Several columns a row take a third less work a tile, but a group is then 4 or 8 rows and not 16. That pays for a
+    // token's own query heads, and for several tokens while every group has a compute unit (the host does not know whether
+    // tokens share their cells; 32 heads of 8, D 128, us with 4 and 16 rows a group): 8 tokens behind 4000 cells of one
+    // sequence 16.2 / 14.8, of 8 sequences with 2000 cells each 15.4 / 23.8; 32 tokens 30.5 / 20.3 and 20.8 / 31.2; 64
+    // tokens 45.5 / 29.7 and 42.0 / 51.0.
+    const uint32_t C = G <= 4u && D >= 128u ? 4u : G <= 8u ? 2u : 1u;
+    p.C = C > 1u && (R <= 16u / C || wgs(16u / C) <= n_cu) ? C : 1u;
+    // Two groups a workgroup share the unpacking of the codes, once that leaves every compute unit two workgroups (512
+    // tokens behind 1536 cells 57 -> 52 us, 2048 behind 6144 710 -> 630; 100 tokens 7.9 -> 12). D 256 has no registers
+    // for it.
+    p.NT = p.C == 1u && D <= 128u && wgs(32u) >= 2u * (uint64_t)n_cu ? 2u : 1u;
+    // Splits fill the compute units with one workgroup each (a token behind 8192 cells: 16, 32, 64 splits 12.6, 11.8, 12.2
+    // us), with two where a wave then still has eight tiles (131072 cells: 32, 64, 96 splits 43.6, 39.0, 40.6). A split is
+    // a second launch and a pass through memory, about the time of five tiles of a wave: none below 20 tiles (512 cells 8.3
+    // us in one piece, 9.3 in four), and none where half the compute units have work (300 tokens 33 -> 42).
+    const uint64_t n = wgs(16u / p.C * p.NT), fill = n_cu / n;
+    const uint64_t S = tiles <= 20u ? 1u : tiles >= 64u * fill && T <= 2u ? 2u * fill : fill;
+    p.S = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ S, (tiles + 3u) / 4u, kSplitsMax }));
     p.ws_bytes = p.S > 1u ? 4u * (size_t)p.S * T * n_head * (2u + D) : 0u;
     return p;
 }

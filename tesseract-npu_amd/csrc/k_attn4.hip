@@ -69,10 +69,6 @@ __device__ __forceinline__ float rows_sum(float x) {
     return bf(b[0]) + bf(b[1]);
 }
 
-#ifndef FENCE
-#define FENCE 256
-#endif
-constexpr int kFence = FENCE;
 constexpr uint32_t kWaves = 4;                  // of a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 6.0f;                  // weights are at most 2^6: a maximum is followed when it is passed by more
@@ -131,16 +127,16 @@ __device__ __forceinline__ float columns_sum(float x) {
     return x;
 }
 
-// SPLIT: the waves of a workgroup have the same rows and take different tiles; else each has rows of its own.
+// The waves of a workgroup have the same rows and take different tiles.
 // C: columns of the matrix instruction a query row. With few rows (a decode token's G query heads) 16 / C rows fill the
 // 16 columns: column C r + c is row r and meets the blocks C k + c alone (its q is zero for the others, and of its results
 // for the values of other blocks nothing is used), so that a lane scales the products and splits the weights of D / 32 / C
 // blocks and not of all D / 32.
-template <int D, int NT, int C, uint32_t TYPE, bool SPLIT>
+template <int D, int NT, int C, uint32_t TYPE>
 struct Attn4 {
     static constexpr int NB = D / 32, NK = NB / C;                 // blocks of a head, of a column
     static constexpr int RW = 16 / C;                              // query rows of a group of 16 columns
-    static constexpr int AHEAD = D >= 512 ? 1 : 2;                 // tiles loaded ahead
+    static constexpr int AHEAD = D == 512 ? 1 : 2;                 // tiles loaded ahead
     using Tl = Tile<D, C, TYPE>;
     struct Row {                                                   // of the lane's query row in each group of 16
         uint32_t lo0, hi0, lo1, hi1, t;
@@ -182,7 +178,7 @@ struct Attn4 {
             l[n] = 0.0f;
         }
     }
-    // The queries; their pieces go to `lds`, [row group][block][piece][lane]. With SPLIT the waves share the blocks out.
+    // The queries; their pieces go to `lds`, [row group][block][piece][lane], the blocks shared out over the waves.
     __device__ __forceinline__ void load_queries(float scale, uint32_t lane, h8 * lds, uint32_t wave) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -214,7 +210,7 @@ struct Attn4 {
                     const float z = rows_sum(sum);
                     if (mine) qs[n][b / C] = z;
                 }
-                if (!SPLIT || (b % kWaves) == wave) {
+                if (b % kWaves == wave) {
                     const float z[8] = { y[0], y[2], y[4], y[6], y[1], y[3], y[5], y[7] };
                     uint32_t hi[4], lo[4];
 #pragma unroll
@@ -313,7 +309,6 @@ struct Attn4 {
 #pragma unroll
             for (int bb = 0; bb < 2; ++bb) {
                 const int b = 2 * j + bb;
-                if constexpr (D >= kFence) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const uint32_t w = u ? (bb ? k.w[j].w : k.w[j].z) : (bb ? k.w[j].y : k.w[j].x);
@@ -454,7 +449,6 @@ struct Attn4 {
                 if constexpr (TYPE == kKvQ4_1) all_cells(v.m[j], mw);
 #pragma unroll
                 for (int bb = 0; bb < 2; ++bb) {
-                    if constexpr (D >= kFence) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) pieces(n, 2 * j + bb, dw[bb], mw[bb], ph[n], pl[n]);
                     add(2 * j + bb, ph, pl);
@@ -591,21 +585,26 @@ struct Attn4 {
     }
 };
 
+constexpr uint32_t values_at_once(uint32_t D, uint32_t most) { return D <= most ? D : values_at_once(D / 2u, most); }
+
 // Workgroup (KV head, split, group of rows), KV heads fastest: with eight of them every XCD's L2 holds one head.
-template <int D, int NT, int C, uint32_t TYPE, bool SPLIT>
-__global__ __launch_bounds__(256, D == 64 ? 4 : D == 128 && C == 4 ? 3 : D <= 256 ? 2 : 1) void k_attn4(Attn4Args a) {
-    using A = Attn4<D, NT, C, TYPE, SPLIT>;
-    constexpr uint32_t RT = A::RW * NT, kRows = RT * (SPLIT ? 1u : kWaves);    // rows of a wave, of the workgroup
+template <int D, int NT, int C, uint32_t TYPE>
+__global__ __launch_bounds__(256, D * NT == 64 ? 4 : D == 128 && C != 2 && NT == 1 ? 3 : D <= 256 ? 2 : 1) void k_attn4(Attn4Args a) {
+    using A = Attn4<D, NT, C, TYPE>;
+    constexpr uint32_t RT = A::RW * NT;                            // rows of the workgroup
     const uint32_t h = blockIdx.x, split = blockIdx.y, rg = gridDim.z - 1u - blockIdx.z;   // causal: the long rows first
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u, g = lane >> 4;
     const uint32_t c = lane & (C - 1u), rl = (lane & 15u) / C;
-    const uint32_t r0 = rg * kRows + (SPLIT ? 0u : RT * wave), R = a.T * a.G, nh = a.G * a.n_head_kv;
+    const uint32_t r0 = rg * RT, R = a.T * a.G, nh = a.G * a.n_head_kv;
     const size_t nr = (size_t)a.T * nh;
-    __shared__ h8 lq[(SPLIT ? 1 : kWaves) * NT * A::NB * 2 * 64];
+    // the queries' pieces, then the waves' sums, DC values of every row at a time
+    constexpr uint32_t kQ = NT * A::NB * 2u * 64u * 16u, kRoom = kQ < 16384u ? 16384u : kQ;
+    constexpr uint32_t DC = values_at_once(D, kRoom / (16u * RT));
+    __shared__ __align__(16) uint8_t room[kRoom];
+    h8 * lq = (h8 *)room;
     A w;
     w.load_runs(a, h, r0, lane);
-    if constexpr (SPLIT) w.run(a, h, split * kWaves + wave, a.S * kWaves, lq, wave, lane);
-    else w.run(a, h, split, a.S, lq + wave * NT * A::NB * 2 * 64, wave, lane);
+    w.run(a, h, split * kWaves + wave, a.S * kWaves, lq, wave, lane);
     w.finish();
     // where row r's result goes: the output, or its place in the split's partial rows
     auto place = [&](uint32_t r) {
@@ -617,57 +616,42 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : D == 128 && C == 4 ? 3 : D <= 25
         const uint32_t t = token(a, r);
         *(float2 *)(a.part + 2u * (split * nr + (size_t)t * nh + h * a.G + r - t * a.G)) = make_float2(m, l);
     };
-    if constexpr (SPLIT) {                                         // the waves' sums joined
-        constexpr uint32_t DC = D < 128 ? D : 128;                 // values joined at a time
-        __shared__ float2 ml[kWaves * RT];
-        __shared__ __align__(16) float lo[kWaves * RT * DC];
+    // the waves' sums joined
+    static_assert(DC % 16u == 0u && D % DC == 0u, "whole groups of 16 values");
+    __shared__ float2 ml[kWaves * RT];
+    float * lo = (float *)room;
 #pragma unroll
-        for (uint32_t z = 0; z < D / DC; ++z) {
-            if (z != 0u) __syncthreads();
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (z == 0u && g == 0u && c == 0u) ml[wave * RT + A::RW * n + rl] = make_float2(w.m[n], w.l[n]);
-#pragma unroll
-                for (uint32_t j = 0; j < DC / 16; ++j) {
-                    const f4 x = w.o[n][z * (DC / 16) + j];
-                    if (C == 1 || ((z * (DC / 16) + j) / 2u) % C == c)
-                        *(float4 *)(lo + (wave * RT + A::RW * n + rl) * DC + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
-                }
-            }
-            __syncthreads();
-            for (uint32_t e = threadIdx.x; e < RT * (DC / 4); e += 64u * kWaves) {
-                const uint32_t r = e / (DC / 4), d = 4u * (e % (DC / 4));
-                if (r0 + r >= R) continue;
-                float2 u[kWaves];
-                float M = -__builtin_inff(), L = 0.0f;
-#pragma unroll
-                for (uint32_t x = 0; x < kWaves; ++x) { u[x] = ml[x * RT + r]; M = fmaxf(M, u[x].x); }
-                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (uint32_t x = 0; x < kWaves; ++x) {
-                    const float f = u[x].x == M ? 1.0f : __builtin_amdgcn_exp2f(u[x].x - M);
-                    const float4 v = *(const float4 *)(lo + (x * RT + r) * DC + d);
-                    L += u[x].y * f;
-                    y.x += v.x * f; y.y += v.y * f; y.z += v.z * f; y.w += v.w * f;
-                }
-                const float il = a.S > 1u ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
-                *(float4 *)(place(r0 + r) + z * DC + d) = make_float4(y.x * il, y.y * il, y.z * il, y.w * il);
-                if (a.S > 1u && z == 0u && d == 0u) sums(r0 + r, M, L);
-            }
-        }
-    } else {
+    for (uint32_t z = 0; z < D / DC; ++z) {
+        __syncthreads();                                       // (the queries, the values before have been read)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const uint32_t r = r0 + A::RW * n + rl;
-            if (r >= R) continue;
-            const float f = a.S > 1u ? 1.0f : w.l[n] == 0.0f ? 0.0f : 1.0f / w.l[n];
-            float * y = place(r);
+            if (z == 0u && g == 0u && c == 0u) ml[wave * RT + A::RW * n + rl] = make_float2(w.m[n], w.l[n]);
 #pragma unroll
-            for (int j = 0; j < 2 * A::NB; ++j) {
-                const f4 x = w.o[n][j] * f;
-                if (C == 1 || (uint32_t)(j / 2) % C == c) *(float4 *)(y + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
+            for (uint32_t j = 0; j < DC / 16; ++j) {
+                const f4 x = w.o[n][z * (DC / 16) + j];
+                if (C == 1 || ((z * (DC / 16) + j) / 2u) % C == c)
+                    *(float4 *)(lo + (wave * RT + A::RW * n + rl) * DC + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
             }
-            if (a.S > 1u && g == 0u && c == 0u) sums(r, w.m[n], w.l[n]);
+        }
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < RT * (DC / 4); e += 64u * kWaves) {
+            const uint32_t r = e / (DC / 4), d = 4u * (e % (DC / 4));
+            if (r0 + r >= R) continue;
+            float2 u[kWaves];
+            float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+            for (uint32_t x = 0; x < kWaves; ++x) { u[x] = ml[x * RT + r]; M = fmaxf(M, u[x].x); }
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t x = 0; x < kWaves; ++x) {
+                const float f = u[x].x == M ? 1.0f : __builtin_amdgcn_exp2f(u[x].x - M);
+                const float4 v = *(const float4 *)(lo + (x * RT + r) * DC + d);
+                L += u[x].y * f;
+                y.x += v.x * f; y.y += v.y * f; y.z += v.z * f; y.w += v.w * f;
+            }
+            const float il = a.S > 1u ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+            *(float4 *)(place(r0 + r) + z * DC + d) = make_float4(y.x * il, y.y * il, y.z * il, y.w * il);
+            if (a.S > 1u && z == 0u && d == 0u) sums(r0 + r, M, L);
         }
     }
 }
@@ -734,22 +718,23 @@ __global__ __launch_bounds__(256) void k_attn4_join(Attn4Args a) {
     }
 }
 
-template <int D, int NT, int C, uint32_t TYPE, bool SPLIT>
+template <int D, int NT, int C, uint32_t TYPE>
 static int launch(const Attn4Args & a, hipStream_t s) {
-    const uint32_t rows = 16u / C * NT * (SPLIT ? 1u : kWaves), n_rg = (a.T * a.G + rows - 1u) / rows;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4<D, NT, C, TYPE, SPLIT>), dim3(a.n_head_kv, a.S, n_rg), dim3(64u * kWaves), 0, s, a);
+    const uint32_t rows = 16u / C * NT, n_rg = (a.T * a.G + rows - 1u) / rows;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4<D, NT, C, TYPE>), dim3(a.n_head_kv, a.S, n_rg), dim3(64u * kWaves), 0, s, a);
     if (a.S > 1u) hipLaunchKernelGGL(k_attn4_join<D>, dim3(a.T * a.G * a.n_head_kv), dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
 template <int D, uint32_t TYPE>
 static int launch_d(const Attn4Args & a, const Attn4Plan & p, hipStream_t s) {
-    if (!p.split_waves) return launch<D, 1, 1, TYPE, false>(a, s);
+    if constexpr (D <= 128)
+        if (p.NT == 2u) return launch<D, 2, 1, TYPE>(a, s);
     switch (p.C) {
-        case 2: return launch<D, 1, 2, TYPE, true>(a, s);
+        case 2: return launch<D, 1, 2, TYPE>(a, s);
         case 4:
-            if constexpr (D >= 128) return launch<D, 1, 4, TYPE, true>(a, s);
-        default: return launch<D, 1, 1, TYPE, true>(a, s);
+            if constexpr (D >= 128) return launch<D, 1, 4, TYPE>(a, s);
+        default: return launch<D, 1, 1, TYPE>(a, s);
     }
 }
 

@@ -1,6 +1,7 @@
 // tsr_kv4.hip -- host side of the attention over 4-bit KV caches.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 
@@ -9,6 +10,8 @@
 #include "kv4.hpp"
 #include "runtime.hpp"
 #include "tsr_hip.h"
+
+constexpr uint32_t kTokens = 16000u;     // of one launch
 
 static bool shape_ok(uint32_t D, uint32_t n_head, uint32_t n_head_kv) {
     return (D == 64u || D == 128u || D == 256u || D == 512u) && n_head_kv != 0u && n_head != 0u && n_head % n_head_kv == 0u &&
@@ -37,7 +40,7 @@ int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, u
         ((uintptr_t)mask_f16_dev & 1u) != 0u || (T > 1u && (q_stride % 4u != 0u || q_stride < K || out_stride % 4u != 0u ||
                                                             out_stride < K || (mask_f16_dev && mask_stride < n_kv))))
         return TSR_HIP_E_ARG;
-    const tsr::Attn4Plan p = tsr::attn4_plan(T, D, n_head, n_head_kv, n_kv, (uint32_t)ctx->n_cu);
+    const tsr::Attn4Plan p = tsr::attn4_plan(T, D, n_head, n_head_kv, n_kv, (uint32_t)ctx->n_cu);   // (S 1 beyond kTokens)
     if (ws_dev != nullptr && (ws_bytes < p.ws_bytes || ((uintptr_t)ws_dev & 15u) != 0u)) return TSR_HIP_E_ARG;
     tsr::Attn4Args a{};
     a.q = q_dev;
@@ -51,7 +54,6 @@ int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, u
     a.out_stride = out_stride;
     a.type = kc->type;
     a.D = D;
-    a.T = T;
     a.G = n_head / n_head_kv;
     a.inv_G = a.G == 1u ? 0u : (uint32_t)((1ull << 32) / a.G) + 1u;
     a.n_head_kv = n_head_kv;
@@ -73,5 +75,14 @@ int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, u
     }
     ctx->ctr.flash_attn_calls++;
     ctx->ctr.flash_attn_kv_bytes += (uint64_t)n_kv * (E / 32u) * tsr::kv4_block_bytes(kc->type) * 2u;
-    return tsr_launch_attn4(a, p, s) ? TSR_HIP_E_HIP : TSR_HIP_OK;
+    // (a launch holds 65535 groups of at least 16 rows along its third axis: 16000 tokens of up to 64 query heads)
+    for (uint32_t t0 = 0; t0 < T; t0 += kTokens) {
+        a.T = std::min(T - t0, kTokens);
+        a.q = q_dev + t0 * q_stride;
+        a.out = out_dev + t0 * out_stride;
+        if (runs_dev) a.runs = runs_dev + 4u * (size_t)t0;
+        if (mask_f16_dev) a.mask = mask_f16_dev + t0 * mask_stride;
+        if (tsr_launch_attn4(a, p, s)) return TSR_HIP_E_HIP;
+    }
+    return TSR_HIP_OK;
 }

@@ -304,3 +304,16 @@ def test_precision(dev, typ, nh, nkv, D, T, n_kv, kind):
     got = attend(dev, q, kc, vc, D, nh, nkv, scale, n_kv, runs, mask).astype(np.float64)
     rel = np.linalg.norm(got - want, axis=-1) / np.linalg.norm(want, axis=-1)
     assert rel.max() <= 2.0 ** -19, (rel.max(), np.unravel_index(rel.argmax(), rel.shape))
+
+
+def test_many_rows(dev):
+    """More tokens than one launch holds."""
+    D, T, n_kv, typ = 64, 16500, 70, H.KV_Q4_0
+    ki, kc, vi, vc = caches(dev, typ, n_kv, D, 91)
+    q = S.normal(93, T * D).reshape(T, D)
+    runs = np.zeros((T, 4), np.uint32)
+    runs[:, 1] = 1 + np.arange(T) % n_kv
+    got = attend(dev, q, kc, vc, D, 1, 1, 0.125, n_kv, runs)
+    pick = np.r_[0:40, 15980:16020, T - 40:T]
+    want, tol = R.attention(q[pick], ki, vi, typ, D, 1, 1, 0.125, runs[pick])
+    R.check(got[pick], want, tol, "many rows")
