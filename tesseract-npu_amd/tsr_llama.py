@@ -16,6 +16,9 @@ One decode step (T = 1) runs the op list of the reference's decoder-layer test
 
 then logits = MUL_MAT(Woutput, RMS_NORM(X) * output_norm) and the greedy token is the ARGMAX.
 
+kv_type picks the caches' type. Over q8_0 caches (the default) attention is the reference's; over 4-bit ones (q4_0, q4_1)
+A = tsr_hip_flash_attn_kv4, behind tsr_hip_rope_kv (fused) or ROPE and two SET_ROWS_KV, its visible cells in device memory.
+
 With fused=True (the default) RMS_NORM + MUL runs inside the Q|K|V and gate|up MUL_MATs
 (tsr_hip_mul_mat_norm), SWIGLU in the epilogue of the gate|up MUL_MAT (TSR_HIP_MM_GLU over gate / up
 rows interleaved), and ROPE with both SET_ROWS_KV inside the planned FLASH_ATTN_EXT
@@ -150,8 +153,9 @@ class LlamaDecoder:
     cells, and the activation buffers of one decode token."""
 
     def __init__(self, dev: H.Device, cfg: LlamaConfig, weights: SyntheticWeights, kv_size: int, fused: bool = True,
-                 qkv_in_attn: bool = True):
-        self.dev, self.cfg, self.kv_size = dev, cfg, kv_size
+                 qkv_in_attn: bool = True, kv_type: int = H.KV_Q8_0):
+        self.dev, self.cfg, self.kv_size, self.kv_type = dev, cfg, kv_size, kv_type
+        self.kv4 = kv_type != H.KV_Q8_0
         self.fused = fused
         self.qkv_in_attn = qkv_in_attn     # planned decode: the Q|K|V MUL_MAT inside the attention launch
         c = cfg
@@ -170,8 +174,8 @@ class LlamaDecoder:
                 "wgu": dev.weight(c.wfmt, np.stack([t["ffn_gate"], t["ffn_up"]], axis=1).reshape(2 * c.n_ff, -1)
                                   if fused else np.concatenate([t["ffn_gate"], t["ffn_up"]]), 2 * c.n_ff, c.n_embd),
                 "wd": dev.weight(c.wfmt, t["ffn_down"], c.n_embd, c.n_ff),
-                "kc": dev.kv(c.E, kv_size),
-                "vc": dev.kv(c.E, kv_size),
+                "kc": dev.kv(c.E, kv_size, kv_type),
+                "vc": dev.kv(c.E, kv_size, kv_type),
             }
             del t
             self.layers.append(L)
@@ -190,18 +194,25 @@ class LlamaDecoder:
         self.logits = H.BufferPart(self._out, 0, c.n_vocab * f4)
         self.bad = H.BufferPart(self._out, c.n_vocab * f4, 4).fill(0)
         self.next = dev.alloc(4)           # int32 greedy token (ARGMAX) of an eager step
-        # int32 position (ROPE) at 0, int64 cell (SET_ROWS_KV) at 8, int32 token id (GET_ROWS ids) at 16
-        self.params = dev.alloc(24)
+        # int32 position (ROPE) at 0, int64 cell (SET_ROWS_KV) at 8, int32 token id (GET_ROWS ids) at 16; in front of them
+        # the runs of visible cells (attention over 4-bit caches)
+        self._in = dev.alloc(40)
+        self.params = H.BufferPart(self._in, 16, 24)
         self.tok = H.BufferPart(self.params, 16, 4)
         self.rtab = dev.alloc(4 * c.head_dim)  # ROPE angles of the token's position (tsr_hip_rope_table)
         self.scale = 1.0 / math.sqrt(c.head_dim)
-        self.plan = dev.fa_plan(c.head_dim, c.n_head, c.n_head_kv, 1, kv_size)
+        self.plan = None if self.kv4 else dev.fa_plan(c.head_dim, c.n_head, c.n_head_kv, 1, kv_size)
+        self.ws, self.n_kv_graph = None, 0   # 4-bit caches: the graph's workspace and the cells it may touch
         # the planned FLASH_ATTN_EXT can take the ROPE + SET_ROWS_KV (tsr_hip_flash_attn_plan_rope) at these shapes
-        self.fa_rope = (c.head_dim in (64, 128) and (c.n_head // c.n_head_kv + 2) * c.head_dim <= 1024 and
+        self.fa_rope = (not self.kv4 and c.head_dim in (64, 128) and (c.n_head // c.n_head_kv + 2) * c.head_dim <= 1024 and
                         c.head_dim % 8 == 0)
         self.graph = None
         self.captures = 0
         self._pf = None                    # activations of a prefill ubatch (prefill)
+
+    @property
+    def runs_ptr(self) -> int:
+        return self._in.ptr
 
     @property
     def pos_ptr(self) -> int:
@@ -233,10 +244,12 @@ class LlamaDecoder:
         self._pf = {"U": U, "x": d.alloc(U * c.n_embd * f4), "h": d.alloc(U * c.n_embd * f4),
                     "xn": d.alloc(U * c.n_embd * f4), "qkv": d.alloc(U * (c.n_q + 2 * c.E) * f4),
                     "att": d.alloc(U * c.n_q * f4), "gu": d.alloc(U * 2 * c.n_ff * f4),
-                    "glu": d.alloc(U * c.n_ff * f4), "in": d.alloc(U * 16)}
+                    "glu": d.alloc(U * c.n_ff * f4), "in": d.alloc(U * (32 if self.kv4 else 16))}
         # a ubatch's cells (int64), positions and token ids (int32), written with one copy
         self._pf.update(cell=H.BufferPart(self._pf["in"], 0, U * 8), pos=H.BufferPart(self._pf["in"], U * 8, U * 4),
                         ids=H.BufferPart(self._pf["in"], U * 12, U * 4))
+        if self.kv4:                       # and their runs of visible cells
+            self._pf.update(runs=H.BufferPart(self._pf["in"], U * 16, U * 16))
         return self._pf
 
     def prefill(self, tokens, pos0: int = 0, ubatch: int = 512) -> None:
@@ -272,10 +285,12 @@ class LlamaDecoder:
         pf = self._prefill_buffers(T)
         x, h, xn, qkv, att, gu, glu = (pf[k] for k in ("x", "h", "xn", "qkv", "att", "gu", "glu"))
         U, pos = pf["U"], pos0 + np.arange(T, dtype=np.int64)
-        ins = np.zeros(4 * U, np.int32)
+        ins = np.zeros((8 if self.kv4 else 4) * U, np.int32)
         ins[:2 * T].view(np.int64)[:] = pos
         ins[2 * U:2 * U + T] = pos
         ins[3 * U:3 * U + T] = toks
+        if self.kv4:
+            ins[4 * U:].reshape(U, 4)[:T, 1] = pos + 1
         if ins.nbytes <= 16384:                                   # queued behind the ubatch before, no wait
             d.write_async(pf["in"], ins)
         else:
@@ -310,8 +325,12 @@ class LlamaDecoder:
                        c.rope_base, qkv, w3)
                 d.kv_set_rows(L["kc"], 0, qkv.ptr + nq * f4, T, w3, pf["cell"], self.bad)
                 d.kv_set_rows(L["vc"], 1, qkv.ptr + (nq + E) * f4, T, w3, pf["cell"], self.bad)
-            d.flash_attn(qkv, T, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, msum, att, nq,
-                         new_runs=runs)
+            if self.kv4:
+                d.flash_attn_kv4(qkv, T, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, pos0 + T, att,
+                                 nq, runs=pf["runs"])
+            else:
+                d.flash_attn(qkv, T, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, msum, att, nq,
+                             new_runs=runs)
             d.mul_mat(L["wo"], att, T, nq, h, n, add=x, add_stride=n)
             if self.fused and mma:
                 d.rms_norm(h, n, T, n, c.eps, xn, n, w=L["ffn_norm"], w_stride=n)
@@ -341,9 +360,15 @@ class LlamaDecoder:
             p[4] = token
         return p
 
-    def _ops(self, out_tok, msum=None, runs=None, stream=None) -> None:
+    def _inputs(self, pos: int, token: int | None = None):
+        """Where a token's input bytes go, and they: with 4-bit caches the runs (cells [0, pos]) in front."""
+        p = self._params(pos, token)
+        return (self._in, np.concatenate([np.array([0, pos + 1, 0, 0], np.int32), p])) if self.kv4 else (self.params, p)
+
+    def _ops(self, out_tok, msum=None, runs=None, stream=None, n_kv=None) -> None:
         """The launches of one decode token. msum given: FLASH_ATTN_EXT planned on the host per call
-        (eager); else the device-resident plan (capturable)."""
+        (eager); else the device-resident plan (capturable). Over 4-bit caches of at most n_kv cells in use: the
+        workspace of the graph, or without one the context's scratch."""
         c, d = self.cfg, self.dev
         nq, E, n = c.n_q, c.E, c.n_embd
         f4 = 4
@@ -378,6 +403,9 @@ class LlamaDecoder:
                 d.kv_set_rows(L["vc"], 1, self.qkv.ptr + (nq + E) * f4, 1, E, self.cell_ptr, self.bad, stream=stream)
             if fa_done:
                 pass
+            elif self.kv4:
+                d.flash_attn_kv4(self.qkv, 1, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, n_kv,
+                                 self.att, nq, runs=self.runs_ptr, ws=self.ws, stream=stream)
             elif msum is not None:
                 d.flash_attn(self.qkv, 1, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale,
                              msum, self.att, nq, new_runs=runs, stream=stream)
@@ -408,8 +436,29 @@ class LlamaDecoder:
         rounded up to 256, at most kv_size)."""
         msum, runs = self._mask(pos, n_kv)
         self.tok.write(np.array([token], np.int32) if token is not None else self.next.read(np.int32, (1,)))
-        self.params.write(self._params(pos))
-        self._ops(self.next, msum, runs)
+        buf, ins = self._inputs(pos)
+        buf.write(ins)
+        if self.kv4:
+            self._graph_cells(pos)
+        self._ops(self.next, msum, runs, n_kv=pos + 1)
+
+    def _graph_cells(self, pos: int) -> bool:
+        """4-bit caches: a decode graph is captured for 256, 512, 1024 .. cells (what splits its attention). True when
+        position pos is beyond the last one's; the workspace then fits the next."""
+        if pos < self.n_kv_graph:
+            return False
+        c, n = self.cfg, 256
+        while n <= pos:
+            n *= 2
+        self.n_kv_graph = min(n, self.kv_size)
+        if self.graph is not None:         # (it reads the workspace)
+            self.graph.free()
+            self.graph = None
+        need = self.dev.flash_attn_kv4_ws(1, c.head_dim, c.n_head, c.n_head_kv, self.n_kv_graph)
+        if self.ws is not None:
+            self.ws.free()
+        self.ws = self.dev.alloc(need) if need else None
+        return True
 
     def step_graph(self, token: int | None, pos: int, n_kv: int | None = None) -> None:
         """One decode token as one graph replay. Per token the host only plans the attention chunks and
@@ -418,14 +467,14 @@ class LlamaDecoder:
         call and again whenever the plan's shape changes. Nothing waits for the device."""
         d = self.dev
         msum, runs = self._mask(pos, n_kv)
-        d.write_async(self.params, self._params(pos, token))
-        changed = self.plan.set(msum, runs)
+        d.write_async(*self._inputs(pos, token))
+        changed = self._graph_cells(pos) if self.kv4 else self.plan.set(msum, runs)
         if self.graph is None or changed:
             if self.graph is not None:
                 self.graph.free()
             d.graph_begin()
             try:
-                self._ops(self.tok)
+                self._ops(self.tok, n_kv=self.n_kv_graph)
             finally:
                 g = d.graph_end()
             self.graph = g
@@ -438,9 +487,12 @@ class LlamaDecoder:
         Nothing waits for the device."""
         d = self.dev
         msum, runs = self._mask(pos, n_kv)
-        d.write_async(self.params, self._params(pos, token))
-        self.plan.set(msum, runs)
-        self._ops(self.tok)
+        d.write_async(*self._inputs(pos, token))
+        if self.kv4:
+            self._graph_cells(pos)
+        else:
+            self.plan.set(msum, runs)
+        self._ops(self.tok, n_kv=self.n_kv_graph)
 
     def generate_graph(self, first_token: int, pos0: int, n_tokens: int, hist=None, check: bool = True) -> None:
         """Greedy decode of n_tokens by graph replays, queued without waiting for the device; the token
@@ -505,7 +557,11 @@ class LlamaDecoder:
         if self.graph is not None:
             self.graph.free()
             self.graph = None
-        self.plan.free()
+        if self.plan is not None:
+            self.plan.free()
+        if self.ws is not None:
+            self.ws.free()
+            self.ws = None
         if self._pf is not None:
             for k, b in self._pf.items():
                 if k != "U":
