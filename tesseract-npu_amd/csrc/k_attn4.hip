@@ -136,7 +136,7 @@ template <int D, int NT, int C, uint32_t TYPE>
 struct Attn4 {
     static constexpr int NB = D / 32, NK = NB / C;                 // blocks of a head, of a column
     static constexpr int RW = 16 / C;                              // query rows of a group of 16 columns
-    static constexpr int AHEAD = D == 512 ? 1 : 2;                 // tiles loaded ahead
+    static constexpr int AHEAD = D >= 256 ? 1 : 2;                 // tiles loaded ahead
     using Tl = Tile<D, C, TYPE>;
     struct Row {                                                   // of the lane's query row in each group of 16
         uint32_t lo0, hi0, lo1, hi1, t;
@@ -343,20 +343,29 @@ struct Attn4 {
             if constexpr (MASKED) {
                 vis[n] = 0u;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t c = c0 + 16u * u + 4u * g;
+                    uint2 w = make_uint2(0u, 0u);                  // the mask's four values
+                    if (a.mask != nullptr) {
+                        const uint16_t * mp = a.mask + (size_t)row[n].t * a.mask_stride + c;
+                        if (a.mask_by4 && c + 4u <= a.n_kv) {
+                            w = *(const uint2 *)mp;
+                        } else {
+                            if (c < a.n_kv) w.x = mp[0];
+                            if (c + 1u < a.n_kv) w.x |= (uint32_t)mp[1] << 16;
+                            if (c + 2u < a.n_kv) w.y = mp[2];
+                            if (c + 3u < a.n_kv) w.y |= (uint32_t)mp[3] << 16;
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t c = c0 + 16u * u + 4u * g + i;
-                        bool in = sees(n, c);
-                        float x = s[n][u][i] * csc[n];
-                        if (a.mask != nullptr && in) {
-                            const float w = h2f_fast(a.mask[(size_t)row[n].t * a.mask_stride + c]);
-                            in = w != -__builtin_inff();
-                            x = __builtin_fmaf(w, kLog2e, x);
-                        }
+                        const float z = half_of(i < 2 ? w.x : w.y, i & 1);
+                        const bool in = sees(n, c + i) && z != -__builtin_inff();
+                        const float x = __builtin_fmaf(z, kLog2e, s[n][u][i] * csc[n]);
                         vis[n] |= in ? 1u << (4 * u + i) : 0u;
                         s[n][u][i] = in ? x : -__builtin_inff();
                     }
+                }
             }
             float x = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3]));
             x = fmaxf(x, fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));

@@ -108,6 +108,7 @@ struct Attn4Args {
     const uint32_t * runs;   // nullable: [T][4] the cells [lo0, hi0) and [lo1, hi1) that a token sees
     const uint16_t * mask;   // nullable: f16 [T], rows of mask_stride
     uint64_t mask_stride;
+    uint32_t mask_by4;       // four of its values, from a multiple of four on, are 8-byte aligned
     float * out;             // [T][n_head][D], token t at out + t * out_stride
     uint64_t out_stride;
     float * part;            // S > 1: [split][T n_head] (maximum, sum), then [split][T n_head][D] unnormalised rows

@@ -50,6 +50,7 @@ int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, u
     a.runs = runs_dev;
     a.mask = mask_f16_dev;
     a.mask_stride = mask_stride;
+    a.mask_by4 = (((uintptr_t)mask_f16_dev | (T > 1u ? 2u * mask_stride : 0u)) & 7u) == 0u ? 1u : 0u;
     a.out = out_dev;
     a.out_stride = out_stride;
     a.type = kc->type;
