@@ -107,13 +107,21 @@ __global__ __launch_bounds__(256) void k_kv4_set_rows(Kv4Args a, uint32_t which,
         atomicMax((uint32_t *)a.base, dmax);                       // rare once the plane has seen its values
 }
 
-// Cells as f32 rows: workgroup (pair of blocks, 32 rows), a thread eight values. d n - 8 d and d n are exact in f32;
-// q4_1's sum is rounded once.
+// Stores past the caches: rows read back are not read again by these kernels.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void store_row(float * p, float a, float b, float c, float d) {
+    __builtin_nontemporal_store(f32x4{ a, b, c, d }, (f32x4 *)p);
+}
+
+// Cells as f32 rows: workgroup (pair of blocks, 32 rows), a thread values 4 q .. 4 q + 3 of both blocks. Bound: the
+// rows' bytes. Every store covers whole lines of the rows and goes past the caches; 32768 rows of 1024 values (151 MB)
+// take 24 us from K and 28 from V, 6.3 and 5.4 TB/s. With half a line a store and no hint they took 41 us from K and 50 from V, with either alone 38
+// and 46. d n - 8 d and d n are exact in f32; q4_1's sum is rounded once.
 template <uint32_t TYPE>
 __global__ __launch_bounds__(256) void k_kv4_get_rows(Kv4Args a, uint32_t which, const int64_t * idx, uint32_t n_rows,
                                                       float * dst, uint64_t dst_stride, int32_t * bad) {
     const uint32_t r = blockIdx.y * kRowsPerWg + threadIdx.x / 8u, q = threadIdx.x & 7u, k = q & 3u;
-    const uint32_t b = 2u * blockIdx.x + (q >> 2);
+    const uint32_t b = 2u * blockIdx.x;
     if (r >= n_rows) return;
     const int64_t cell64 = idx[r];
     if (cell64 < 0 || cell64 >= (int64_t)a.kv_size) {
@@ -122,25 +130,33 @@ __global__ __launch_bounds__(256) void k_kv4_get_rows(Kv4Args a, uint32_t which,
     }
     const uint32_t cell = (uint32_t)cell64;
     const uint8_t * t = a.base + kv4_tile(TYPE, a.n_tiles, cell, b);
-    uint32_t w = 0u;
+    uint32_t w[2] = { 0u, 0u };
     if (which == 0u) {
-        w = *(const uint32_t *)(t + kv4_code(0u, cell, b, 4u * k));
+        const uint2 v = *(const uint2 *)(t + kv4_code(0u, cell, b, 4u * k));
+        w[0] = v.x;
+        w[1] = v.y;
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) w |= (uint32_t)t[kv4_code(1u, cell, b, 4u * k + i)] << (8u * i);
+        for (uint32_t i = 0; i < 4; ++i) {
+            w[0] |= (uint32_t)t[kv4_code(1u, cell, b, 4u * k + i)] << (8u * i);
+            w[1] |= (uint32_t)t[kv4_code(1u, cell, b + 1u, 4u * k + i)] << (8u * i);
+        }
     }
-    const uint16_t * sc = (const uint16_t *)(t + kv4_scale(TYPE, cell, b));
-    const float d = h2f_fast(sc[0]);
-    const float m = TYPE == kKvQ4_1 ? h2f_fast(sc[TYPE == kKvQ4_1 ? 2 : 0]) : 0.0f;
-    float y[8];
+    float * row = dst + (size_t)r * dst_stride + 32u * b + 4u * q;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float n = (float)((w >> (8 * (i & 3) + (i >> 2) * 4)) & 15u);
-        y[i] = TYPE == kKvQ4_0 ? d * (n - 8.0f) : d * n + m;
+    for (uint32_t p = 0; p < 2; ++p) {
+        const uint16_t * sc = (const uint16_t *)(t + kv4_scale(TYPE, cell, b + p));
+        const float d = h2f_fast(sc[0]);
+        const float m = TYPE == kKvQ4_1 ? h2f_fast(sc[TYPE == kKvQ4_1 ? 2 : 0]) : 0.0f;
+        const uint32_t v = w[p] >> (q & 4u);                       // threads 4 .. 7: the high nibbles
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float n = (float)((v >> (8 * i)) & 15u);
+            y[i] = TYPE == kKvQ4_0 ? d * (n - 8.0f) : d * n + m;
+        }
+        store_row(row + 32u * p, y[0], y[1], y[2], y[3]);
     }
-    float * row = dst + (size_t)r * dst_stride + 32u * b + 4u * k;
-    *(float4 *)row = make_float4(y[0], y[1], y[2], y[3]);
-    *(float4 *)(row + 16) = make_float4(y[4], y[5], y[6], y[7]);
 }
 
 // q8_0 cells as f32 rows (the layout of k_kv.hip): a wave 256 values of a row. d q is exact in f32.
@@ -163,7 +179,7 @@ __global__ __launch_bounds__(64) void k_kv_get_rows(KvArgs a, uint32_t which, co
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = (int8_t)qb[(size_t)(i + j) * 16u + rr];
     }
-    *(float4 *)(dst + (size_t)r * dst_stride + i) = make_float4(d * v[0], d * v[1], d * v[2], d * v[3]);
+    store_row(dst + (size_t)r * dst_stride + i, d * v[0], d * v[1], d * v[2], d * v[3]);
 }
 
 // One thread a byte [off, off + n) of the ggml image (row j = cell j, E / 32 blocks of {d[, m], 16 code bytes}).
