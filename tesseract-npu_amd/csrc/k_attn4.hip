@@ -520,6 +520,9 @@ struct Attn4 {
         uint32_t vis[NT];
         const size_t c = (size_t)ahead * kv4_tile_bytes(TYPE);
         scores(k, lds + ql, s);
+        if constexpr (!WHOLE)                                      // (made here: moved behind the mask's branches they would
+#pragma unroll                                                     // keep the products and scales of every block in registers)
+            for (int n = 0; n < NT; ++n) asm volatile("" : "+v"(s[n][0]), "+v"(s[n][1]));
         load<false>(k, kp + c, pair, lane);
         weights<!WHOLE>(a, s, vis, 32u * i, lane, kexp);
         values<!WHOLE>(v, s, vis);
