@@ -8,13 +8,21 @@
 //            pieces (22 bits). q4_1 (d n + m) adds m sum(q) a block.
 //   softmax  in base 2, f32: a lane holds the scores of one row for four cells of every 16, which is, cells
 //            permuted, the second operand of the next product: P stays where it is.
-//   P V      O^T[value][row]: the first operand are n - 8 again, the second p d[cell] of a block in two f16 pieces (one instruction makes each: f16(p d),
-//            f16(p d - hi)). Sums of raw codes would be large and nearly cancel: an error that grows with the root of the
-//            cells. p carries 2^k with 2^k max|d| in [2^8, 2^9) from the plane's header and is at most 2^6 (the maximum
-//            follows when it is passed by that), so that no piece overflows and the pieces keep 2^-33 of the largest.
-//            q4_1: sum p (m + 8 d) is summed aside in f32.
+//   P V      O^T[value][row]: the first operand are n - 8 again, the second p d[cell] of a block in two f16 pieces, f16(p) d
+//            rounded once and what p d leaves of it. Sums of raw codes would be large and nearly cancel: an error that grows
+//            with the root of the cells. p carries 2^k with 2^k max|d| in [2^8, 2^9) from the plane's header (k at most 9) and
+//            is at most 2^6 (the maximum follows when it is passed by that), so that no piece overflows and the pieces keep
+//            2^-33 of the largest. q4_1: sum p (m + 8 d) is summed aside in f32.
 // The scales meet the f32 sums only, where a cell that its row does not see is replaced by nothing: an infinity or a
 // NaN in a masked cell reaches no result. Sums, maxima and results are f32; both splits keep 22 bits of f32's 24.
+//
+// Bound. Few rows: the cells' bytes and two launches: a token of 32 heads of 128 (8 KV heads) takes 12.8 us behind 8192
+// cells (a call of a graph of them: 6.5 the cells, 2.8 the join, the rest between launches) and 42 us behind 131071 of q4_1
+// (168 MB, 4.0 TB/s; a plain read of them 29 us). Many rows: vector instructions, about 130 a 16 x 16 tile of scores and
+// D 128 (a third the unpacking, a quarter the pieces of p d) against 32 matrix instructions: 2048 tokens behind 4096 .. 6144
+// cells take 544 us (316 TFLOP/s), vector units 80 %, matrix units 35 % busy. Unpacking once for four waves through LDS,
+// V in two pieces, left 270 vector instructions of 466 a tile of 32 rows and gave 4 %: with 239 registers two waves a
+// SIMD hide neither kind behind the other; four groups of rows a workgroup gave nothing.
 #include "attn4_plan.hpp"
 #include "kernels.hpp"
 #include "kv4.hpp"
@@ -599,9 +607,17 @@ struct Attn4 {
 
 constexpr uint32_t values_at_once(uint32_t D, uint32_t most) { return D <= most ? D : values_at_once(D / 2u, most); }
 
+// Waves a SIMD has registers for: the most that need no spills (q4_1's sums aside take up to 40 more: a third wave with
+// 12 registers spilled made 128 rows behind 3000 cells, D 128, 41 us and not 37).
+constexpr int waves_of(int D, int NT, int C, uint32_t TYPE) {
+    if (D * NT == 64) return 4;
+    if (NT == 1 && (D == 128 ? C == 4 || (C == 1 && TYPE == kKvQ4_0) : D == 256 && C == 1 && TYPE == kKvQ4_0)) return 3;
+    return D <= 256 ? 2 : 1;
+}
+
 // Workgroup (KV head, split, group of rows), KV heads fastest: with eight of them every XCD's L2 holds one head.
 template <int D, int NT, int C, uint32_t TYPE>
-__global__ __launch_bounds__(256, D * NT == 64 ? 4 : D == 128 && C != 2 && NT == 1 ? 3 : D <= 256 ? 2 : 1) void k_attn4(Attn4Args a) {
+__global__ __launch_bounds__(256, waves_of(D, NT, C, TYPE)) void k_attn4(Attn4Args a) {
     using A = Attn4<D, NT, C, TYPE>;
     constexpr uint32_t RT = A::RW * NT;                            // rows of the workgroup
     const uint32_t h = blockIdx.x, split = blockIdx.y, rg = gridDim.z - 1u - blockIdx.z;   // causal: the long rows first
