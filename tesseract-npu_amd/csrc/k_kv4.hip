@@ -70,7 +70,8 @@ __device__ __forceinline__ uint32_t quantize4(float (&x)[8], uint32_t k, uint16_
     return w;
 }
 
-// SET_ROWS: workgroup (pair of blocks, 32 rows). Bound: the rows' bytes (a launch for few rows).
+// SET_ROWS: workgroup (pair of blocks, 32 rows). Bound: the rows' bytes, 32768 rows of 1024 values in 25 us (6.1 TB/s); a
+// launch for few rows.
 template <uint32_t TYPE>
 __global__ __launch_bounds__(256) void k_kv4_set_rows(Kv4Args a, uint32_t which, const float * src, uint64_t src_stride,
                                                       uint32_t n_rows, const int64_t * idx, int32_t * bad) {
@@ -114,9 +115,9 @@ __device__ __forceinline__ void store_row(float * p, float a, float b, float c, 
 }
 
 // Cells as f32 rows: workgroup (pair of blocks, 32 rows), a thread values 4 q .. 4 q + 3 of both blocks. Bound: the
-// rows' bytes. Every store covers whole lines of the rows and goes past the caches; 32768 rows of 1024 values (151 MB)
-// take 24 us from K and 28 from V, 6.3 and 5.4 TB/s. With half a line a store and no hint they took 41 us from K and 50 from V, with either alone 38
-// and 46. d n - 8 d and d n are exact in f32; q4_1's sum is rounded once.
+// rows' bytes. Every store covers whole lines of the rows and goes past the caches: 32768 rows of 1024 values (153 MB)
+// take 24 us from K and 28 from V, 6.3 and 5.4 TB/s. With half a line a store and no hint they took 41 and 50, with the
+// hint alone 38 and 46. d n - 8 d and d n are exact in f32; q4_1's sum is rounded once.
 template <uint32_t TYPE>
 __global__ __launch_bounds__(256) void k_kv4_get_rows(Kv4Args a, uint32_t which, const int64_t * idx, uint32_t n_rows,
                                                       float * dst, uint64_t dst_stride, int32_t * bad) {
