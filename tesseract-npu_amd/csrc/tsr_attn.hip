@@ -90,17 +90,23 @@ static int kv_bytes(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t which, si
     if (bytes == 0) return TSR_HIP_OK;
     std::lock_guard<std::mutex> lk(ctx->mtx);
     (void)hipSetDevice(ctx->device);
-    int rc = ctx->scratch.reserve(bytes, ctx->stream);
-    if (rc) return rc;
-    uint8_t * stage = (uint8_t *)ctx->scratch.ptr;
-    if (to_dev) rc = hip_err(hipMemcpyAsync(stage, host, bytes, hipMemcpyHostToDevice, ctx->stream), "kv H2D");
-    if (rc == 0) {
-        const int k = kv->type == TSR_HIP_KV_Q8_0
-                          ? tsr_launch_kv_bytes(kv_args(kv), which, off, bytes, stage, to_dev, ctx->stream)
-                          : tsr_launch_kv4_bytes(kv4_args(kv), which, off, bytes, stage, to_dev, ctx->stream);
-        rc = k ? TSR_HIP_E_HIP : 0;
+    // In pieces of whole rows, at most kBytesAtOnce: a launch holds fewer than 2^32 threads (one a byte), a cache may
+    // hold more bytes. Each piece goes through the same scratch, in the stream's order.
+    constexpr size_t kBytesAtOnce = (size_t)64 << 20;
+    const size_t row = (size_t)(kv->E / 32u) * block, most = kBytesAtOnce / row * row;   // (a row is at most 34816 bytes)
+    int rc = ctx->scratch.reserve(std::min(bytes, most), ctx->stream);
+    for (size_t done = 0, n; rc == 0 && done < bytes; done += n) {
+        n = std::min(bytes - done, most - (off + done) % row);
+        uint8_t * stage = (uint8_t *)ctx->scratch.ptr, * h = (uint8_t *)host + done;
+        if (to_dev) rc = hip_err(hipMemcpyAsync(stage, h, n, hipMemcpyHostToDevice, ctx->stream), "kv H2D");
+        if (rc == 0) {
+            const int k = kv->type == TSR_HIP_KV_Q8_0
+                              ? tsr_launch_kv_bytes(kv_args(kv), which, off + done, n, stage, to_dev, ctx->stream)
+                              : tsr_launch_kv4_bytes(kv4_args(kv), which, off + done, n, stage, to_dev, ctx->stream);
+            rc = k ? TSR_HIP_E_HIP : 0;
+        }
+        if (rc == 0 && !to_dev) rc = hip_err(hipMemcpyAsync(h, stage, n, hipMemcpyDeviceToHost, ctx->stream), "kv D2H");
     }
-    if (rc == 0 && !to_dev) rc = hip_err(hipMemcpyAsync(host, stage, bytes, hipMemcpyDeviceToHost, ctx->stream), "kv D2H");
     if (rc == 0) rc = hip_err(hipStreamSynchronize(ctx->stream), "hipStreamSynchronize");
     return rc;
 }

@@ -57,6 +57,21 @@ def test_image_round_trip(dev, typ, E, kv_size):
         kv.free()
 
 
+@pytest.mark.parametrize("typ", [H.KV_Q8_0, H.KV_Q4_0, H.KV_Q4_1])
+def test_image_in_pieces(dev, typ):
+    """An image of more bytes than one piece of the conversion (64 MiB), from the middle of a row to the middle of one."""
+    E, kv_size = 1024, 150_000
+    kv = dev.kv(E, kv_size, typ)
+    img = np.random.default_rng(typ).integers(0, 256, kv_size * kv.row_bytes, dtype=np.uint8)
+    off, end = 5 * kv.row_bytes + 77, img.size - 300
+    assert end - off > 80 << 20
+    kv.set_bytes(H.KV_K, img[off:end], off)
+    assert (kv.get_bytes(H.KV_K, off, end - off) == img[off:end]).all()
+    img[:off], img[end:] = 0, 0
+    assert (kv.get_bytes(H.KV_K) == img).all()
+    kv.free()
+
+
 @pytest.mark.parametrize("typ", TYPES)
 @pytest.mark.parametrize("which", [0, 1])
 @pytest.mark.parametrize("E,kv_size,n,stride", [(1024, 64, 1, 1024), (128, 300, 33, 132), (64, 40, 40, 64),
