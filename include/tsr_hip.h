@@ -14,7 +14,9 @@
  *   - Pointers named *_dev are device addresses (from tsr_hip_alloc or any HIP allocation on the
  *     context's device); every other pointer is host memory.
  *   - `stream` is a hipStream_t of the context's device, or NULL for the context's own stream.
- *     Kernel entry points are asynchronous on that stream; tsr_hip_sync waits.
+ *     Kernel entry points are asynchronous on that stream; tsr_hip_sync waits. The context orders the next
+ *     user of its scratch memory behind the last one's stream: a stream on which a call used the scratch is
+ *     destroyed after a later call has used it on another stream, or after tsr_hip_close.
  *   - A context is thread-safe: calls on one context are serialized by its mutex (the reference
  *     backend's device mutex, ggml-tesseract.cpp:3932).
  *   - Strides are in elements (floats) unless named *_bytes.

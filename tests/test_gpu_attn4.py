@@ -177,7 +177,7 @@ def test_a_huge_value_written_before(dev):
 
 def test_graph_replays_follow_runs_and_cells(dev):
     """A captured call with a workspace of its own, replayed with eager work between: each replay attends over the runs and
-    cells of its time; a second graph with another workspace on another stream in turn with it."""
+    cells of its time; a second graph with a workspace of its own in turn with it."""
     nh, nkv, D, kv_size = 32, 8, 128, 3000
     typ = H.KV_Q4_0
     E, scale = nkv * D, 1.0 / math.sqrt(D)
@@ -317,3 +317,91 @@ def test_many_rows(dev):
     pick = np.r_[0:40, 15980:16020, T - 40:T]
     want, tol = R.attention(q[pick], ki, vi, typ, D, 1, 1, 0.125, runs[pick])
     R.check(got[pick], want, tol, "many rows")
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("nh,nkv,D,T,n_kv", [(32, 8, 64, 600, 75), (32, 8, 128, 520, 200), (8, 4, 256, 150, 131),
+                                              (4, 2, 512, 20, 97), (12, 2, 512, 2, 300), (16, 1, 256, 1, 900)])
+def test_masks_at_every_head_size(dev, typ, nh, nkv, D, T, n_kv):
+    """Masks that hide and weigh cells, their rows aligned to eight bytes and not, a row that sees nothing."""
+    ki, kc, vi, vc = caches(dev, typ, n_kv, nkv * D, 101)
+    rng = np.random.default_rng(D + T)
+    q = S.normal(103, T * nh * D).reshape(T, nh * D)
+    for width in (n_kv + 1, (n_kv + 7) // 4 * 4):
+        mask = rng.standard_normal((T, width)).astype(np.float16)
+        mask[rng.random((T, width)) < 0.5] = -np.inf
+        mask[T - 1] = -np.inf
+        mask[:, n_kv:] = np.nan
+        want, tol = R.attention(q, ki, vi, typ, D, nh, nkv, 0.15, None, mask)
+        got = attend(dev, q, kc, vc, D, nh, nkv, 0.15, n_kv, mask=mask)
+        R.check(got, want, tol, f"rows of {width}")
+        assert (got[T - 1] == 0).all()
+
+
+def test_two_streams(dev):
+    """Calls on two streams at once: each with a workspace of its own, and both with the context's scratch; rows stored,
+    read back and attended to on a stream that is not the context's."""
+    other = H.Device(0)
+    nh, nkv, D, n_kv, typ = 32, 8, 128, 6000, H.KV_Q4_1
+    ki, kc, vi, vc = caches(dev, typ, n_kv, nkv * D, 111)
+    qs = S.normal(113, 2 * nh * D).reshape(2, nh * D)
+    bq = [dev.upload(qs[i]) for i in range(2)]
+    streams = (None, other.stream)
+    need = dev.flash_attn_kv4_ws(1, D, nh, nkv, n_kv)
+    assert need > 0
+    wants = [R.attention(qs[i:i + 1], ki, vi, typ, D, nh, nkv, 0.1) for i in range(2)]
+    for ws in ([dev.alloc(need), dev.alloc(need)], [None, None]):
+        outs = [[dev.alloc(4 * nh * D).fill(0xFF) for _ in range(6)] for _ in range(2)]
+        dev.sync()
+        for j in range(6):
+            for i in range(2):
+                dev.flash_attn_kv4(bq[i], 1, nh * D, kc, vc, D, nh, nkv, 0.1, n_kv, outs[i][j], nh * D, ws=ws[i],
+                                   stream=streams[i])
+        for st in streams:
+            dev.sync(st)
+        for i in range(2):
+            for out in outs[i]:
+                R.check(out.read(np.float32, (1, nh, D)), *wants[i], f"stream {i}")
+    x = S.normal(117, 3 * nkv * D).reshape(3, nkv * D)
+    cells = np.array([5, 17, 4000], np.int64)
+    bx, bi, back = dev.upload(x), dev.upload(cells), dev.alloc(x.nbytes).fill(0xFF)
+    out = dev.alloc(4 * nh * D)
+    dev.sync()
+    dev.kv_set_rows(vc, 1, bx, 3, nkv * D, bi, stream=streams[1])
+    dev.kv_get_rows(vc, 1, bi, 3, back, nkv * D, stream=streams[1])
+    dev.flash_attn_kv4(bq[0], 1, nh * D, kc, vc, D, nh, nkv, 0.1, n_kv, out, nh * D, stream=streams[1])
+    dev.sync(streams[1])
+    vi[cells] = R.quantize(x, typ)
+    assert (back.read(np.float32, x.shape) == R.values_f32(vi[cells], typ)).all()
+    R.check(out.read(np.float32, (1, nh, D)), *R.attention(qs[:1], ki, vi, typ, D, nh, nkv, 0.1), "behind the rows")
+    # (the scratch goes back to the context's stream before the other one ends)
+    R.check(attend(dev, qs[:1], kc, vc, D, nh, nkv, 0.1, n_kv), *R.attention(qs[:1], ki, vi, typ, D, nh, nkv, 0.1), "after it")
+    other.close()
+
+
+def test_offsets_past_32_bits(dev):
+    """A plane of more than 4 GiB: its last cells and heads stored, read back and attended to."""
+    nh = nkv = 64
+    D, kv_size, n, typ = 128, 1 << 20, 45, H.KV_Q4_0
+    E = nkv * D
+    assert kv_size * (E // 32) * R.BLOCK[typ] > 1 << 32
+    cells = kv_size - n + np.arange(n, dtype=np.int64)
+    bi, imgs, cs = dev.upload(cells), [], []
+    for which in (0, 1):
+        x = S.normal(121 + which, n * E).reshape(n, E)
+        imgs.append(R.quantize(x, typ))
+        cs.append(dev.kv(E, kv_size, typ))
+        dev.kv_set_rows(cs[which], which, dev.upload(x), n, E, bi)
+        back = dev.alloc(4 * n * E)
+        dev.kv_get_rows(cs[which], which, bi, n, back, E)
+        dev.sync()
+        assert (back.read(np.float32, (n, E)) == R.values_f32(imgs[which], typ)).all()
+        assert (cs[which].get_bytes(which, int(cells[0]) * cs[which].row_bytes, imgs[which].nbytes) == imgs[which].reshape(-1)).all()
+    T = 3
+    q = S.normal(125, T * nh * D).reshape(T, nh * D)
+    runs = np.zeros((T, 4), np.uint32)
+    runs[:, 0], runs[:, 1] = cells[0], cells[0] + [1, 20, n]
+    want, tol = R.attention(q, imgs[0], imgs[1], typ, D, nh, nkv, 0.1, runs - np.array([cells[0], cells[0], 0, 0], np.uint32))
+    R.check(attend(dev, q, cs[0], cs[1], D, nh, nkv, 0.1, kv_size, runs), want, tol, "the last cells")
+    for c in cs:
+        c.free()
