@@ -35,9 +35,14 @@ inline Attn4Plan attn4_plan(uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_
     // Splits fill the compute units with one workgroup each (a token behind 8192 cells: 16, 32, 64 splits 12.6, 11.8, 12.2
     // us), with two where a wave then still has eight tiles (131072 cells: 32, 64, 96 splits 43.6, 39.0, 40.6). A split is
     // a second launch and a pass through memory, about the time of five tiles of a wave: none below 20 tiles (512 cells 8.3
-    // us in one piece, 9.3 in four), and none where half the compute units have work (300 tokens 33 -> 42).
+    // us in one piece, 9.3 in four), and none where half the compute units have work (300 tokens 33 -> 42). Several
+    // tokens behind many cells are mostly sequences of their own and of all lengths, and a group waits for its longest:
+    // two workgroups a compute unit from 8192 cells on (64 tokens of up to 2000 cells, 128 groups: 2, 4, 8 splits 57.8, 42.8,
+    // 48.9; 96, 192 groups: 1, 2, 4 splits 91, 72, 54; 64 tokens of one sequence behind 1000 cells 19.2, 21.1, 26.9), but
+    // not where a group is one token's and each unit has one (32 tokens of up to 1000 cells: 13.3, 17.2).
     const uint64_t n = wgs(16u / p.C * p.NT), fill = n_cu / n;
-    const uint64_t S = tiles <= 20u ? 1u : tiles >= 64u * fill && T <= 2u ? 2u * fill : fill;
+    const bool twice = n <= n_cu && (p.C == 1u || n < n_cu) && tiles >= std::max<uint64_t>(T <= 2u ? 0u : 256u, 64u * fill);
+    const uint64_t S = tiles <= 20u ? 1u : twice ? (2u * (uint64_t)n_cu + n - 1u) / n : fill;
     p.S = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ S, (tiles + 3u) / 4u, kSplitsMax }));
     p.ws_bytes = p.S > 1u ? 4u * (size_t)p.S * T * n_head * (2u + D) : 0u;
     return p;
