@@ -20,8 +20,8 @@
 // cells (a call of a graph of them: 6.5 the cells, 2.8 the join, the rest between launches) and 42 us behind 131071 of q4_1
 // (168 MB, 4.0 TB/s; a plain read of them 29 us). Many rows: vector instructions, about 130 a 16 x 16 tile of scores and
 // D 128 (a third the unpacking, a quarter the pieces of p d) against 16 matrix instructions: 2048 tokens behind 6144
-// cells take 544 us (442 TFLOP/s), vector units 80 %, matrix units 35 % busy. Unpacking once for four waves through LDS,
-// V in two pieces, left 270 vector instructions of 466 a tile of 32 rows and gave 4 %: with 239 registers two waves a
+// cells take 544 to 573 us (420 to 442 TFLOP/s), vector units 80 %, matrix units 35 % busy. Unpacking once for four waves through LDS,
+// V in two pieces, left 270 vector instructions of 466 a tile of 32 rows and was no faster: with 239 registers two waves a
 // SIMD hide neither kind behind the other; four groups of rows a workgroup gave nothing.
 #include "attn4_plan.hpp"
 #include "kernels.hpp"
