@@ -156,6 +156,7 @@ struct Attn4 {
     f4 o[NT][2 * NB];
     float bias[NT][TYPE == kKvQ4_1 ? NK : 1];                      // q4_1: sum p (m + 8 d)
     float m[NT], l[NT];
+    float kexp;                                                    // l, bias and o are 2^kexp times their sums (until finish)
     uint32_t magic;                                                // 0x64006400 (f16 1024) in a vector register
 
     __device__ __forceinline__ bool sees(int n, uint32_t c) const {
@@ -340,8 +341,7 @@ struct Attn4 {
     // The weights of a tile from its scores: s becomes p 2^k. MASKED when some row does not see all of it (or a mask is
     // given): vis gets the cells that the lane's row sees (bit 4 u + i: its cell i of group u). c0: the first cell.
     template <bool MASKED>
-    __device__ __forceinline__ void weights(const Attn4Args & a, f4 (&s)[NT][2], uint32_t (&vis)[NT], uint32_t c0, uint32_t lane,
-                                            float kexp) {
+    __device__ __forceinline__ void weights(const Attn4Args & a, f4 (&s)[NT][2], uint32_t (&vis)[NT], uint32_t c0, uint32_t lane) {
         const uint32_t g = lane >> 4;
         bool grow = false;
         float top[NT];
@@ -521,7 +521,7 @@ struct Attn4 {
     // The scores and the values of one tile, its registers loaded again from tile `ahead` behind their last use.
     template <bool WHOLE>
     __device__ __forceinline__ void one(const Attn4Args & a, Tl & k, Tl & v, uint32_t i, uint32_t ahead, const uint8_t * kp,
-                                        const uint8_t * vp, size_t pair, float kexp, const h8 * lds, uint32_t lane) {
+                                        const uint8_t * vp, size_t pair, const h8 * lds, uint32_t lane) {
         uint32_t ql = lane;                                        // q's pieces: read from LDS for every tile where registers
         if constexpr (D * NT > 128) asm volatile("" : "+v"(ql));   // would spill, kept where they do not
         f4 s[NT][2];
@@ -532,7 +532,7 @@ struct Attn4 {
 #pragma unroll                                                     // keep the products and scales of every block in registers)
             for (int n = 0; n < NT; ++n) asm volatile("" : "+v"(s[n][0]), "+v"(s[n][1]));
         load<false>(k, kp + c, pair, lane);
-        weights<!WHOLE>(a, s, vis, 32u * i, lane, kexp);
+        weights<!WHOLE>(a, s, vis, 32u * i, lane);
         values<!WHOLE>(v, s, vis);
         load<true>(v, vp + c, pair, lane);
     }
@@ -546,7 +546,7 @@ struct Attn4 {
         // 2^k: the largest |d| of the V plane times 2^k in [2^8, 2^9) (an infinite one counts as the largest finite), k <= 9
         const uint32_t dm = *(const uint32_t *)a.v;
         const float top = (float)__builtin_bit_cast(_Float16, (uint16_t)min(dm, 0x7BFFu));
-        const float kexp = top == 0.0f ? 0.0f : (float)min(8 - ((int)(fb(top) >> 23) - 127), 9);
+        kexp = top == 0.0f ? 0.0f : (float)min(8 - ((int)(fb(top) >> 23) - 127), 9);
         Span w0, w1, all;
         spans(a, w0, w1, all);
         const uint32_t n0 = w0.size(), nw = n0 + w1.size();
@@ -566,10 +566,10 @@ struct Attn4 {
         }
         load_queries(a.scale, lane, lds, wave);
         __syncthreads();
-        if (odd) one<true>(a, k1, v1, nth(0u), nth(2u), kp, vp, pair, kexp, lds, lane);
+        if (odd) one<true>(a, k1, v1, nth(0u), nth(2u), kp, vp, pair, lds, lane);
         for (uint32_t x = odd; x < cnt; x += AHEAD) {
-            one<true>(a, k0, v0, nth(x), nth(x + AHEAD), kp, vp, pair, kexp, lds, lane);
-            if constexpr (AHEAD == 2) one<true>(a, k1, v1, nth(x + 1u), nth(x + 3u), kp, vp, pair, kexp, lds, lane);
+            one<true>(a, k0, v0, nth(x), nth(x + AHEAD), kp, vp, pair, lds, lane);
+            if constexpr (AHEAD == 2) one<true>(a, k1, v1, nth(x + 1u), nth(x + 3u), kp, vp, pair, lds, lane);
         }
         // the others: the hull without w0 and w1, dealt on from the wave after the one that took the last whole tile
         const uint32_t g0 = w0.lo - all.lo, g1 = g0 + (w1.lo - w0.hi), np = all.size() - nw;
@@ -583,17 +583,20 @@ struct Attn4 {
         for (;;) {
             uint32_t nx = x + parts;
             while (nx < np && !any(other(nx))) nx += parts;
-            one<false>(a, k0, v0, other(x), other(nx < np ? nx : x), kp, vp, pair, kexp, lds, lane);
+            one<false>(a, k0, v0, other(x), other(nx < np ? nx : x), kp, vp, pair, lds, lane);
             if (nx >= np) break;
             x = nx;
         }
     }
 
-    // Rows summed over their lanes; o becomes sum p v (2^k times), value 32 b + 16 c + 4 g + i in o[2 b + c][i].
+    // Rows summed over their lanes; o becomes sum p v, value 32 b + 16 c + 4 g + i in o[2 b + c][i]. What leaves the wave
+    // carries no 2^k: waves that read the header at different times (a store into other cells may raise it while the call
+    // runs) differ in it, and the joins weigh by the maxima alone.
     __device__ __forceinline__ void finish() {
+        const float unit = __builtin_ldexpf(1.0f, -(int)kexp);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            l[n] = rows_sum(l[n]);
+            l[n] = rows_sum(l[n]) * unit;
             if constexpr (TYPE == kKvQ4_1)
 #pragma unroll
                 for (int k = 0; k < NK; ++k) {
@@ -601,6 +604,8 @@ struct Attn4 {
 #pragma unroll
                     for (int j = 2 * C * k; j < 2 * C * (k + 1); ++j) o[n][j] += z;
                 }
+#pragma unroll
+            for (int j = 0; j < 2 * NB; ++j) o[n][j] *= unit;
         }
     }
 };
