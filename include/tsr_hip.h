@@ -356,7 +356,9 @@ int tsr_hip_flash_attn_noalloc(tsr_hip_ctx * ctx, const float * q_dev, uint32_t 
 
 /* FLASH_ATTN_EXT over a 4-bit cache (TSR_HIP_KV_Q4_0 / _Q4_1; no counterpart in the reference, whose cache is
  * q8_0): out = softmax(scale q K^T + mask) V on the values that the blocks stand for, f32 queries and
- * results, in f32 arithmetic (q and the weights p enter the matrix cores as two f16 pieces of 22 bits).
+ * results, in f32 arithmetic, but that two operands enter the matrix cores as two f16 pieces: q with 22 bits of its row's
+ * largest value, and each weight times a V block's d with 22 bits, or 2^-30 of the largest |d| that the row sees in its KV
+ * head where that is more.
  *   q_dev, out_dev  as tsr_hip_flash_attn; 16-byte aligned, strides multiples of 4
  *   kc, vc          caches of one 4-bit type, E = n_head_kv * D
  *   n_kv            cells of the caches that the call may touch, <= kv_size (0: every row is empty)
@@ -370,10 +372,10 @@ int tsr_hip_flash_attn_noalloc(tsr_hip_ctx * ctx, const float * q_dev, uint32_t 
  *                   graph capture a call whose workspace is not of 0 bytes needs one here (else
  *                   TSR_HIP_E_ARG): graphs that may run at once take one each.
  * A row that sees no cell (or whose scores are all -inf) is 0. What a cell holds that a row does not see
- * (infinities and NaN too) does not reach the row. The masks and runs are read when the kernels run: a captured
- * call replays over what they hold then, within its n_kv. D in {64, 128, 256, 512}, n_head % n_head_kv == 0,
- * n_head / n_head_kv <= 64, n_head D <= 32768, T <= 65535; scale finite, normal and > 0. Results do not depend
- * on the order in which workgroups run. */
+ * (infinities and NaN too) does not reach the row, nor its precision; it may be written meanwhile. The masks and
+ * runs are read when the kernels run: a captured call replays over what they hold then, within its n_kv. D in
+ * {64, 128, 256, 512}, n_head % n_head_kv == 0, n_head / n_head_kv <= 64, n_head D <= 32768, T <= 65535; scale
+ * finite, normal and > 0. Results do not depend on the order in which workgroups run. */
 int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const tsr_hip_kv * kc,
                            const tsr_hip_kv * vc, uint32_t D, uint32_t n_head, uint32_t n_head_kv, float scale,
                            uint32_t n_kv, const uint32_t * runs_dev, const uint16_t * mask_f16_dev, uint64_t mask_stride,

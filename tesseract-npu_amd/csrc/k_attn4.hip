@@ -10,9 +10,13 @@
 //            permuted, the second operand of the next product: P stays where it is.
 //   P V      O^T[value][row]: the first operand are n - 8 again, the second p d[cell] of a block in two f16 pieces, f16(p) d
 //            rounded once and what p d leaves of it. Sums of raw codes would be large and nearly cancel: an error that grows
-//            with the root of the cells. p carries 2^k with 2^k max|d| in [2^8, 2^9) from the plane's header (k at most 9) and
-//            is at most 2^6 (the maximum follows when it is passed by that), so that no piece overflows and the pieces keep
-//            2^-33 of the largest. q4_1: sum p (m + 8 d) is summed aside in f32.
+//            with the root of the cells. p d carries 2^e with 2^e max|d| in [2^5, 2^9), max|d| the largest finite scale that
+//            the row has seen so far, followed like the maximum of its scores; p takes k = min(e, 9) of it and d, exactly, the
+//            rest. p is at most 2^6 (the maximum follows when it is passed by that), so that no piece overflows and the
+//            pieces keep 2^-30 of the largest. What a row does not see has no part in e: cells of other rows, heads and
+//            times change no result's precision. Following e takes 1 to 3 % of a call (512 tokens behind 1536 cells 48.9 ->
+//            49.8 us, a token behind 8192 cells 12.7 -> 13.0; heads of 512 over q4_1 up to 17 %, whose registers spill).
+//            q4_1: sum p (m + 8 d) is summed aside in f32.
 // The scales meet the f32 sums only, where a cell that its row does not see is replaced by nothing: an infinity or a
 // NaN in a masked cell reaches no result. Sums, maxima and results are f32; both splits keep 22 bits of f32's 24.
 //
@@ -113,6 +117,33 @@ __device__ __forceinline__ void all_cells(uint32_t w, uint32_t (&x)[2][4]) {
     x[1][0] = from_row<4>(w); x[1][1] = from_row<5>(w); x[1][2] = from_row<6>(w); x[1][3] = from_row<7>(w);
 }
 
+// The scales of two cells by their size (|d|'s bits), without those that are not finite where FINITE.
+typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u2 larger(u2 a, u2 b) { return __builtin_elementwise_max(a, b); }
+__device__ __forceinline__ uint32_t larger(u2 a) { return max((uint32_t)a[0], (uint32_t)a[1]); }
+template <bool FINITE>
+__device__ __forceinline__ u2 sizes(uint32_t w) {
+    u2 x = __builtin_bit_cast(u2, w & 0x7FFF7FFFu);
+    if constexpr (FINITE) x = u2{ x[0] < 0x7C00u ? x[0] : (uint16_t)0u, x[1] < 0x7C00u ? x[1] : (uint16_t)0u };
+    return x;
+}
+// e of a largest scale: the largest of 21, 17 .. 9 .. -7 with 2^e |d| < 2^9 (steps of 2^4, so that it seldom changes). A wave starts
+// with 9, right for 2^-4 <= |d| < 1. The least size for which e is too large, and whether one is small enough for the next.
+constexpr int kMostE = 21, kMostK = 9, kFirstE = 9;
+__device__ __forceinline__ int e_of(uint32_t size) { return ((30 - (int)(size >> 10)) & ~3) - 7; }
+__device__ __forceinline__ uint32_t beyond(int e) { return (uint32_t)(24 - e) << 10; }
+__device__ __forceinline__ bool below(uint32_t size, int e) { return e < kMostE && size < beyond(e + 4); }
+__device__ __forceinline__ int k_of(int e) { return min(e, kMostK); }
+// 2^(e - k), as an f16 pair
+__device__ __forceinline__ h2 rest_of(int e) {
+    return __builtin_bit_cast(h2, (uint32_t)(15 + e - k_of(e)) * 0x04000400u);
+}
+__device__ __forceinline__ uint32_t rows_max_u(uint32_t x) {      // over the four lanes that hold one row
+    auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(b[0], b[1]);
+}
 // The token of row r of a KV head: r / G by a product (r < 2^22, G <= 64: exact).
 __device__ __forceinline__ uint32_t token(const Attn4Args & a, uint32_t r) {
     return a.T == 1u ? 0u : a.inv_G == 0u ? r : __umulhi(r, a.inv_G);
@@ -126,6 +157,13 @@ __device__ __forceinline__ uint32_t rows16_min(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
 }
 __device__ __forceinline__ uint32_t rows16_max(uint32_t v) { return ~rows16_min(~v); }
+// Maximum over the C columns of a row (aligned groups of C lanes).
+template <int C>
+__device__ __forceinline__ uint32_t columns_max(uint32_t x) {
+    if constexpr (C >= 2) x = max(x, (uint32_t)dpp_i<kDppXor1>((int)x));
+    if constexpr (C >= 4) x = max(x, (uint32_t)dpp_i<kDppXor2>((int)x));
+    return x;
+}
 // Sum over the C columns of a row (aligned groups of C lanes).
 template <int C>
 __device__ __forceinline__ float columns_sum(float x) {
@@ -156,7 +194,7 @@ struct Attn4 {
     f4 o[NT][2 * NB];
     float bias[NT][TYPE == kKvQ4_1 ? NK : 1];                      // q4_1: sum p (m + 8 d)
     float m[NT], l[NT];
-    float kexp;                                                    // l, bias and o are 2^kexp times their sums (until finish)
+    int e[NT];                                                     // o is 2^e, l and bias are 2^min(e, 9) times their sums (until finish)
     uint32_t magic;                                                // 0x64006400 (f16 1024) in a vector register
 
     __device__ __forceinline__ bool sees(int n, uint32_t c) const {
@@ -338,13 +376,60 @@ struct Attn4 {
         }
     }
 
-    // The weights of a tile from its scores: s becomes p 2^k. MASKED when some row does not see all of it (or a mask is
-    // given): vis gets the cells that the lane's row sees (bit 4 u + i: its cell i of group u). c0: the first cell.
+    // The scales' sizes of a tile of V: of the lane's cells 2 x, 2 x + 1 (MASKED, C > 1), or of all that the lane holds.
     template <bool MASKED>
-    __device__ __forceinline__ void weights(const Attn4Args & a, f4 (&s)[NT][2], uint32_t (&vis)[NT], uint32_t c0, uint32_t lane) {
+    using Sizes = u2[MASKED || C > 1 ? 4 : 1];
+    template <bool MASKED, bool FINITE>
+    static __device__ __forceinline__ void sizes_of(const Tl & v, Sizes<MASKED> & size) {
+        if constexpr (C > 1) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                size[x] = sizes<FINITE>(v.dk(0, x));
+#pragma unroll
+                for (int y = 1; y < NK; ++y) size[x] = larger(size[x], sizes<FINITE>(v.dk(y, x)));
+            }
+        } else {
+            size[0] = sizes<FINITE>(v.d[0]);
+#pragma unroll
+            for (int j = 1; j < D / 64; ++j) size[0] = larger(size[0], sizes<FINITE>(v.d[j]));
+            if constexpr (MASKED) {
+                uint32_t z = __builtin_bit_cast(uint32_t, size[0]);    // (the other block of a pair is four lanes on in a row)
+                z = __builtin_bit_cast(uint32_t, larger(size[0], __builtin_bit_cast(u2, (uint32_t)__builtin_amdgcn_mov_dpp((int)z, 0x124, 0xF, 0xF, true))));
+                size[0] = __builtin_bit_cast(u2, from_row<0>(z));
+                size[1] = __builtin_bit_cast(u2, from_row<1>(z));
+                size[2] = __builtin_bit_cast(u2, from_row<2>(z));
+                size[3] = __builtin_bit_cast(u2, from_row<3>(z));
+            }
+        }
+    }
+
+    // The bits of the lane's cells 2 x, 2 x + 1 that its row sees, as a mask of halves.
+    static __device__ __forceinline__ uint32_t cells_in(uint32_t vis, int x) {
+        return ((vis >> (2 * x)) & 1u ? 0x0000FFFFu : 0u) | ((vis >> (2 * x)) & 2u ? 0xFFFF0000u : 0u);
+    }
+    // The largest of them; of the cells that the lane's row sees.
+    template <bool MASKED>
+    static __device__ __forceinline__ uint32_t all_of(const Sizes<MASKED> & size) {
+        if constexpr (C > 1) return larger(larger(larger(size[0], size[1]), larger(size[2], size[3])));
+        else return larger(size[0]);
+    }
+    static __device__ __forceinline__ uint32_t all_seen(const Sizes<true> & size, uint32_t vis) {
+        u2 z = { 0, 0 };
+#pragma unroll
+        for (int y = 0; y < 4; ++y) z = larger(z, __builtin_bit_cast(u2, __builtin_bit_cast(uint32_t, size[y]) & cells_in(vis, y)));
+        return larger(z);
+    }
+    // The weights of a tile from its scores: s becomes p 2^k. MASKED when some row does not see all of it (or a mask is
+    // given): vis gets the cells that the lane's row sees (bit 4 u + i: its cell i of group u). c0: the first cell. A larger
+    // maximum of the scores, or of the scales of V that a row sees, shrinks what is summed so far: `whole` is e of the
+    // tiles that every row sees, the same for all of them.
+    template <bool MASKED>
+    __device__ __forceinline__ void weights(const Attn4Args & a, f4 (&s)[NT][2], uint32_t (&vis)[NT], const Tl & v, const Sizes<MASKED> & size,
+                                            int & whole, bool & first, uint32_t c0, uint32_t lane) {
         const uint32_t g = lane >> 4;
         bool grow = false;
         float top[NT];
+        if constexpr (!MASKED) grow = all_of<false>(size) >= beyond(whole);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             vis[n] = 0xFFu;
@@ -379,12 +464,15 @@ struct Attn4 {
             x = fmaxf(x, fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
             top[n] = MASKED ? x : x * csc[n];
             grow |= top[n] > m[n] + kSlack;
+            if constexpr (MASKED) grow |= all_seen(size, vis[n]) >= beyond(e[n]);
         }
-        if (__ballot(grow)) {                                      // a larger maximum: what is summed so far shrinks
+        if (__ballot(grow)) {
+            bool fresh[NT];                                        // nothing was summed yet
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float mn = fmaxf(m[n], rows_max(top[n]));
                 const float f = mn == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+                fresh[n] = m[n] == -__builtin_inff() && mn != m[n];
                 m[n] = mn;
                 l[n] *= f;
 #pragma unroll
@@ -392,10 +480,48 @@ struct Attn4 {
 #pragma unroll
                 for (int j = 0; j < 2 * NB; ++j) o[n][j] *= f;
             }
+            bool other;                                            // another e for a row, perhaps
+            if constexpr (MASKED) {
+                other = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint32_t z = columns_max<C>(rows_max_u(all_seen(size, vis[n])));
+                    other |= z >= beyond(e[n]) || (fresh[n] && below(z, e[n]));
+                }
+                other = __ballot(other) != 0ull;
+            } else {
+                const uint32_t z = all_of<false>(size);
+                other = __ballot(z >= beyond(whole)) != 0ull || (first && __ballot(!below(z, whole)) == 0ull);
+            }
+            if (other) {
+                Sizes<MASKED> finite;
+                sizes_of<MASKED, true>(v, finite);
+                const int was = whole;
+                if constexpr (!MASKED) {
+                    whole = e_of(rows16_max(rows_max_u(all_of<false>(finite))));
+                    if (!first) whole = min(whole, was);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    int e0 = was, e1 = whole;
+                    if constexpr (MASKED) {
+                        e0 = e[n];
+                        e1 = e_of(columns_max<C>(rows_max_u(all_seen(finite, vis[n]))));
+                        e[n] = e1 = fresh[n] ? e1 : min(e0, e1);
+                    }
+                    const float fk = __builtin_ldexpf(1.0f, k_of(e1) - k_of(e0)), fe = __builtin_ldexpf(1.0f, e1 - e0);
+                    l[n] *= fk;
+#pragma unroll
+                    for (int k = 0; k < (TYPE == kKvQ4_1 ? NK : 1); ++k) bias[n][k] *= fk;
+#pragma unroll
+                    for (int j = 0; j < 2 * NB; ++j) o[n][j] *= fe;
+                }
+            }
+            first = false;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float sub = kexp - (m[n] == -__builtin_inff() ? 0.0f : m[n]), unit = MASKED ? 1.0f : csc[n];
+            const float sub = (float)k_of(MASKED ? e[n] : whole) - (m[n] == -__builtin_inff() ? 0.0f : m[n]), unit = MASKED ? 1.0f : csc[n];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -407,27 +533,38 @@ struct Attn4 {
     }
 
     template <bool MASKED>
-    __device__ __forceinline__ void values(const Tl & v, const f4 (&s)[NT][2], const uint32_t (&vis)[NT]) {
+    __device__ __forceinline__ void values(const Tl & v, const f4 (&s)[NT][2], const uint32_t (&vis)[NT], int whole) {
+        // the scales times their part of 2^e: a tile's, or where the rows differ in it a row's
+        h2 rest[NT];
+        float eight[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int en = MASKED ? e[n] : whole;
+            rest[n] = rest_of(en);
+            eight[n] = __builtin_ldexpf(8.0f, k_of(en) - en);
+        }
+        auto scaled = [&](uint32_t d, int n) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, d) * rest[n]); };
+        auto of_tile = [&](uint32_t d) { return MASKED ? d : scaled(d, 0); };
         uint32_t p16[NT][4], in[NT][4];                            // of the cells 2 x, 2 x + 1 of the lane's eight
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 p16[n][x] = pair_of(s[n][x >> 1][2 * (x & 1)], s[n][x >> 1][2 * (x & 1) + 1]);
-                in[n][x] = ((vis[n] >> (2 * x)) & 1u ? 0x0000FFFFu : 0u) | ((vis[n] >> (2 * x)) & 2u ? 0xFFFF0000u : 0u);
+                in[n][x] = cells_in(vis[n], x);
             }
         // the pieces of the weights times the scales of a block, {d, d of the next cell} in d and {m, m} in mm
         auto pieces = [&](int n, int k, const uint32_t (&dd)[4], const uint32_t (&mm)[4], uint32_t (&ph)[4], uint32_t (&pl)[4]) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const float p0 = s[n][x >> 1][2 * (x & 1)], p1 = s[n][x >> 1][2 * (x & 1) + 1];
-                const uint32_t d = MASKED ? dd[x] & in[n][x] : dd[x];
+                const uint32_t d = MASKED ? scaled(dd[x] & in[n][x], n) : dd[x];
                 ph[x] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, p16[n][x]) * __builtin_bit_cast(h2, d));
                 pl[x] = pair_of(__builtin_fmaf(p0, half_of(d, 0), -half_of(ph[x], 0)), __builtin_fmaf(p1, half_of(d, 1), -half_of(ph[x], 1)));
                 if constexpr (TYPE == kKvQ4_1) {
                     const uint32_t m = MASKED ? mm[x] & in[n][x] : mm[x];
-                    bias[n][k] = __builtin_fmaf(p0, __builtin_fmaf(half_of(d, 0), 8.0f, half_of(m, 0)), bias[n][k]);
-                    bias[n][k] = __builtin_fmaf(p1, __builtin_fmaf(half_of(d, 1), 8.0f, half_of(m, 1)), bias[n][k]);
+                    bias[n][k] = __builtin_fmaf(p0, __builtin_fmaf(half_of(d, 0), eight[n], half_of(m, 0)), bias[n][k]);
+                    bias[n][k] = __builtin_fmaf(p1, __builtin_fmaf(half_of(d, 1), eight[n], half_of(m, 1)), bias[n][k]);
                 }
             }
         };
@@ -448,7 +585,7 @@ struct Attn4 {
         if constexpr (C > 1) {
 #pragma unroll
             for (int y = 0; y < NK; ++y) {
-                const uint32_t dd[4] = { v.dk(y, 0), v.dk(y, 1), v.dk(y, 2), v.dk(y, 3) };
+                const uint32_t dd[4] = { of_tile(v.dk(y, 0)), of_tile(v.dk(y, 1)), of_tile(v.dk(y, 2)), of_tile(v.dk(y, 3)) };
                 uint32_t mm[4] = {};
                 if constexpr (TYPE == kKvQ4_1)
 #pragma unroll
@@ -462,7 +599,7 @@ struct Attn4 {
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
                 uint32_t dw[2][4], mw[2][4] = {};
-                all_cells(v.d[j], dw);
+                all_cells(of_tile(v.d[j]), dw);
                 if constexpr (TYPE == kKvQ4_1) all_cells(v.m[j], mw);
 #pragma unroll
                 for (int bb = 0; bb < 2; ++bb) {
@@ -521,19 +658,31 @@ struct Attn4 {
     // The scores and the values of one tile, its registers loaded again from tile `ahead` behind their last use.
     template <bool WHOLE>
     __device__ __forceinline__ void one(const Attn4Args & a, Tl & k, Tl & v, uint32_t i, uint32_t ahead, const uint8_t * kp,
-                                        const uint8_t * vp, size_t pair, const h8 * lds, uint32_t lane) {
+                                        const uint8_t * vp, size_t pair, int & whole, bool & first, const h8 * lds, uint32_t lane) {
         uint32_t ql = lane;                                        // q's pieces: read from LDS for every tile where registers
         if constexpr (D * NT > 128) asm volatile("" : "+v"(ql));   // would spill, kept where they do not
         f4 s[NT][2];
         uint32_t vis[NT];
         const size_t c = (size_t)ahead * kv4_tile_bytes(TYPE);
+        Sizes<!WHOLE> size;
+        sizes_of<!WHOLE, false>(v, size);
         scores(k, lds + ql, s);
         if constexpr (!WHOLE)                                      // (made here: moved behind the mask's branches they would
 #pragma unroll                                                     // keep the products and scales of every block in registers)
             for (int n = 0; n < NT; ++n) asm volatile("" : "+v"(s[n][0]), "+v"(s[n][1]));
         load<false>(k, kp + c, pair, lane);
-        weights<!WHOLE>(a, s, vis, 32u * i, lane);
-        values<!WHOLE>(v, s, vis);
+        weights<!WHOLE>(a, s, vis, v, size, whole, first, 32u * i, lane);
+        if constexpr (C == 1) {                                    // (from here on: scaled and spread before the softmax they would
+#pragma unroll                                                     // take registers of every block)
+            for (int j = 0; j < D / 64; ++j) asm volatile("" : "+v"(v.d[j]));
+        } else {
+#pragma unroll
+            for (int y = 0; y < NK; ++y)
+#pragma unroll
+                for (int z = 0; z < (TYPE == kKvQ4_1 ? 2 : 1); ++z)
+                    asm volatile("" : "+v"(v.sc[y][z].x), "+v"(v.sc[y][z].y), "+v"(v.sc[y][z].z), "+v"(v.sc[y][z].w));
+        }
+        values<!WHOLE>(v, s, vis, whole);
         load<true>(v, vp + c, pair, lane);
     }
     // The tiles that the rows see, every parts-th: those that all rows see whole with the next AHEAD tiles loaded ahead,
@@ -543,10 +692,6 @@ struct Attn4 {
         constexpr size_t tb = kv4_tile_bytes(TYPE);
         const size_t pair = (size_t)a.n_tiles * tb;
         const uint8_t * kp = a.k + kKv4Header + (size_t)h * (D / 64) * pair, * vp = a.v + kKv4Header + (size_t)h * (D / 64) * pair;
-        // 2^k: the largest |d| of the V plane times 2^k in [2^8, 2^9) (an infinite one counts as the largest finite), k <= 9
-        const uint32_t dm = *(const uint32_t *)a.v;
-        const float top = (float)__builtin_bit_cast(_Float16, (uint16_t)min(dm, 0x7BFFu));
-        kexp = top == 0.0f ? 0.0f : (float)min(8 - ((int)(fb(top) >> 23) - 127), 9);
         Span w0, w1, all;
         spans(a, w0, w1, all);
         const uint32_t n0 = w0.size(), nw = n0 + w1.size();
@@ -566,11 +711,15 @@ struct Attn4 {
         }
         load_queries(a.scale, lane, lds, wave);
         __syncthreads();
-        if (odd) one<true>(a, k1, v1, nth(0u), nth(2u), kp, vp, pair, lds, lane);
+        int whole_e = kFirstE;
+        bool first = true;                                         // no tile has been summed
+        if (odd) one<true>(a, k1, v1, nth(0u), nth(2u), kp, vp, pair, whole_e, first, lds, lane);
         for (uint32_t x = odd; x < cnt; x += AHEAD) {
-            one<true>(a, k0, v0, nth(x), nth(x + AHEAD), kp, vp, pair, lds, lane);
-            if constexpr (AHEAD == 2) one<true>(a, k1, v1, nth(x + 1u), nth(x + 3u), kp, vp, pair, lds, lane);
+            one<true>(a, k0, v0, nth(x), nth(x + AHEAD), kp, vp, pair, whole_e, first, lds, lane);
+            if constexpr (AHEAD == 2) one<true>(a, k1, v1, nth(x + 1u), nth(x + 3u), kp, vp, pair, whole_e, first, lds, lane);
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) e[n] = whole_e;
         // the others: the hull without w0 and w1, dealt on from the wave after the one that took the last whole tile
         const uint32_t g0 = w0.lo - all.lo, g1 = g0 + (w1.lo - w0.hi), np = all.size() - nw;
         uint32_t x = part + parts - nw % parts;
@@ -583,29 +732,28 @@ struct Attn4 {
         for (;;) {
             uint32_t nx = x + parts;
             while (nx < np && !any(other(nx))) nx += parts;
-            one<false>(a, k0, v0, other(x), other(nx < np ? nx : x), kp, vp, pair, lds, lane);
+            one<false>(a, k0, v0, other(x), other(nx < np ? nx : x), kp, vp, pair, whole_e, first, lds, lane);
             if (nx >= np) break;
             x = nx;
         }
     }
 
     // Rows summed over their lanes; o becomes sum p v, value 32 b + 16 c + 4 g + i in o[2 b + c][i]. What leaves the wave
-    // carries no 2^k: waves that read the header at different times (a store into other cells may raise it while the call
-    // runs) differ in it, and the joins weigh by the maxima alone.
+    // carries no power of two: waves differ in it, and the joins weigh by the maxima alone.
     __device__ __forceinline__ void finish() {
-        const float unit = __builtin_ldexpf(1.0f, -(int)kexp);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            const float unit = __builtin_ldexpf(1.0f, -k_of(e[n])), ounit = __builtin_ldexpf(1.0f, -e[n]);
             l[n] = rows_sum(l[n]) * unit;
+#pragma unroll
+            for (int j = 0; j < 2 * NB; ++j) o[n][j] *= ounit;
             if constexpr (TYPE == kKvQ4_1)
 #pragma unroll
                 for (int k = 0; k < NK; ++k) {
-                    const float z = rows_sum(bias[n][k]);          // (used where column and block belong together)
+                    const float z = rows_sum(bias[n][k]) * unit;   // (used where column and block belong together)
 #pragma unroll
                     for (int j = 2 * C * k; j < 2 * C * (k + 1); ++j) o[n][j] += z;
                 }
-#pragma unroll
-            for (int j = 0; j < 2 * NB; ++j) o[n][j] *= unit;
         }
     }
 };

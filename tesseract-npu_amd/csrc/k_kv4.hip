@@ -77,7 +77,6 @@ __global__ __launch_bounds__(256) void k_kv4_set_rows(Kv4Args a, uint32_t which,
                                                       uint32_t n_rows, const int64_t * idx, int32_t * bad) {
     const uint32_t r = blockIdx.y * kRowsPerWg + threadIdx.x / 8u, q = threadIdx.x & 7u, k = q & 3u;
     const uint32_t b = 2u * blockIdx.x + (q >> 2);
-    uint32_t dmax = 0u;
     if (r < n_rows) {
         const int64_t cell64 = idx[r];
         const float * row = src + (size_t)r * src_stride + 32u * b + 4u * k;
@@ -95,7 +94,6 @@ __global__ __launch_bounds__(256) void k_kv4_set_rows(Kv4Args a, uint32_t which,
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) t[kv4_code(1u, cell, b, 4u * k + i)] = (uint8_t)(w >> (8u * i));
-                dmax = d16 & 0x7FFFu;
             }
             if (k == 0u) {
                 uint16_t * sc = (uint16_t *)(t + kv4_scale(TYPE, cell, b));
@@ -104,8 +102,6 @@ __global__ __launch_bounds__(256) void k_kv4_set_rows(Kv4Args a, uint32_t which,
             }
         }
     }
-    if (which != 0u && dmax > __hip_atomic_load((uint32_t *)a.base, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-        atomicMax((uint32_t *)a.base, dmax);                       // rare once the plane has seen its values
 }
 
 // Stores past the caches: rows read back are not read again by these kernels.
@@ -197,16 +193,6 @@ __global__ __launch_bounds__(256) void k_kv4_bytes(Kv4Args a, uint32_t which, ui
     else stage[i] = *p;
 }
 
-// The largest |d| of cells [c0, c0 + n) joins the plane's (after bytes were written into a V plane): a thread a block.
-__global__ __launch_bounds__(256) void k_kv4_dmax(Kv4Args a, uint32_t c0, uint32_t n) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-    const uint32_t nb = a.E / 32u;
-    if (i >= (uint64_t)n * nb) return;
-    const uint32_t cell = c0 + (uint32_t)(i / nb), b = (uint32_t)(i % nb);
-    const uint32_t d = *(const uint16_t *)(a.base + kv4_tile(a.type, a.n_tiles, cell, b) + kv4_scale(a.type, cell, b)) & 0x7FFFu;
-    if (d > __hip_atomic_load((uint32_t *)a.base, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax((uint32_t *)a.base, d);
-}
-
 }  // namespace tsr
 
 static int launched() { return hipGetLastError() == hipSuccess ? 0 : -4; }
@@ -244,11 +230,5 @@ int tsr_launch_kv4_bytes(const tsr::Kv4Args & a, uint32_t which, uint64_t off, u
                          hipStream_t s) {
     if (n == 0u) return 0;
     hipLaunchKernelGGL(tsr::k_kv4_bytes, dim3((uint32_t)((n + 255u) / 256u)), dim3(256), 0, s, a, which, off, n, stage, to_dev);
-    if (to_dev && which == 1u) {
-        const uint64_t rowb = (uint64_t)(a.E / 32u) * tsr::kv4_block_bytes(a.type);
-        const uint64_t c0 = off / rowb, c1 = (off + n + rowb - 1u) / rowb, blocks = (c1 - c0) * (a.E / 32u);
-        hipLaunchKernelGGL(tsr::k_kv4_dmax, dim3((uint32_t)((blocks + 255u) / 256u)), dim3(256), 0, s, a, (uint32_t)c0,
-                           (uint32_t)(c1 - c0));
-    }
     return launched();
 }

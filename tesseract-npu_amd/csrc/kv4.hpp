@@ -4,10 +4,9 @@
 // A block is 32 consecutive values of a cell's row, as ggml lays it out: q4_0 {f16 d, 16 bytes} stands for
 // d (n - 8), q4_1 {f16 d, f16 m, 16 bytes} for d n + m; byte j holds n of value j (low nibble) and of value j + 16.
 //
-// Device layout of one plane: a header of 256 bytes (word 0: the largest |d| ever stored in a V plane, as f16 bits),
-// then for every pair of blocks (64 values of a row) a run of tiles of 32 cells, 1024 bytes of codes and 4 (q4_1: 8)
-// bytes of scales a cell. A tile is the operands of the matrix instruction 16x16x32 as its lanes hold them, so that a
-// wave loads them with full-width loads and unpacks them with a mask alone (k_attn4.hip):
+// Device layout of one plane: for every pair of blocks (64 values of a row) a run of tiles of 32 cells, 1024 bytes of
+// codes and 4 (q4_1: 8) bytes of scales a cell. A tile is the operands of the matrix instruction 16x16x32 as its lanes
+// hold them, so that a wave loads them with full-width loads and unpacks them with a mask alone (k_attn4.hip):
 //   K codes  [2 groups of 16 cells][lane 16 g + cell][2 blocks] words: bytes 4 g .. 4 g + 3 of the block
 //   V codes  [lane 16 g + j][2 blocks][2 groups of 16 cells] words: byte j of the block for cells 4 g + 0, 2, 1, 3
 //   scales   [g][2 blocks][2 groups of 16 cells][2] words {d of cell 4 g + 2 x, of the next one} (q4_1: and {m, m})
@@ -18,7 +17,7 @@
 
 namespace tsr {
 
-constexpr uint32_t kKv4Header = 256u;
+constexpr uint32_t kKv4Header = 0u;                // bytes in front of a plane's first tile
 __host__ __device__ constexpr uint32_t kv4_tile_bytes(uint32_t type) { return type == kKvQ4_1 ? 1280u : 1152u; }
 __host__ __device__ constexpr uint32_t kv4_block_bytes(uint32_t type) { return type == kKvQ4_1 ? 20u : 18u; }
 __host__ __device__ inline uint32_t kv4_tiles(uint32_t kv_size) { return (uint32_t)(((uint64_t)kv_size + 31u) / 32u); }
