@@ -119,8 +119,9 @@ int tsr_hip_kv_get_bytes(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t whic
     return kv_bytes(ctx, kv, which, off, dst, bytes, 0);
 }
 
-int tsr_hip_kv_set_rows(tsr_hip_ctx * ctx, tsr_hip_kv * kv, uint32_t which, const float * src_dev, uint32_t n_rows,
-                        uint64_t src_stride, const int64_t * idx_dev, int32_t * bad_dev, void * stream) {
+// Rows into the first `cells` cells of a cache: a row of a cell beyond them is stored nowhere.
+static int kv_set_rows(tsr_hip_ctx * ctx, tsr_hip_kv * kv, uint32_t cells, uint32_t which, const float * src_dev,
+                       uint32_t n_rows, uint64_t src_stride, const int64_t * idx_dev, int32_t * bad_dev, void * stream) {
     if (ctx == nullptr || kv == nullptr || src_dev == nullptr || idx_dev == nullptr || which > 1u) return TSR_HIP_E_ARG;
     if (n_rows == 0u) return TSR_HIP_OK;
     if (((uintptr_t)src_dev & 15u) != 0u || (n_rows > 1u && (src_stride % 4u != 0u || src_stride < kv->E)) ||
@@ -129,12 +130,22 @@ int tsr_hip_kv_set_rows(tsr_hip_ctx * ctx, tsr_hip_kv * kv, uint32_t which, cons
     std::lock_guard<std::mutex> lk(ctx->mtx);
     (void)hipSetDevice(ctx->device);
     ctx->ctr.set_rows_calls++;
-    const int rc = kv->type == TSR_HIP_KV_Q8_0
-                       ? tsr_launch_kv_set_rows(kv_args(kv), which, src_dev, n_rows, src_stride, idx_dev,
-                                                ctx->flag(bad_dev), ctx->pick(stream))
-                       : tsr_launch_kv4_set_rows(kv4_args(kv), which, src_dev, n_rows, src_stride, idx_dev,
-                                                 ctx->flag(bad_dev), ctx->pick(stream));
+    int rc;
+    if (kv->type == TSR_HIP_KV_Q8_0) {
+        tsr::KvArgs a = kv_args(kv);
+        a.kv_size = cells;
+        rc = tsr_launch_kv_set_rows(a, which, src_dev, n_rows, src_stride, idx_dev, ctx->flag(bad_dev), ctx->pick(stream));
+    } else {
+        tsr::Kv4Args a = kv4_args(kv);
+        a.kv_size = cells;
+        rc = tsr_launch_kv4_set_rows(a, which, src_dev, n_rows, src_stride, idx_dev, ctx->flag(bad_dev), ctx->pick(stream));
+    }
     return rc ? TSR_HIP_E_HIP : TSR_HIP_OK;
+}
+
+int tsr_hip_kv_set_rows(tsr_hip_ctx * ctx, tsr_hip_kv * kv, uint32_t which, const float * src_dev, uint32_t n_rows,
+                        uint64_t src_stride, const int64_t * idx_dev, int32_t * bad_dev, void * stream) {
+    return kv_set_rows(ctx, kv, kv != nullptr ? kv->kv_size : 0u, which, src_dev, n_rows, src_stride, idx_dev, bad_dev, stream);
 }
 
 int tsr_hip_kv_get_rows(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t which, const int64_t * idx_dev,
@@ -174,8 +185,9 @@ int tsr_hip_rope_kv(tsr_hip_ctx * ctx, float * qkv_dev, uint32_t T, uint64_t str
         int rc = tsr_hip_rope(ctx, qkv_dev, T, stride, head_dim, n_head + n_head_kv, n_dims, mode, pos_dev, freq_base, 1.0f,
                               attn_factor, nullptr, qkv_dev, stride, stream);
         const float * k = qkv_dev + (size_t)n_head * head_dim;
-        if (rc == 0) rc = tsr_hip_kv_set_rows(ctx, kc, TSR_HIP_KV_K, k, T, stride, cell_dev, bad_dev, stream);
-        if (rc == 0) rc = tsr_hip_kv_set_rows(ctx, vc, TSR_HIP_KV_V, k + E, T, stride, cell_dev, bad_dev, stream);
+        const uint32_t cells = std::min(kc->kv_size, vc->kv_size);
+        if (rc == 0) rc = kv_set_rows(ctx, kc, cells, TSR_HIP_KV_K, k, T, stride, cell_dev, bad_dev, stream);
+        if (rc == 0) rc = kv_set_rows(ctx, vc, cells, TSR_HIP_KV_V, k + E, T, stride, cell_dev, bad_dev, stream);
         return rc;
     }
     tsr::RopeKvArgs a{};
