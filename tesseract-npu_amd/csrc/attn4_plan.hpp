@@ -9,6 +9,13 @@ namespace tsr {
 
 constexpr uint32_t kSplitsMax = 256u;
 
+// The workspace of S splits of nr rows, in floats: the splits' rows of D values, which are read and written 16 bytes at a
+// time and so come first, behind them a (maximum, sum) each.
+constexpr size_t attn4_part_row(uint64_t nr, uint32_t D, uint32_t split, uint64_t row) { return (split * nr + row) * D; }
+constexpr size_t attn4_part_sum(uint64_t nr, uint32_t D, uint32_t S, uint32_t split, uint64_t row) {
+    return attn4_part_row(nr, D, S, 0u) + 2u * (split * nr + row);
+}
+
 struct Attn4Plan {
     uint32_t C;              // columns of the matrix instruction a row (k_attn4.hip): 16 / C rows a group
     uint32_t NT;             // groups of rows of a workgroup

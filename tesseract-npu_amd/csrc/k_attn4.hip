@@ -790,12 +790,12 @@ __global__ __launch_bounds__(256, waves_of(D, NT, C, TYPE)) void k_attn4(Attn4Ar
     // where row r's result goes: the output, or its place in the split's partial rows
     auto place = [&](uint32_t r) {
         const uint32_t t = token(a, r), hq = h * a.G + r - t * a.G;
-        return a.S > 1u ? a.part + 2u * a.S * nr + (split * nr + (size_t)t * nh + hq) * D
+        return a.S > 1u ? a.part + attn4_part_row(nr, D, split, (size_t)t * nh + hq)
                         : a.out + (size_t)t * a.out_stride + (size_t)hq * D;
     };
     auto sums = [&](uint32_t r, float m, float l) {
         const uint32_t t = token(a, r);
-        *(float2 *)(a.part + 2u * (split * nr + (size_t)t * nh + h * a.G + r - t * a.G)) = make_float2(m, l);
+        *(float2 *)(a.part + attn4_part_sum(nr, D, a.S, split, (size_t)t * nh + h * a.G + r - t * a.G)) = make_float2(m, l);
     };
     // the waves' sums joined
     static_assert(DC % 16u == 0u && D % DC == 0u, "whole groups of 16 values");
@@ -846,7 +846,7 @@ __global__ __launch_bounds__(256) void k_attn4_join(Attn4Args a) {
     __shared__ float wt[kSplitsMax], red[8];
     const uint32_t ro = blockIdx.x, nh = a.G * a.n_head_kv, tid = threadIdx.x, c = tid % W, s0 = tid / W;
     const size_t nr = (size_t)a.T * nh;
-    const float4 * po = (const float4 *)(a.part + 2u * a.S * nr + (size_t)ro * D) + c;
+    const float4 * po = (const float4 *)(a.part + attn4_part_row(nr, D, 0u, ro)) + c;
     float4 x[N];
     auto fetch = [&](uint32_t i0) {
 #pragma unroll
@@ -858,7 +858,7 @@ __global__ __launch_bounds__(256) void k_attn4_join(Attn4Args a) {
     fetch(0u);
     static_assert(kSplitsMax == 256u, "a thread a split");
     float2 e = make_float2(-__builtin_inff(), 0.0f);
-    if (tid < a.S) e = ((const float2 *)a.part)[tid * nr + ro];
+    if (tid < a.S) e = *(const float2 *)(a.part + attn4_part_sum(nr, D, a.S, tid, ro));
     float M = e.x;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));

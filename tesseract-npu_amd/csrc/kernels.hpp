@@ -111,7 +111,7 @@ struct Attn4Args {
     uint32_t mask_by4;       // four of its values, from a multiple of four on, are 8-byte aligned
     float * out;             // [T][n_head][D], token t at out + t * out_stride
     uint64_t out_stride;
-    float * part;            // S > 1: [split][T n_head] (maximum, sum), then [split][T n_head][D] unnormalised rows
+    float * part;            // S > 1: [split][T n_head][D] unnormalised rows, then [split][T n_head] (maximum, sum)
     uint32_t type, D, T, G, n_head_kv, n_kv, n_tiles;
     uint32_t inv_G;          // floor(2^32 / G) + 1 (G 1: 0)
     uint32_t S;              // splits of the cells

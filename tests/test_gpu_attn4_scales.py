@@ -80,9 +80,10 @@ def test_stores_into_other_cells_meanwhile(dev, typ):
     other.close()
 
 
-SHAPES = [  # n_head, n_head_kv, D, T, n_kv: one and several tokens, cells in splits and not, several columns a row and one
+SHAPES = [  # n_head, n_head_kv, D, T, n_kv: one and several tokens, cells in splits and not, several columns a row and one,
+            # an odd number of rows in an odd number of splits
     (32, 8, 128, 1, 8192), (14, 2, 64, 5, 3000), (32, 8, 128, 80, 1000), (8, 4, 256, 90, 500), (16, 1, 512, 3, 700),
-    (32, 8, 64, 600, 333),
+    (32, 8, 64, 600, 333), (7, 1, 64, 1, 1056),
 ]
 
 
