@@ -240,7 +240,7 @@ struct Attn4 {
             top = rows_max(top);
             if constexpr (D > 128) asm volatile("" : "+v"(q));     // (read again rather than kept: no registers for it)
             const int e = 140 - (int)(fb(top) >> 23);              // 2^e top in [2^13, 2^14)
-            csc[n] = __builtin_ldexpf(scale * kLog2e, -e);
+            csc[n] = __builtin_ldexpf(scale, -e) * kLog2e;         // (in this order: scale log2(e) may pass f32's range)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const float4 u = *(const float4 *)(q + 32 * b), v = *(const float4 *)(q + 32 * b + 16);
