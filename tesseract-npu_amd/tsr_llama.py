@@ -450,14 +450,16 @@ class LlamaDecoder:
         c, n = self.cfg, 256
         while n <= pos:
             n *= 2
-        self.n_kv_graph = min(n, self.kv_size)
         if self.graph is not None:         # (it reads the workspace)
             self.graph.free()
             self.graph = None
-        need = self.dev.flash_attn_kv4_ws(1, c.head_dim, c.n_head, c.n_head_kv, self.n_kv_graph)
         if self.ws is not None:
             self.ws.free()
+        self.ws, self.n_kv_graph = None, 0   # (until there is another: an allocation may fail)
+        n_kv = min(n, self.kv_size)
+        need = self.dev.flash_attn_kv4_ws(1, c.head_dim, c.n_head, c.n_head_kv, n_kv)
         self.ws = self.dev.alloc(need) if need else None
+        self.n_kv_graph = n_kv
         return True
 
     def step_graph(self, token: int | None, pos: int, n_kv: int | None = None) -> None:
