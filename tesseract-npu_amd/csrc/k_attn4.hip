@@ -760,8 +760,9 @@ struct Attn4 {
 
 constexpr uint32_t values_at_once(uint32_t D, uint32_t most) { return D <= most ? D : values_at_once(D / 2u, most); }
 
-// Waves a SIMD has registers for: the most that need no spills (q4_1's sums aside take up to 40 more: a third wave with
-// 12 registers spilled made 128 rows behind 3000 cells, D 128, 41 us and not 37).
+// Waves a SIMD that a kernel has registers for: the most that need no spills, but for heads of 512 over q4_1 with two columns a
+// row, which keep 78 of one wave's 512 in memory (the scales and sums of 16 blocks: 60 rows behind 500 cells, 8 heads on 1, 41
+// us against 30 over q4_0).
 constexpr int waves_of(int D, int NT, int C, uint32_t TYPE) {
     if (D * NT == 64) return 4;
     if (NT == 1 && (D == 128 ? C == 4 || (C == 1 && TYPE == kKvQ4_0) : D == 256 && C == 1 && TYPE == kKvQ4_0)) return 3;
