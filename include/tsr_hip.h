@@ -358,7 +358,7 @@ int tsr_hip_flash_attn_noalloc(tsr_hip_ctx * ctx, const float * q_dev, uint32_t 
  * q8_0): out = softmax(scale q K^T + mask) V on the values that the blocks stand for, f32 queries and
  * results, in f32 arithmetic, but that two operands enter the matrix cores as two f16 pieces: q with 22 bits of its row's
  * largest value, and each weight times a V block's d with 22 bits, or 2^-30 of the largest |d| that the row sees in its KV
- * head where that is more.
+ * head (at least 2^-46) where that is more. Scaled scores stay below 2^24 in magnitude.
  *   q_dev, out_dev  as tsr_hip_flash_attn; 16-byte aligned, strides multiples of 4
  *   kc, vc          caches of one 4-bit type, E = n_head_kv * D
  *   n_kv            cells of the caches that the call may touch, <= kv_size (0: every row is empty)

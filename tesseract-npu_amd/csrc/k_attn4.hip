@@ -20,11 +20,11 @@
 // The scales meet the f32 sums only, where a cell that its row does not see is replaced by nothing: an infinity or a
 // NaN in a masked cell reaches no result. Sums, maxima and results are f32; both splits keep 22 bits of f32's 24.
 //
-// Bound. Few rows: the cells' bytes and two launches: a token of 32 heads of 128 (8 KV heads) takes 12.8 us behind 8192
-// cells (a call of a graph of them: 6.5 the cells, 2.8 the join, the rest between launches) and 42 us behind 131071 of q4_1
-// (168 MB, 4.0 TB/s; a plain read of them 29 us). Many rows: vector instructions, about 130 a 16 x 16 tile of scores and
+// Bound. Few rows: the cells' bytes and two launches: a token of 32 heads of 128 (8 KV heads) takes 13.1 us behind 8192
+// cells (a call of a graph of them: 7 the cells, 2.8 the join, the rest between launches) and 43 us behind 131071 of q4_1
+// (168 MB, 3.9 TB/s; a plain read of them 29 us). Many rows: vector instructions, about 130 a 16 x 16 tile of scores and
 // D 128 (a third the unpacking, a quarter the pieces of p d) against 16 matrix instructions: 2048 tokens behind 6144
-// cells take 544 to 573 us (420 to 442 TFLOP/s), vector units 80 %, matrix units 35 % busy. Unpacking once for four waves through LDS,
+// cells take 553 to 574 us (418 to 435 TFLOP/s), vector units 80 %, matrix units 35 % busy. Unpacking once for four waves through LDS,
 // V in two pieces, left 270 vector instructions of 466 a tile of 32 rows and was no faster: with 239 registers two waves a
 // SIMD hide neither kind behind the other; four groups of rows a workgroup gave nothing.
 #include "attn4_plan.hpp"

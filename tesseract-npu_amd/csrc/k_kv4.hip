@@ -70,7 +70,7 @@ __device__ __forceinline__ uint32_t quantize4(float (&x)[8], uint32_t k, uint16_
     return w;
 }
 
-// SET_ROWS: workgroup (pair of blocks, 32 rows). Bound: the rows' bytes, 32768 rows of 1024 values in 25 us (6.1 TB/s); a
+// SET_ROWS: workgroup (pair of blocks, 32 rows). Bound: the rows' bytes, 32768 rows of 1024 values in 23 us (6.6 TB/s); a
 // launch for few rows.
 template <uint32_t TYPE>
 __global__ __launch_bounds__(256) void k_kv4_set_rows(Kv4Args a, uint32_t which, const float * src, uint64_t src_stride,
