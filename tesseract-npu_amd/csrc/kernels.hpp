@@ -221,6 +221,22 @@ struct RopeArgs {
     uint32_t fs;             // freq_scale != 1
 };
 
+// ROPE with positions scaled for long contexts (k_rope_scaled.hip): pair i turns by pos 2^(log2_step i) / ff[i] times
+// freq_scale (1 - w) + w, w = ext (1 - clamp((i - ramp_lo) / ramp_len, 0, 1)).
+struct RopeScaledArgs {
+    const float * x;         // head h of token t at x + t * x_stride + h * head_dim
+    uint64_t x_stride;
+    float * y;               // x itself, or apart from it
+    uint64_t y_stride;
+    const int32_t * pos;     // [T] positions, of either sign
+    const float * ff;        // nullable: [n_dims / 2] frequency factors
+    uint32_t head_dim, n_heads, n_dims, halves;
+    uint32_t units, inv_units;   // set by the launch: units of a head, floor(2^32 / units) + 1
+    double log2_step;        // -2 log2(base) / n_dims
+    double freq_scale, ext, ramp_lo, ramp_len;
+    double m;                // of cosine and sine
+};
+
 // ROPE of the q and k heads of a fused Q|K|V row, then SET_ROWS_KV of the rotated k and of v
 // (one workgroup per token). Token t's row is at qkv + t * stride: n_head q heads, n_head_kv k
 // heads, n_head_kv v heads of head_dim values; q and k are rotated in place.
@@ -274,6 +290,8 @@ int tsr_launch_rms_norm(const float * x, uint64_t x_stride, uint32_t n, uint32_t
                         const float * w, uint64_t w_stride, uint32_t w_period, float * y, uint64_t y_stride, hipStream_t s);
 int tsr_launch_rope(const tsr::RopeArgs & a, uint32_t T, hipStream_t s);
 int tsr_launch_rope_table(const int32_t * pos, uint32_t half, float ts, float m, float * tab, hipStream_t s);
+int tsr_launch_rope_scaled(tsr::RopeScaledArgs a, uint32_t T, hipStream_t s);
+int tsr_launch_rope_scaled_table(const tsr::RopeScaledArgs & a, float * tab, hipStream_t s);
 int tsr_launch_mm_epilogue(float * y, uint64_t y_stride, uint32_t N, uint32_t T, uint32_t mode, float fs, float sc,
                            const tsr::ExpkTab & ex, hipStream_t s);
 int tsr_launch_swiglu(const float * g, uint64_t g_stride, const float * u, uint64_t u_stride, float * y, uint64_t y_stride,

@@ -42,7 +42,18 @@ EXPORTS = (
     "tsr_hip_flash_attn_noalloc", "tsr_hip_get_flags", "tsr_hip_msum_mask_f32", "tsr_hip_attn_qkv_plan_rope_tab",
     "tsr_hip_fa_plan_set_epoch",
     "tsr_hip_kv_create_type", "tsr_hip_kv_get_rows", "tsr_hip_flash_attn_kv4", "tsr_hip_flash_attn_kv4_ws",
+    "tsr_hip_rope_scaled", "tsr_hip_rope_scaled_table",
 )
+
+
+class RopeScaling(C.Structure):
+    """tsr_hip_rope_scaling: how rotary positions are scaled beyond the trained length n_ctx_orig."""
+    _fields_ = [("freq_base", C.c_float), ("freq_scale", C.c_float), ("ext_factor", C.c_float), ("attn_factor", C.c_float),
+                ("beta_fast", C.c_float), ("beta_slow", C.c_float), ("n_ctx_orig", C.c_uint32)]
+
+    def __init__(self, freq_base: float = 10000.0, freq_scale: float = 1.0, ext_factor: float = 0.0, attn_factor: float = 1.0,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, n_ctx_orig: int = 0):
+        super().__init__(freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow, n_ctx_orig)
 
 
 class TsrHipError(RuntimeError):
@@ -131,6 +142,8 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         "tsr_hip_flash_attn_kv4": ([vp, vp, u32, u64, vp, vp, u32, u32, u32, C.c_float, u32, vp, vp, u64, vp, u64, vp, sz,
                                     vp], C.c_int),
         "tsr_hip_flash_attn_kv4_ws": ([vp, u32, u32, u32, u32, u32], sz),
+        "tsr_hip_rope_scaled": ([vp, vp, u32, u64, u32, u32, u32, C.c_int, vp, C.POINTER(RopeScaling), vp, vp, u64, vp], C.c_int),
+        "tsr_hip_rope_scaled_table": ([vp, vp, u32, C.POINTER(RopeScaling), vp, vp, vp], C.c_int),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -560,6 +573,17 @@ class Device:
         _check(self.L.tsr_hip_rope(self.ctx, self._p(x), T, x_stride, head_dim, n_heads, n_dims, mode, self._p(pos),
                                    float(freq_base), float(freq_scale), float(attn_factor), self._p(freq_factors),
                                    self._p(y), y_stride, stream), "rope")
+
+    def rope_scaled(self, x, T: int, x_stride: int, head_dim: int, n_heads: int, n_dims: int, mode: int, pos,
+                    scaling: RopeScaling, y, y_stride: int, freq_factors=None, stream=None) -> None:
+        """ROPE with positions scaled for long contexts (YaRN, interpolation, frequency factors); y may be x."""
+        _check(self.L.tsr_hip_rope_scaled(self.ctx, self._p(x), T, x_stride, head_dim, n_heads, n_dims, mode, self._p(pos),
+                                          C.byref(scaling), self._p(freq_factors), self._p(y), y_stride, stream), "rope_scaled")
+
+    def rope_scaled_table(self, pos, n_dims: int, scaling: RopeScaling, tab, freq_factors=None, stream=None) -> None:
+        """The angles of rope_scaled at *pos as a rope_table for flash_attn_plan_rope_tab and attn_qkv_plan_rope_tab."""
+        _check(self.L.tsr_hip_rope_scaled_table(self.ctx, self._p(pos), n_dims, C.byref(scaling), self._p(freq_factors),
+                                                self._p(tab), stream), "rope_scaled_table")
 
     def swiglu(self, g, g_stride: int, u, u_stride: int, n: int, rows: int, y, y_stride: int, stream=None) -> None:
         _check(self.L.tsr_hip_swiglu(self.ctx, self._p(g), g_stride, self._p(u), u_stride, n, rows, self._p(y),
