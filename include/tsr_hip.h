@@ -384,6 +384,22 @@ int tsr_hip_flash_attn_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, u
 size_t tsr_hip_flash_attn_kv4_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv,
                                  uint32_t n_kv);
 
+/* ---- sparse attention over a 4-bit cache ---------------------------------------------------------
+ * For a long context: attention of each token and KV head over a few blocks of `block` consecutive cells (a multiple of
+ * 32, <= 1024; block b: cells block b .. block (b + 1) - 1), those that can matter most by bounds of their keys. No counterpart in
+ * the reference. */
+
+/* The bounds: bounds_dev[(h * nb + b) * D + c] of KV head h, block b and channel c holds two bf16, in the low half the
+ * nearest not above the smallest, in the high half the nearest not below the largest of the block's values of that channel (nb =
+ * ceil(kv_size / block): of all blocks of the cache, kc->E * nb words, 16-byte aligned). kc: a 4-bit K cache; E a
+ * multiple of D, D in {64, 128, 256, 512}. Of the cells only those below n_kv (<= kv_size) count; cells_dev NULL: every block with
+ * one of them is made. cells_dev, two uint32 in device memory that are read when the kernel runs: {lo, hi}, only the blocks of cells
+ * lo .. hi - 1 are made, of their cells below hi, ends beyond n_kv cut to it; hi - lo <= n_new (>= 1; the blocks of cells further
+ * on are left as they were): what a decode loop's graph or a ubatch calls behind its SET_ROWS. A d or m that is not finite
+ * counts as the largest f16 of its sign (a NaN as the lowest), so that bounds are finite. */
+int tsr_hip_kv4_bounds(tsr_hip_ctx * ctx, const tsr_hip_kv * kc, uint32_t D, uint32_t block, uint32_t n_kv, uint32_t * bounds_dev,
+                       const uint32_t * cells_dev, uint32_t n_new, void * stream);
+
 /* ---- decode-layer glue ops ----------------------------------------------------------------------
  * The f32 ops around MUL_MAT and FLASH_ATTN in a decoder layer, on the vector unit's f32 rules
  * (every input denormal-as-zero, one IEEE round-to-nearest-even operation, result flushed to zero,

@@ -118,6 +118,16 @@ struct Attn4Args {
     float scale;
 };
 
+// The bounds of the blocks of a 4-bit K cache (k_kv4_bounds.hip).
+struct Kv4BoundsArgs {
+    const uint8_t * k;       // the plane
+    const uint32_t * cells;  // nullable: {lo, hi} the cells whose blocks are made anew, those from hi on not in use
+    uint32_t * bounds;       // [E / D][stride][D] words: lo in the low half, hi in the high half
+    uint32_t type, E, D, n_tiles, block, n_kv;
+    uint32_t n_blocks;       // of the grid
+    uint32_t stride;         // blocks of a head
+};
+
 // The work list of one call. Small lists (decode) travel inline in the kernel arguments; larger ones
 // are copied to device memory once per call and the kernels read them there (FaArgs::items != 0).
 struct FaPlan {
@@ -281,6 +291,7 @@ int tsr_launch_kv4_get_rows(const tsr::Kv4Args & a, uint32_t which, const int64_
                             uint64_t dst_stride, int32_t * bad, hipStream_t s);
 int tsr_launch_kv_get_rows(const tsr::KvArgs & a, uint32_t which, const int64_t * idx, uint32_t n_rows, float * dst,
                            uint64_t dst_stride, int32_t * bad, hipStream_t s);
+int tsr_launch_kv4_bounds(const tsr::Kv4BoundsArgs & a, hipStream_t s);
 // attention over a 4-bit cache, cut as attn4_plan.hpp says (k_attn4.hip)
 int tsr_launch_attn4(const tsr::Attn4Args & a, const tsr::Attn4Plan & p, hipStream_t s);
 int tsr_launch_fa(const tsr::FaArgs & a, const tsr::FaPlan & p, uint32_t T, uint32_t n_cu, hipStream_t s);

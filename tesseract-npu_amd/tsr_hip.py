@@ -43,6 +43,7 @@ EXPORTS = (
     "tsr_hip_fa_plan_set_epoch",
     "tsr_hip_kv_create_type", "tsr_hip_kv_get_rows", "tsr_hip_flash_attn_kv4", "tsr_hip_flash_attn_kv4_ws",
     "tsr_hip_rope_scaled", "tsr_hip_rope_scaled_table",
+    "tsr_hip_kv4_bounds",
 )
 
 
@@ -142,6 +143,7 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         "tsr_hip_flash_attn_kv4": ([vp, vp, u32, u64, vp, vp, u32, u32, u32, C.c_float, u32, vp, vp, u64, vp, u64, vp, sz,
                                     vp], C.c_int),
         "tsr_hip_flash_attn_kv4_ws": ([vp, u32, u32, u32, u32, u32], sz),
+        "tsr_hip_kv4_bounds": ([vp, vp, u32, u32, u32, vp, vp, u32, vp], C.c_int),
         "tsr_hip_rope_scaled": ([vp, vp, u32, u64, u32, u32, u32, C.c_int, vp, C.POINTER(RopeScaling), vp, vp, u64, vp], C.c_int),
         "tsr_hip_rope_scaled_table": ([vp, vp, u32, C.POINTER(RopeScaling), vp, vp, vp], C.c_int),
     }
@@ -477,6 +479,12 @@ class Device:
         _check(self.L.tsr_hip_flash_attn_kv4(self.ctx, self._p(q), T, q_stride, kc.h, vc.h, D, n_head, n_head_kv, scale,
                                              n_kv, self._p(runs), self._p(mask), mask_stride, self._p(out), out_stride,
                                              self._p(ws), 0 if ws is None else ws.nbytes, stream), "flash_attn_kv4")
+
+    def kv4_bounds(self, kc: KvCache, D: int, block: int, n_kv: int, bounds, cells=None, n_new: int = 0, stream=None) -> None:
+        """Smallest and largest values (bf16 pairs) of every channel over each block of a 4-bit K cache's cells: of all n_kv cells,
+        or of the blocks of at most n_new cells from cells[0] to cells[1] (device uint32)."""
+        _check(self.L.tsr_hip_kv4_bounds(self.ctx, kc.h, D, block, n_kv, self._p(bounds), self._p(cells), n_new, stream),
+               "kv4_bounds")
 
     def flash_attn(self, q, T: int, q_stride: int, kc: KvCache, vc: KvCache, D: int, n_head: int, n_head_kv: int,
                    scale: float, msum, out, out_stride: int, mask_f32=None, new_runs=None, stream=None) -> None:

@@ -1,0 +1,59 @@
+"""Block bounds, selection and attention over the selected blocks of 4-bit K caches in plain numpy."""
+import numpy as np
+
+import kv4_ref as R
+
+
+def bf16_down(x):
+    """The largest bf16 value that is not above x (f32 or exact f64 of f32), as f64."""
+    x = np.asarray(x, np.float64)
+    m, e = np.frexp(x)
+    return np.ldexp(np.floor(m * 256.0), e - 8)
+
+
+def bf16_up(x):
+    return -bf16_down(-np.asarray(x, np.float64))
+
+
+def bounds(values, D, block, n_kv=None):
+    """f32 values [cells, E] -> f64 [E / D, blocks, D] lo and hi of the blocks of the first n_kv cells."""
+    n_kv = values.shape[0] if n_kv is None else n_kv
+    E = values.shape[1]
+    lo, hi = [], []
+    for c0 in range(0, n_kv, block):
+        part = values[c0:min(n_kv, c0 + block)]
+        lo.append(bf16_down(part.min(0)))
+        hi.append(bf16_up(part.max(0)))
+    return (np.stack(x).reshape(-1, E // D, D).transpose(1, 0, 2) for x in (lo, hi))
+
+
+def words(w):
+    """uint32 words -> f64 lo, hi."""
+    w = np.ascontiguousarray(w, np.uint32)
+    return (w << np.uint32(16)).view(np.float32).astype(np.float64), (w & np.uint32(0xFFFF0000)).view(np.float32).astype(np.float64)
+
+
+def pack(lo, hi):
+    """The words of bf16 values."""
+    lo, hi = (np.ascontiguousarray(x, np.float32).view(np.uint32) for x in (lo, hi))
+    assert not ((lo | hi) & 0xFFFF).any()
+    return (lo >> np.uint32(16)) | hi
+
+
+def cache_rows(seed, n, E):
+    """K rows with channels of different sizes and signs, exact zeros and a drift along the cells."""
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((n, E)).astype(np.float32)
+    x[:, ::7] *= np.float32(5.0)
+    x[:, 3::11] = np.abs(x[:, 3::11])
+    x[:, 5::13] = 0.0
+    x += np.float32(0.7) * np.sin(np.arange(n) / 90.0)[:, None].astype(np.float32)
+    return x
+
+
+def fill(dev, x, typ, which=0, cells=None):
+    """A cache of the library that holds the image of x, and what it stands for (f32)."""
+    img = R.quantize(x, typ)
+    kv = dev.kv(x.shape[1], cells or x.shape[0], typ)
+    kv.set_bytes(which, img)
+    return kv, R.values_f32(img, typ)
