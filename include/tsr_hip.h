@@ -400,6 +400,23 @@ size_t tsr_hip_flash_attn_kv4_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t D, uint
 int tsr_hip_kv4_bounds(tsr_hip_ctx * ctx, const tsr_hip_kv * kc, uint32_t D, uint32_t block, uint32_t n_kv, uint32_t * bounds_dev,
                        const uint32_t * cells_dev, uint32_t n_new, void * stream);
 
+/* The selection: blocks_dev[(t * n_head_kv + h) * n_sel + i] (int32) for token t and KV head h, ascending, -1 behind the last. A token's
+ * candidates are the blocks with a cell that it sees: of runs_dev's two runs a token as tsr_hip_flash_attn_kv4 takes
+ * them (NULL: all n_kv cells). Where they are more than n_sel, the n_first lowest and the n_last highest are taken (a context's
+ * start, its newest cells; n_first + n_last <= n_sel) and of the others those with the largest scores: max over the KV
+ * head's query heads of sum over channels of max(q lo, q hi), at least the score of each of the block's cells; in f64, so
+ * that sums' rounding decides between no two blocks but equal ones, of which the lowest is taken (a score that is NaN is the lowest).
+ *   q_dev          as tsr_hip_flash_attn_kv4; 16-byte aligned, the stride a multiple of 4
+ *   bounds_dev     as tsr_hip_kv4_bounds, bounds_blocks >= ceil(n_kv / block) blocks a head (that entry point's nb)
+ *   ws_dev         tsr_hip_kv4_select_ws(...) bytes, with tsr_hip_flash_attn_kv4's rules (never of 0 bytes); the
+ *                  workspace of this call may be that of the attention behind it
+ * D, heads, T <= 65535 as tsr_hip_flash_attn_kv4; 1 <= n_sel <= 65536. */
+int tsr_hip_kv4_select(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const uint32_t * bounds_dev,
+                       uint32_t bounds_blocks, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t block, uint32_t n_kv,
+                       const uint32_t * runs_dev, uint32_t n_sel, uint32_t n_first, uint32_t n_last, int32_t * blocks_dev,
+                       void * ws_dev, size_t ws_bytes, void * stream);
+size_t tsr_hip_kv4_select_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t n_head_kv, uint32_t block, uint32_t n_kv);
+
 /* ---- decode-layer glue ops ----------------------------------------------------------------------
  * The f32 ops around MUL_MAT and FLASH_ATTN in a decoder layer, on the vector unit's f32 rules
  * (every input denormal-as-zero, one IEEE round-to-nearest-even operation, result flushed to zero,

@@ -128,6 +128,17 @@ struct Kv4BoundsArgs {
     uint32_t stride;         // blocks of a head
 };
 
+// The blocks that tokens attend to (k_kv4_select.hip).
+struct Kv4SelectArgs {
+    const float * q;         // [T][n_head][D], token t at q + t * q_stride
+    uint64_t q_stride;
+    const uint32_t * bounds; // [n_head_kv][stride][D]
+    const uint32_t * runs;   // nullable: [T][4]
+    uint64_t * keys;         // [T][n_head_kv][n_blocks]
+    int32_t * blocks;        // [T][n_head_kv][n_sel]
+    uint32_t stride, D, T, G, n_head_kv, n_kv, block, n_blocks, n_sel, n_first, n_last;
+};
+
 // The work list of one call. Small lists (decode) travel inline in the kernel arguments; larger ones
 // are copied to device memory once per call and the kernels read them there (FaArgs::items != 0).
 struct FaPlan {
@@ -291,6 +302,7 @@ int tsr_launch_kv4_get_rows(const tsr::Kv4Args & a, uint32_t which, const int64_
                             uint64_t dst_stride, int32_t * bad, hipStream_t s);
 int tsr_launch_kv_get_rows(const tsr::KvArgs & a, uint32_t which, const int64_t * idx, uint32_t n_rows, float * dst,
                            uint64_t dst_stride, int32_t * bad, hipStream_t s);
+int tsr_launch_kv4_select(const tsr::Kv4SelectArgs & a, hipStream_t s);
 int tsr_launch_kv4_bounds(const tsr::Kv4BoundsArgs & a, hipStream_t s);
 // attention over a 4-bit cache, cut as attn4_plan.hpp says (k_attn4.hip)
 int tsr_launch_attn4(const tsr::Attn4Args & a, const tsr::Attn4Plan & p, hipStream_t s);

@@ -1,4 +1,5 @@
-// tsr_sparse4.hip -- host side of the sparse attention over 4-bit KV caches: the bounds of a K cache's blocks.
+// tsr_sparse4.hip -- host side of the sparse attention over 4-bit KV caches: the bounds of a K cache's blocks and
+// their selection.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -7,6 +8,7 @@
 #include "kernels.hpp"
 #include "kv4.hpp"
 #include "runtime.hpp"
+#include "sparse4_plan.hpp"
 #include "tsr_hip.h"
 
 static bool block_ok(uint32_t block) { return block != 0u && block % 32u == 0u && block <= 1024u; }
@@ -37,4 +39,73 @@ int tsr_hip_kv4_bounds(tsr_hip_ctx * ctx, const tsr_hip_kv * kc, uint32_t D, uin
     std::lock_guard<std::mutex> lk(ctx->mtx);
     (void)hipSetDevice(ctx->device);
     return tsr_launch_kv4_bounds(a, ctx->pick(stream)) ? TSR_HIP_E_HIP : TSR_HIP_OK;
+}
+
+static bool heads_ok(uint32_t D, uint32_t n_head, uint32_t n_head_kv) {
+    return head_ok(D) && n_head_kv != 0u && n_head != 0u && n_head % n_head_kv == 0u && n_head / n_head_kv <= 64u &&
+           (uint64_t)n_head * D <= 32768u;
+}
+static uint32_t blocks_of(uint32_t n_kv, uint32_t block) { return (uint32_t)(((uint64_t)n_kv + block - 1u) / block); }
+
+// A call's workspace: the caller's, or eagerly the context's scratch, which orders calls across streams; a graph's replays
+// are ordered by nobody, so that a captured call brings its own. `lk` holds the context.
+static int workspace(tsr_hip_ctx * ctx, size_t need, void * ws_dev, hipStream_t s, void ** ws) {
+    *ws = ws_dev;
+    if (ws_dev != nullptr || need == 0u) return TSR_HIP_OK;
+    if (tsr_capturing(s)) return TSR_HIP_E_ARG;
+    const int rc = ctx->scratch.reserve(need, s);
+    *ws = ctx->scratch.ptr;
+    return rc;
+}
+
+size_t tsr_hip_kv4_select_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t n_head_kv, uint32_t block, uint32_t n_kv) {
+    if (ctx == nullptr || T == 0u || T > 65535u || n_head_kv == 0u || n_head_kv > 512u || !block_ok(block) || n_kv > 0x7FFFFFFFu)
+        return 0u;
+    return tsr::kv4_select_ws(T, n_head_kv, blocks_of(n_kv, block));
+}
+
+int tsr_hip_kv4_select(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const uint32_t * bounds_dev,
+                       uint32_t bounds_blocks, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t block, uint32_t n_kv,
+                       const uint32_t * runs_dev, uint32_t n_sel, uint32_t n_first, uint32_t n_last, int32_t * blocks_dev,
+                       void * ws_dev, size_t ws_bytes, void * stream) {
+    if (ctx == nullptr || q_dev == nullptr || bounds_dev == nullptr || blocks_dev == nullptr || T == 0u || T > 65535u)
+        return TSR_HIP_E_ARG;
+    if (!heads_ok(D, n_head, n_head_kv) || !block_ok(block) || n_sel == 0u || n_sel > 65536u || n_first > n_sel || n_last > n_sel - n_first)
+        return TSR_HIP_E_SHAPE;
+    if (n_kv > 0x7FFFFFFFu || bounds_blocks < blocks_of(n_kv, block)) return TSR_HIP_E_RANGE;
+    if ((((uintptr_t)q_dev | (uintptr_t)bounds_dev | (uintptr_t)runs_dev) & 15u) != 0u || ((uintptr_t)blocks_dev & 3u) != 0u ||
+        (T > 1u && (q_stride % 4u != 0u || q_stride < (uint64_t)n_head * D)))
+        return TSR_HIP_E_ARG;
+    const uint32_t nb = blocks_of(n_kv, block);
+    const size_t need = tsr::kv4_select_ws(T, n_head_kv, nb);
+    if (ws_dev != nullptr && (ws_bytes < need || ((uintptr_t)ws_dev & 15u) != 0u)) return TSR_HIP_E_ARG;
+    tsr::Kv4SelectArgs a{};
+    a.q_stride = q_stride;
+    a.bounds = bounds_dev;
+    a.stride = bounds_blocks;
+    a.D = D;
+    a.G = n_head / n_head_kv;
+    a.n_head_kv = n_head_kv;
+    a.n_kv = n_kv;
+    a.block = block;
+    a.n_blocks = nb;
+    a.n_sel = n_sel;
+    a.n_first = n_first;
+    a.n_last = n_last;
+    std::lock_guard<std::mutex> lk(ctx->mtx);
+    (void)hipSetDevice(ctx->device);
+    hipStream_t s = ctx->pick(stream);
+    void * ws = nullptr;
+    const int rc = workspace(ctx, need, ws_dev, s, &ws);
+    if (rc) return rc;
+    a.keys = (uint64_t *)ws;
+    const uint32_t step = tsr::kv4_select_tokens(T, n_head_kv, nb);
+    for (uint32_t t0 = 0; t0 < T; t0 += step) {
+        a.T = std::min(T - t0, step);
+        a.q = q_dev + t0 * q_stride;
+        a.runs = runs_dev ? runs_dev + 4u * (size_t)t0 : nullptr;
+        a.blocks = blocks_dev + (size_t)t0 * n_head_kv * n_sel;
+        if (tsr_launch_kv4_select(a, s)) return TSR_HIP_E_HIP;
+    }
+    return TSR_HIP_OK;
 }

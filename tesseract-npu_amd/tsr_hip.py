@@ -43,7 +43,7 @@ EXPORTS = (
     "tsr_hip_fa_plan_set_epoch",
     "tsr_hip_kv_create_type", "tsr_hip_kv_get_rows", "tsr_hip_flash_attn_kv4", "tsr_hip_flash_attn_kv4_ws",
     "tsr_hip_rope_scaled", "tsr_hip_rope_scaled_table",
-    "tsr_hip_kv4_bounds",
+    "tsr_hip_kv4_bounds", "tsr_hip_kv4_select", "tsr_hip_kv4_select_ws",
 )
 
 
@@ -144,6 +144,8 @@ def load(path: str = LIB_PATH) -> C.CDLL:
                                     vp], C.c_int),
         "tsr_hip_flash_attn_kv4_ws": ([vp, u32, u32, u32, u32, u32], sz),
         "tsr_hip_kv4_bounds": ([vp, vp, u32, u32, u32, vp, vp, u32, vp], C.c_int),
+        "tsr_hip_kv4_select": ([vp, vp, u32, u64, vp, u32, u32, u32, u32, u32, u32, vp, u32, u32, u32, vp, vp, sz, vp], C.c_int),
+        "tsr_hip_kv4_select_ws": ([vp, u32, u32, u32, u32], sz),
         "tsr_hip_rope_scaled": ([vp, vp, u32, u64, u32, u32, u32, C.c_int, vp, C.POINTER(RopeScaling), vp, vp, u64, vp], C.c_int),
         "tsr_hip_rope_scaled_table": ([vp, vp, u32, C.POINTER(RopeScaling), vp, vp, vp], C.c_int),
     }
@@ -485,6 +487,19 @@ class Device:
         or of the blocks of at most n_new cells from cells[0] to cells[1] (device uint32)."""
         _check(self.L.tsr_hip_kv4_bounds(self.ctx, kc.h, D, block, n_kv, self._p(bounds), self._p(cells), n_new, stream),
                "kv4_bounds")
+
+    def kv4_select_ws(self, T: int, n_head_kv: int, block: int, n_kv: int) -> int:
+        """Bytes of workspace that kv4_select needs."""
+        return int(self.L.tsr_hip_kv4_select_ws(self.ctx, T, n_head_kv, block, n_kv))
+
+    def kv4_select(self, q, T: int, q_stride: int, bounds, bounds_blocks: int, D: int, n_head: int, n_head_kv: int, block: int,
+                   n_kv: int, n_sel: int, n_first: int, n_last: int, blocks, runs=None, ws: "Buffer | None" = None,
+                   stream=None) -> None:
+        """The blocks (device int32 [T, n_head_kv, n_sel]) of each token and KV head: the first, the last and those whose bounds
+        allow the largest scores."""
+        _check(self.L.tsr_hip_kv4_select(self.ctx, self._p(q), T, q_stride, self._p(bounds), bounds_blocks, D, n_head, n_head_kv,
+                                         block, n_kv, self._p(runs), n_sel, n_first, n_last, self._p(blocks), self._p(ws),
+                                         0 if ws is None else ws.nbytes, stream), "kv4_select")
 
     def flash_attn(self, q, T: int, q_stride: int, kc: KvCache, vc: KvCache, D: int, n_head: int, n_head_kv: int,
                    scale: float, msum, out, out_stride: int, mask_f32=None, new_runs=None, stream=None) -> None:

@@ -57,3 +57,32 @@ def fill(dev, x, typ, which=0, cells=None):
     kv = dev.kv(x.shape[1], cells or x.shape[0], typ)
     kv.set_bytes(which, img)
     return kv, R.values_f32(img, typ)
+
+
+def candidates(run, n_kv, block):
+    """The blocks with a cell of a token's two runs, ascending."""
+    see = np.zeros(n_kv, bool)
+    for lo, hi in ((run[0], run[1]), (run[2], run[3])):
+        see[int(lo):max(int(lo), min(int(hi), n_kv))] = True
+    return np.unique(np.flatnonzero(see) // block)
+
+
+def select(q, lo, hi, n_head, block, n_kv, n_sel, n_first, n_last, runs=None):
+    """q f32 [T, n_head, D], bounds f64 [n_head_kv, blocks, D] -> int32 [T, n_head_kv, n_sel]."""
+    T, nkv = q.shape[0], lo.shape[0]
+    G = n_head // nkv
+    out = np.full((T, nkv, n_sel), -1, np.int32)
+    for t in range(T):
+        c = candidates(runs[t] if runs is not None else (0, n_kv, 0, 0), n_kv, block)
+        for h in range(nkv):
+            mine = c
+            if c.size > n_sel:
+                qh = q[t, h * G:(h + 1) * G].astype(np.float64)[:, None]
+                with np.errstate(invalid="ignore"):
+                    s = (np.where(qh < 0, 0.0, qh) * hi[h, c] + np.where(qh > 0, 0.0, qh) * lo[h, c]).sum(-1)
+                s = np.where(np.isnan(s).any(0), -np.inf, s.max(0))
+                mid = np.arange(n_first, c.size - n_last)
+                best = mid[np.argsort(-s[mid], kind="stable")[:n_sel - n_first - n_last]]
+                mine = c[np.sort(np.concatenate([np.arange(n_first), best, np.arange(c.size - n_last, c.size)]))]
+            out[t, h, :mine.size] = mine
+    return out
