@@ -417,6 +417,18 @@ int tsr_hip_kv4_select(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint6
                        void * ws_dev, size_t ws_bytes, void * stream);
 size_t tsr_hip_kv4_select_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t n_head_kv, uint32_t block, uint32_t n_kv);
 
+/* The attention: tsr_hip_flash_attn_kv4 of each token and KV head over the cells of its listed blocks that its runs allow.
+ * Arguments, precision, empty rows and the workspace (tsr_hip_flash_attn_kv4_blocks_ws) as there; no mask.
+ *   blocks_dev     [T][n_head_kv][n_sel] int32, 4-byte aligned, read when the kernels run: as tsr_hip_kv4_select gives
+ *                  them, or others in any order; an entry that is negative or of no cell below n_kv is passed over, a block that is
+ *                  listed twice counts twice. */
+int tsr_hip_flash_attn_kv4_blocks(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const tsr_hip_kv * kc,
+                                  const tsr_hip_kv * vc, uint32_t D, uint32_t n_head, uint32_t n_head_kv, float scale, uint32_t n_kv,
+                                  const uint32_t * runs_dev, const int32_t * blocks_dev, uint32_t n_sel, uint32_t block, float * out_dev,
+                                  uint64_t out_stride, void * ws_dev, size_t ws_bytes, void * stream);
+size_t tsr_hip_flash_attn_kv4_blocks_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_sel,
+                                        uint32_t block);
+
 /* ---- decode-layer glue ops ----------------------------------------------------------------------
  * The f32 ops around MUL_MAT and FLASH_ATTN in a decoder layer, on the vector unit's f32 rules
  * (every input denormal-as-zero, one IEEE round-to-nearest-even operation, result flushed to zero,

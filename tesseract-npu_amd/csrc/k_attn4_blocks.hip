@@ -1,0 +1,73 @@
+// k_attn4_blocks.hip -- attention of f32 query rows over listed blocks of a 4-bit KV cache (attn4.hpp has the mathematics and
+// what a wave does): a token's query heads of one KV head share a list and are the rows of its workgroups, whose waves take
+// the lists' tiles in turn.
+#include "attn4.hpp"
+
+namespace tsr {
+
+// Workgroup (KV head, split, token and group of its rows).
+template <int D, int C, uint32_t TYPE>
+__global__ __launch_bounds__(256, waves_of(D, 1, C, TYPE)) void k_attn4_blocks(Attn4BlocksArgs b) {
+    using A = Attn4<D, 1, C, TYPE>;
+    Attn4Args a = b.a;
+    const uint32_t n_rg = (a.G + A::RW - 1u) / A::RW, t = blockIdx.z / n_rg, r0 = (blockIdx.z - t * n_rg) * A::RW;
+    const uint32_t h = blockIdx.x, split = blockIdx.y, nh = a.G * a.n_head_kv;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u;
+    const size_t nr = (size_t)a.T * nh, row0 = (size_t)t * nh + h * a.G;
+    float * out = a.out + (size_t)t * a.out_stride + (size_t)h * a.G * D;
+    a.T = 1u;                                                      // the token alone
+    a.mask = nullptr;
+    a.q += (size_t)t * a.q_stride;
+    if (a.runs != nullptr) a.runs += 4u * (size_t)t;
+    __shared__ __align__(16) uint8_t room[A::kRoom];
+    __shared__ float2 ml[kWaves * A::RT];
+    __shared__ uint32_t list[kWaves][64];
+    const int32_t * ids = b.blocks + ((size_t)t * a.n_head_kv + h) * b.n_sel;
+    const uint32_t per = b.block / 32u, n_blocks = (a.n_kv + b.block - 1u) / b.block;
+    auto entry = [&](uint32_t j) {
+        const uint32_t i = j / per, id = (uint32_t)ids[i];
+        return id < n_blocks ? id * per + (j - i * per) : ~0u;
+    };
+    A w;
+    w.load_runs(a, h, r0, lane);
+    w.run_list(a, h, split * kWaves + wave, a.S * kWaves, b.n_sel * per, entry, list[wave], (h8 *)room, wave, lane);
+    w.finish();
+    auto place = [&](uint32_t r) { return a.S > 1u ? a.part + attn4_part_row(nr, D, split, row0 + r) : out + (size_t)r * D; };
+    auto sums = [&](uint32_t r, float m, float l) { *(float2 *)(a.part + attn4_part_sum(nr, D, a.S, split, row0 + r)) = make_float2(m, l); };
+    w.join(room, ml, r0, a.G, a.S > 1u, wave, lane, place, sums);
+}
+
+template <int D, int C, uint32_t TYPE>
+static int launch_blocks(const Attn4BlocksArgs & b, hipStream_t s) {
+    const uint32_t n_rg = (b.a.G + 16u / C - 1u) / (16u / C);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4_blocks<D, C, TYPE>), dim3(b.a.n_head_kv, b.a.S, b.a.T * n_rg), dim3(64u * kWaves), 0, s, b);
+    if (b.a.S > 1u) return tsr_launch_attn4_join(b.a, s);
+    return hipGetLastError() == hipSuccess ? 0 : -4;
+}
+
+template <int D, uint32_t TYPE>
+static int launch_blocks_d(const Attn4BlocksArgs & b, uint32_t C, hipStream_t s) {
+    switch (C) {
+        case 2: return launch_blocks<D, 2, TYPE>(b, s);
+        case 4:
+            if constexpr (D >= 128) return launch_blocks<D, 4, TYPE>(b, s);
+        default: return launch_blocks<D, 1, TYPE>(b, s);
+    }
+}
+
+template <uint32_t TYPE>
+static int launch_blocks_t(const Attn4BlocksArgs & b, uint32_t C, hipStream_t s) {
+    switch (b.a.D) {
+        case 64: return launch_blocks_d<64, TYPE>(b, C, s);
+        case 128: return launch_blocks_d<128, TYPE>(b, C, s);
+        case 256: return launch_blocks_d<256, TYPE>(b, C, s);
+        case 512: return launch_blocks_d<512, TYPE>(b, C, s);
+        default: return -2;
+    }
+}
+
+}  // namespace tsr
+
+int tsr_launch_attn4_blocks(const tsr::Attn4BlocksArgs & b, uint32_t C, hipStream_t s) {
+    return b.a.type == tsr::kKvQ4_0 ? tsr::launch_blocks_t<tsr::kKvQ4_0>(b, C, s) : tsr::launch_blocks_t<tsr::kKvQ4_1>(b, C, s);
+}

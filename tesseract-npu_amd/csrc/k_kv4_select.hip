@@ -12,6 +12,7 @@
 // is one value; two passes do for a few thousand keys.
 #include "kernels.hpp"
 #include "tsr_dev.hpp"
+#include "wave_lds.hpp"
 
 namespace tsr {
 
@@ -30,13 +31,6 @@ struct BlockRange { uint32_t lo, hi; };
 __device__ __forceinline__ BlockRange blocks_of(uint32_t lo, uint32_t hi, uint32_t n_kv, uint32_t block) {
     hi = min(hi, n_kv);
     return lo < hi ? BlockRange{ lo / block, (hi + block - 1u) / block } : BlockRange{ 0u, 0u };
-}
-
-// Behind a wave's writes to LDS that its other lanes read, and the other way round: a wave's operations run in order there.
-__device__ __forceinline__ void own_room() {
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_wave_barrier();
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
 // Workgroup (64 blocks, KV heads fastest; tokens), a wave 16 blocks. C columns hold 16 / G tokens' G query heads, or a token's 16 at

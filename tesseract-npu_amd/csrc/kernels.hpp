@@ -118,6 +118,13 @@ struct Attn4Args {
     float scale;
 };
 
+// The same over listed blocks of cells (k_attn4_blocks.hip).
+struct Attn4BlocksArgs {
+    Attn4Args a;             // no mask
+    const int32_t * blocks;  // [T][n_head_kv][n_sel] blocks of `block` cells; those without a cell below n_kv are passed over
+    uint32_t n_sel, block;
+};
+
 // The bounds of the blocks of a 4-bit K cache (k_kv4_bounds.hip).
 struct Kv4BoundsArgs {
     const uint8_t * k;       // the plane
@@ -306,6 +313,9 @@ int tsr_launch_kv4_select(const tsr::Kv4SelectArgs & a, hipStream_t s);
 int tsr_launch_kv4_bounds(const tsr::Kv4BoundsArgs & a, hipStream_t s);
 // attention over a 4-bit cache, cut as attn4_plan.hpp says (k_attn4.hip)
 int tsr_launch_attn4(const tsr::Attn4Args & a, const tsr::Attn4Plan & p, hipStream_t s);
+int tsr_launch_attn4_blocks(const tsr::Attn4BlocksArgs & b, uint32_t C, hipStream_t s);
+// the splits' partial rows joined into the output
+int tsr_launch_attn4_join(const tsr::Attn4Args & a, hipStream_t s);
 int tsr_launch_fa(const tsr::FaArgs & a, const tsr::FaPlan & p, uint32_t T, uint32_t n_cu, hipStream_t s);
 int tsr_launch_fa_dec(const tsr::FaDecArgs & a, hipStream_t s);
 int tsr_launch_xcd_probe(uint32_t * out64, hipStream_t s);

@@ -17,4 +17,21 @@ inline size_t kv4_select_ws(uint32_t T, uint32_t n_head_kv, uint64_t n_blocks) {
     return (size_t)kv4_select_tokens(T, n_head_kv, n_blocks) * n_head_kv * (size_t)std::max<uint64_t>(1u, n_blocks) * 8u;
 }
 
+// Attention over listed blocks: columns of the matrix instruction a row (attn4.hpp) and splits of a token's tiles.
+struct Attn4BlocksPlan {
+    uint32_t C, S;
+    size_t ws_bytes;
+};
+inline Attn4BlocksPlan attn4_blocks_plan(uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_sel, uint32_t block,
+                                         uint32_t n_cu) {
+    Attn4BlocksPlan p{};
+    const uint64_t G = n_head / n_head_kv, tiles = (uint64_t)n_sel * (block / 32u);
+    p.C = G <= 4u && D >= 128u ? 4u : G <= 8u ? 2u : 1u;           // a workgroup's rows are one token's: as few columns as hold them
+    const uint64_t rows = 16u / p.C, n = (uint64_t)T * n_head_kv * ((G + rows - 1u) / rows), fill = n_cu / n;
+    const uint64_t S = tiles <= 20u ? 1u : fill;
+    p.S = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ S, (tiles + 3u) / 4u, 256u }));
+    p.ws_bytes = p.S > 1u ? 4u * (size_t)p.S * T * n_head * (2u + D) : 0u;
+    return p;
+}
+
 }  // namespace tsr

@@ -44,6 +44,7 @@ EXPORTS = (
     "tsr_hip_kv_create_type", "tsr_hip_kv_get_rows", "tsr_hip_flash_attn_kv4", "tsr_hip_flash_attn_kv4_ws",
     "tsr_hip_rope_scaled", "tsr_hip_rope_scaled_table",
     "tsr_hip_kv4_bounds", "tsr_hip_kv4_select", "tsr_hip_kv4_select_ws",
+    "tsr_hip_flash_attn_kv4_blocks", "tsr_hip_flash_attn_kv4_blocks_ws",
 )
 
 
@@ -146,6 +147,9 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         "tsr_hip_kv4_bounds": ([vp, vp, u32, u32, u32, vp, vp, u32, vp], C.c_int),
         "tsr_hip_kv4_select": ([vp, vp, u32, u64, vp, u32, u32, u32, u32, u32, u32, vp, u32, u32, u32, vp, vp, sz, vp], C.c_int),
         "tsr_hip_kv4_select_ws": ([vp, u32, u32, u32, u32], sz),
+        "tsr_hip_flash_attn_kv4_blocks": ([vp, vp, u32, u64, vp, vp, u32, u32, u32, C.c_float, u32, vp, vp, u32, u32, vp, u64, vp,
+                                           sz, vp], C.c_int),
+        "tsr_hip_flash_attn_kv4_blocks_ws": ([vp, u32, u32, u32, u32, u32, u32], sz),
         "tsr_hip_rope_scaled": ([vp, vp, u32, u64, u32, u32, u32, C.c_int, vp, C.POINTER(RopeScaling), vp, vp, u64, vp], C.c_int),
         "tsr_hip_rope_scaled_table": ([vp, vp, u32, C.POINTER(RopeScaling), vp, vp, vp], C.c_int),
     }
@@ -500,6 +504,18 @@ class Device:
         _check(self.L.tsr_hip_kv4_select(self.ctx, self._p(q), T, q_stride, self._p(bounds), bounds_blocks, D, n_head, n_head_kv,
                                          block, n_kv, self._p(runs), n_sel, n_first, n_last, self._p(blocks), self._p(ws),
                                          0 if ws is None else ws.nbytes, stream), "kv4_select")
+
+    def flash_attn_kv4_blocks_ws(self, T: int, D: int, n_head: int, n_head_kv: int, n_sel: int, block: int) -> int:
+        """Bytes of workspace that flash_attn_kv4_blocks needs (0: none)."""
+        return int(self.L.tsr_hip_flash_attn_kv4_blocks_ws(self.ctx, T, D, n_head, n_head_kv, n_sel, block))
+
+    def flash_attn_kv4_blocks(self, q, T: int, q_stride: int, kc: KvCache, vc: KvCache, D: int, n_head: int, n_head_kv: int,
+                              scale: float, n_kv: int, blocks, n_sel: int, block: int, out, out_stride: int, runs=None,
+                              ws: "Buffer | None" = None, stream=None) -> None:
+        """flash_attn_kv4 over the cells of listed blocks (device int32 [T, n_head_kv, n_sel], as kv4_select gives them)."""
+        _check(self.L.tsr_hip_flash_attn_kv4_blocks(self.ctx, self._p(q), T, q_stride, kc.h, vc.h, D, n_head, n_head_kv, scale,
+                                                    n_kv, self._p(runs), self._p(blocks), n_sel, block, self._p(out), out_stride,
+                                                    self._p(ws), 0 if ws is None else ws.nbytes, stream), "flash_attn_kv4_blocks")
 
     def flash_attn(self, q, T: int, q_stride: int, kc: KvCache, vc: KvCache, D: int, n_head: int, n_head_kv: int,
                    scale: float, msum, out, out_stride: int, mask_f32=None, new_runs=None, stream=None) -> None:

@@ -86,3 +86,21 @@ def select(q, lo, hi, n_head, block, n_kv, n_sel, n_first, n_last, runs=None):
                 mine = c[np.sort(np.concatenate([np.arange(n_first), best, np.arange(c.size - n_last, c.size)]))]
             out[t, h, :mine.size] = mine
     return out
+
+
+def attention(q, kimg, vimg, typ, D, n_head, nkv, scale, blocks, block, n_kv, runs=None):
+    """f64 attention over listed blocks [T, nkv, n_sel] and how far an f32 result may be from it (kv4_ref.attention's terms,
+    which do not depend on the order of the tiles)."""
+    T, G, nb = q.shape[0], n_head // nkv, D // 32
+    out, tol = np.zeros((T, n_head, D)), np.zeros((T, n_head, D))
+    per = kimg.shape[1] // (nkv * nb)
+    for h in range(nkv):
+        mask = np.full((T, n_kv), -np.inf, np.float16)
+        for t in range(T):
+            for b in blocks[t, h]:
+                if b >= 0:
+                    mask[t, b * block:(b + 1) * block] = 0
+        part = slice(h * nb * per, (h + 1) * nb * per)
+        o, x = R.attention(q.reshape(T, n_head, D)[:, h * G:(h + 1) * G], kimg[:n_kv, part], vimg[:n_kv, part], typ, D, G, 1, scale, runs, mask)
+        out[:, h * G:(h + 1) * G], tol[:, h * G:(h + 1) * G] = o, x
+    return out, tol
