@@ -1,15 +1,18 @@
 // k_kv4_select.hip -- for every token and KV head the blocks of cells whose bounds (k_kv4_bounds.hip) allow the largest
 // scores.
 //
-// The score of a block is max over the KV head's query heads of sum over channels of max(q lo, q hi) = max(q, 0) hi + min(q, 0) lo.
-// It decides between blocks that may lie close together, so that it is f64: products of f32 and bf16 are exact there
-// and a sum of 512 is off by 2^-52 of its terms, far below what tells two blocks apart. Equal scores go to the lowest block.
+// The score of a block is max over the KV head's query heads of sum over channels of max(q lo, q hi).
+// It decides between blocks that may lie close together, so that it is f64, made as q (hi + lo) + |q| (hi - lo), twice the score:
+// products of f32 and sums of bf16 are exact or off by 2^-53 there, far below what tells two blocks apart. Equal scores go to
+// the lowest block.
 //
-// k_kv4_scores is a matrix product of bounds and queries on the f64 matrix instruction 16x16x4 (the rate of f64's vector units,
-// without their registers): rows 16 blocks, columns 16 query heads (whole tokens), each channel once with hi and
-// once with lo. What leaves is a key a block, an unsigned number in the order of the scores. k_kv4_pick_blocks then finds the
-// cut: the keys' range is counted into 1024 bins, the bin with the cut becomes the range, until all of a bin is taken or it
-// is one value; two passes do for a few thousand keys.
+// k_kv4_scores is a product of bounds and queries on the f64 matrix instruction 4x4x4 (four of them at once: 16 blocks by
+// four query heads, each channel once with q and once with |q|), 18 cycles an instruction; k_kv4_scores_many on 16x16x4, 64 cycles,
+// whose 16 columns several tokens fill that look at the same blocks. What leaves is a key a block, an unsigned number in
+// the order of the scores. k_kv4_pick_blocks then finds the cut: the keys' range is counted into bins, the bin with the cut becomes
+// the range, until all of a bin is taken or it is one value; two or three passes do for a few thousand keys. Both are a few
+// microseconds of waiting for memory and for each other's steps, not work: reductions and scans run on DPP, keys are asked for
+// before the runs that say which of them count.
 #include "kernels.hpp"
 #include "tsr_dev.hpp"
 #include "wave_lds.hpp"
@@ -27,16 +30,117 @@ __device__ __forceinline__ uint64_t order_of(double x) {
 constexpr uint32_t kScoreWaves = 4u;
 
 // The blocks that cells [lo, hi) touch.
-struct BlockRange { uint32_t lo, hi; };
+struct BlockRange {
+    uint32_t lo, hi;
+    __device__ __forceinline__ bool has(uint32_t b) const { return b >= lo && b < hi; }
+    __device__ __forceinline__ bool meets(uint32_t b0, uint32_t b1) const { return lo < b1 && hi > b0 && lo < hi; }
+};
 __device__ __forceinline__ BlockRange blocks_of(uint32_t lo, uint32_t hi, uint32_t n_kv, uint32_t block) {
     hi = min(hi, n_kv);
     return lo < hi ? BlockRange{ lo / block, (hi + block - 1u) / block } : BlockRange{ 0u, 0u };
 }
 
-// Workgroup (64 blocks, KV heads fastest; tokens), a wave 16 blocks. C columns hold 16 / G tokens' G query heads, or a token's 16 at
+// hi + lo and hi - lo of a word of bounds.
+struct Bounds2 { double mid, half; };
+__device__ __forceinline__ Bounds2 bounds2(uint32_t w) {
+    const double lo = (double)bf(w << 16), hi = (double)bf(w & 0xFFFF0000u);
+    return Bounds2{ hi + lo, hi - lo };
+}
+
+// Few tokens: workgroup (KV heads fastest, part of the blocks; token), a wave 16 blocks at a time and the token's query heads, NG
+// groups of four at a time. Lane 16 k + 4 u + i of the instruction's operands: block 4 u + i (query head i), channels 4 k .. 4
+// k + 3 of every 16, one a step; of its result: block 4 u + k, query head i. One token: a part is 64 blocks, whose bounds are asked
+// for ahead of the runs. Several may be sequences of their own, which look at a few of the blocks: the parts share a token's out.
+template <int D, int NG>
+__global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores(Kv4SelectArgs a, uint32_t parts) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u, g = lane >> 4;
+    const uint32_t h = blockIdx.x % a.n_head_kv, t = blockIdx.y;
+    constexpr int most = 16 / NG, AT = D / 16 < most ? D / 16 : most;   // loads of 16 channels in flight
+    const uint32_t * hp = a.bounds + (size_t)h * a.stride * D + 4u * g;
+    uint32_t b0 = (blockIdx.x / a.n_head_kv * kScoreWaves + wave) * 16u, end = a.n_blocks;
+    auto row = [&](uint32_t b) { return hp + (size_t)min(b + (lane & 15u), a.n_blocks - 1u) * D; };
+    uint4 w[AT];
+    if (a.T == 1u)
+#pragma unroll
+        for (int m = 0; m < AT; ++m) w[m] = *(const uint4 *)(row(b0) + 16 * m);
+    BlockRange x = { 0u, end }, y = { 0u, 0u };
+    if (a.runs != nullptr) {
+        const uint4 u = *(const uint4 *)(a.runs + 4u * (size_t)t);
+        x = blocks_of(u.x, u.y, a.n_kv, a.block);
+        y = blocks_of(u.z, u.w, a.n_kv, a.block);
+        const uint32_t lo = min(x.lo < x.hi ? x.lo : end, y.lo < y.hi ? y.lo : end);
+        end = max(x.lo < x.hi ? x.hi : 0u, y.lo < y.hi ? y.hi : 0u);
+        if (a.T != 1u) b0 += lo & ~15u;
+    }
+    bool here = a.T == 1u;                                         // w holds this tile's first bounds
+    for (; b0 < end; b0 += parts * kScoreWaves * 16u) {
+        if (!x.meets(b0, b0 + 16u) && !y.meets(b0, b0 + 16u)) {
+            here = false;
+            continue;
+        }
+        const uint32_t * bp = row(b0);
+        double best = -__builtin_inf();                                // over the lane's query heads
+        bool nan = false;
+        for (uint32_t q0 = 0; q0 < a.G; q0 += 4u * NG) {
+            const float * qp[NG];
+#pragma unroll
+            for (int n = 0; n < NG; ++n)                               // (past the last: it again)
+                qp[n] = a.q + (size_t)t * a.q_stride + ((size_t)h * a.G + min(q0 + 4u * n + (lane & 3u), a.G - 1u)) * D + 4u * g;
+            double acc[NG][2];
+#pragma unroll
+            for (int n = 0; n < NG; ++n) acc[n][0] = acc[n][1] = 0.0;
+#pragma unroll 1
+            for (int m0 = 0; m0 < D / 16; m0 += AT) {
+                if (!here || m0 != 0 || (D / 16 > AT && q0 != 0u))
+#pragma unroll
+                    for (int m = 0; m < AT; ++m) w[m] = *(const uint4 *)(bp + 16 * (m0 + m));
+                float4 q[NG][AT];
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+#pragma unroll
+                    for (int m = 0; m < AT; ++m) q[n][m] = *(const float4 *)(qp[n] + 16 * (m0 + m));
+#pragma unroll
+                for (int m = 0; m < AT; ++m) {
+                    const uint32_t x[4] = { w[m].x, w[m].y, w[m].z, w[m].w };
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const Bounds2 z = bounds2(x[i]);
+#pragma unroll
+                        for (int n = 0; n < NG; ++n) {
+                            const float y[4] = { q[n][m].x, q[n][m].y, q[n][m].z, q[n][m].w };
+                            const double v = (double)y[i];
+                            acc[n][0] = __builtin_amdgcn_mfma_f64_4x4x4f64(z.mid, v, acc[n][0], 0, 0, 0);
+                            acc[n][1] = __builtin_amdgcn_mfma_f64_4x4x4f64(z.half, __builtin_fabs(v), acc[n][1], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                const double s = acc[n][0] + acc[n][1];
+                nan |= s != s;
+                best = fmax(best, s);
+            }
+        }
+        // the most over the four lanes of a block
+        auto xor_of = [](double v, auto f) {
+            const uint64_t u = __builtin_bit_cast(uint64_t, v);
+            return __builtin_bit_cast(double, (uint64_t)(uint32_t)f((int)(uint32_t)u) | (uint64_t)(uint32_t)f((int)(uint32_t)(u >> 32)) << 32);
+        };
+        best = fmax(best, xor_of(best, [](int v) { return dpp_i<kDppXor1>(v); }));
+        best = fmax(best, xor_of(best, [](int v) { return dpp_i<kDppXor2>(v); }));
+        const bool none = ((__ballot(nan) >> (lane & 60u)) & 15u) != 0u;
+        const uint32_t b = b0 + (lane & 12u) + g;
+        if ((lane & 3u) == 0u && b < a.n_blocks)
+            a.keys[((size_t)t * a.n_head_kv + h) * a.n_blocks + b] = none ? 0u : order_of(best);
+        here = false;
+    }
+}
+
+// Many tokens: workgroup (64 blocks, KV heads fastest; tokens), a wave 16 blocks. The instruction's 16 columns hold 16 / G tokens' G query heads, or a token's 16 at
 // a time where G > 16.
 template <int D>
-__global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores(Kv4SelectArgs a) {
+__global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores_many(Kv4SelectArgs a) {
     __shared__ double room[kScoreWaves][16 * 17];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
     const uint32_t h = blockIdx.x % a.n_head_kv, b0 = (blockIdx.x / a.n_head_kv * kScoreWaves + wave) * 16u;
@@ -47,7 +151,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores(Kv4SelectArgs a
         if (lane < tpt && t0 + lane < a.T) {
             const uint4 u = *(const uint4 *)(a.runs + 4u * (size_t)(t0 + lane));
             const BlockRange x = blocks_of(u.x, u.y, a.n_kv, a.block), y = blocks_of(u.z, u.w, a.n_kv, a.block);
-            any = (x.lo < b0 + 16u && x.hi > b0) || (y.lo < b0 + 16u && y.hi > b0);
+            any = x.meets(b0, b0 + 16u) || y.meets(b0, b0 + 16u);
         }
         if (__ballot(any) == 0ull) return;
     }
@@ -80,9 +184,10 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores(Kv4SelectArgs a
                 const float y[4] = { q[m].x, q[m].y, q[m].z, q[m].w };
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float up = y[i] < 0.0f ? 0.0f : y[i], down = y[i] > 0.0f ? 0.0f : y[i];   // (a NaN stays one)
-                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)bf(x[i] & 0xFFFF0000u), (double)up, acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)bf(x[i] << 16), (double)down, acc, 0, 0, 0);
+                    const Bounds2 z = bounds2(x[i]);
+                    const double v = (double)y[i];
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(z.mid, v, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(z.half, __builtin_fabs(v), acc, 0, 0, 0);
                 }
             }
         }
@@ -111,23 +216,57 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores(Kv4SelectArgs a
 }
 
 __device__ __forceinline__ uint64_t lesser(uint64_t a, uint64_t b) { return a < b ? a : b; }
-__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a < b ? b : a; }
-
-constexpr uint32_t kPickWaves = 4u, kBins = 1024u;
-
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int d) {
-    return (uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)x, d) | (uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)(x >> 32), d) << 32;
+// Over the wave: the least, and the sum of the lanes up to each (row shifts, then broadcasts of the rows' ends).
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+    v = min(v, (uint32_t)dpp_i<kDppXor1>((int)v));
+    v = min(v, (uint32_t)dpp_i<kDppXor2>((int)v));
+    v = min(v, (uint32_t)dpp_i<kDppRowHalfMirror>((int)v));
+    v = min(v, (uint32_t)dpp_i<kDppRowMirror>((int)v));
+    auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = min(x[0], x[1]);
+    auto y = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return min(y[0], y[1]);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
 }
 
-// Workgroup (KV head, token). The keys of the candidates between the first and the last ones lie in the waves' registers, wave
-// w the w-th quarter, rows of 64; where they are more than ROWS rows a wave, they are read from memory whenever they are needed.
-template <uint32_t ROWS>
-__global__ __launch_bounds__(64 * kPickWaves) void k_kv4_pick_blocks(Kv4SelectArgs a) {
-    __shared__ uint32_t bins[kBins], part[kPickWaves][2], found[3];
-    __shared__ uint64_t ends[kPickWaves][2];
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u;
-    const uint32_t h = blockIdx.x, t = blockIdx.y;
-    BlockRange x = { 0u, (a.n_kv + a.block - 1u) / a.block }, y = { 0u, 0u };
+constexpr uint32_t pick_waves(uint32_t WAVES) { return WAVES == 1u ? 4u : WAVES; }   // of a workgroup
+
+// WAVES 16: a workgroup a token and KV head; WAVES 1: each of its four waves. The keys lie in the waves' registers, wave w of a
+// list the w-th part of the blocks, rows of 64; where they are more than ROWS rows (ROWS 0), they are read from memory whenever they
+// are needed.
+template <uint32_t ROWS, uint32_t WAVES>
+__global__ __launch_bounds__(64 * pick_waves(WAVES)) void k_kv4_pick_blocks(Kv4SelectArgs a) {
+    constexpr uint32_t LISTS = pick_waves(WAVES) / WAVES, kBins = 256u * WAVES, kBits = WAVES == 1u ? 8u : 12u;
+    static_assert(kBins == 1u << kBits, "bins");
+    __shared__ uint32_t room[LISTS][kBins], parts[LISTS][WAVES][2], founds[LISTS][3];
+    const uint32_t wv = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u;
+    const uint32_t list = WAVES == 1u ? wv : 0u, wave = WAVES == 1u ? 0u : wv, tid = 64u * wave + lane;
+    uint32_t * bins = room[list], (*part)[2] = parts[list], * found = founds[list];
+    auto sync = [] {
+        if constexpr (WAVES == 1u) own_room();
+        else __syncthreads();
+    };
+    const uint32_t id = blockIdx.x * LISTS + list;                 // token and KV head
+    if (id >= a.T * a.n_head_kv) return;
+    const uint32_t t = id / a.n_head_kv;
+    const uint64_t * keys = a.keys + (size_t)id * a.n_blocks;
+    uint32_t from = 0u, rows = (a.n_blocks + 64u * WAVES - 1u) / (64u * WAVES);
+    uint64_t mine[ROWS == 0u ? 1u : ROWS];
+    if constexpr (ROWS != 0u)
+#pragma unroll
+        for (uint32_t j = 0; j < ROWS; ++j) {
+            const uint32_t b = (wave * rows + j) * 64u + lane;
+            mine[j] = j < rows && b < a.n_blocks ? keys[b] : 0u;
+        }
+    BlockRange x = { 0u, a.n_blocks }, y = { 0u, 0u };
     if (a.runs != nullptr) {
         const uint4 u = *(const uint4 *)(a.runs + 4u * (size_t)t);
         x = blocks_of(u.x, u.y, a.n_kv, a.block);
@@ -136,109 +275,108 @@ __global__ __launch_bounds__(64 * kPickWaves) void k_kv4_pick_blocks(Kv4SelectAr
         y.lo = max(y.lo, x.hi);
         if (y.lo > y.hi) y.hi = y.lo;
     }
+    if constexpr (ROWS == 0u) {                                    // the candidates' hull
+        from = x.lo;
+        rows = (max(x.hi, y.lo < y.hi ? y.hi : 0u) - from + 64u * WAVES - 1u) / (64u * WAVES);
+    }
     const uint32_t nx = x.hi - x.lo, n = nx + (y.hi - y.lo);
     auto block = [&](uint32_t i) { return i < nx ? x.lo + i : y.lo + (i - nx); };
-    int32_t * out = a.blocks + ((size_t)t * a.n_head_kv + h) * a.n_sel;
-    const uint32_t nf = min(a.n_first, n), take = min(n, a.n_sel);
-    for (uint32_t i = threadIdx.x; i < a.n_sel; i += 64u * kPickWaves) {
+    int32_t * out = a.blocks + (size_t)id * a.n_sel;
+    const uint32_t nf = min(a.n_first, n);
+    for (uint32_t i = tid; i < a.n_sel; i += 64u * WAVES) {
         if (n <= a.n_sel) out[i] = i < n ? (int32_t)block(i) : -1;
         else if (i < nf) out[i] = (int32_t)block(i);
         else if (i >= a.n_sel - a.n_last) out[i] = (int32_t)block(n - (a.n_sel - i));
     }
-    uint32_t m = take - nf - a.n_last;                             // wanted of the others
-    if (n <= a.n_sel || m == 0u) return;
-    const uint32_t others = n - nf - a.n_last, rows = (others + 64u * kPickWaves - 1u) / (64u * kPickWaves), first = wave * rows * 64u;
-    const uint64_t * keys = a.keys + ((size_t)t * a.n_head_kv + h) * a.n_blocks;
-    auto fetch = [&](uint32_t j) {
-        const uint32_t i = first + 64u * j + lane;
-        return i < others ? keys[block(nf + i)] : 0u;
-    };
-    uint64_t mine[ROWS == 0u ? 1u : ROWS];
-    if constexpr (ROWS != 0u)
-#pragma unroll
-        for (uint32_t j = 0; j < ROWS; ++j) mine[j] = j < rows ? fetch(j) : 0u;
-    // f(place, key, whether there is one) for every row of the wave, the lanes together
+    if (n <= a.n_sel || a.n_sel == nf + a.n_last) return;
+    uint32_t m = a.n_sel - nf - a.n_last;                          // wanted of the others
+    // f(block, key, whether it is one of them) for every row of the wave, the lanes together
     auto each = [&](auto f) {
+        auto one = [&](uint32_t j, uint64_t k) {
+            const uint32_t b = from + (wave * rows + j) * 64u + lane;
+            const uint32_t i = x.has(b) ? b - x.lo : y.has(b) ? nx + (b - y.lo) : ~0u;
+            f(b, k, i >= nf && i < n - a.n_last);
+        };
         if constexpr (ROWS != 0u) {
 #pragma unroll
             for (uint32_t j = 0; j < ROWS; ++j)
-                if (j < rows) f(first + 64u * j + lane, mine[j], first + 64u * j + lane < others);
+                if (j < rows) one(j, mine[j]);
         } else {
-            for (uint32_t j = 0; j < rows; ++j) f(first + 64u * j + lane, fetch(j), first + 64u * j + lane < others);
+            for (uint32_t j = 0; j < rows; ++j) one(j, keys[min(from + (wave * rows + j) * 64u + lane, a.n_blocks - 1u)]);
         }
     };
-    uint64_t lo = ~0ull, hi = 0u;
+    uint32_t least = ~0u, most = 0u;                               // of the keys' high words
     each([&](uint32_t, uint64_t k, bool real) {
-        lo = real ? lesser(lo, k) : lo;
-        hi = real ? larger(hi, k) : hi;
+        least = real ? min(least, (uint32_t)(k >> 32)) : least;
+        most = real ? max(most, (uint32_t)(k >> 32)) : most;
     });
+    least = wave_min(least);
+    most = ~wave_min(~most);
+    if constexpr (WAVES > 1u) {
+        if (lane == 0u) { part[wave][0] = least; part[wave][1] = most; }
+        sync();
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        lo = lesser(lo, shfl_xor64(lo, d));
-        hi = larger(hi, shfl_xor64(hi, d));
+        for (uint32_t v = 0; v < WAVES; ++v) { least = min(least, part[v][0]); most = max(most, part[v][1]); }
     }
-    if (lane == 0u) { ends[wave][0] = lo; ends[wave][1] = hi; }
-    __syncthreads();
-#pragma unroll
-    for (uint32_t v = 0; v < kPickWaves; ++v) { lo = lesser(lo, ends[v][0]); hi = larger(hi, ends[v][1]); }
+    uint64_t lo = (uint64_t)least << 32, hi = (uint64_t)most << 32 | 0xFFFFFFFFu;
     // keys above hi are taken, those below lo are not, m of those between are
-    bool whole = others == m;
+    bool whole = false;
     while (!whole && lo != hi) {
-        const uint32_t bits = 64u - (uint32_t)__builtin_clzll(hi - lo), shift = bits > 10u ? bits - 10u : 0u;
-        for (uint32_t i = threadIdx.x; i < kBins; i += 64u * kPickWaves) bins[i] = 0u;
-        __syncthreads();
+        const uint32_t bits = 64u - (uint32_t)__builtin_clzll(hi - lo);
+        const uint32_t shift = bits > kBits ? bits - kBits : 0u;
+        *(uint4 *)(bins + 4u * tid) = make_uint4(0u, 0u, 0u, 0u);
+        sync();
         each([&](uint32_t, uint64_t k, bool real) {
             if (real && k >= lo && k <= hi) atomicAdd(&bins[(uint32_t)((k - lo) >> shift)], 1u);
         });
-        __syncthreads();
+        sync();
         // thread i has four bins from the top down: how many keys lie above them, and where m is passed
-        uint32_t c[4], sum = 0u;
+        const uint4 z = *(const uint4 *)(bins + kBins - 4u - 4u * tid);
+        const uint32_t c[4] = { z.w, z.z, z.y, z.x }, sum = (z.x + z.y) + (z.z + z.w);
+        uint32_t above = wave_scan(sum);
+        if constexpr (WAVES > 1u) {
+            if (lane == 63u) part[wave][0] = above;
+            sync();
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) { c[i] = bins[kBins - 1u - (4u * threadIdx.x + i)]; sum += c[i]; }
-        uint32_t above = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t v = (uint32_t)__shfl_up((int)above, d);
-            above += lane >= (uint32_t)d ? v : 0u;
+            for (uint32_t v = 0; v < WAVES; ++v) above += v < wave ? part[v][0] : 0u;
         }
-        if (lane == 63u) part[wave][0] = above;
-        __syncthreads();
         above -= sum;
 #pragma unroll
-        for (uint32_t v = 0; v < kPickWaves; ++v) above += v < wave ? part[v][0] : 0u;
-#pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
-            if (above < m && above + c[i] >= m) { found[0] = kBins - 1u - (4u * threadIdx.x + i); found[1] = above; found[2] = c[i]; }
+            if (above < m && above + c[i] >= m) { found[0] = kBins - 1u - (4u * tid + i); found[1] = above; found[2] = c[i]; }
             above += c[i];
         }
-        __syncthreads();
+        sync();
         lo += (uint64_t)found[0] << shift;
         hi = lesser(hi, lo + (((uint64_t)1 << shift) - 1u));
         m -= found[1];
         whole = found[2] == m;
     }
     // the cut: keys above hi, and of those from lo to hi all or, equal ones, the first m
-    uint32_t n_above = 0u, n_in = 0u;
-    each([&](uint32_t, uint64_t k, bool real) {
-        n_above += (uint32_t)__popcll(__ballot(real && k > hi));
-        n_in += (uint32_t)__popcll(__ballot(real && k >= lo && k <= hi));
-    });
-    if (lane == 0u) { part[wave][0] = n_above; part[wave][1] = n_in; }
-    __syncthreads();
-    uint32_t at = 0u, in = 0u;
+    uint32_t at = nf, in = 0u;
+    if constexpr (WAVES > 1u) {
+        uint32_t n_above = 0u, n_in = 0u;
+        each([&](uint32_t, uint64_t k, bool real) {
+            n_above += (uint32_t)__popcll(__ballot(real && k > hi));
+            n_in += (uint32_t)__popcll(__ballot(real && k >= lo && k <= hi));
+        });
+        sync();                                                    // (the bins' partial sums have been read)
+        if (lane == 0u) { part[wave][0] = n_above; part[wave][1] = n_in; }
+        sync();
 #pragma unroll
-    for (uint32_t v = 0; v < kPickWaves; ++v) {
-        at += v < wave ? part[v][0] : 0u;
-        in += v < wave ? part[v][1] : 0u;
+        for (uint32_t v = 0; v < WAVES; ++v) {
+            at += v < wave ? part[v][0] : 0u;
+            in += v < wave ? part[v][1] : 0u;
+        }
+        at += min(in, m);
     }
-    at += nf + min(in, m);
     const uint64_t below = (1ull << lane) - 1u;
-    each([&](uint32_t i, uint64_t k, bool real) {
+    each([&](uint32_t b, uint64_t k, bool real) {
         const bool mid = real && k >= lo && k <= hi;
         const uint64_t mids = __ballot(mid);
         const bool sel = (real && k > hi) || (mid && in + (uint32_t)__popcll(mids & below) < m);
         const uint64_t sels = __ballot(sel);
-        if (sel) out[at + (uint32_t)__popcll(sels & below)] = (int32_t)block(nf + i);
+        if (sel) out[at + (uint32_t)__popcll(sels & below)] = (int32_t)b;
         at += (uint32_t)__popcll(sels);
         in += (uint32_t)__popcll(mids);
     });
@@ -246,9 +384,12 @@ __global__ __launch_bounds__(64 * kPickWaves) void k_kv4_pick_blocks(Kv4SelectAr
 
 template <int D>
 static void launch_scores(const Kv4SelectArgs & a, hipStream_t s) {
-    const uint32_t tpt = a.G <= 16u ? 16u / a.G : 1u;
-    hipLaunchKernelGGL(k_kv4_scores<D>, dim3(a.n_head_kv * ((a.n_blocks + 16u * kScoreWaves - 1u) / (16u * kScoreWaves)), (a.T + tpt - 1u) / tpt),
-                       dim3(64u * kScoreWaves), 0, s, a);
+    const uint32_t all = (a.n_blocks + 16u * kScoreWaves - 1u) / (16u * kScoreWaves), tpt = a.G <= 16u ? 16u / a.G : 1u;
+    const uint32_t lists = a.T * a.n_head_kv, parts = a.T == 1u ? all : min(all, max(1u, 1024u / lists));
+    const dim3 grid(a.n_head_kv * parts, a.T), wg(64u * kScoreWaves);
+    if (a.T >= 64u) hipLaunchKernelGGL(k_kv4_scores_many<D>, dim3(a.n_head_kv * all, (a.T + tpt - 1u) / tpt), wg, 0, s, a);
+    else if (a.G <= 4u) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_kv4_scores<D, 1>), grid, wg, 0, s, a, parts);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_kv4_scores<D, 2>), grid, wg, 0, s, a, parts);
 }
 
 }  // namespace tsr
@@ -263,10 +404,12 @@ int tsr_launch_kv4_select(const tsr::Kv4SelectArgs & a, hipStream_t s) {
             default: return -2;
         }
     }
-    const dim3 grid(a.n_head_kv, a.T), wg(64u * tsr::kPickWaves);
-    const uint32_t rows = (a.n_blocks + 64u * tsr::kPickWaves - 1u) / (64u * tsr::kPickWaves);
-    if (rows <= 2u) hipLaunchKernelGGL(tsr::k_kv4_pick_blocks<2>, grid, wg, 0, s, a);
-    else if (rows <= 16u) hipLaunchKernelGGL(tsr::k_kv4_pick_blocks<16>, grid, wg, 0, s, a);
-    else hipLaunchKernelGGL(tsr::k_kv4_pick_blocks<0>, grid, wg, 0, s, a);
+    const uint32_t lists = a.T * a.n_head_kv;
+    const dim3 grid(lists), grid4((lists + 3u) / 4u), wg(1024), wg4(256);
+    if (a.n_blocks <= 128u) hipLaunchKernelGGL(HIP_KERNEL_NAME(tsr::k_kv4_pick_blocks<2, 1>), grid4, wg4, 0, s, a);
+    else if (a.n_blocks <= 512u) hipLaunchKernelGGL(HIP_KERNEL_NAME(tsr::k_kv4_pick_blocks<8, 1>), grid4, wg4, 0, s, a);
+    else if (a.n_blocks <= 2048u) hipLaunchKernelGGL(HIP_KERNEL_NAME(tsr::k_kv4_pick_blocks<2, 16>), grid, wg, 0, s, a);
+    else if (a.n_blocks <= 8192u) hipLaunchKernelGGL(HIP_KERNEL_NAME(tsr::k_kv4_pick_blocks<8, 16>), grid, wg, 0, s, a);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(tsr::k_kv4_pick_blocks<0, 16>), grid, wg, 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
