@@ -742,10 +742,11 @@ struct Attn4 {
 
     // run() over listed tiles, for rows that see the same cells (one token's): entry(j) of the list, j < total, is a tile or one
     // behind all cells; the wave takes every parts-th. 64 entries at a time, those that its rows see whole come first, in
-    // `list` (64 words of LDS, the wave's own) and from there one a lane; a second pass takes those that they see in part.
+    // `list` (64 words of LDS, the wave's own) and from there one a lane; a second pass takes those that they see in part. e0: the
+    // lane's entry of the first 64, which the caller asks for ahead of everything else.
     template <class Entry>
-    __device__ __forceinline__ void run_list(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, uint32_t total, Entry entry,
-                                             uint32_t * list, h8 * lds, uint32_t wave, uint32_t lane) {
+    __device__ __forceinline__ void run_list(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, uint32_t total, uint32_t e0,
+                                             Entry entry, uint32_t * list, h8 * lds, uint32_t wave, uint32_t lane) {
         constexpr size_t tb = kv4_tile_bytes(TYPE);
         const size_t pair = (size_t)a.n_tiles * tb;
         const uint8_t * kp = a.k + kKv4Header + (size_t)h * (D / 64) * pair, * vp = a.v + kKv4Header + (size_t)h * (D / 64) * pair;
@@ -756,7 +757,7 @@ struct Attn4 {
             bool mine = false;
             uint32_t i = 0u;
             if (j < total) {
-                i = entry(j);
+                i = round == 0u ? e0 : entry(j);
                 const uint32_t c0 = 32u * min(i, 0x03FFFFFFu), c1 = c0 + 32u;   // (cells stay below 2^31)
                 const bool w = (r.lo0 <= c0 && r.hi0 >= c1) || (r.lo1 <= c0 && r.hi1 >= c1);
                 const bool some = (r.lo0 < r.hi0 && r.lo0 < c1 && r.hi0 > c0) || (r.lo1 < r.hi1 && r.lo1 < c1 && r.hi1 > c0);

@@ -28,9 +28,11 @@ __global__ __launch_bounds__(256, waves_of(D, 1, C, TYPE)) void k_attn4_blocks(A
         const uint32_t i = j / per, id = (uint32_t)ids[i];
         return id < n_blocks ? id * per + (j - i * per) : ~0u;
     };
+    const uint32_t part = split * kWaves + wave, parts = a.S * kWaves, total = b.n_sel * per;
+    const uint32_t e0 = entry(min(part + parts * lane, total - 1u));
     A w;
     w.load_runs(a, h, r0, lane);
-    w.run_list(a, h, split * kWaves + wave, a.S * kWaves, b.n_sel * per, entry, list[wave], (h8 *)room, wave, lane);
+    w.run_list(a, h, part, parts, total, e0, entry, list[wave], (h8 *)room, wave, lane);
     w.finish();
     auto place = [&](uint32_t r) { return a.S > 1u ? a.part + attn4_part_row(nr, D, split, row0 + r) : out + (size_t)r * D; };
     auto sums = [&](uint32_t r, float m, float l) { *(float2 *)(a.part + attn4_part_sum(nr, D, a.S, split, row0 + r)) = make_float2(m, l); };
