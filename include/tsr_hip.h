@@ -429,6 +429,22 @@ int tsr_hip_flash_attn_kv4_blocks(tsr_hip_ctx * ctx, const float * q_dev, uint32
 size_t tsr_hip_flash_attn_kv4_blocks_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_sel,
                                         uint32_t block);
 
+/* ---- eviction by attention weight -----------------------------------------------------------------
+ * For a context that outgrows its cache: what each cell gets of the tokens' attention, the cells that get most, and their
+ * move to the front of the cache. No counterpart in the reference. */
+
+/* out_dev[c] = decay * before_dev[c] + sum over tokens t and query heads of softmax(scale q K^T)[c], c < n_kv (f32): the weights that
+ * tsr_hip_flash_attn_kv4 of the same arguments gives cell c (0 of rows that do not see it, and of rows that see nothing). Scores
+ * and precision as there; no mask. before_dev NULL or decay 0: no addend, before_dev is not read; before_dev may be out_dev. The
+ * sums' order is fixed: the same call gives the same bits.
+ *   kc             a 4-bit K cache, E = n_head_kv * D
+ *   runs_dev       as tsr_hip_flash_attn_kv4
+ *   ws_dev         tsr_hip_attn_weights_kv4_ws(...) bytes, with tsr_hip_flash_attn_kv4's rules (never of 0 bytes for n_kv > 0) */
+int tsr_hip_attn_weights_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const tsr_hip_kv * kc, uint32_t D,
+                             uint32_t n_head, uint32_t n_head_kv, float scale, uint32_t n_kv, const uint32_t * runs_dev,
+                             const float * before_dev, float decay, float * out_dev, void * ws_dev, size_t ws_bytes, void * stream);
+size_t tsr_hip_attn_weights_kv4_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_kv);
+
 /* ---- decode-layer glue ops ----------------------------------------------------------------------
  * The f32 ops around MUL_MAT and FLASH_ATTN in a decoder layer, on the vector unit's f32 rules
  * (every input denormal-as-zero, one IEEE round-to-nearest-even operation, result flushed to zero,

@@ -1,0 +1,246 @@
+// k_attn4_weights.hip -- the attention weight that each cell of a 4-bit K cache gets, summed over tokens and query heads:
+// out[c] = decay before[c] + sum over rows of exp(s[row][c] - max[row]) / sum[row], s the scores of attn4.hpp.
+//
+// A row's sum has to be known before any of its weights is, and the weights of all rows are too many to keep (64 tokens of 32 heads
+// behind 32768 cells: 268 MB), so that the scores are made twice, from the codes, which stay in the caches:
+//   k_attn4_rowsums  every row's maximum and sum of exp2, a lane a row and a quarter of the cells, joined over lanes and waves
+//   k_attn4_weights  the weights of a workgroup's rows, summed over them: a lane sums its row of each group of 16, the 16 lanes
+//                    then meet; 32 sums a tile and row set go to memory
+//   k_attn4_cells    the row sets' sums added up, in their order: no atomic decides a rounding
+// A workgroup's waves have the same rows (up to four groups of 16: nothing but scores to hold) and take tiles in turn.
+#include "attn4.hpp"
+#include "weights4_plan.hpp"
+
+namespace tsr {
+
+template <int D, int NT, uint32_t TYPE>
+struct Weights4 : Attn4<D, NT, 1, TYPE> {
+    using A = Attn4<D, NT, 1, TYPE>;
+    using typename A::Tl;
+    using typename A::Span;
+
+    // The lane's cells of tile i that its row n sees: bit 4 u + k its cell 16 u + 4 g + k.
+    __device__ __forceinline__ uint32_t seen(int n, uint32_t i, uint32_t g) const {
+        uint32_t v = 0u;
+#pragma unroll
+        for (uint32_t u = 0; u < 2u; ++u)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) v |= this->sees(n, 32u * i + 16u * u + 4u * g + k) ? 1u << (4u * u + k) : 0u;
+        return v;
+    }
+
+    // one(tile's codes, its number, whether every row sees all of it) for the wave's tiles, every parts-th; none(number) for
+    // those that no row sees. `lds`: the queries' pieces go there first.
+    template <class One, class None>
+    __device__ __forceinline__ void walk(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, h8 * lds, uint32_t wave, uint32_t lane,
+                                         One one, None none) {
+        constexpr size_t tb = kv4_tile_bytes(TYPE);
+        const size_t pair = (size_t)a.n_tiles * tb;
+        const uint8_t * kp = a.k + kKv4Header + (size_t)h * (D / 64) * pair;
+        Span w0, w1, all;
+        this->spans(a, w0, w1, all);
+        const uint32_t n0 = w0.size(), nw = n0 + w1.size();
+        const uint32_t cnt = part < nw ? (nw - 1u - part) / parts + 1u : 0u;
+        auto nth = [&](uint32_t x) {                               // (past the last: it again)
+            const uint32_t j = part + min(x, cnt - 1u) * parts;
+            return j < n0 ? w0.lo + j : w1.lo + (j - n0);
+        };
+        Tl k0, k1;
+        if (cnt != 0u) {
+            A::template load<false>(k0, kp + nth(0u) * tb, pair, lane);
+            A::template load<false>(k1, kp + nth(1u) * tb, pair, lane);
+        }
+        this->load_queries(a.scale, lane, lds, wave);
+        __syncthreads();
+        for (uint32_t x = 0; x < cnt; x += 2u) {                   // two tiles ahead
+            one(k0, nth(x), true);
+            A::template load<false>(k0, kp + nth(x + 2u) * tb, pair, lane);
+            if (x + 1u < cnt) one(k1, nth(x + 1u), true);
+            A::template load<false>(k1, kp + nth(x + 3u) * tb, pair, lane);
+        }
+        // the others: what is left of all tiles, dealt on from the wave after the one that took the last whole tile
+        const uint32_t g0 = w0.lo, g1 = g0 + (w1.lo - w0.hi), np = (a.n_kv + 31u) / 32u - nw;
+        auto other = [&](uint32_t y) { return y < g0 ? y : y < g1 ? w0.hi + (y - g0) : w1.hi + (y - g1); };
+        uint32_t x = part + parts - nw % parts;
+        x = x >= parts ? x - parts : x;
+        for (; x < np; x += parts) {
+            const uint32_t i = other(x);
+            if (!this->any(i)) {
+                none(i);
+                continue;
+            }
+            A::template load<false>(k0, kp + i * tb, pair, lane);
+            one(k0, i, false);
+        }
+    }
+};
+
+constexpr int weights_waves(int D, int NT) { return D * NT <= 128 ? 4 : D <= 256 ? 2 : 1; }
+
+// Workgroup (KV head, split, row set), KV heads fastest.
+template <int D, int NT, uint32_t TYPE>
+__global__ __launch_bounds__(256, weights_waves(D, NT)) void k_attn4_rowsums(Attn4Args a, Weights4Plan p) {
+    using W = Weights4<D, NT, TYPE>;
+    __shared__ __align__(16) uint8_t room[W::kQ];
+    __shared__ float2 ml[kWaves][16 * NT];
+    const uint32_t h = blockIdx.x, split = blockIdx.y, rg = blockIdx.z, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+    W w;
+    w.load_runs(a, h, rg * 16u * NT, lane);
+    w.walk(a, h, split * kWaves + wave, a.S * kWaves, (h8 *)room, wave, lane,
+           [&](const typename W::Tl & k, uint32_t i, bool whole) {
+               f4 s[NT][2];
+               uint32_t ql = lane;                                 // (q's pieces: read from LDS for every tile)
+               asm volatile("" : "+v"(ql));
+               w.scores(k, (h8 *)room + ql, s);
+#pragma unroll
+               for (int n = 0; n < NT; ++n) {
+                   const uint32_t in = whole ? 0xFFu : w.seen(n, i, g);
+                   float top = -__builtin_inff();
+#pragma unroll
+                   for (int u = 0; u < 2; ++u)
+#pragma unroll
+                       for (int c = 0; c < 4; ++c) {
+                           const float x = s[n][u][c] * w.csc[n];
+                           s[n][u][c] = whole || ((in >> (4 * u + c)) & 1u) ? x : -__builtin_inff();
+                           top = fmaxf(top, s[n][u][c]);
+                       }
+                   const float m = fmaxf(w.m[n], top), sub = m == -__builtin_inff() ? 0.0f : m;
+                   float l = w.l[n] * __builtin_amdgcn_exp2f(w.m[n] - sub);
+#pragma unroll
+                   for (int u = 0; u < 2; ++u)
+#pragma unroll
+                       for (int c = 0; c < 4; ++c) l += __builtin_amdgcn_exp2f(s[n][u][c] - sub);
+                   w.m[n] = m;
+                   w.l[n] = l;
+               }
+           },
+           [](uint32_t) {});
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const float m = rows_max(w.m[n]), f = w.m[n] == m ? 1.0f : __builtin_amdgcn_exp2f(w.m[n] - m), l = rows_sum(w.l[n] * f);
+        if (g == 0u) ml[wave][16 * n + lane] = make_float2(m, l);
+    }
+    __syncthreads();
+    const uint32_t r = threadIdx.x;
+    if (r < 16u * NT) {
+        float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+        for (uint32_t v = 0; v < kWaves; ++v) m = fmaxf(m, ml[v][r].x);
+#pragma unroll
+        for (uint32_t v = 0; v < kWaves; ++v) l += ml[v][r].y * (ml[v][r].x == m ? 1.0f : __builtin_amdgcn_exp2f(ml[v][r].x - m));
+        ((float2 *)a.part)[weights4_pair(p, a.n_head_kv, split, h, rg, r)] = make_float2(m, l);
+    }
+}
+
+template <int D, int NT, uint32_t TYPE>
+__global__ __launch_bounds__(256, weights_waves(D, NT)) void k_attn4_weights(Attn4Args a, Weights4Plan p) {
+    using W = Weights4<D, NT, TYPE>;
+    __shared__ __align__(16) uint8_t room[W::kQ];
+    const uint32_t h = blockIdx.x, split = blockIdx.y, rg = blockIdx.z, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+    W w;
+    w.load_runs(a, h, rg * 16u * NT, lane);
+    // each row's maximum and the inverse of its sum over the splits, the four lanes of a row taking them in turn
+    float M[NT], il[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const float2 * pairs = (const float2 *)a.part + weights4_pair(p, a.n_head_kv, 0u, h, rg, 16u * n + (lane & 15u));
+        const size_t step = weights4_pair(p, a.n_head_kv, 1u, 0u, 0u, 0u);
+        float m = -__builtin_inff(), l = 0.0f;
+        for (uint32_t s = g; s < a.S; s += 4u) {
+            const float2 x = pairs[s * step];
+            const float z = fmaxf(m, x.x);
+            l = l * (m == z ? 1.0f : __builtin_amdgcn_exp2f(m - z)) + x.y * (x.x == z ? 1.0f : __builtin_amdgcn_exp2f(x.x - z));
+            m = z;
+        }
+        M[n] = rows_max(m);
+        l = rows_sum(l * (m == M[n] ? 1.0f : __builtin_amdgcn_exp2f(m - M[n])));
+        const bool empty = l == 0.0f || rg * 16u * NT + 16u * n + (lane & 15u) >= a.T * a.G;
+        il[n] = empty ? 0.0f : 1.0f / l;
+        M[n] = empty ? 0.0f : M[n];
+    }
+    float * sums = (float *)((uint8_t *)a.part + p.sums) + ((size_t)h * p.n_rg + rg) * p.n_pad;
+    w.walk(a, h, split * kWaves + wave, a.S * kWaves, (h8 *)room, wave, lane,
+           [&](const typename W::Tl & k, uint32_t i, bool whole) {
+               f4 s[NT][2];
+               uint32_t ql = lane;
+               asm volatile("" : "+v"(ql));
+               w.scores(k, (h8 *)room + ql, s);
+               float x[8] = {};
+#pragma unroll
+               for (int n = 0; n < NT; ++n) {
+                   const uint32_t in = il[n] == 0.0f ? 0u : whole ? 0xFFu : w.seen(n, i, g);
+#pragma unroll
+                   for (int c = 0; c < 8; ++c) {
+                       const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][c >> 2][c & 3], w.csc[n], -M[n]));
+                       x[c] += (in >> c) & 1u ? e * il[n] : 0.0f;
+                   }
+               }
+               // over the 16 lanes of a row of the wave: halves handed over between lanes 7 - x and x, 2 and 1 apart; then all eight
+               const bool b2 = (lane & 4u) != 0u, b1 = (lane & 2u) != 0u, b0 = (lane & 1u) != 0u;
+#pragma unroll
+               for (int c = 0; c < 4; ++c) x[c] = (b2 ? x[c + 4] : x[c]) + dpp_f<kDppRowHalfMirror>(b2 ? x[c] : x[c + 4]);
+#pragma unroll
+               for (int c = 0; c < 2; ++c) x[c] = (b1 ? x[c + 2] : x[c]) + dpp_f<kDppXor2>(b1 ? x[c] : x[c + 2]);
+               x[0] = (b0 ? x[1] : x[0]) + dpp_f<kDppXor1>(b0 ? x[0] : x[1]);
+               x[0] += dpp_f<kDppRowMirror>(dpp_f<kDppRowHalfMirror>(x[0]));   // (lane l and l ^ 8)
+               if ((lane & 8u) == 0u) sums[32u * i + 16u * ((lane >> 2) & 1u) + 4u * g + (lane & 3u)] = x[0];
+           },
+           [&](uint32_t i) {
+               if (lane < 32u) sums[32u * i + lane] = 0.0f;
+           });
+}
+
+// Cells' sums over n row sets: 64 cells a workgroup, its four waves every fourth row set, joined in their order.
+__global__ __launch_bounds__(256) void k_attn4_cells(const float * sums, uint32_t n, uint32_t n_pad, uint32_t n_kv, const float * before, float decay,
+                                                     float * out) {
+    __shared__ float part[4][64];
+    const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u, c = blockIdx.x * 64u + lane;
+    float x = 0.0f;
+    if (c < n_kv)
+        for (uint32_t i = wave; i < n; i += 4u) x += sums[(size_t)i * n_pad + c];
+    part[wave][lane] = x;
+    __syncthreads();
+    if (wave == 0u && c < n_kv) {
+        x = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+        out[c] = before == nullptr ? x : __builtin_fmaf(decay, before[c], x);
+    }
+}
+
+template <int D, int NT, uint32_t TYPE>
+static int launch_weights(const Attn4Args & a, const Weights4Plan & p, hipStream_t s) {
+    const dim3 grid(a.n_head_kv, a.S, (a.T * a.G + 16u * NT - 1u) / (16u * NT)), wg(64u * kWaves);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4_rowsums<D, NT, TYPE>), grid, wg, 0, s, a, p);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4_weights<D, NT, TYPE>), grid, wg, 0, s, a, p);
+    return hipGetLastError() == hipSuccess ? 0 : -4;
+}
+
+template <uint32_t TYPE>
+static int launch_weights_t(const Attn4Args & a, const Weights4Plan & p, hipStream_t s) {
+    switch (a.D * 8u + p.NT) {
+        case 64 * 8 + 1: return launch_weights<64, 1, TYPE>(a, p, s);
+        case 64 * 8 + 2: return launch_weights<64, 2, TYPE>(a, p, s);
+        case 64 * 8 + 4: return launch_weights<64, 4, TYPE>(a, p, s);
+        case 128 * 8 + 1: return launch_weights<128, 1, TYPE>(a, p, s);
+        case 128 * 8 + 2: return launch_weights<128, 2, TYPE>(a, p, s);
+        case 128 * 8 + 4: return launch_weights<128, 4, TYPE>(a, p, s);
+        case 256 * 8 + 1: return launch_weights<256, 1, TYPE>(a, p, s);
+        case 256 * 8 + 2: return launch_weights<256, 2, TYPE>(a, p, s);
+        case 512 * 8 + 1: return launch_weights<512, 1, TYPE>(a, p, s);
+        default: return -2;
+    }
+}
+
+}  // namespace tsr
+
+int tsr_launch_attn4_weights(const tsr::Attn4Args & a, const tsr::Weights4Plan & p, const float * before, float decay, hipStream_t s) {
+    if (a.n_kv != 0u) {
+        const int rc = a.type == tsr::kKvQ4_0 ? tsr::launch_weights_t<tsr::kKvQ4_0>(a, p, s) : tsr::launch_weights_t<tsr::kKvQ4_1>(a, p, s);
+        if (rc) return rc;
+        const uint32_t n = a.n_head_kv * p.n_rg;
+        hipLaunchKernelGGL(tsr::k_attn4_cells, dim3((a.n_kv + 63u) / 64u), dim3(256), 0, s, (const float *)((uint8_t *)a.part + p.sums), n, p.n_pad,
+                           a.n_kv, before, decay, a.out);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -4;
+}

@@ -314,6 +314,9 @@ int tsr_launch_kv4_bounds(const tsr::Kv4BoundsArgs & a, hipStream_t s);
 // attention over a 4-bit cache, cut as attn4_plan.hpp says (k_attn4.hip)
 int tsr_launch_attn4(const tsr::Attn4Args & a, const tsr::Attn4Plan & p, hipStream_t s);
 int tsr_launch_attn4_blocks(const tsr::Attn4BlocksArgs & b, uint32_t C, hipStream_t s);
+// the weights that cells gather (k_attn4_weights.hip): out[c] = decay before[c] (none: 0) + their sum over rows, c < n_kv
+namespace tsr { struct Weights4Plan; }
+int tsr_launch_attn4_weights(const tsr::Attn4Args & a, const tsr::Weights4Plan & p, const float * before, float decay, hipStream_t s);
 // the splits' partial rows joined into the output
 int tsr_launch_attn4_join(const tsr::Attn4Args & a, hipStream_t s);
 int tsr_launch_fa(const tsr::FaArgs & a, const tsr::FaPlan & p, uint32_t T, uint32_t n_cu, hipStream_t s);

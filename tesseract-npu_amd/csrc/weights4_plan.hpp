@@ -1,0 +1,46 @@
+// weights4_plan.hpp -- how a call that sums attention weights a cell is cut, and its workspace. Plain C++.
+#pragma once
+
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+
+namespace tsr {
+
+constexpr uint32_t kWeightsSplits = 64u;
+
+struct Weights4Plan {
+    uint32_t NT;             // groups of 16 rows of a workgroup
+    uint32_t tokens;         // of a launch
+    uint32_t n_rg;           // workgroups' row sets of a KV head
+    uint32_t S;              // splits of the cells
+    uint32_t n_pad;          // cells in whole tiles
+    size_t sums;             // byte offset of the sums behind the (maximum, sum) pairs
+    size_t ws_bytes;
+};
+
+// (maximum, sum) of row r of a KV head's row set in one split, and the sums over a row set's rows for every cell.
+constexpr size_t weights4_pair(const Weights4Plan & p, uint32_t n_head_kv, uint32_t split, uint32_t h, uint32_t rg, uint32_t r) {
+    return ((size_t)split * n_head_kv * p.n_rg + (size_t)h * p.n_rg + rg) * (16u * p.NT) + r;
+}
+
+inline Weights4Plan weights4_plan(uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_kv, uint32_t n_cu) {
+    Weights4Plan p{};
+    const uint64_t G = n_head / n_head_kv, tiles = std::max<uint64_t>(1u, ((uint64_t)n_kv + 31u) / 32u);
+    // Four groups of rows share the unpacking of a tile's codes (heads up to 128, whose queries' pieces leave LDS for three workgroups)
+    // where there are that many rows; heads of 256 two.
+    const uint64_t R = T * G;
+    p.NT = D <= 128u && R > 32u ? 4u : D <= 256u && R > 16u ? 2u : 1u;
+    p.n_pad = (uint32_t)(32u * tiles);
+    // a launch's sums take at most 64 MiB, or are one token's
+    const uint64_t rows = 16u * p.NT, most = std::max<uint64_t>(1u, ((uint64_t)64 << 20) / (4u * (uint64_t)p.n_pad * n_head_kv));   // row sets of a KV head
+    p.tokens = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ T, most * rows / G, 16384u }));
+    p.n_rg = (uint32_t)((p.tokens * G + rows - 1u) / rows);
+    const uint64_t n = (uint64_t)n_head_kv * p.n_rg;
+    p.S = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ (2u * (uint64_t)n_cu + n - 1u) / n, (tiles + 3u) / 4u, kWeightsSplits }));
+    p.sums = 8u * (size_t)p.S * n * rows;
+    p.ws_bytes = p.sums + 4u * (size_t)n * p.n_pad;
+    return p;
+}
+
+}  // namespace tsr

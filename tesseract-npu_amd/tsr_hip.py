@@ -45,6 +45,7 @@ EXPORTS = (
     "tsr_hip_rope_scaled", "tsr_hip_rope_scaled_table",
     "tsr_hip_kv4_bounds", "tsr_hip_kv4_select", "tsr_hip_kv4_select_ws",
     "tsr_hip_flash_attn_kv4_blocks", "tsr_hip_flash_attn_kv4_blocks_ws",
+    "tsr_hip_attn_weights_kv4", "tsr_hip_attn_weights_kv4_ws",
 )
 
 
@@ -150,6 +151,8 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         "tsr_hip_flash_attn_kv4_blocks": ([vp, vp, u32, u64, vp, vp, u32, u32, u32, C.c_float, u32, vp, vp, u32, u32, vp, u64, vp,
                                            sz, vp], C.c_int),
         "tsr_hip_flash_attn_kv4_blocks_ws": ([vp, u32, u32, u32, u32, u32, u32], sz),
+        "tsr_hip_attn_weights_kv4": ([vp, vp, u32, u64, vp, u32, u32, u32, C.c_float, u32, vp, vp, C.c_float, vp, vp, sz, vp], C.c_int),
+        "tsr_hip_attn_weights_kv4_ws": ([vp, u32, u32, u32, u32, u32], sz),
         "tsr_hip_rope_scaled": ([vp, vp, u32, u64, u32, u32, u32, C.c_int, vp, C.POINTER(RopeScaling), vp, vp, u64, vp], C.c_int),
         "tsr_hip_rope_scaled_table": ([vp, vp, u32, C.POINTER(RopeScaling), vp, vp, vp], C.c_int),
     }
@@ -516,6 +519,17 @@ class Device:
         _check(self.L.tsr_hip_flash_attn_kv4_blocks(self.ctx, self._p(q), T, q_stride, kc.h, vc.h, D, n_head, n_head_kv, scale,
                                                     n_kv, self._p(runs), self._p(blocks), n_sel, block, self._p(out), out_stride,
                                                     self._p(ws), 0 if ws is None else ws.nbytes, stream), "flash_attn_kv4_blocks")
+
+    def attn_weights_kv4_ws(self, T: int, D: int, n_head: int, n_head_kv: int, n_kv: int) -> int:
+        """Bytes of workspace that attn_weights_kv4 needs."""
+        return int(self.L.tsr_hip_attn_weights_kv4_ws(self.ctx, T, D, n_head, n_head_kv, n_kv))
+
+    def attn_weights_kv4(self, q, T: int, q_stride: int, kc: KvCache, D: int, n_head: int, n_head_kv: int, scale: float, n_kv: int,
+                         out, before=None, decay: float = 1.0, runs=None, ws: "Buffer | None" = None, stream=None) -> None:
+        """The attention weight of each cell, summed over tokens and query heads, on top of decay * before (device f32 [n_kv])."""
+        _check(self.L.tsr_hip_attn_weights_kv4(self.ctx, self._p(q), T, q_stride, kc.h, D, n_head, n_head_kv, scale, n_kv,
+                                               self._p(runs), self._p(before), float(decay), self._p(out), self._p(ws),
+                                               0 if ws is None else ws.nbytes, stream), "attn_weights_kv4")
 
     def flash_attn(self, q, T: int, q_stride: int, kc: KvCache, vc: KvCache, D: int, n_head: int, n_head_kv: int,
                    scale: float, msum, out, out_stride: int, mask_f32=None, new_runs=None, stream=None) -> None:
