@@ -75,7 +75,7 @@ struct Weights4 : Attn4<D, NT, 1, TYPE> {
     }
 };
 
-constexpr int weights_waves(int D, int NT) { return D * NT <= 128 ? 4 : D <= 256 ? 2 : 1; }
+constexpr int weights_waves(int D, int NT) { return D * NT <= 128 ? 4 : D * NT <= 256 || D <= 128 ? 2 : 1; }
 
 // Workgroup (KV head, split, row set), KV heads fastest.
 template <int D, int NT, uint32_t TYPE>
@@ -87,38 +87,38 @@ __global__ __launch_bounds__(256, weights_waves(D, NT)) void k_attn4_rowsums(Att
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
     W w;
     w.load_runs(a, h, rg * 16u * NT, lane);
+    float sub[NT] = {};                                            // the maxima in base 2 (0: none yet)
     w.walk(a, h, split * kWaves + wave, a.S * kWaves, (h8 *)room, wave, lane,
            [&](const typename W::Tl & k, uint32_t i, bool whole) {
                f4 s[NT][2];
                uint32_t ql = lane;                                 // (q's pieces: read from LDS for every tile)
                asm volatile("" : "+v"(ql));
                w.scores(k, (h8 *)room + ql, s);
+               // maxima of the scores in the row's own unit, which is positive; a lane's sum is in units of its maximum's exp2
 #pragma unroll
                for (int n = 0; n < NT; ++n) {
-                   const uint32_t in = whole ? 0xFFu : w.seen(n, i, g);
-                   float top = -__builtin_inff();
+                   if (!whole) {
+                       const uint32_t in = w.seen(n, i, g);
 #pragma unroll
-                   for (int u = 0; u < 2; ++u)
+                       for (int c = 0; c < 8; ++c) s[n][c >> 2][c & 3] = (in >> c) & 1u ? s[n][c >> 2][c & 3] : -__builtin_inff();
+                   }
+                   float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])), s[n][1][0]);
+                   top = fmaxf(fmaxf(fmaxf(top, s[n][1][1]), s[n][1][2]), s[n][1][3]);
+                   if (__ballot(top > w.m[n])) {
+                       const float m = fmaxf(w.m[n], top);
+                       w.l[n] = w.m[n] == m ? w.l[n] : w.l[n] * __builtin_amdgcn_exp2f((w.m[n] - m) * w.csc[n]);
+                       w.m[n] = m;
+                       sub[n] = m == -__builtin_inff() ? 0.0f : m * w.csc[n];
+                   }
 #pragma unroll
-                       for (int c = 0; c < 4; ++c) {
-                           const float x = s[n][u][c] * w.csc[n];
-                           s[n][u][c] = whole || ((in >> (4 * u + c)) & 1u) ? x : -__builtin_inff();
-                           top = fmaxf(top, s[n][u][c]);
-                       }
-                   const float m = fmaxf(w.m[n], top), sub = m == -__builtin_inff() ? 0.0f : m;
-                   float l = w.l[n] * __builtin_amdgcn_exp2f(w.m[n] - sub);
-#pragma unroll
-                   for (int u = 0; u < 2; ++u)
-#pragma unroll
-                       for (int c = 0; c < 4; ++c) l += __builtin_amdgcn_exp2f(s[n][u][c] - sub);
-                   w.m[n] = m;
-                   w.l[n] = l;
+                   for (int c = 0; c < 8; ++c) w.l[n] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][c >> 2][c & 3], w.csc[n], -sub[n]));
                }
            },
            [](uint32_t) {});
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const float m = rows_max(w.m[n]), f = w.m[n] == m ? 1.0f : __builtin_amdgcn_exp2f(w.m[n] - m), l = rows_sum(w.l[n] * f);
+        const float m0 = w.m[n] == -__builtin_inff() ? w.m[n] : sub[n], m = rows_max(m0);
+        const float l = rows_sum(w.l[n] * (m0 == m ? 1.0f : __builtin_amdgcn_exp2f(m0 - m)));
         if (g == 0u) ml[wave][16 * n + lane] = make_float2(m, l);
     }
     __syncthreads();
@@ -147,18 +147,20 @@ __global__ __launch_bounds__(256, weights_waves(D, NT)) void k_attn4_weights(Att
     for (int n = 0; n < NT; ++n) {
         const float2 * pairs = (const float2 *)a.part + weights4_pair(p, a.n_head_kv, 0u, h, rg, 16u * n + (lane & 15u));
         const size_t step = weights4_pair(p, a.n_head_kv, 1u, 0u, 0u, 0u);
+        float2 x[kWeightsSplits / 4];                              // (all on their way at once)
+#pragma unroll
+        for (uint32_t j = 0; j < kWeightsSplits / 4; ++j)
+            x[j] = g + 4u * j < a.S ? pairs[(g + 4u * j) * step] : make_float2(-__builtin_inff(), 0.0f);
         float m = -__builtin_inff(), l = 0.0f;
-        for (uint32_t s = g; s < a.S; s += 4u) {
-            const float2 x = pairs[s * step];
-            const float z = fmaxf(m, x.x);
-            l = l * (m == z ? 1.0f : __builtin_amdgcn_exp2f(m - z)) + x.y * (x.x == z ? 1.0f : __builtin_amdgcn_exp2f(x.x - z));
-            m = z;
-        }
+#pragma unroll
+        for (uint32_t j = 0; j < kWeightsSplits / 4; ++j) m = fmaxf(m, x[j].x);
+#pragma unroll
+        for (uint32_t j = 0; j < kWeightsSplits / 4; ++j) l += x[j].y * (x[j].x == m ? 1.0f : __builtin_amdgcn_exp2f(x[j].x - m));
         M[n] = rows_max(m);
         l = rows_sum(l * (m == M[n] ? 1.0f : __builtin_amdgcn_exp2f(m - M[n])));
         const bool empty = l == 0.0f || rg * 16u * NT + 16u * n + (lane & 15u) >= a.T * a.G;
         il[n] = empty ? 0.0f : 1.0f / l;
-        M[n] = empty ? 0.0f : M[n];
+        M[n] = empty ? __builtin_inff() : M[n];                    // (weights of 0, whatever the scores are)
     }
     float * sums = (float *)((uint8_t *)a.part + p.sums) + ((size_t)h * p.n_rg + rg) * p.n_pad;
     w.walk(a, h, split * kWaves + wave, a.S * kWaves, (h8 *)room, wave, lane,
@@ -170,11 +172,12 @@ __global__ __launch_bounds__(256, weights_waves(D, NT)) void k_attn4_weights(Att
                float x[8] = {};
 #pragma unroll
                for (int n = 0; n < NT; ++n) {
-                   const uint32_t in = il[n] == 0.0f ? 0u : whole ? 0xFFu : w.seen(n, i, g);
+                   const uint32_t in = whole ? 0xFFu : w.seen(n, i, g);
 #pragma unroll
                    for (int c = 0; c < 8; ++c) {
                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][c >> 2][c & 3], w.csc[n], -M[n]));
-                       x[c] += (in >> c) & 1u ? e * il[n] : 0.0f;
+                       const float z = __builtin_fmaf(e, il[n], x[c]);
+                       x[c] = whole || ((in >> c) & 1u) ? z : x[c];
                    }
                }
                // over the 16 lanes of a row of the wave: halves handed over between lanes 7 - x and x, 2 and 1 apart; then all eight
