@@ -445,6 +445,23 @@ int tsr_hip_attn_weights_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T,
                              const float * before_dev, float decay, float * out_dev, void * ws_dev, size_t ws_bytes, void * stream);
 size_t tsr_hip_attn_weights_kv4_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_kv);
 
+/* The n_keep of n_kv cells that are kept, idx_dev[0 .. n_keep - 1] (int64, 8-byte aligned) ascending: the n_first first, the n_last
+ * last (n_first + n_last <= n_keep <= n_kv < 2^31) and of those between the ones with the largest weights_dev[c] (f32), equal ones the
+ * lowest cells, a NaN below every number. kept_dev (nullable, not weights_dev): their weights in that order, the addend of a next
+ * tsr_hip_attn_weights_kv4 over the moved cells. */
+int tsr_hip_kv_pick(tsr_hip_ctx * ctx, const float * weights_dev, uint32_t n_kv, uint32_t n_keep, uint32_t n_first, uint32_t n_last,
+                    int64_t * idx_dev, float * kept_dev, void * stream);
+
+/* Cell i of plane dst becomes cell idx_dev[i] (int64, 8-byte aligned) of plane src, i < n <= dst's kv_size, bit for bit; both of one
+ * type (any) and row length and of the same `which`. dst may be src: every cell is read before any is written (through the
+ * workspace, tsr_hip_kv_gather_ws(ctx, src, n) bytes with tsr_hip_flash_attn_kv4's rules; another dst needs none), in any order of the
+ * list, which may name a cell twice. An index outside src leaves its cell as it was and sets *bad_dev (nullable: the context's
+ * flag). Cells from n on are left as they were, but with dst src the up to 31 that share the last one's group of 32 are written with what
+ * they hold: nothing else writes the cache meanwhile. */
+int tsr_hip_kv_gather(tsr_hip_ctx * ctx, tsr_hip_kv * dst, const tsr_hip_kv * src, uint32_t which, const int64_t * idx_dev, uint32_t n,
+                      int32_t * bad_dev, void * ws_dev, size_t ws_bytes, void * stream);
+size_t tsr_hip_kv_gather_ws(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t n);
+
 /* ---- decode-layer glue ops ----------------------------------------------------------------------
  * The f32 ops around MUL_MAT and FLASH_ATTN in a decoder layer, on the vector unit's f32 rules
  * (every input denormal-as-zero, one IEEE round-to-nearest-even operation, result flushed to zero,

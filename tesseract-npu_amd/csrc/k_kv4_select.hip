@@ -9,23 +9,15 @@
 // k_kv4_scores is a product of bounds and queries on the f64 matrix instruction 4x4x4 (four of them at once: 16 blocks by
 // four query heads, each channel once with q and once with |q|), 18 cycles an instruction; k_kv4_scores_many on 16x16x4, 64 cycles,
 // whose 16 columns several tokens fill that look at the same blocks. What leaves is a key a block, an unsigned number in
-// the order of the scores. k_kv4_pick_blocks then finds the cut: the keys' range is counted into bins, the bin with the cut becomes
-// the range, until all of a bin is taken or it is one value; two or three passes do for a few thousand keys. Both are a few
-// microseconds of waiting for memory and for each other's steps, not work: reductions and scans run on DPP, keys are asked for
-// before the runs that say which of them count.
+// the order of the scores. k_kv4_pick_blocks then finds the cut (pick.hpp). Both are a few microseconds of waiting for memory
+// and for each other's steps, not work: reductions and scans run on DPP, keys are asked for before the runs that say which
+// of them count.
 #include "kernels.hpp"
-#include "tsr_dev.hpp"
-#include "wave_lds.hpp"
+#include "pick.hpp"
 
 namespace tsr {
 
 typedef double d4 __attribute__((ext_vector_type(4)));
-
-// The order of f64 as unsigned numbers; a NaN is the lowest.
-__device__ __forceinline__ uint64_t order_of(double x) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    return x != x ? 0u : u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
-}
 
 constexpr uint32_t kScoreWaves = 4u;
 
@@ -215,28 +207,6 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores_many(Kv4SelectA
     }
 }
 
-__device__ __forceinline__ uint64_t lesser(uint64_t a, uint64_t b) { return a < b ? a : b; }
-// Over the wave: the least, and the sum of the lanes up to each (row shifts, then broadcasts of the rows' ends).
-__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
-    v = min(v, (uint32_t)dpp_i<kDppXor1>((int)v));
-    v = min(v, (uint32_t)dpp_i<kDppXor2>((int)v));
-    v = min(v, (uint32_t)dpp_i<kDppRowHalfMirror>((int)v));
-    v = min(v, (uint32_t)dpp_i<kDppRowMirror>((int)v));
-    auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = min(x[0], x[1]);
-    auto y = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return min(y[0], y[1]);
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
-    return v;
-}
-
 constexpr uint32_t pick_waves(uint32_t WAVES) { return WAVES == 1u ? 4u : WAVES; }   // of a workgroup
 
 // WAVES 16: a workgroup a token and KV head; WAVES 1: each of its four waves. The keys lie in the waves' registers, wave w of a
@@ -244,16 +214,10 @@ constexpr uint32_t pick_waves(uint32_t WAVES) { return WAVES == 1u ? 4u : WAVES;
 // are needed.
 template <uint32_t ROWS, uint32_t WAVES>
 __global__ __launch_bounds__(64 * pick_waves(WAVES)) void k_kv4_pick_blocks(Kv4SelectArgs a) {
-    constexpr uint32_t LISTS = pick_waves(WAVES) / WAVES, kBins = 256u * WAVES, kBits = WAVES == 1u ? 8u : 12u;
-    static_assert(kBins == 1u << kBits, "bins");
-    __shared__ uint32_t room[LISTS][kBins], parts[LISTS][WAVES][2], founds[LISTS][3];
+    constexpr uint32_t LISTS = pick_waves(WAVES) / WAVES;
+    __shared__ __align__(16) PickRoom<WAVES> room[LISTS];
     const uint32_t wv = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u;
     const uint32_t list = WAVES == 1u ? wv : 0u, wave = WAVES == 1u ? 0u : wv, tid = 64u * wave + lane;
-    uint32_t * bins = room[list], (*part)[2] = parts[list], * found = founds[list];
-    auto sync = [] {
-        if constexpr (WAVES == 1u) own_room();
-        else __syncthreads();
-    };
     const uint32_t id = blockIdx.x * LISTS + list;                 // token and KV head
     if (id >= a.T * a.n_head_kv) return;
     const uint32_t t = id / a.n_head_kv;
@@ -289,7 +253,6 @@ __global__ __launch_bounds__(64 * pick_waves(WAVES)) void k_kv4_pick_blocks(Kv4S
         else if (i >= a.n_sel - a.n_last) out[i] = (int32_t)block(n - (a.n_sel - i));
     }
     if (n <= a.n_sel || a.n_sel == nf + a.n_last) return;
-    uint32_t m = a.n_sel - nf - a.n_last;                          // wanted of the others
     // f(block, key, whether it is one of them) for every row of the wave, the lanes together
     auto each = [&](auto f) {
         auto one = [&](uint32_t j, uint64_t k) {
@@ -305,81 +268,8 @@ __global__ __launch_bounds__(64 * pick_waves(WAVES)) void k_kv4_pick_blocks(Kv4S
             for (uint32_t j = 0; j < rows; ++j) one(j, keys[min(from + (wave * rows + j) * 64u + lane, a.n_blocks - 1u)]);
         }
     };
-    uint32_t least = ~0u, most = 0u;                               // of the keys' high words
-    each([&](uint32_t, uint64_t k, bool real) {
-        least = real ? min(least, (uint32_t)(k >> 32)) : least;
-        most = real ? max(most, (uint32_t)(k >> 32)) : most;
-    });
-    least = wave_min(least);
-    most = ~wave_min(~most);
-    if constexpr (WAVES > 1u) {
-        if (lane == 0u) { part[wave][0] = least; part[wave][1] = most; }
-        sync();
-#pragma unroll
-        for (uint32_t v = 0; v < WAVES; ++v) { least = min(least, part[v][0]); most = max(most, part[v][1]); }
-    }
-    uint64_t lo = (uint64_t)least << 32, hi = (uint64_t)most << 32 | 0xFFFFFFFFu;
-    // keys above hi are taken, those below lo are not, m of those between are
-    bool whole = false;
-    while (!whole && lo != hi) {
-        const uint32_t bits = 64u - (uint32_t)__builtin_clzll(hi - lo);
-        const uint32_t shift = bits > kBits ? bits - kBits : 0u;
-        *(uint4 *)(bins + 4u * tid) = make_uint4(0u, 0u, 0u, 0u);
-        sync();
-        each([&](uint32_t, uint64_t k, bool real) {
-            if (real && k >= lo && k <= hi) atomicAdd(&bins[(uint32_t)((k - lo) >> shift)], 1u);
-        });
-        sync();
-        // thread i has four bins from the top down: how many keys lie above them, and where m is passed
-        const uint4 z = *(const uint4 *)(bins + kBins - 4u - 4u * tid);
-        const uint32_t c[4] = { z.w, z.z, z.y, z.x }, sum = (z.x + z.y) + (z.z + z.w);
-        uint32_t above = wave_scan(sum);
-        if constexpr (WAVES > 1u) {
-            if (lane == 63u) part[wave][0] = above;
-            sync();
-#pragma unroll
-            for (uint32_t v = 0; v < WAVES; ++v) above += v < wave ? part[v][0] : 0u;
-        }
-        above -= sum;
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            if (above < m && above + c[i] >= m) { found[0] = kBins - 1u - (4u * tid + i); found[1] = above; found[2] = c[i]; }
-            above += c[i];
-        }
-        sync();
-        lo += (uint64_t)found[0] << shift;
-        hi = lesser(hi, lo + (((uint64_t)1 << shift) - 1u));
-        m -= found[1];
-        whole = found[2] == m;
-    }
-    // the cut: keys above hi, and of those from lo to hi all or, equal ones, the first m
-    uint32_t at = nf, in = 0u;
-    if constexpr (WAVES > 1u) {
-        uint32_t n_above = 0u, n_in = 0u;
-        each([&](uint32_t, uint64_t k, bool real) {
-            n_above += (uint32_t)__popcll(__ballot(real && k > hi));
-            n_in += (uint32_t)__popcll(__ballot(real && k >= lo && k <= hi));
-        });
-        sync();                                                    // (the bins' partial sums have been read)
-        if (lane == 0u) { part[wave][0] = n_above; part[wave][1] = n_in; }
-        sync();
-#pragma unroll
-        for (uint32_t v = 0; v < WAVES; ++v) {
-            at += v < wave ? part[v][0] : 0u;
-            in += v < wave ? part[v][1] : 0u;
-        }
-        at += min(in, m);
-    }
-    const uint64_t below = (1ull << lane) - 1u;
-    each([&](uint32_t b, uint64_t k, bool real) {
-        const bool mid = real && k >= lo && k <= hi;
-        const uint64_t mids = __ballot(mid);
-        const bool sel = (real && k > hi) || (mid && in + (uint32_t)__popcll(mids & below) < m);
-        const uint64_t sels = __ballot(sel);
-        if (sel) out[at + (uint32_t)__popcll(sels & below)] = (int32_t)b;
-        at += (uint32_t)__popcll(sels);
-        in += (uint32_t)__popcll(mids);
-    });
+    Pick<WAVES>{ room[list], wave, lane }.template run<uint64_t>(a.n_sel - nf - a.n_last, each,
+                                                                 [&](uint32_t at, uint32_t b, uint64_t) { out[nf + at] = (int32_t)b; });
 }
 
 template <int D>

@@ -135,6 +135,18 @@ struct Kv4BoundsArgs {
     uint32_t stride;         // blocks of a head
 };
 
+// Cells gathered into the first n of a plane (k_kv_gather.hip): cell i is cell idx[i] of src, or, where that is none, cell i of
+// src for i < stay_size (the workspace of a plane that is gathered into itself) and else left as it is.
+struct KvGatherArgs {
+    uint8_t * dst;
+    const uint8_t * src;
+    const int64_t * idx;
+    int32_t * bad;
+    uint32_t n, E, src_size, stay_size;
+    uint32_t dst_tiles, src_tiles;   // 4-bit planes: tiles of a pair of blocks
+    size_t dst_off, src_off;         // q8_0: byte offsets of the quant regions
+};
+
 // The blocks that tokens attend to (k_kv4_select.hip).
 struct Kv4SelectArgs {
     const float * q;         // [T][n_head][D], token t at q + t * q_stride
@@ -314,6 +326,11 @@ int tsr_launch_kv4_bounds(const tsr::Kv4BoundsArgs & a, hipStream_t s);
 // attention over a 4-bit cache, cut as attn4_plan.hpp says (k_attn4.hip)
 int tsr_launch_attn4(const tsr::Attn4Args & a, const tsr::Attn4Plan & p, hipStream_t s);
 int tsr_launch_attn4_blocks(const tsr::Attn4BlocksArgs & b, uint32_t C, hipStream_t s);
+// the n_keep of n cells that are kept, ascending (k_kv_pick.hip); kept: their weights (nullable)
+int tsr_launch_kv_pick(const float * weights, uint32_t n, uint32_t keep, uint32_t first, uint32_t last, int64_t * idx, float * kept,
+                       hipStream_t s);
+int tsr_launch_kv_gather(const tsr::KvGatherArgs & a, uint32_t type, uint32_t which, hipStream_t s);
+int tsr_launch_kv_rows_copy(uint8_t * to, size_t to_step, const uint8_t * from, size_t from_step, size_t bytes, uint32_t rows, hipStream_t s);
 // the weights that cells gather (k_attn4_weights.hip): out[c] = decay before[c] (none: 0) + their sum over rows, c < n_kv
 namespace tsr { struct Weights4Plan; }
 int tsr_launch_attn4_weights(const tsr::Attn4Args & a, const tsr::Weights4Plan & p, const float * before, float decay, hipStream_t s);

@@ -1,4 +1,5 @@
-// tsr_evict4.hip -- host side of eviction by attention weight: the weights that cells of a 4-bit K cache gather.
+// tsr_evict4.hip -- host side of eviction by attention weight: the weights that cells of a 4-bit K cache gather, the cells that
+// are kept, and their move (caches of every type).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -80,4 +81,88 @@ int tsr_hip_attn_weights_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T,
         before = out_dev;
     }
     return TSR_HIP_OK;
+}
+
+int tsr_hip_kv_pick(tsr_hip_ctx * ctx, const float * weights_dev, uint32_t n_kv, uint32_t n_keep, uint32_t n_first, uint32_t n_last,
+                    int64_t * idx_dev, float * kept_dev, void * stream) {
+    if (ctx == nullptr || weights_dev == nullptr || idx_dev == nullptr) return TSR_HIP_E_ARG;
+    if (n_keep > n_kv || n_kv > 0x7FFFFFFFu) return TSR_HIP_E_RANGE;
+    if (n_first > n_keep || n_last > n_keep - n_first) return TSR_HIP_E_SHAPE;
+    if ((((uintptr_t)weights_dev | (uintptr_t)kept_dev) & 3u) != 0u || ((uintptr_t)idx_dev & 7u) != 0u || kept_dev == weights_dev)
+        return TSR_HIP_E_ARG;
+    if (n_keep == 0u) return TSR_HIP_OK;
+    std::lock_guard<std::mutex> lk(ctx->mtx);
+    (void)hipSetDevice(ctx->device);
+    return tsr_launch_kv_pick(weights_dev, n_kv, n_keep, n_first, n_last, idx_dev, kept_dev, ctx->pick(stream)) ? TSR_HIP_E_HIP : TSR_HIP_OK;
+}
+
+// A plane's first n cells by themselves: bytes, and where q8_0's quants begin.
+static size_t part_bytes(const tsr_hip_kv * kv, uint32_t n, size_t * quants) {
+    *quants = 0u;
+    if (kv->type != TSR_HIP_KV_Q8_0) return (size_t)(kv->E / 64u) * tsr::kv4_tiles(n) * tsr::kv4_tile_bytes(kv->type);
+    const size_t ng = ((size_t)n + 15u) / 16u;
+    *quants = (ng * 16u * kv->meta_row + 255u) & ~(size_t)255u;
+    return *quants + ng * 16u * kv->E;
+}
+
+size_t tsr_hip_kv_gather_ws(tsr_hip_ctx * ctx, const tsr_hip_kv * kv, uint32_t n) {
+    if (ctx == nullptr || kv == nullptr || n == 0u || n > kv->kv_size) return 0u;
+    size_t quants;
+    return part_bytes(kv, n, &quants);
+}
+
+int tsr_hip_kv_gather(tsr_hip_ctx * ctx, tsr_hip_kv * dst, const tsr_hip_kv * src, uint32_t which, const int64_t * idx_dev, uint32_t n,
+                      int32_t * bad_dev, void * ws_dev, size_t ws_bytes, void * stream) {
+    if (ctx == nullptr || dst == nullptr || src == nullptr || idx_dev == nullptr || which > 1u) return TSR_HIP_E_ARG;
+    if (dst->type != src->type) return TSR_HIP_E_FMT;
+    if (dst->E != src->E) return TSR_HIP_E_SHAPE;
+    if (n > dst->kv_size) return TSR_HIP_E_RANGE;
+    if (((uintptr_t)idx_dev & 7u) != 0u || ((uintptr_t)bad_dev & 3u) != 0u) return TSR_HIP_E_ARG;
+    if (n == 0u) return TSR_HIP_OK;
+    const bool self = dst == src, q8 = dst->type == TSR_HIP_KV_Q8_0;
+    size_t quants = 0u;
+    const size_t need = self ? part_bytes(dst, n, &quants) : 0u;
+    if (ws_dev != nullptr && (ws_bytes < need || ((uintptr_t)ws_dev & 15u) != 0u)) return TSR_HIP_E_ARG;
+    tsr::KvGatherArgs a{};
+    a.src = src->dev;
+    a.idx = idx_dev;
+    a.n = n;
+    a.E = dst->E;
+    a.src_size = src->kv_size;
+    if (q8) a.src_off = src->quant_off;
+    else a.src_tiles = tsr::kv4_tiles(src->kv_size);
+    std::lock_guard<std::mutex> lk(ctx->mtx);
+    (void)hipSetDevice(ctx->device);
+    hipStream_t s = ctx->pick(stream);
+    a.bad = ctx->flag(bad_dev);
+    if (!self) {
+        a.dst = dst->dev;
+        if (q8) a.dst_off = dst->quant_off;
+        else a.dst_tiles = tsr::kv4_tiles(dst->kv_size);
+        return tsr_launch_kv_gather(a, dst->type, which, s) ? TSR_HIP_E_HIP : TSR_HIP_OK;
+    }
+    void * ws = nullptr;
+    const int rc = workspace(ctx, need, ws_dev, s, &ws);
+    if (rc) return rc;
+    a.dst = (uint8_t *)ws;
+    // (cells stay that have no source, and those behind the last of the part's tiles)
+    if (q8) {
+        a.dst_off = quants;
+        a.stay_size = (uint32_t)std::min<uint64_t>(((uint64_t)dst->kv_size + 15u) & ~(uint64_t)15u, 0xFFFFFFF0u);
+    } else {
+        a.dst_tiles = tsr::kv4_tiles(n);
+        a.stay_size = 32u * a.src_tiles;
+    }
+    if (tsr_launch_kv_gather(a, dst->type, which, s)) return TSR_HIP_E_HIP;
+    int e = 0;
+    if (q8) {
+        const size_t ng = ((size_t)n + 15u) / 16u;
+        e = tsr_launch_kv_rows_copy(dst->dev, 0u, a.dst, 0u, ng * 16u * dst->meta_row, 1u, s);
+        if (e == 0) e = tsr_launch_kv_rows_copy(dst->dev + dst->quant_off, 0u, a.dst + quants, 0u, ng * 16u * dst->E, 1u, s);
+    } else {
+        const size_t tb = tsr::kv4_tile_bytes(dst->type);
+        e = tsr_launch_kv_rows_copy(dst->dev + tsr::kKv4Header, a.src_tiles * tb, a.dst + tsr::kKv4Header, a.dst_tiles * tb, a.dst_tiles * tb,
+                                    dst->E / 64u, s);
+    }
+    return e ? TSR_HIP_E_HIP : TSR_HIP_OK;
 }

@@ -45,7 +45,7 @@ EXPORTS = (
     "tsr_hip_rope_scaled", "tsr_hip_rope_scaled_table",
     "tsr_hip_kv4_bounds", "tsr_hip_kv4_select", "tsr_hip_kv4_select_ws",
     "tsr_hip_flash_attn_kv4_blocks", "tsr_hip_flash_attn_kv4_blocks_ws",
-    "tsr_hip_attn_weights_kv4", "tsr_hip_attn_weights_kv4_ws",
+    "tsr_hip_attn_weights_kv4", "tsr_hip_attn_weights_kv4_ws", "tsr_hip_kv_pick", "tsr_hip_kv_gather", "tsr_hip_kv_gather_ws",
 )
 
 
@@ -153,6 +153,9 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         "tsr_hip_flash_attn_kv4_blocks_ws": ([vp, u32, u32, u32, u32, u32, u32], sz),
         "tsr_hip_attn_weights_kv4": ([vp, vp, u32, u64, vp, u32, u32, u32, C.c_float, u32, vp, vp, C.c_float, vp, vp, sz, vp], C.c_int),
         "tsr_hip_attn_weights_kv4_ws": ([vp, u32, u32, u32, u32, u32], sz),
+        "tsr_hip_kv_pick": ([vp, vp, u32, u32, u32, u32, vp, vp, vp], C.c_int),
+        "tsr_hip_kv_gather": ([vp, vp, vp, u32, vp, u32, vp, vp, sz, vp], C.c_int),
+        "tsr_hip_kv_gather_ws": ([vp, vp, u32], sz),
         "tsr_hip_rope_scaled": ([vp, vp, u32, u64, u32, u32, u32, C.c_int, vp, C.POINTER(RopeScaling), vp, vp, u64, vp], C.c_int),
         "tsr_hip_rope_scaled_table": ([vp, vp, u32, C.POINTER(RopeScaling), vp, vp, vp], C.c_int),
     }
@@ -530,6 +533,21 @@ class Device:
         _check(self.L.tsr_hip_attn_weights_kv4(self.ctx, self._p(q), T, q_stride, kc.h, D, n_head, n_head_kv, scale, n_kv,
                                                self._p(runs), self._p(before), float(decay), self._p(out), self._p(ws),
                                                0 if ws is None else ws.nbytes, stream), "attn_weights_kv4")
+
+    def kv_pick(self, weights, n_kv: int, n_keep: int, n_first: int, n_last: int, idx, kept=None, stream=None) -> None:
+        """The n_keep cells (device int64, ascending) that are kept: the first, the last and those with the largest weights; kept:
+        their weights."""
+        _check(self.L.tsr_hip_kv_pick(self.ctx, self._p(weights), n_kv, n_keep, n_first, n_last, self._p(idx), self._p(kept), stream),
+               "kv_pick")
+
+    def kv_gather_ws(self, kv: KvCache, n: int) -> int:
+        """Bytes of workspace that kv_gather of n cells within a cache needs."""
+        return int(self.L.tsr_hip_kv_gather_ws(self.ctx, kv.h, n))
+
+    def kv_gather(self, dst: KvCache, src: KvCache, which: int, idx, n: int, bad=None, ws: "Buffer | None" = None, stream=None) -> None:
+        """Cells idx (device int64) of src, bit for bit, as cells 0 .. n - 1 of dst, which may be src."""
+        _check(self.L.tsr_hip_kv_gather(self.ctx, dst.h, src.h, which, self._p(idx), n, self._p(bad), self._p(ws),
+                                        0 if ws is None else ws.nbytes, stream), "kv_gather")
 
     def flash_attn(self, q, T: int, q_stride: int, kc: KvCache, vc: KvCache, D: int, n_head: int, n_head_kv: int,
                    scale: float, msum, out, out_stride: int, mask_f32=None, new_runs=None, stream=None) -> None:
