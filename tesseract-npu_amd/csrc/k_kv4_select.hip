@@ -124,7 +124,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores(Kv4SelectArgs a
         const bool none = ((__ballot(nan) >> (lane & 60u)) & 15u) != 0u;
         const uint32_t b = b0 + (lane & 12u) + g;
         if ((lane & 3u) == 0u && b < a.n_blocks)
-            a.keys[((size_t)t * a.n_head_kv + h) * a.n_blocks + b] = none ? 0u : order_of(best);
+            a.keys[((size_t)t * a.n_head_kv + h) * a.n_blocks + b] = none ? kNan64 : order_of(best);
         here = false;
     }
 }
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores_many(Kv4SelectA
     for (uint32_t k = 0; k < 4u; ++k) {
         const uint32_t e = lane + 64u * k, b = b0 + (e & 15u), t = t0 + (e >> 4);
         if (e < items && t < a.T && b < a.n_blocks)
-            a.keys[((size_t)t * a.n_head_kv + h) * a.n_blocks + b] = nan[k] ? 0u : order_of(best[k]);
+            a.keys[((size_t)t * a.n_head_kv + h) * a.n_blocks + b] = nan[k] ? kNan64 : order_of(best[k]);
     }
 }
 
@@ -253,12 +253,12 @@ __global__ __launch_bounds__(64 * pick_waves(WAVES)) void k_kv4_pick_blocks(Kv4S
         else if (i >= a.n_sel - a.n_last) out[i] = (int32_t)block(n - (a.n_sel - i));
     }
     if (n <= a.n_sel || a.n_sel == nf + a.n_last) return;
-    // f(block, key, whether it is one of them) for every row of the wave, the lanes together
+    // f(block, key) for every row of the wave, the lanes together; key 0: not one of them
     auto each = [&](auto f) {
         auto one = [&](uint32_t j, uint64_t k) {
             const uint32_t b = from + (wave * rows + j) * 64u + lane;
             const uint32_t i = x.has(b) ? b - x.lo : y.has(b) ? nx + (b - y.lo) : ~0u;
-            f(b, k, i >= nf && i < n - a.n_last);
+            f(b, i >= nf && i < n - a.n_last ? k : 0u);
         };
         if constexpr (ROWS != 0u) {
 #pragma unroll
@@ -268,8 +268,7 @@ __global__ __launch_bounds__(64 * pick_waves(WAVES)) void k_kv4_pick_blocks(Kv4S
             for (uint32_t j = 0; j < rows; ++j) one(j, keys[min(from + (wave * rows + j) * 64u + lane, a.n_blocks - 1u)]);
         }
     };
-    Pick<WAVES>{ room[list], wave, lane }.template run<uint64_t>(a.n_sel - nf - a.n_last, each,
-                                                                 [&](uint32_t at, uint32_t b, uint64_t) { out[nf + at] = (int32_t)b; });
+    Pick<WAVES>{ room[list], wave, lane }.template run<uint64_t>(a.n_sel - nf - a.n_last, each, [&](uint32_t at, uint32_t b, uint64_t) { out[nf + at] = (int32_t)b; });
 }
 
 template <int D>

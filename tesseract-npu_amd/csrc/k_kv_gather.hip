@@ -1,8 +1,9 @@
 // k_kv_gather.hip -- cells of a KV cache of any type, bit for bit, as cells 0 .. n - 1 of another one or of itself.
 //
 // A thread makes 16 bytes of the destination's codes, from 2 cells (K) or 8 (V, where a cell owns single bytes: 16 loads of one,
-// a wave's 64 in eight lines), or a word of scales. A list in ascending order has a tile's source cells close together. Bound: the
-// cells' bytes in and out; V's codes, the loads.
+// a wave's 64 in eight lines), or a word of scales. A list in ascending order has a tile's source cells close together. Bound: memory,
+// and there the lines that the cells lie in, which 16 (K) or 8 (V) cells share: 16384 of 65536 cells of 1024 values (9.4 MB, of 37.7
+// MB whose every line has some) take 10 us for K and 12.3 for V, 4.7 and 3.8 TB/s of lines.
 //
 // Into itself: cells may move onto one another, so that they first go to a workspace laid out like the cache's first n
 // cells (with the cells that stay, where a source is none) and from there over them.

@@ -2,7 +2,7 @@
 // weights (pick.hpp), in the order of their cells.
 //
 // One workgroup of 16 waves finds the cut and writes the list; up to 65536 weights stay in its registers. Bound: what one compute unit
-// loads and counts: 16384 of 65536 cells take 20 us.
+// loads and counts: 16384 of 65536 cells take 31 us (its 64 weights a lane some 2000 instructions), 777 of 1500 5 us.
 #include "kernels.hpp"
 #include "pick.hpp"
 
@@ -15,13 +15,14 @@ __global__ __launch_bounds__(1024) void k_kv_pick(const float * weights, uint32_
     __shared__ __align__(16) PickRoom<16> room;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u;
     const uint32_t rows = (n + 1023u) / 1024u, c0 = wave * rows * 64u + lane;
+    auto counts = [&](uint32_t c) { return c >= first && c < n - last; };
     uint32_t mine[ROWS == 0u ? 1u : ROWS];
     if constexpr (ROWS != 0u) {
         float x[ROWS];
 #pragma unroll
         for (uint32_t j = 0; j < ROWS; ++j) x[j] = j < rows && c0 + 64u * j < n ? weights[c0 + 64u * j] : 0.0f;
 #pragma unroll
-        for (uint32_t j = 0; j < ROWS; ++j) mine[j] = order_of(x[j]);
+        for (uint32_t j = 0; j < ROWS; ++j) mine[j] = j < rows && counts(c0 + 64u * j) ? order_of(x[j]) : 0u;
     }
     auto store = [&](uint32_t at, uint32_t c, float w) {
         idx[at] = c;
@@ -35,13 +36,14 @@ __global__ __launch_bounds__(1024) void k_kv_pick(const float * weights, uint32_
     auto each = [&](auto f) {
         if constexpr (ROWS != 0u) {
 #pragma unroll
-            for (uint32_t j = 0; j < ROWS; ++j)
-                if (j < rows) f(c0 + 64u * j, mine[j], c0 + 64u * j >= first && c0 + 64u * j < n - last);
+            for (uint32_t j0 = 0; j0 < ROWS; j0 += 4u)
+                if (j0 < rows)
+#pragma unroll
+                    for (uint32_t j = j0; j < j0 + 4u; ++j) f(c0 + 64u * j, mine[j]);
         } else {
             for (uint32_t j = 0; j < rows; ++j) {
                 const uint32_t c = c0 + 64u * j;
-                const bool real = c >= first && c < n - last;
-                f(c, real ? order_of(weights[c]) : 0u, real);
+                f(c, counts(c) ? order_of(weights[c]) : 0u);
             }
         }
     };

@@ -10,14 +10,17 @@
 
 namespace tsr {
 
-// The order of f64 and f32 as unsigned numbers; a NaN is the lowest, zeros are equal.
+// The order of f64 and f32 as unsigned numbers; a NaN is the lowest, zeros are equal. Nothing but what takes no part is 0 (of f64:
+// in the high word).
+constexpr uint64_t kNan64 = (uint64_t)1 << 32;
+constexpr uint32_t kNan32 = 1u;
 __device__ __forceinline__ uint64_t order_of(double x) {
     const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
-    return x != x ? 0u : u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
+    return x != x ? kNan64 : u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
 }
 __device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t u = fb(x + 0.0f);
-    return x != x ? 0u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    return x != x ? kNan32 : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
 // The number of an order (a NaN for a NaN's, 0 for zeros').
@@ -62,18 +65,18 @@ struct Pick {
         else __syncthreads();
     }
 
-    // each(f) calls f(place, key, whether it takes part) for every row of the wave, the lanes together, rows and waves in the
-    // order of the places. At least m keys take part, m >= 1. put(position, place, key) for the m that are taken, positions
-    // from 0 on in the order of the places.
+    // each(f) calls f(place, key) for every row of the wave, the lanes together, rows and waves in the order of the places; key 0
+    // takes no part, at least m others do, m >= 1. put(position, place, key) for the m that are taken, positions from 0 on in the
+    // order of the places.
     template <class Key, class Each, class Put>
     __device__ __forceinline__ void run(uint32_t m, Each each, Put put) {
         constexpr uint32_t kHigh = 8u * sizeof(Key) - 32u;
         const uint32_t tid = 64u * wave + lane;
         uint32_t (*part)[2] = room.part, * found = room.found;
-        uint32_t least = ~0u, most = 0u;                           // of the keys' high words
-        each([&](uint32_t, Key k, bool real) {
-            least = real ? min(least, (uint32_t)(k >> kHigh)) : least;
-            most = real ? max(most, (uint32_t)(k >> kHigh)) : most;
+        uint32_t least = ~0u, most = 0u;                           // of the keys' high words, the least less one
+        each([&](uint32_t, Key k) {
+            least = min(least, (uint32_t)(k >> kHigh) - 1u);
+            most = max(most, (uint32_t)(k >> kHigh));
         });
         least = wave_min(least);
         most = ~wave_min(~most);
@@ -84,15 +87,15 @@ struct Pick {
             for (uint32_t v = 0; v < WAVES; ++v) { least = min(least, part[v][0]); most = max(most, part[v][1]); }
         }
         const Key ones = ((Key)1 << kHigh) - 1u;
-        Key lo = (Key)least << kHigh, hi = ((Key)most << kHigh) | ones;
+        Key lo = (Key)(least + 1u) << kHigh, hi = ((Key)most << kHigh) | ones;   // (lo > 0)
         // keys above hi are taken, those below lo are not, m of those between are
         bool whole = false;
         while (!whole && lo != hi) {
             const uint32_t bits = 64u - (uint32_t)__builtin_clzll((uint64_t)(hi - lo)), shift = bits > kBits ? bits - kBits : 0u;
             *(uint4 *)(room.bins + 4u * tid) = make_uint4(0u, 0u, 0u, 0u);
             sync();
-            each([&](uint32_t, Key k, bool real) {
-                if (real && k >= lo && k <= hi) atomicAdd(&room.bins[(uint32_t)((k - lo) >> shift)], 1u);
+            each([&](uint32_t, Key k) {
+                if (k - lo <= hi - lo) atomicAdd(&room.bins[(uint32_t)((k - lo) >> shift)], 1u);
             });
             sync();
             // thread i has four bins from the top down: how many keys lie above them, and where m is passed
@@ -113,21 +116,21 @@ struct Pick {
             }
             sync();
             lo += (Key)found[0] << shift;
-            const Key end = lo + (((Key)1 << shift) - 1u);
-            hi = end < hi ? end : hi;
+            const Key span = ((Key)1 << shift) - 1u;
+            hi = hi - lo < span ? hi : lo + span;
             m -= found[1];
             whole = found[2] == m;
         }
-        // the cut: keys above hi, and of those from lo to hi all or, equal ones, the first m
+        // all keys from lo on are taken or, where lo is the only one left, those above it and its first m
         uint32_t at = 0u, in = 0u;
         if constexpr (WAVES > 1u) {
-            uint32_t n_above = 0u, n_in = 0u;
-            each([&](uint32_t, Key k, bool real) {
-                n_above += (uint32_t)__popcll(__ballot(real && k > hi));
-                n_in += (uint32_t)__popcll(__ballot(real && k >= lo && k <= hi));
-            });
+            uint32_t n_from = 0u, n_in = 0u;                       // keys from lo on, those that are lo
+            each([&](uint32_t, Key k) { n_from += k >= lo ? 1u : 0u; });
+            if (!whole) each([&](uint32_t, Key k) { n_in += k == lo ? 1u : 0u; });
+            n_from = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n_from), 63);
+            n_in = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n_in), 63);
             sync();                                                // (the bins' partial sums have been read)
-            if (lane == 0u) { part[wave][0] = n_above; part[wave][1] = n_in; }
+            if (lane == 0u) { part[wave][0] = n_from - n_in; part[wave][1] = n_in; }
             sync();
 #pragma unroll
             for (uint32_t v = 0; v < WAVES; ++v) {
@@ -136,16 +139,23 @@ struct Pick {
             }
             at += min(in, m);
         }
-        const uint64_t below = (1ull << lane) - 1u;
-        each([&](uint32_t b, Key k, bool real) {
-            const bool mid = real && k >= lo && k <= hi;
-            const uint64_t mids = __ballot(mid);
-            const bool sel = (real && k > hi) || (mid && in + (uint32_t)__popcll(mids & below) < m);
-            const uint64_t sels = __ballot(sel);
-            if (sel) put(at + (uint32_t)__popcll(sels & below), b, k);
-            at += (uint32_t)__popcll(sels);
-            in += (uint32_t)__popcll(mids);
-        });
+        auto rank = [](uint64_t lanes) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u)); };
+        if (whole) {
+            each([&](uint32_t b, Key k) {
+                const uint64_t sels = __ballot(k >= lo);
+                if (k >= lo) put(at + rank(sels), b, k);
+                at += (uint32_t)__builtin_popcountll(sels);
+            });
+        } else {
+            each([&](uint32_t b, Key k) {
+                const uint64_t mids = __ballot(k == lo);
+                const bool sel = k > lo || (k == lo && in + rank(mids) < m);
+                const uint64_t sels = __ballot(sel);
+                if (sel) put(at + rank(sels), b, k);
+                at += (uint32_t)__builtin_popcountll(sels);
+                in += (uint32_t)__builtin_popcountll(mids);
+            });
+        }
     }
 };
 
