@@ -34,7 +34,7 @@ inline Weights4Plan weights4_plan(uint32_t T, uint32_t D, uint32_t n_head, uint3
     p.n_pad = (uint32_t)(32u * tiles);
     // a launch's sums take at most 64 MiB, or are one token's
     const uint64_t rows = 16u * p.NT, most = std::max<uint64_t>(1u, ((uint64_t)64 << 20) / (4u * (uint64_t)p.n_pad * n_head_kv));   // row sets of a KV head
-    p.tokens = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ T, most * rows / G, 16384u }));
+    p.tokens = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ T, most * rows / G, 16000u }));   // (16-row sets fit a grid)
     p.n_rg = (uint32_t)((p.tokens * G + rows - 1u) / rows);
     const uint64_t n = (uint64_t)n_head_kv * p.n_rg;
     p.S = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ (2u * (uint64_t)n_cu + n - 1u) / n, (tiles + 3u) / 4u, kWeightsSplits }));
