@@ -504,8 +504,8 @@ int tsr_hip_rope_table(tsr_hip_ctx * ctx, const int32_t * pos_dev, uint32_t n_di
  *   w_i = ext_factor (1 - clamp((i - lo) / max(0.001, hi - lo), 0, 1)),  lo = max(0, floor(c(beta_fast))),
  *   hi = min(n_dims - 1, ceil(c(beta_slow))),  c(b) = n_dims ln(n_ctx_orig / (2 pi b)) / (2 ln freq_base)
  * and its values are multiplied by m = attn_factor, with ext_factor != 0 by attn_factor (1 + 0.1 ln(1 / s)): the parameters
- * of GGML_OP_ROPE under its names. Angles in f64, a pair's result off by at most two roundings of its products. Modes, layouts and
- * rows as tsr_hip_rope (dims from n_dims on are copied; y may be x), positions of either sign: -p turns back what p has turned (K
+ * of GGML_OP_ROPE under its names. Angles, cosines and sines in f64, rounded to f32 once; a pair is then turned by tsr_hip_rope's
+ * operations. Modes, layouts and rows as tsr_hip_rope (dims from n_dims on are copied; y may be x), positions of either sign: -p turns back what p has turned (K
  * rows of a context shift; m twice). Its angles are not tsr_hip_rope's, which follow the reference's f32 recurrence. freq_base > 1;
  * s > 0; 0 <= ext_factor <= 1; n_ctx_orig and the betas are read where ext_factor != 0 and are > 0 there; head_dim <= 16384,
  * n_heads head_dim <= 2^18. 16-byte aligned rows of whole quads are fastest, any are taken. */
@@ -523,7 +523,8 @@ int tsr_hip_rope_scaled(tsr_hip_ctx * ctx, const float * x_dev, uint32_t T, uint
                         const tsr_hip_rope_scaling * scaling, const float * freq_factors_dev, float * y_dev, uint64_t y_stride,
                         void * stream);
 /* Its angles at *pos_dev as a table for tsr_hip_flash_attn_plan_rope_tab and tsr_hip_attn_qkv_plan_rope_tab: tab_dev[2 i]
- * = m cos, tab_dev[2 i + 1] = m sin of pair i, i < n_dims / 2; n_dims even, 2 <= n_dims <= 128; tab_dev 8-byte aligned. */
+ * = m cos, tab_dev[2 i + 1] = m sin of pair i, i < n_dims / 2; n_dims even, 2 <= n_dims <= 128; tab_dev 8-byte aligned. Those calls
+ * are then bit-identical to tsr_hip_rope_scaled, tsr_hip_kv_set_rows and the attention. */
 int tsr_hip_rope_scaled_table(tsr_hip_ctx * ctx, const int32_t * pos_dev, uint32_t n_dims, const tsr_hip_rope_scaling * scaling,
                               const float * freq_factors_dev, float * tab_dev, void * stream);
 

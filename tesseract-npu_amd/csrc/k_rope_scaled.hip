@@ -10,8 +10,8 @@
 // values of its units are on their way. A unit is four values (interleaved pairs) or two times four (halves), and where rows
 // are not of whole aligned quads a pair, or a single value to copy; one thread reads and writes all of it, so that y may be x.
 //
-// Bound: the rows' bytes, once in and once out. 2047 tokens of 40 heads of 128 (84 MB) take 17.9 us, 4.7 TB/s, what a large
-// copy reaches here; the f64 angles hide behind them. One token is a launch (5.0 us a call).
+// Bound: the rows' bytes, once in and once out. 2047 tokens of 40 heads of 128 (84 MB) take 18.6 us, 4.5 TB/s where a large
+// copy reaches 4.65; the f64 angles hide behind them. One token is a launch (5.0 us a call).
 #include "kernels.hpp"
 #include "tsr_dev.hpp"
 
@@ -62,9 +62,31 @@ __device__ __forceinline__ void rs_store(float * p, const RsVec<V> & r) {
     }
 }
 
-// One value of a turned pair: a c -+ b s, one of the products unrounded.
-__device__ __forceinline__ float rs_first(float a, float b, float2 cs) { return __builtin_fmaf(a, cs.x, -(b * cs.y)); }
-__device__ __forceinline__ float rs_second(float a, float b, float2 cs) { return __builtin_fmaf(b, cs.x, a * cs.y); }
+// Pairs turned by ROPE's operations (k_glue.hip: subnormals are 0, a NaN is the canonical one), so that the fused attention calls,
+// which take the angles as a table, give the same bits. Plain products and sums are these but for values that a class test finds,
+// and then all of a unit's are made again by the rules (2047 tokens of 40 heads: 22.4 us by the rules alone).
+__device__ __forceinline__ bool rs_odd(float x) { return __builtin_amdgcn_classf(x, 0x93); }   // subnormal or a NaN
+template <int N>
+__device__ __forceinline__ void rs_turn(float (&p)[N], float (&q)[N], const float2 (&cs)[N]) {
+    float x[N], y[N];
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float pc = p[i] * cs[i].x, qs = q[i] * cs[i].y, ps = p[i] * cs[i].y, qc = q[i] * cs[i].x;
+        x[i] = pc - qs;
+        y[i] = ps + qc;
+        odd |= rs_odd(p[i]) | rs_odd(q[i]) | rs_odd(pc) | rs_odd(qs) | rs_odd(ps) | rs_odd(qc) | rs_odd(x[i]) | rs_odd(y[i]);
+    }
+    if (__builtin_expect(odd, 0)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] = ssub(smul(p[i], cs[i].x), smul(q[i], cs[i].y));
+            y[i] = sadd(smul(p[i], cs[i].y), smul(q[i], cs[i].x));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = x[i], q[i] = y[i];
+}
 
 // Units of a head: first those that turn (n_dims / V interleaved; n_dims / (2 V) halves), then those that are copied, of V
 // values where V is 4, else of one.
@@ -102,7 +124,10 @@ __global__ __launch_bounds__(kRsThreads) void k_rope_scaled(RopeScaledArgs a) {
         }
     }
     const int32_t pos = a.pos[t];
-    for (uint32_t i = threadIdx.x; i < half; i += kRsThreads) cs[i] = rope_scaled_cs(a, pos, i);
+    for (uint32_t i = threadIdx.x; i < half; i += kRsThreads) {
+        const float2 c = rope_scaled_cs(a, pos, i);
+        cs[i] = make_float2(daz(c.x), daz(c.y));
+    }
     __syncthreads();
 #pragma unroll
     for (uint32_t k = 0; k < kRsUnits; ++k) {
@@ -112,26 +137,24 @@ __global__ __launch_bounds__(kRsThreads) void k_rope_scaled(RopeScaledArgs a) {
             if constexpr (V == CW) rs_store<V>(y + w.at, w.p);
             else y[w.at] = w.p.v[0];
         } else {
-            if constexpr (HALVES) {
-                RsVec<V> p, q;
+            constexpr int N = HALVES ? V : V / 2;
+            float p[N], q[N];
+            float2 c[N];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float2 c = cs[w.j * V + i];
-                    p.v[i] = rs_first(w.p.v[i], w.q.v[i], c);
-                    q.v[i] = rs_second(w.p.v[i], w.q.v[i], c);
-                }
-                rs_store<V>(y + w.at, p);
-                rs_store<V>(y + w.at + half, q);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    const float2 c = cs[(w.j * V + i) / 2u];
-                    const float p = w.p.v[i], q = w.p.v[i + 1];
-                    w.p.v[i] = rs_first(p, q, c);
-                    w.p.v[i + 1] = rs_second(p, q, c);
-                }
-                rs_store<V>(y + w.at, w.p);
+            for (int i = 0; i < N; ++i) {
+                p[i] = w.p.v[HALVES ? i : 2 * i];
+                q[i] = HALVES ? w.q.v[i] : w.p.v[2 * i + 1];
+                c[i] = cs[HALVES ? w.j * V + i : w.j * V / 2u + i];
             }
+            rs_turn(p, q, c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                w.p.v[HALVES ? i : 2 * i] = p[i];
+                if constexpr (HALVES) w.q.v[i] = q[i];
+                else w.p.v[2 * i + 1] = q[i];
+            }
+            rs_store<V>(y + w.at, w.p);
+            if constexpr (HALVES) rs_store<V>(y + w.at + half, w.q);
         }
     }
 }

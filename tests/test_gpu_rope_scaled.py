@@ -95,6 +95,37 @@ def test_values_that_are_not_finite_stay_in_their_pairs(dev):
     assert bad.tolist() == [6, 7, 8, 9, 200]
 
 
+@pytest.mark.parametrize("hd,n,mode", [(64, 64, 0), (64, 48, 2), (24, 20, 2), (10, 6, 0)])
+def test_rope_s_operations(dev, hd, n, mode):
+    """The angles are those of the table; products and sums flush subnormals and give one NaN, bit for bit."""
+    rng = np.random.default_rng(hd + n)
+    x = (rng.standard_normal((5, 3 * hd)) * 10.0 ** rng.choice([0, 0, -37.5, -38.5, 38], (5, 3 * hd))).astype(np.float32)
+    x[1] = rng.standard_normal(3 * hd)
+    x[2, ::7], x[3, ::5], x[3, 1::6] = np.nan, np.inf, -0.0
+    x.view(np.uint32)[4, ::9] = 0xFFC01234
+    sc = H.RopeScaling(freq_base=10000.0, freq_scale=0.25, ext_factor=1.0, n_ctx_orig=256)
+    pos, tab, cs = np.array([0, 1, 77, 1000, 131071], np.int32), dev.alloc(4 * n), []
+    for p in pos:
+        dev.rope_scaled_table(dev.upload(np.array([p], np.int32)), n, sc, tab)
+        cs.append(tab.read(np.float32, (n // 2, 2)))
+    c, s = np.stack(cs)[:, None].transpose(3, 0, 1, 2)
+
+    def daz(v):
+        return np.where(np.abs(v) < np.float32(2.0 ** -126), np.copysign(np.float32(0), v), v)
+
+    def fin(v):
+        return np.where(np.isnan(v), np.uint32(0x7FC00000).view(np.float32), daz(v))
+
+    h = x.reshape(5, 3, hd)
+    i, j = (np.arange(0, n, 2), np.arange(1, n, 2)) if mode == 0 else (np.arange(n // 2), n // 2 + np.arange(n // 2))
+    want, a, b = h.copy(), daz(h[:, :, i]), daz(h[:, :, j])
+    with np.errstate(all="ignore"):
+        want[:, :, i] = fin(fin(a * c) - fin(b * s))
+        want[:, :, j] = fin(fin(a * s) + fin(b * c))
+    got = run(dev, x, pos, 3, hd, n, mode, sc)
+    assert (got.view(np.uint32) == want.reshape(got.shape).view(np.uint32)).all()
+
+
 def test_in_a_graph(dev):
     """A captured call reads the positions that are there when it is replayed."""
     rng = np.random.default_rng(8)
