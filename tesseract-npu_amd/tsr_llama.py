@@ -20,6 +20,12 @@ kv_type picks the caches' type. Over q8_0 caches (the default) attention is the 
 A = tsr_hip_flash_attn_kv4, behind tsr_hip_rope_kv (fused) or ROPE and two SET_ROWS_KV, its visible cells in device memory:
 half the bytes, in more launches (Llama-3-8B, tokens/s over q8_0 and q4_0: 634 and 513 at 4096 cells, 482 and 488 at 16384).
 
+Contexts beyond the trained one: rope_scale in the config turns positions by tsr_hip_rope_scaled, over caches of either kind. Over
+4-bit caches `sparse` lets decode tokens attend to the blocks of cells that can matter most (tsr_hip_kv4_bounds of the cells as they
+are written, tsr_hip_kv4_select, tsr_hip_flash_attn_kv4_blocks), and `track` sums up what attention weight each cell gets
+(tsr_hip_attn_weights_kv4), by which evict() thins the caches out (tsr_hip_kv_pick, tsr_hip_kv_gather): positions go on, cells
+start again behind the kept ones.
+
 With fused=True (the default) RMS_NORM + MUL runs inside the Q|K|V and gate|up MUL_MATs
 (tsr_hip_mul_mat_norm), SWIGLU in the epilogue of the gate|up MUL_MAT (TSR_HIP_MM_GLU over gate / up
 rows interleaved), and ROPE with both SET_ROWS_KV inside the planned FLASH_ATTN_EXT
@@ -49,6 +55,27 @@ class DecodeError(RuntimeError):
 
 
 @dataclass(frozen=True)
+class RopeScale:
+    """Rotary positions scaled from a trained length n_ctx_orig to factor times it (tsr_hip_rope_scaled)."""
+    factor: float
+    ext_factor: float = 1.0
+    n_ctx_orig: int = 8192
+    attn_factor: float = 1.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    freq_factors: tuple[float, ...] | None = None
+
+
+@dataclass(frozen=True)
+class SparseAttention:
+    """Decode tokens attend to n_blocks blocks of `block` cells a KV head, the first and the last ones among them."""
+    block: int = 64
+    n_blocks: int = 32
+    first: int = 1
+    last: int = 4
+
+
+@dataclass(frozen=True)
 class LlamaConfig:
     name: str
     n_layer: int
@@ -64,6 +91,7 @@ class LlamaConfig:
     wfmt: int = H.FMT_Q4_K           # layer weights
     ofmt: int = H.FMT_Q4_K           # output head
     std: float = 0.02
+    rope_scale: RopeScale | None = None
 
     @property
     def E(self) -> int:
@@ -151,12 +179,27 @@ def msum_causal(pos0: int, T: int, n_kv: int) -> np.ndarray:
 
 class LlamaDecoder:
     """The model on one device: weights uploaded once, one q8_0 K and V cache per layer of kv_size
-    cells, and the activation buffers of one decode token."""
+    cells, and the activation buffers of one decode token. sparse, track: over 4-bit caches alone; track is what earlier
+    weights are multiplied by at every token (1: nothing is forgotten), None: no weights."""
+
+    scaling = rope_ff = sparse = track = None
+    dropped = n_cells = 0                  # evicted cells; cells in use
+    TRACKED_ROWS = 64                      # of a prompt's ubatch: its last tokens' weights
 
     def __init__(self, dev: H.Device, cfg: LlamaConfig, weights: SyntheticWeights, kv_size: int, fused: bool = True,
-                 qkv_in_attn: bool = True, kv_type: int = H.KV_Q8_0):
+                 qkv_in_attn: bool = True, kv_type: int = H.KV_Q8_0, sparse: SparseAttention | None = None,
+                 track: float | None = None):
         self.dev, self.cfg, self.kv_size, self.kv_type = dev, cfg, kv_size, kv_type
         self.kv4 = kv_type != H.KV_Q8_0
+        if not self.kv4 and (sparse is not None or track is not None):
+            raise ValueError("sparse attention and weights of cells are of 4-bit caches")
+        self.sparse, self.track = sparse, track
+        if cfg.rope_scale is not None:
+            r = cfg.rope_scale
+            self.scaling = H.RopeScaling(cfg.rope_base, 1.0 / r.factor, r.ext_factor, r.attn_factor, r.beta_fast, r.beta_slow,
+                                         r.n_ctx_orig)
+            if r.freq_factors is not None:
+                self.rope_ff = dev.upload(np.array(r.freq_factors, np.float32))
         self.fused = fused
         self.qkv_in_attn = qkv_in_attn     # planned decode: the Q|K|V MUL_MAT inside the attention launch
         c = cfg
@@ -178,6 +221,10 @@ class LlamaDecoder:
                 "kc": dev.kv(c.E, kv_size, kv_type),
                 "vc": dev.kv(c.E, kv_size, kv_type),
             }
+            if sparse is not None:
+                L["bounds"] = dev.alloc(c.E * self.n_bounds * f4)
+            if track is not None:
+                L["weights"] = dev.alloc(kv_size * f4).fill(0)
             del t
             self.layers.append(L)
         self.out_norm = dev.upload(weights.norm("output_norm.weight"))
@@ -196,11 +243,12 @@ class LlamaDecoder:
         self.bad = H.BufferPart(self._out, c.n_vocab * f4, 4).fill(0)
         self.next = dev.alloc(4)           # int32 greedy token (ARGMAX) of an eager step
         # int32 position (ROPE) at 0, int64 cell (SET_ROWS_KV) at 8, int32 token id (GET_ROWS ids) at 16; in front of them
-        # the runs of visible cells (attention over 4-bit caches)
-        self._in = dev.alloc(40)
-        self.params = H.BufferPart(self._in, 16, 24)
+        # the runs of visible cells (attention over 4-bit caches), and {cell, cell + 1} (bounds of new cells)
+        self._in = dev.alloc(56)
+        self.params = H.BufferPart(self._in, 32, 24)
         self.tok = H.BufferPart(self.params, 16, 4)
         self.rtab = dev.alloc(4 * c.head_dim)  # ROPE angles of the token's position (tsr_hip_rope_table)
+        self.blocks = dev.alloc(c.n_head_kv * sparse.n_blocks * f4) if sparse is not None else None
         self.scale = 1.0 / math.sqrt(c.head_dim)
         self.plan = None if self.kv4 else dev.fa_plan(c.head_dim, c.n_head, c.n_head_kv, 1, kv_size)
         self.ws, self.n_kv_graph = None, 0   # 4-bit caches: the graph's workspace and the cells it may touch
@@ -214,6 +262,15 @@ class LlamaDecoder:
     @property
     def runs_ptr(self) -> int:
         return self._in.ptr
+
+    @property
+    def new_ptr(self) -> int:
+        return self._in.ptr + 16
+
+    @property
+    def n_bounds(self) -> int:
+        """Blocks of a cache (tsr_hip_kv4_bounds)."""
+        return -(-self.kv_size // self.sparse.block)
 
     @property
     def pos_ptr(self) -> int:
@@ -231,7 +288,14 @@ class LlamaDecoder:
                 rows = self.dev.upload(np.ascontiguousarray(weights.kv_history(il, which, n), np.float32))
                 self.dev.kv_set_rows(kv, which, rows, n, self.cfg.E, idx, self.bad)
                 rows.free()
+            if self.sparse is not None:
+                self._all_bounds(L, n)
+        self.n_cells = n
         self.dev.sync()
+
+    def _all_bounds(self, L: dict, n: int) -> None:
+        """The bounds of a layer's first n cells."""
+        self.dev.kv4_bounds(L["kc"], self.cfg.head_dim, self.sparse.block, n, L["bounds"])
 
     def _prefill_buffers(self, U: int) -> dict:
         """Activations of a ubatch of U tokens (allocated on first use, grown when a larger one comes)."""
@@ -245,12 +309,14 @@ class LlamaDecoder:
         self._pf = {"U": U, "x": d.alloc(U * c.n_embd * f4), "h": d.alloc(U * c.n_embd * f4),
                     "xn": d.alloc(U * c.n_embd * f4), "qkv": d.alloc(U * (c.n_q + 2 * c.E) * f4),
                     "att": d.alloc(U * c.n_q * f4), "gu": d.alloc(U * 2 * c.n_ff * f4),
-                    "glu": d.alloc(U * c.n_ff * f4), "in": d.alloc(U * (32 if self.kv4 else 16))}
+                    "glu": d.alloc(U * c.n_ff * f4), "in": d.alloc(U * (32 if self.kv4 else 16) + (8 if self.sparse else 0))}
         # a ubatch's cells (int64), positions and token ids (int32), written with one copy
         self._pf.update(cell=H.BufferPart(self._pf["in"], 0, U * 8), pos=H.BufferPart(self._pf["in"], U * 8, U * 4),
                         ids=H.BufferPart(self._pf["in"], U * 12, U * 4))
         if self.kv4:                       # and their runs of visible cells
             self._pf.update(runs=H.BufferPart(self._pf["in"], U * 16, U * 16))
+        if self.sparse is not None:        # and {first cell, end} of the ubatch
+            self._pf.update(new=H.BufferPart(self._pf["in"], U * 32, 8))
         return self._pf
 
     def prefill(self, tokens, pos0: int = 0, ubatch: int = 512) -> None:
@@ -263,7 +329,12 @@ class LlamaDecoder:
         toks = np.ascontiguousarray(tokens, np.int32).reshape(-1)
         if toks.size == 0:
             raise ValueError("prefill of no tokens")
-        if pos0 < 0 or pos0 + toks.size > self.kv_size:
+        if pos0 == 0:                      # another context
+            self.dropped = self.n_cells = 0
+            if self.track is not None:
+                for L in self.layers:
+                    L["weights"].fill(0)
+        if pos0 < self.dropped or pos0 - self.dropped + toks.size > self.kv_size:
             raise ValueError(f"positions {pos0} .. {pos0 + toks.size - 1} outside the cache of {self.kv_size} cells")
         for u0 in range(0, toks.size, ubatch):
             self._prefill_ubatch(toks[u0:u0 + ubatch], pos0 + u0)
@@ -286,12 +357,15 @@ class LlamaDecoder:
         pf = self._prefill_buffers(T)
         x, h, xn, qkv, att, gu, glu = (pf[k] for k in ("x", "h", "xn", "qkv", "att", "gu", "glu"))
         U, pos = pf["U"], pos0 + np.arange(T, dtype=np.int64)
-        ins = np.zeros((8 if self.kv4 else 4) * U, np.int32)
-        ins[:2 * T].view(np.int64)[:] = pos
+        cell0 = pos0 - self.dropped
+        ins = np.zeros((8 if self.kv4 else 4) * U + (2 if self.sparse else 0), np.int32)
+        ins[:2 * T].view(np.int64)[:] = pos - self.dropped
         ins[2 * U:2 * U + T] = pos
         ins[3 * U:3 * U + T] = toks
         if self.kv4:
-            ins[4 * U:].reshape(U, 4)[:T, 1] = pos + 1
+            ins[4 * U:8 * U].reshape(U, 4)[:T, 1] = pos - self.dropped + 1
+        if self.sparse is not None:
+            ins[8 * U:] = cell0, cell0 + T
         if ins.nbytes <= 16384:                                   # queued behind the ubatch before, no wait
             d.write_async(pf["in"], ins)
         else:
@@ -317,18 +391,21 @@ class LlamaDecoder:
                 else:
                     fused_rows(lambda t0, tt: d.mul_mat_norm(L["wqkv"], x.ptr + t0 * n * f4, tt, n, c.eps,
                                                              L["attn_norm"], qkv.ptr + t0 * w3 * f4, w3))
-                d.rope_kv(qkv, T, w3, c.head_dim, c.n_head, c.n_head_kv, c.head_dim, c.rope_mode, pf["pos"],
-                          c.rope_base, L["kc"], L["vc"], pf["cell"], self.bad)
+                self._rope_kv(qkv, T, w3, pf["pos"], L, pf["cell"])
             else:
                 d.rms_norm(x, n, T, n, c.eps, xn, n, w=L["attn_norm"], w_stride=n)
                 d.mul_mat(L["wqkv"], xn, T, n, qkv, w3)
-                d.rope(qkv, T, w3, c.head_dim, c.n_head + c.n_head_kv, c.head_dim, c.rope_mode, pf["pos"],
-                       c.rope_base, qkv, w3)
-                d.kv_set_rows(L["kc"], 0, qkv.ptr + nq * f4, T, w3, pf["cell"], self.bad)
-                d.kv_set_rows(L["vc"], 1, qkv.ptr + (nq + E) * f4, T, w3, pf["cell"], self.bad)
+                self._rope_kv(qkv, T, w3, pf["pos"], L, pf["cell"], separate=True)
             if self.kv4:
-                d.flash_attn_kv4(qkv, T, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, pos0 + T, att,
+                d.flash_attn_kv4(qkv, T, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, cell0 + T, att,
                                  nq, runs=pf["runs"])
+                if self.sparse is not None:
+                    d.kv4_bounds(L["kc"], c.head_dim, self.sparse.block, cell0 + T, L["bounds"], cells=pf["new"], n_new=T)
+                if self.track is not None:
+                    r = min(T, self.TRACKED_ROWS)
+                    d.attn_weights_kv4(qkv.ptr + (T - r) * w3 * f4, r, w3, L["kc"], c.head_dim, c.n_head, c.n_head_kv, self.scale,
+                                       cell0 + T, L["weights"], before=L["weights"], decay=self.track,
+                                       runs=pf["runs"].ptr + (T - r) * 16)
             else:
                 d.flash_attn(qkv, T, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, msum, att, nq,
                              new_runs=runs)
@@ -344,9 +421,26 @@ class LlamaDecoder:
                 d.mul_mat(L["wgu"], xn, T, n, gu, 2 * ff)
                 d.swiglu(gu, 2 * ff, gu.ptr + ff * f4, 2 * ff, ff, T, glu, ff)
             d.mul_mat(L["wd"], glu, T, ff, x, n, add=h, add_stride=n)
+        self.n_cells = cell0 + T
+
+    def _rope_kv(self, qkv, T: int, w3: int, pos, L: dict, cell, separate: bool = False, stream=None) -> None:
+        """ROPE of q and k in place, and both SET_ROWS_KV: in one call where there is one."""
+        c, d = self.cfg, self.dev
+        if self.scaling is None and not separate:
+            d.rope_kv(qkv, T, w3, c.head_dim, c.n_head, c.n_head_kv, c.head_dim, c.rope_mode, pos, c.rope_base, L["kc"],
+                      L["vc"], cell, self.bad, stream=stream)
+            return
+        heads = c.n_head + c.n_head_kv
+        if self.scaling is None:
+            d.rope(qkv, T, w3, c.head_dim, heads, c.head_dim, c.rope_mode, pos, c.rope_base, qkv, w3, stream=stream)
+        else:
+            d.rope_scaled(qkv, T, w3, c.head_dim, heads, c.head_dim, c.rope_mode, pos, self.scaling, qkv, w3,
+                          freq_factors=self.rope_ff, stream=stream)
+        d.kv_set_rows(L["kc"], 0, qkv.ptr + c.n_q * 4, T, w3, cell, self.bad, stream=stream)
+        d.kv_set_rows(L["vc"], 1, qkv.ptr + (c.n_q + c.E) * 4, T, w3, cell, self.bad, stream=stream)
 
     def _mask(self, pos: int, n_kv: int | None):
-        if not 0 <= pos < self.kv_size:
+        if not 0 <= pos - self.dropped < self.kv_size:
             raise ValueError(f"position {pos} outside the cache of {self.kv_size} cells")
         if n_kv is None:
             n_kv = min(self.kv_size, (pos + 1 + 255) // 256 * 256)
@@ -362,9 +456,13 @@ class LlamaDecoder:
         return p
 
     def _inputs(self, pos: int, token: int | None = None):
-        """Where a token's input bytes go, and they: with 4-bit caches the runs (cells [0, pos]) in front."""
+        """Where a token's input bytes go, and they: with 4-bit caches the runs (the cells up to its own) and its cell in front."""
         p = self._params(pos, token)
-        return (self._in, np.concatenate([np.array([0, pos + 1, 0, 0], np.int32), p])) if self.kv4 else (self.params, p)
+        if not self.kv4:
+            return self.params, p
+        cell = pos - self.dropped
+        p[2] = cell
+        return self._in, np.concatenate([np.array([0, cell + 1, 0, 0, cell, cell + 1, 0, 0], np.int32), p])
 
     def _ops(self, out_tok, msum=None, runs=None, stream=None, n_kv=None) -> None:
         """The launches of one decode token. msum given: FLASH_ATTN_EXT planned on the host per call
@@ -377,7 +475,10 @@ class LlamaDecoder:
         w3 = nq + 2 * E
         fa_tab = self.fused and msum is None and self.fa_rope
         if fa_tab:                                                # the position's angles, once per token
-            d.rope_table(self.pos_ptr, c.head_dim, c.rope_base, self.rtab, stream=stream)
+            if self.scaling is None:
+                d.rope_table(self.pos_ptr, c.head_dim, c.rope_base, self.rtab, stream=stream)
+            else:
+                d.rope_scaled_table(self.pos_ptr, c.head_dim, self.scaling, self.rtab, freq_factors=self.rope_ff, stream=stream)
         for L in self.layers:
             fa_done = False
             if fa_tab and self.qkv_in_attn:                       # Q|K|V, ROPE, SET_ROWS_KV and FA: one call
@@ -393,20 +494,15 @@ class LlamaDecoder:
                                                stream=stream)
                     fa_done = True
                 else:
-                    d.rope_kv(self.qkv, 1, w3, c.head_dim, c.n_head, c.n_head_kv, c.head_dim, c.rope_mode,
-                              self.pos_ptr, c.rope_base, L["kc"], L["vc"], self.cell_ptr, self.bad, stream=stream)
+                    self._rope_kv(self.qkv, 1, w3, self.pos_ptr, L, self.cell_ptr, stream=stream)
             else:
                 d.rms_norm(self.x, n, 1, n, c.eps, self.xn, n, w=L["attn_norm"], w_stride=n, stream=stream)
                 d.mul_mat(L["wqkv"], self.xn, 1, n, self.qkv, w3, stream=stream)
-                d.rope(self.qkv, 1, w3, c.head_dim, c.n_head + c.n_head_kv, c.head_dim, c.rope_mode, self.pos_ptr,
-                       c.rope_base, self.qkv, w3, stream=stream)
-                d.kv_set_rows(L["kc"], 0, self.qkv.ptr + nq * f4, 1, E, self.cell_ptr, self.bad, stream=stream)
-                d.kv_set_rows(L["vc"], 1, self.qkv.ptr + (nq + E) * f4, 1, E, self.cell_ptr, self.bad, stream=stream)
+                self._rope_kv(self.qkv, 1, w3, self.pos_ptr, L, self.cell_ptr, separate=True, stream=stream)
             if fa_done:
                 pass
             elif self.kv4:
-                d.flash_attn_kv4(self.qkv, 1, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, n_kv,
-                                 self.att, nq, runs=self.runs_ptr, ws=self.ws, stream=stream)
+                self._attend4(L, w3, n_kv, stream)
             elif msum is not None:
                 d.flash_attn(self.qkv, 1, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale,
                              msum, self.att, nq, new_runs=runs, stream=stream)
@@ -430,6 +526,50 @@ class LlamaDecoder:
             d.mul_mat(self.wout, self.xn, 1, n, self.logits, c.n_vocab, stream=stream)
         d.argmax(self.logits, c.n_vocab, 1, c.n_vocab, out_tok, stream=stream)
 
+    def _attend4(self, L: dict, w3: int, n_kv: int, stream) -> None:
+        """A decode token's attention over 4-bit caches of at most n_kv cells in use."""
+        c, d = self.cfg, self.dev
+        heads = (c.head_dim, c.n_head, c.n_head_kv)
+        s = self.sparse
+        if s is not None:
+            d.kv4_bounds(L["kc"], c.head_dim, s.block, n_kv, L["bounds"], cells=self.new_ptr, n_new=1, stream=stream)
+        if s is not None and n_kv > s.n_blocks * s.block:
+            d.kv4_select(self.qkv, 1, w3, L["bounds"], self.n_bounds, *heads, s.block, n_kv, s.n_blocks, s.first, s.last, self.blocks,
+                         runs=self.runs_ptr, ws=self.ws, stream=stream)
+            d.flash_attn_kv4_blocks(self.qkv, 1, w3, L["kc"], L["vc"], *heads, self.scale, n_kv, self.blocks, s.n_blocks, s.block,
+                                    self.att, c.n_q, runs=self.runs_ptr, ws=self.ws, stream=stream)
+        else:
+            d.flash_attn_kv4(self.qkv, 1, w3, L["kc"], L["vc"], *heads, self.scale, n_kv, self.att, c.n_q, runs=self.runs_ptr,
+                             ws=self.ws, stream=stream)
+        if self.track is not None:
+            d.attn_weights_kv4(self.qkv, 1, w3, L["kc"], *heads, self.scale, n_kv, L["weights"], before=L["weights"],
+                               decay=self.track, runs=self.runs_ptr, ws=self.ws, stream=stream)
+
+    def evict(self, n_keep: int, first: int = 4, last: int = 64) -> None:
+        """Thin every layer's caches out to n_keep of their cells: the first, the last and those that attention gave most weight
+        (track). Positions go on; the next token's cell is n_keep. Waits for the device."""
+        if self.track is None:
+            raise ValueError("no weights of cells: track was not asked for")
+        n, d, c = self.n_cells, self.dev, self.cfg
+        if not 0 < n_keep <= n or first + last > n_keep:
+            raise ValueError(f"{first} + .. + {last} of {n_keep} of {n} cells")
+        idx, kept = d.alloc(8 * n_keep), d.alloc(4 * n_keep)
+        for L in self.layers:
+            d.kv_pick(L["weights"], n, n_keep, first, last, idx, kept=kept)
+            d.kv_gather(L["kc"], L["kc"], H.KV_K, idx, n_keep, self.bad)
+            d.kv_gather(L["vc"], L["vc"], H.KV_V, idx, n_keep, self.bad)
+            d.copy_async(L["weights"], kept, 4 * n_keep)
+            d.sync()
+            if n > n_keep:
+                H.BufferPart(L["weights"], 4 * n_keep, 4 * (n - n_keep)).fill(0)
+            if self.sparse is not None:
+                self._all_bounds(L, n_keep)
+        d.sync()
+        idx.free()
+        kept.free()
+        self.dropped += n - n_keep
+        self.n_cells = n_keep
+
     def step(self, token: int | None, pos: int, n_kv: int | None = None) -> None:
         """One eager decode token at position pos (cell pos): every op a separate call, FLASH_ATTN_EXT
         planned per call. token: the id to embed, or None for the previous step's greedy token. Logits
@@ -441,15 +581,17 @@ class LlamaDecoder:
         buf.write(ins)
         if self.kv4:
             self._graph_cells(pos)
-        self._ops(self.next, msum, runs, n_kv=pos + 1)
+        self._ops(self.next, msum, runs, n_kv=pos - self.dropped + 1)
+        self.n_cells = pos - self.dropped + 1
 
     def _graph_cells(self, pos: int) -> bool:
         """4-bit caches: a decode graph is captured for 256, 512, 1024 .. cells (what splits its attention). True when
-        position pos is beyond the last one's; the workspace then fits the next."""
-        if pos < self.n_kv_graph:
+        position pos's cell is beyond the last one's; the workspace then fits the next."""
+        cell = pos - self.dropped
+        if cell < self.n_kv_graph:
             return False
         c, n = self.cfg, 256
-        while n <= pos:
+        while n <= cell:
             n *= 2
         if self.graph is not None:         # (it reads the workspace)
             self.graph.free()
@@ -458,10 +600,21 @@ class LlamaDecoder:
             self.ws.free()
         self.ws, self.n_kv_graph = None, 0   # (until there is another: an allocation may fail)
         n_kv = min(n, self.kv_size)
-        need = self.dev.flash_attn_kv4_ws(1, c.head_dim, c.n_head, c.n_head_kv, n_kv)
+        need = self._decode_ws(n_kv)
         self.ws = self.dev.alloc(need) if need else None
         self.n_kv_graph = n_kv
         return True
+
+    def _decode_ws(self, n_kv: int) -> int:
+        """Bytes of workspace of a decode token's calls, which run one after another, over at most n_kv cells."""
+        c, d, s = self.cfg, self.dev, self.sparse
+        need = [d.flash_attn_kv4_ws(1, c.head_dim, c.n_head, c.n_head_kv, n_kv)]
+        if s is not None:
+            need += [d.kv4_select_ws(1, c.n_head_kv, s.block, n_kv),
+                     d.flash_attn_kv4_blocks_ws(1, c.head_dim, c.n_head, c.n_head_kv, s.n_blocks, s.block)]
+        if self.track is not None:
+            need.append(d.attn_weights_kv4_ws(1, c.head_dim, c.n_head, c.n_head_kv, n_kv))
+        return max(need)
 
     def step_graph(self, token: int | None, pos: int, n_kv: int | None = None) -> None:
         """One decode token as one graph replay. Per token the host only plans the attention chunks and
@@ -483,6 +636,7 @@ class LlamaDecoder:
             self.graph = g
             self.captures += 1
         self.graph.launch()
+        self.n_cells = pos - self.dropped + 1
 
     def step_async(self, token: int | None, pos: int, n_kv: int | None = None) -> None:
         """The launches of step_graph issued directly (no graph): the device-resident plan, the
@@ -496,6 +650,7 @@ class LlamaDecoder:
         else:
             self.plan.set(msum, runs)
         self._ops(self.tok, n_kv=self.n_kv_graph)
+        self.n_cells = pos - self.dropped + 1
 
     def generate_graph(self, first_token: int, pos0: int, n_tokens: int, hist=None, check: bool = True) -> None:
         """Greedy decode of n_tokens by graph replays, queued without waiting for the device; the token
