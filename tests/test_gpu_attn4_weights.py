@@ -151,3 +151,90 @@ def test_in_a_graph(dev):
         want, tol = 0.5 * want + w, 0.5 * tol + t + 2.0 ** -24 * (0.5 * want + w)
         check(acc.read(np.float32, (n_kv,)), want, tol)
     g.free()
+
+
+MANY = [
+    # n_head, n_head_kv, D, T, n_kv
+    (8, 2, 64, 40, 700), (32, 8, 128, 33, 500), (4, 1, 256, 70, 400), (3, 3, 64, 200, 130), (8, 1, 128, 16, 31), (16, 1, 64, 9, 2100),
+]
+
+
+@pytest.mark.parametrize("typ", [R.Q4_0, R.Q4_1])
+@pytest.mark.parametrize("nh,nkv,D,T,n_kv", MANY)
+def test_many_rows(dev, typ, nh, nkv, D, T, n_kv):
+    """Rows for several waves: all cells, causal, sequences side by side in one cache, ragged runs, some empty."""
+    rng = np.random.default_rng(D + T)
+    rows = P.cache_rows(nh + D, n_kv + 40, nkv * D)
+    rows[n_kv:] = 6e4                                               # (behind the cells in use)
+    kc, ki = P.fill(dev, rows, typ)[0], R.quantize(rows, typ)
+    q = rng.standard_normal((T, nh * D)).astype(np.float32) * 10.0 ** rng.integers(-2, 1, (T, 1)).astype(np.float32)
+    causal, apart = np.zeros((T, 4), np.uint32), np.zeros((T, 4), np.uint32)
+    causal[:, 1] = np.clip(n_kv - T + 1 + np.arange(T), 0, n_kv)
+    cut = np.sort(rng.integers(0, n_kv + 1, 4))
+    for t in range(T):
+        s = 5 * t // T
+        apart[t] = (0 if s == 0 else cut[s - 1], n_kv if s == 4 else cut[s], 0, 0)
+    ragged = np.sort(rng.integers(0, n_kv + 30, (T, 2, 2)), -1).reshape(T, 4)
+    ragged[::7] = (3, 3, 9, 2)
+    for runs in (None, causal, apart, ragged):
+        check(run(dev, q, kc, D, nh, nkv, n_kv, runs), *W.weights(q, ki, typ, D, nh, nkv, 1 / math.sqrt(D), n_kv, runs))
+
+
+@pytest.mark.parametrize("typ", [R.Q4_0, R.Q4_1])
+@pytest.mark.parametrize("size", [1e-6, 2e-3, 300.0, 6e4])
+def test_many_rows_of_any_size(dev, typ, size):
+    """K from what leaves subnormal scales to what fills f16's range; next to cells that are not seen and hold what is not finite."""
+    nh, nkv, D, T, n_kv = 8, 2, 128, 40, 300
+    rows = np.clip(P.cache_rows(9, n_kv, nkv * D) * size, -6e4, 6e4).astype(np.float32)
+    rows[100:110], rows[290], rows[291] = np.inf, np.nan, 6e4
+    kc, ki = P.fill(dev, rows, typ)[0], R.quantize(rows, typ)
+    q = np.random.default_rng(2).standard_normal((T, nh * D)).astype(np.float32)
+    runs = np.tile(np.array([[0, 100, 110, 290]], np.uint32), (T, 1))
+    runs[5:20, 1] = 64 + np.arange(15)
+    scale = 0.1 / max(size, 1e-6) / math.sqrt(D)
+    check(run(dev, q, kc, D, nh, nkv, n_kv, runs, scale=scale), *W.weights(q, ki, typ, D, nh, nkv, float(np.float32(scale)), n_kv, runs))
+
+
+def test_many_rows_again(dev):
+    """The same bits again, with a workspace, in a graph between eager calls; a row of NaNs."""
+    nh, nkv, D, T, n_kv = 16, 4, 128, 48, 900
+    rows = P.cache_rows(9, n_kv, nkv * D)
+    kc = P.fill(dev, rows, R.Q4_1)[0]
+    q = np.random.default_rng(2).standard_normal((T, nh * D)).astype(np.float32)
+    one = run(dev, q, kc, D, nh, nkv, n_kv)
+    assert (one == run(dev, q, kc, D, nh, nkv, n_kv)).all()
+    ws = dev.alloc(dev.attn_weights_kv4_ws(T, D, nh, nkv, n_kv))
+    assert (one == run(dev, q, kc, D, nh, nkv, n_kv, ws=ws)).all()
+    out, qb = dev.alloc(4 * n_kv), dev.upload(q)
+    dev.graph_begin()
+    dev.attn_weights_kv4(qb, T, nh * D, kc, D, nh, nkv, 1 / math.sqrt(D), n_kv, out, ws=ws)
+    g = dev.graph_end()
+    for i in range(3):
+        g.launch()
+        assert (out.read(np.float32, (n_kv,)) == one).all()
+        assert (run(dev, q[:9], kc, D, nh, nkv, n_kv) >= 0).all()
+    bad = rows.copy()
+    bad[500] = np.nan                                               # (stored as a row of zeros)
+    kc, ki = P.fill(dev, bad, R.Q4_1)[0], R.quantize(bad, R.Q4_1)
+    runs = np.tile(np.array([[0, 500, 501, 900]], np.uint32), (T, 1))
+    runs[7, 1] = 501
+    check(run(dev, q, kc, D, nh, nkv, n_kv, runs), *W.weights(q, ki, R.Q4_1, D, nh, nkv, 1 / math.sqrt(D), n_kv, runs))
+
+
+@pytest.mark.parametrize("typ", [R.Q4_0, R.Q4_1])
+def test_many_rows_and_an_infinity(dev, typ):
+    """A row that sees a cell of infinities gives its cells NaN, the others keep theirs."""
+    nh, nkv, D, T, n_kv = 16, 4, 128, 48, 900
+    rows = P.cache_rows(9, n_kv, nkv * D)
+    rows[500] = np.inf
+    kc, ki = P.fill(dev, rows, typ)[0], R.quantize(rows, typ)
+    q = np.random.default_rng(2).standard_normal((T, nh * D)).astype(np.float32)
+    runs = np.tile(np.array([[0, 500, 501, 900]], np.uint32), (T, 1))
+    check(run(dev, q, kc, D, nh, nkv, n_kv, runs), *W.weights(q, ki, typ, D, nh, nkv, 1 / math.sqrt(D), n_kv, runs))
+    runs[7] = (490, 520, 0, 0)
+    got = run(dev, q, kc, D, nh, nkv, n_kv, runs)
+    others = np.delete(np.arange(T), 7)
+    want, tol = W.weights(q[others], ki, typ, D, nh, nkv, 1 / math.sqrt(D), n_kv, runs[others])
+    assert np.isnan(got[490:520]).all()
+    outside = np.delete(np.arange(n_kv), np.arange(490, 520))
+    check(got[outside], want[outside], tol[outside])
