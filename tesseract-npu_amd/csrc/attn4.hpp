@@ -228,6 +228,8 @@ struct Attn4 {
         }
     }
     // The queries; their pieces go to `lds`, [row group][block][piece][lane], the blocks shared out over the waves.
+    // TOP: 2^e of a row's largest |q| is in [2^(TOP - 127), 2 of it).
+    template <int TOP = 140>
     __device__ __forceinline__ void load_queries(float scale, uint32_t lane, h8 * lds, uint32_t wave) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -241,7 +243,7 @@ struct Attn4 {
             }
             top = rows_max(top);
             if constexpr (D > 128) asm volatile("" : "+v"(q));     // (read again rather than kept: no registers for it)
-            const int e = 140 - (int)(fb(top) >> 23);              // 2^e top in [2^13, 2^14)
+            const int e = TOP - (int)(fb(top) >> 23);              // (140: 2^e top in [2^13, 2^14))
             csc[n] = __builtin_ldexpf(scale, -e) * kLog2e;         // (in this order: scale log2(e) may pass f32's range)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -306,10 +308,14 @@ struct Attn4 {
             }
     }
 
+    // MIN false: without q4_1's minima, added to what s holds (C 1).
+    template <bool MIN = true>
     __device__ __forceinline__ void scores(const Tl & k, const h8 * q, f4 (&s)[NT][2]) const {
         constexpr float zero = TYPE == kKvQ4_0 ? 8.0f : 0.0f;
+        constexpr bool Q41 = TYPE == kKvQ4_1 && MIN;
+        if constexpr (MIN)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f4{ 0.0f, 0.0f, 0.0f, 0.0f };
         if constexpr (C > 1) {
 #pragma unroll
             for (int y = 0; y < NK; ++y) {
@@ -354,7 +360,7 @@ struct Attn4 {
         for (int j = 0; j < D / 64; ++j) {
             uint32_t dw[2][4], mw[2][4];
             all_cells(k.d[j], dw);
-            if constexpr (TYPE == kKvQ4_1) all_cells(k.m[j], mw);
+            if constexpr (Q41) all_cells(k.m[j], mw);
 #pragma unroll
             for (int bb = 0; bb < 2; ++bb) {
                 const int b = 2 * j + bb;
@@ -370,7 +376,7 @@ struct Attn4 {
                         for (int i = 0; i < 4; ++i) {
                             const int y = 2 * u + (i >> 1);
                             s[n][u][i] = __builtin_fmaf(half_of(dw[bb][y], i & 1), x[i], s[n][u][i]);
-                            if constexpr (TYPE == kKvQ4_1) s[n][u][i] = __builtin_fmaf(half_of(mw[bb][y], i & 1), qs[n][b], s[n][u][i]);
+                            if constexpr (Q41) s[n][u][i] = __builtin_fmaf(half_of(mw[bb][y], i & 1), qs[n][b], s[n][u][i]);
                         }
                     }
                 }

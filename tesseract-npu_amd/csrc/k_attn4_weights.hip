@@ -8,6 +8,12 @@
 //                    then meet; 32 sums a tile and row set go to memory
 //   k_attn4_cells    the row sets' sums added up, in their order: no atomic decides a rounding
 // A workgroup's waves have the same rows (up to four groups of 16: nothing but scores to hold) and take tiles in turn.
+//
+// Bound: a decode token's three launches (32 heads of 128 over 8 KV heads behind 8192 cells: 13.1 us, 5.9 + 7.2 + 2.5 by themselves, the
+// codes' 9 MB in 2); for many rows the f32 operations on the scores, 4 for every product of 16 x 16 x 32 and then 4 and an exponential
+// a score: 64 such tokens behind 32768 cells of q4_1 take 108.6 us, 61 + 60, of which the matrix instruction is busy for 14 each.
+// Its time and theirs add up here. K in two f16 pieces with its scales, shared by a workgroup's waves through LDS, needs none of the
+// four and three products for two: 110 us, and 121 for q4_0, which takes 98 so.
 #include "attn4.hpp"
 #include "weights4_plan.hpp"
 
@@ -18,6 +24,65 @@ struct Weights4 : Attn4<D, NT, 1, TYPE> {
     using A = Attn4<D, NT, 1, TYPE>;
     using typename A::Tl;
     using typename A::Span;
+    static constexpr bool MIN = TYPE == kKvQ4_1;
+    static constexpr int NB = D / 32, NW = (NB + 3) / 4;
+
+    // A tile's codes and scales, and q4_1's minima as an operand of the matrix instruction has them: of a group of 16 cells the lane's
+    // cell lane & 15 in blocks 4 k + g. They meet the sums of the blocks' q, in two pieces, in one product for all blocks: 64 tokens
+    // of 32 heads behind 32768 cells take 110 us, with a product and a sum in f32 for every block 125.
+    struct Codes {
+        Tl t;
+        uint32_t m[2][MIN ? NW : 1];
+    };
+    h8 qm[NT];
+    static __device__ __forceinline__ void load(Codes & k, const uint8_t * p, size_t pair, uint32_t lane) {
+        const uint32_t word = 8u * (lane >> 4) + (lane & 7u), c = lane & 15u;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            const uint8_t * t = p + j * pair;
+            const uint2 x = *(const uint2 *)(t + 8u * lane), y = *(const uint2 *)(t + 512u + 8u * lane);
+            k.t.w[j] = make_uint4(x.x, x.y, y.x, y.y);
+            k.t.d[j] = *(const uint32_t *)(t + 1024u + (MIN ? 8u : 4u) * word);
+        }
+        if constexpr (MIN)
+#pragma unroll
+            for (uint32_t u = 0; u < 2u; ++u)
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    const uint32_t b = (4u * i + (lane >> 4)) & (NB - 1u);   // (heads of 64: blocks 2 and 3 meet sums of 0)
+                    k.m[u][i] = *(const uint16_t *)(p + (b >> 1) * pair + 1028u + 8u * (8u * (c >> 2) + 4u * (b & 1u) + 2u * u + ((c >> 1) & 1u)) + 2u * (c & 1u));
+                }
+    }
+    __device__ __forceinline__ void scores(const Codes & k, const h8 * q, f4 (&s)[NT][2]) const {
+        if constexpr (MIN) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t w[4] = {};
+#pragma unroll
+                for (int i = 0; i < NW; ++i) w[i] = k.m[u][i] * 0x10001u;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[n][u] = mfma(of_words(w), qm[n], f4{ 0.0f, 0.0f, 0.0f, 0.0f });
+            }
+        }
+        A::template scores<!MIN>(k.t, q, s);
+    }
+    __device__ __forceinline__ void load_queries(float scale, uint32_t lane, h8 * lds, uint32_t wave) {
+        A::template load_queries<MIN ? 135 : 140>(scale, lane, lds, wave);   // (135: the sum of a block fits f16)
+        if constexpr (MIN)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t w[4] = {};
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    float z = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < 4 && 4 * i + g < NB; ++g) z = (lane >> 4) == (uint32_t)g ? this->qs[n][4 * i + g] : z;
+                    const uint32_t hi = pair_of(z, 0.0f), lo = pair_of(z - half_of(hi, 0), 0.0f);
+                    w[i] = (hi & 0xFFFFu) | (lo << 16);
+                }
+                qm[n] = of_words(w);
+            }
+    }
 
     // The lane's cells of tile i that its row n sees: bit 4 u + k its cell 16 u + 4 g + k.
     __device__ __forceinline__ uint32_t seen(int n, uint32_t i, uint32_t g) const {
@@ -45,18 +110,18 @@ struct Weights4 : Attn4<D, NT, 1, TYPE> {
             const uint32_t j = part + min(x, cnt - 1u) * parts;
             return j < n0 ? w0.lo + j : w1.lo + (j - n0);
         };
-        Tl k0, k1;
+        Codes k0, k1;
         if (cnt != 0u) {
-            A::template load<false>(k0, kp + nth(0u) * tb, pair, lane);
-            A::template load<false>(k1, kp + nth(1u) * tb, pair, lane);
+            load(k0, kp + nth(0u) * tb, pair, lane);
+            load(k1, kp + nth(1u) * tb, pair, lane);
         }
-        this->load_queries(a.scale, lane, lds, wave);
+        load_queries(a.scale, lane, lds, wave);
         __syncthreads();
         for (uint32_t x = 0; x < cnt; x += 2u) {                   // two tiles ahead
             one(k0, nth(x), true);
-            A::template load<false>(k0, kp + nth(x + 2u) * tb, pair, lane);
+            load(k0, kp + nth(x + 2u) * tb, pair, lane);
             if (x + 1u < cnt) one(k1, nth(x + 1u), true);
-            A::template load<false>(k1, kp + nth(x + 3u) * tb, pair, lane);
+            load(k1, kp + nth(x + 3u) * tb, pair, lane);
         }
         // the others: what is left of all tiles, dealt on from the wave after the one that took the last whole tile
         const uint32_t g0 = w0.lo, g1 = g0 + (w1.lo - w0.hi), np = (a.n_kv + 31u) / 32u - nw;
@@ -69,13 +134,13 @@ struct Weights4 : Attn4<D, NT, 1, TYPE> {
                 none(i);
                 continue;
             }
-            A::template load<false>(k0, kp + i * tb, pair, lane);
+            load(k0, kp + i * tb, pair, lane);
             one(k0, i, false);
         }
     }
 };
 
-constexpr int weights_waves(int D, int NT) { return D * NT <= 128 ? 4 : D * NT <= 256 || D <= 128 ? 2 : 1; }
+constexpr int weights_waves(int D, int NT) { return D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2; }
 
 // Workgroup (KV head, split, row set), KV heads fastest.
 template <int D, int NT, uint32_t TYPE>
@@ -89,7 +154,7 @@ __global__ __launch_bounds__(256, weights_waves(D, NT)) void k_attn4_rowsums(Att
     w.load_runs(a, h, rg * 16u * NT, lane);
     float sub[NT] = {};                                            // the maxima in base 2 (0: none yet)
     w.walk(a, h, split * kWaves + wave, a.S * kWaves, (h8 *)room, wave, lane,
-           [&](const typename W::Tl & k, uint32_t i, bool whole) {
+           [&](const typename W::Codes & k, uint32_t i, bool whole) {
                f4 s[NT][2];
                uint32_t ql = lane;                                 // (q's pieces: read from LDS for every tile)
                asm volatile("" : "+v"(ql));
@@ -164,7 +229,7 @@ __global__ __launch_bounds__(256, weights_waves(D, NT)) void k_attn4_weights(Att
     }
     float * sums = (float *)((uint8_t *)a.part + p.sums) + ((size_t)h * p.n_rg + rg) * p.n_pad;
     w.walk(a, h, split * kWaves + wave, a.S * kWaves, (h8 *)room, wave, lane,
-           [&](const typename W::Tl & k, uint32_t i, bool whole) {
+           [&](const typename W::Codes & k, uint32_t i, bool whole) {
                f4 s[NT][2];
                uint32_t ql = lane;
                asm volatile("" : "+v"(ql));
@@ -202,7 +267,13 @@ __global__ __launch_bounds__(256) void k_attn4_cells(const float * sums, uint32_
     const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u, c = blockIdx.x * 64u + lane;
     float x = 0.0f;
     if (c < n_kv)
-        for (uint32_t i = wave; i < n; i += 4u) x += sums[(size_t)i * n_pad + c];
+        for (uint32_t i = wave; i < n; i += 32u) {                 // (eight on their way at once)
+            float v[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8u; ++j) v[j] = i + 4u * j < n ? sums[(size_t)(i + 4u * j) * n_pad + c] : 0.0f;
+#pragma unroll
+            for (uint32_t j = 0; j < 8u; ++j) x += v[j];
+        }
     part[wave][lane] = x;
     __syncthreads();
     if (wave == 0u && c < n_kv) {
@@ -229,7 +300,6 @@ static int launch_weights_t(const Attn4Args & a, const Weights4Plan & p, hipStre
         case 128 * 8 + 2: return launch_weights<128, 2, TYPE>(a, p, s);
         case 128 * 8 + 4: return launch_weights<128, 4, TYPE>(a, p, s);
         case 256 * 8 + 1: return launch_weights<256, 1, TYPE>(a, p, s);
-        case 256 * 8 + 2: return launch_weights<256, 2, TYPE>(a, p, s);
         case 512 * 8 + 1: return launch_weights<512, 1, TYPE>(a, p, s);
         default: return -2;
     }

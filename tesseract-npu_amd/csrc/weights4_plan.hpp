@@ -27,10 +27,12 @@ constexpr size_t weights4_pair(const Weights4Plan & p, uint32_t n_head_kv, uint3
 inline Weights4Plan weights4_plan(uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_kv, uint32_t n_cu) {
     Weights4Plan p{};
     const uint64_t G = n_head / n_head_kv, tiles = std::max<uint64_t>(1u, ((uint64_t)n_kv + 31u) / 32u);
-    // Four groups of rows share the unpacking of a tile's codes (heads up to 128, whose queries' pieces leave LDS for three workgroups)
-    // where there are that many rows; heads of 256 two.
-    const uint64_t R = T * G;
-    p.NT = D <= 128u && R > 32u ? 4u : D <= 256u && R > 16u ? 2u : 1u;
+    // More groups of rows share the unpacking of a tile's codes, fewer start sooner (their queries' pieces are made by every workgroup).
+    // By the products that a SIMD has (of 16 rows, a tile and 32 values): two groups from 64, four from 256. Microseconds of 1, 2 and 4
+    // groups, 32 heads of 128 over 8 KV heads: 64 tokens behind 2048 cells 21.7, 22.9, 30.5, behind 8192 45.5, 41.4, 44.6, behind 32768 129,
+    // 105, 98; 16 tokens behind 8192 22.2, 24.8, 36.0. Heads of 256 keep to one (64 tokens of 8 heads over 4, 32768 cells: 72.6, 91.1).
+    const uint64_t R = T * G, groups = (R + 15u) / 16u, products = groups * n_head_kv * tiles * (D / 32u) / (4u * n_cu);
+    p.NT = D > 128u || groups == 1u || products < 64u ? 1u : groups == 2u || products < 256u ? 2u : 4u;
     p.n_pad = (uint32_t)(32u * tiles);
     // a launch's sums take at most 64 MiB, or are one token's
     const uint64_t rows = 16u * p.NT, most = std::max<uint64_t>(1u, ((uint64_t)64 << 20) / (4u * (uint64_t)p.n_pad * n_head_kv));   // row sets of a KV head
