@@ -505,10 +505,11 @@ int tsr_hip_rope_table(tsr_hip_ctx * ctx, const int32_t * pos_dev, uint32_t n_di
  *   hi = min(n_dims - 1, ceil(c(beta_slow))),  c(b) = n_dims ln(n_ctx_orig / (2 pi b)) / (2 ln freq_base)
  * and its values are multiplied by m = attn_factor, with ext_factor != 0 by attn_factor (1 + 0.1 ln(1 / s)): the parameters
  * of GGML_OP_ROPE under its names. Angles, cosines and sines in f64, rounded to f32 once; a pair is then turned by tsr_hip_rope's
- * operations. Modes, layouts and rows as tsr_hip_rope (dims from n_dims on are copied; y may be x), positions of either sign: -p turns back what p has turned (K
- * rows of a context shift; m twice). Its angles are not tsr_hip_rope's, which follow the reference's f32 recurrence. freq_base > 1;
+ * operations. Modes, layouts and rows as tsr_hip_rope (dims from n_dims on are copied; y may be x), positions of either
+ * sign: -p turns back what p has turned (K rows of a context shift; m twice). Its angles are not tsr_hip_rope's, which follow the reference's f32 recurrence. freq_base > 1;
  * s > 0; 0 <= ext_factor <= 1; n_ctx_orig and the betas are read where ext_factor != 0 and are > 0 there; head_dim <= 16384,
- * n_heads head_dim <= 2^18. 16-byte aligned rows of whole quads are fastest, any are taken. */
+ * n_heads head_dim <= 2^18, T < 2^24; y is x with x's stride or does not overlap it. 16-byte aligned rows of whole quads are
+ * fastest, any are taken. */
 typedef struct tsr_hip_rope_scaling {
     float    freq_base;      /* 10000, 500000, .. */
     float    freq_scale;     /* trained length / new length; 1: none */

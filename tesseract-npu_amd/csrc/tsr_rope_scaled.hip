@@ -47,8 +47,8 @@ int tsr_hip_rope_scaled(tsr_hip_ctx * ctx, const float * x_dev, uint32_t T, uint
     if (mode != TSR_HIP_ROPE_NORMAL && mode != TSR_HIP_ROPE_NEOX && mode != TSR_HIP_ROPE_IMROPE) return TSR_HIP_E_SHAPE;
     if (n_dims < 2u || n_dims % 2u != 0u || n_dims > head_dim || n_dims > 1024u || head_dim > 16384u) return TSR_HIP_E_SHAPE;
     const uint64_t width = (uint64_t)head_dim * n_heads;
-    if (T > 0x7FFFFFFFu || width > (1u << 18)) return TSR_HIP_E_SHAPE;   // (units below 2^32 / units of a head, rows below 2^32)
-    if (T > 1u && (x_stride < width || y_stride < width)) return TSR_HIP_E_ARG;
+    if (T >= 1u << 24 || width > (1u << 18)) return TSR_HIP_E_SHAPE;   // (a launch's threads and units below 2^32)
+    if (T > 1u && (x_stride < width || y_stride < width || (x_dev == y_dev && x_stride != y_stride))) return TSR_HIP_E_ARG;
     if ((((uintptr_t)x_dev | (uintptr_t)y_dev | (uintptr_t)pos_dev | (uintptr_t)freq_factors_dev) & 3u) != 0u) return TSR_HIP_E_ARG;
     tsr::RopeScaledArgs a{};
     if (!scaling_args(*scaling, n_dims, a)) return TSR_HIP_E_ARG;

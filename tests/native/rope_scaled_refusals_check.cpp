@@ -63,6 +63,11 @@ int main() {
     want(arg, 0, "rows that overlap", [](Call & c) { c.xs = 255; });
     want(arg, 0, "results that overlap", [](Call & c) { c.ys = 255; });
     want(0, 0, "one row needs no strides", [](Call & c) { c.T = 1; c.xs = c.ys = 0; });
+    want(0, 0, "in place", [](Call & c) { c.y = c.x; });
+    want(arg, 0, "in place with another stride", [](Call & c) { c.y = c.x; c.ys = 260; });
+    want(0, 0, "one row in place, whatever the strides", [](Call & c) { c.T = 1; c.y = c.x; c.ys = 260; });
+    want(0, 0, "as many tokens as a launch holds", [](Call & c) { c.T = (1u << 24) - 1u; });
+    want(shape, 0, "more", [](Call & c) { c.T = 1u << 24; });
     want(arg, 0, "a misaligned row", [](Call & c) { c.x = 0x1002; });
     want(arg, arg, "base 1", [](Call & c) { c.r.freq_base = 1.0f; });
     want(arg, arg, "base NaN", [](Call & c) { c.r.freq_base = __builtin_nanf(""); });
