@@ -290,8 +290,15 @@ class LlamaDecoder:
                 rows.free()
             if self.sparse is not None:
                 self._all_bounds(L, n)
-        self.n_cells = n
+        self.n_cells, self.dropped = n, 0
         self.dev.sync()
+
+    def _written_from(self, cell: int) -> None:
+        """Cells from here on are written anew: what the tokens that were there got of attention is not theirs."""
+        if self.track is not None and cell < self.n_cells:
+            for L in self.layers:
+                H.BufferPart(L["weights"], 4 * cell, 4 * (self.n_cells - cell)).fill(0)
+        self.n_cells = min(self.n_cells, cell)
 
     def _all_bounds(self, L: dict, n: int) -> None:
         """The bounds of a layer's first n cells."""
@@ -330,12 +337,10 @@ class LlamaDecoder:
         if toks.size == 0:
             raise ValueError("prefill of no tokens")
         if pos0 == 0:                      # another context
-            self.dropped = self.n_cells = 0
-            if self.track is not None:
-                for L in self.layers:
-                    L["weights"].fill(0)
+            self.dropped = 0
         if pos0 < self.dropped or pos0 - self.dropped + toks.size > self.kv_size:
             raise ValueError(f"positions {pos0} .. {pos0 + toks.size - 1} outside the cache of {self.kv_size} cells")
+        self._written_from(pos0 - self.dropped)
         for u0 in range(0, toks.size, ubatch):
             self._prefill_ubatch(toks[u0:u0 + ubatch], pos0 + u0)
         c, d = self.cfg, self.dev
@@ -442,6 +447,7 @@ class LlamaDecoder:
     def _mask(self, pos: int, n_kv: int | None):
         if not 0 <= pos - self.dropped < self.kv_size:
             raise ValueError(f"position {pos} outside the cache of {self.kv_size} cells")
+        self._written_from(pos - self.dropped)
         if n_kv is None:
             n_kv = min(self.kv_size, (pos + 1 + 255) // 256 * 256)
         return msum_decode(pos, n_kv), np.array([[pos, pos + 1]], np.uint32)

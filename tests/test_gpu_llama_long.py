@@ -171,6 +171,29 @@ def test_eviction(dev, typ, sparse):
     m.free()
 
 
+def test_cells_written_anew(dev):
+    """A step back: what the tokens that were there got of attention is forgotten, what the others got is not."""
+    cfg = LL.tiny_config("tiny-evict")
+    m = LL.LlamaDecoder(dev, cfg, LL.SyntheticWeights(cfg), 300, kv_type=H.KV_Q4_0, track=1.0)
+    nh = cfg.n_head
+    L = m.layers[0]
+    m.prefill(np.arange(100, dtype=np.int32), 0)
+    for i in range(4):
+        m.step_graph(7 + i, 100 + i)
+    before = L["weights"].read(np.float32, (300,))
+    assert (before[:104] > 0).all() and (before[104:] == 0).all()
+    before[102:] = 0
+    m.step_graph(3, 102)
+    got = L["weights"].read(np.float32, (300,))
+    assert m.n_cells == 103 and (got[103:] == 0).all() and (got[:103] >= before[:103]).all()
+    assert abs(float((got - before).astype(np.float64).sum()) - nh) <= 103 * nh * 2.0 ** -20
+    m.prefill(np.arange(5, dtype=np.int32), 50)
+    got = L["weights"].read(np.float32, (300,))
+    assert m.n_cells == 55 and (got[:50] >= before[:50]).all() and (got[55:] == 0).all()
+    m.check()
+    m.free()
+
+
 def test_refusals(dev):
     cfg = LL.tiny_config("tiny-evict")
     w = LL.SyntheticWeights(cfg, cache=True)
