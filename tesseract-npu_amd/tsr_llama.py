@@ -21,8 +21,8 @@ A = tsr_hip_flash_attn_kv4, behind tsr_hip_rope_kv (fused) or ROPE and two SET_R
 half the bytes, in more launches (Llama-3-8B, tokens/s over q8_0 and q4_0: 634 and 513 at 4096 cells, 482 and 488 at 16384).
 
 Contexts beyond the trained one: rope_scale in the config turns positions by tsr_hip_rope_scaled, over caches of either kind. Over
-4-bit caches `sparse` lets decode tokens attend to the blocks of cells that can matter most (tsr_hip_kv4_bounds of the cells as they
-are written, tsr_hip_kv4_select, tsr_hip_flash_attn_kv4_blocks), and `track` sums up what attention weight each cell gets
+4-bit caches `sparse` lets decode tokens attend to the blocks of cells that can matter most (tsr_hip_kv4_bounds of a block when it is
+full, tsr_hip_kv4_select, tsr_hip_flash_attn_kv4_blocks), and `track` sums up what attention weight each cell gets
 (tsr_hip_attn_weights_kv4), by which evict() thins the caches out (tsr_hip_kv_pick, tsr_hip_kv_gather): positions go on, cells
 start again behind the kept ones.
 
@@ -243,7 +243,7 @@ class LlamaDecoder:
         self.bad = H.BufferPart(self._out, c.n_vocab * f4, 4).fill(0)
         self.next = dev.alloc(4)           # int32 greedy token (ARGMAX) of an eager step
         # int32 position (ROPE) at 0, int64 cell (SET_ROWS_KV) at 8, int32 token id (GET_ROWS ids) at 16; in front of them
-        # the runs of visible cells (attention over 4-bit caches), and {cell, cell + 1} (bounds of new cells)
+        # the runs of visible cells (attention over 4-bit caches), and {first cell, end} (bounds of new cells)
         self._in = dev.alloc(56)
         self.params = H.BufferPart(self._in, 32, 24)
         self.tok = H.BufferPart(self.params, 16, 4)
@@ -468,7 +468,22 @@ class LlamaDecoder:
             return self.params, p
         cell = pos - self.dropped
         p[2] = cell
-        return self._in, np.concatenate([np.array([0, cell + 1, 0, 0, cell, cell + 1, 0, 0], np.int32), p])
+        first, end = (cell - self.sparse.block, cell) if self._block_done(cell) else (cell, cell + 1)
+        return self._in, np.concatenate([np.array([0, cell + 1, 0, 0, first, end, 0, 0], np.int32), p])
+
+    def _block_done(self, cell: int) -> bool:
+        """Whether the token of this cell is the first behind a block whose bounds no token has needed so far: the newest blocks are
+        attended to without a look at them."""
+        return self.sparse is not None and self.sparse.last > 0 and cell > 0 and cell % self.sparse.block == 0
+
+    def _queue_inputs(self, pos: int, token: int | None, write) -> None:
+        """A token's input bytes to the device by write(buffer, bytes), and the bounds of the block that the token before it filled."""
+        write(*self._inputs(pos, token))
+        cell = pos - self.dropped
+        if self._block_done(cell):
+            for L in self.layers:
+                self.dev.kv4_bounds(L["kc"], self.cfg.head_dim, self.sparse.block, cell, L["bounds"], cells=self.new_ptr,
+                                    n_new=self.sparse.block)
 
     def _ops(self, out_tok, msum=None, runs=None, stream=None, n_kv=None) -> None:
         """The launches of one decode token. msum given: FLASH_ATTN_EXT planned on the host per call
@@ -537,7 +552,7 @@ class LlamaDecoder:
         c, d = self.cfg, self.dev
         heads = (c.head_dim, c.n_head, c.n_head_kv)
         s = self.sparse
-        if s is not None:
+        if s is not None and s.last == 0:  # (else once a block: _queue_inputs)
             d.kv4_bounds(L["kc"], c.head_dim, s.block, n_kv, L["bounds"], cells=self.new_ptr, n_new=1, stream=stream)
         if s is not None and n_kv > s.n_blocks * s.block:
             d.kv4_select(self.qkv, 1, w3, L["bounds"], self.n_bounds, *heads, s.block, n_kv, s.n_blocks, s.first, s.last, self.blocks,
@@ -583,8 +598,7 @@ class LlamaDecoder:
         rounded up to 256, at most kv_size)."""
         msum, runs = self._mask(pos, n_kv)
         self.tok.write(np.array([token], np.int32) if token is not None else self.next.read(np.int32, (1,)))
-        buf, ins = self._inputs(pos)
-        buf.write(ins)
+        self._queue_inputs(pos, None, lambda buf, ins: buf.write(ins))
         if self.kv4:
             self._graph_cells(pos)
         self._ops(self.next, msum, runs, n_kv=pos - self.dropped + 1)
@@ -629,7 +643,7 @@ class LlamaDecoder:
         call and again whenever the plan's shape changes. Nothing waits for the device."""
         d = self.dev
         msum, runs = self._mask(pos, n_kv)
-        d.write_async(*self._inputs(pos, token))
+        self._queue_inputs(pos, token, d.write_async)
         changed = self._graph_cells(pos) if self.kv4 else self.plan.set(msum, runs)
         if self.graph is None or changed:
             if self.graph is not None:
@@ -650,7 +664,7 @@ class LlamaDecoder:
         Nothing waits for the device."""
         d = self.dev
         msum, runs = self._mask(pos, n_kv)
-        d.write_async(*self._inputs(pos, token))
+        self._queue_inputs(pos, token, d.write_async)
         if self.kv4:
             self._graph_cells(pos)
         else:

@@ -73,13 +73,15 @@ def test_scaled_positions_over_4_bit_caches(dev, monkeypatch, scale, mode):
 SPARSE = LL.SparseAttention(block=32, n_blocks=8, first=1, last=2)
 
 
-@pytest.mark.parametrize("typ,kw", [(H.KV_Q4_0, {}), (H.KV_Q4_1, dict(n_head=8, n_head_kv=1, head_dim=128, n_embd=512, n_ff=768))],
-                         ids=["q4_0", "q4_1-gqa8"])
-def test_sparse_decode(dev, monkeypatch, typ, kw):
+@pytest.mark.parametrize("typ,kw,sparse", [
+    (H.KV_Q4_0, {}, SPARSE), (H.KV_Q4_1, dict(n_head=8, n_head_kv=1, head_dim=128, n_embd=512, n_ff=768), SPARSE),
+    (H.KV_Q4_0, {}, LL.SparseAttention(block=32, n_blocks=8, first=1, last=0)),
+    (H.KV_Q4_1, {}, LL.SparseAttention(block=64, n_blocks=4, first=0, last=1))], ids=["q4_0", "q4_1-gqa8", "no-last", "one-last"])
+def test_sparse_decode(dev, monkeypatch, typ, kw, sparse):
     """Every layer's list and attention of eager tokens, and graph replays with the same bits across the growth of their cells."""
     cfg = LL.tiny_config("tiny-sparse", rope_scale=YARN, **kw)
     w = LL.SyntheticWeights(cfg, cache=True)
-    m, g = (LL.LlamaDecoder(dev, cfg, w, 1200, kv_type=typ, sparse=SPARSE) for _ in range(2))
+    m, g = (LL.LlamaDecoder(dev, cfg, w, 1200, kv_type=typ, sparse=sparse) for _ in range(2))
     prompt = np.random.default_rng(2).integers(0, cfg.n_vocab, 510).astype(np.int32)
     for x in (m, g):
         x.prefill(prompt, 0, 200)
@@ -91,13 +93,14 @@ def test_sparse_decode(dev, monkeypatch, typ, kw):
         L = next(x for x in m.layers if x["kc"] is kc)
         ki, vi = images(m, L)
         lo, hi = P.words(L["bounds"].read(np.uint32, (nkv, nb, D)))
-        used = -(-n_kv // block)
-        want = P.bounds(R.values_f32(ki[:n_kv], typ), D, block)
+        want = tuple(P.bounds(R.values_f32(ki[:n_kv], typ), D, block))
+        used = (n_kv - 1) // block if sparse.last else -(-n_kv // block)   # (the token's own block is listed without its bounds)
         for a, b in zip((lo, hi), want):
-            assert (a[:, :used] == b).all()
+            assert (a[:, :used] == b[:, :used]).all()
+        lo, hi = want
         qs = q.read(np.float32, (1, q_stride))[:, :nh * D]
         ids = blocks.read(np.int32, (1, nkv, n_sel))
-        assert (ids == P.select(qs.reshape(1, nh, D), lo, hi, nh, block, n_kv, n_sel, 1, 2)).all()
+        assert (ids == P.select(qs.reshape(1, nh, D), lo, hi, nh, block, n_kv, n_sel, sparse.first, sparse.last)).all()
         o, tol = P.attention(qs, ki, vi, typ, D, nh, nkv, np.float64(np.float32(scale)), ids, block, n_kv)
         R.check(out.read(np.float32, (1, nh, D)), o, tol, f"{n_kv} cells")
         calls[0] += 1
