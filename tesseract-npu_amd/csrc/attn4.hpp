@@ -228,8 +228,8 @@ struct Attn4 {
         }
     }
     // The queries; their pieces go to `lds`, [row group][block][piece][lane], the blocks shared out over the waves.
-    // TOP: 2^e of a row's largest |q| is in [2^(TOP - 127), 2 of it).
-    template <int TOP = 140>
+    // TOP: 2^e of a row's largest |q| is in [2^(TOP - 127), 2 of it). OWN: the wave's own rows, all blocks by itself.
+    template <int TOP = 140, bool OWN = false>
     __device__ __forceinline__ void load_queries(float scale, uint32_t lane, h8 * lds, uint32_t wave) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -261,7 +261,7 @@ struct Attn4 {
                     const float z = rows_sum(sum);
                     if (mine) qs[n][b / C] = z;
                 }
-                if (b % kWaves == wave) {
+                if (OWN || b % kWaves == wave) {
                     const float z[8] = { y[0], y[2], y[4], y[6], y[1], y[3], y[5], y[7] };
                     uint32_t hi[4], lo[4];
 #pragma unroll

@@ -7,6 +7,7 @@
 //   k_attn4_weights  the weights of a workgroup's rows, summed over them: a lane sums its row of each group of 16, the 16 lanes
 //                    then meet; 32 sums a tile and row set go to memory
 //   k_attn4_cells    the row sets' sums added up, in their order: no atomic decides a rounding
+// or, for one group of rows of few heads, both at once: k_attn4_weights_one.
 // A workgroup's waves have the same rows (up to four groups of 16: nothing but scores to hold) and take tiles in turn.
 //
 // Bound: a decode token's three launches (32 heads of 128 over 8 KV heads behind 8192 cells: 13.1 us, 5.9 + 7.2 + 2.5 by themselves, the
@@ -66,8 +67,9 @@ struct Weights4 : Attn4<D, NT, 1, TYPE> {
         }
         A::template scores<!MIN>(k.t, q, s);
     }
+    template <bool OWN>
     __device__ __forceinline__ void load_queries(float scale, uint32_t lane, h8 * lds, uint32_t wave) {
-        A::template load_queries<MIN ? 135 : 140>(scale, lane, lds, wave);   // (135: the sum of a block fits f16)
+        A::template load_queries<MIN ? 135 : 140, OWN>(scale, lane, lds, wave);   // (135: the sum of a block fits f16)
         if constexpr (MIN)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -94,9 +96,61 @@ struct Weights4 : Attn4<D, NT, 1, TYPE> {
         return v;
     }
 
+    // Each row's maximum and the inverse of its sum over the splits, the four lanes of a row taking them in turn.
+    float top[NT], il[NT];
+    __device__ __forceinline__ void load_sums(const Attn4Args & a, const Weights4Plan & p, uint32_t h, uint32_t rg, uint32_t lane) {
+        const uint32_t g = lane >> 4;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float2 * pairs = (const float2 *)a.part + weights4_pair(p, a.n_head_kv, 0u, h, rg, 16u * n + (lane & 15u));
+            const size_t step = weights4_pair(p, a.n_head_kv, 1u, 0u, 0u, 0u);
+            float2 x[kWeightsSplits / 4];                          // (all on their way at once)
+#pragma unroll
+            for (uint32_t j = 0; j < kWeightsSplits / 4; ++j)
+                x[j] = g + 4u * j < a.S ? pairs[(g + 4u * j) * step] : make_float2(-__builtin_inff(), 0.0f);
+            float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+            for (uint32_t j = 0; j < kWeightsSplits / 4; ++j) m = fmaxf(m, x[j].x);
+#pragma unroll
+            for (uint32_t j = 0; j < kWeightsSplits / 4; ++j) l += x[j].y * (x[j].x == m ? 1.0f : __builtin_amdgcn_exp2f(x[j].x - m));
+            top[n] = rows_max(m);
+            l = rows_sum(l * (m == top[n] ? 1.0f : __builtin_amdgcn_exp2f(m - top[n])));
+            const bool empty = l == 0.0f || rg * 16u * NT + 16u * n + (lane & 15u) >= a.T * a.G;
+            il[n] = empty ? 0.0f : 1.0f / l;
+            top[n] = empty ? __builtin_inff() : top[n];            // (weights of 0, whatever the scores are)
+        }
+    }
+    // The rows' weights of tile i, summed: of its cell place(lane), in the lanes without bit 3.
+    static __device__ __forceinline__ uint32_t place(uint32_t lane) { return 16u * ((lane >> 2) & 1u) + 4u * (lane >> 4) + (lane & 3u); }
+    __device__ __forceinline__ float sums(const Codes & k, uint32_t i, bool whole, const h8 * lds, uint32_t lane) const {
+        f4 s[NT][2];
+        uint32_t ql = lane;
+        asm volatile("" : "+v"(ql));
+        scores(k, lds + ql, s);
+        float x[8] = {};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t in = whole ? 0xFFu : seen(n, i, lane >> 4);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][c >> 2][c & 3], this->csc[n], -top[n]));
+                const float z = __builtin_fmaf(e, il[n], x[c]);
+                x[c] = whole || ((in >> c) & 1u) ? z : x[c];
+            }
+        }
+        // over the 16 lanes of a row of the wave: halves handed over between lanes 7 - x and x, 2 and 1 apart; then all eight
+        const bool b2 = (lane & 4u) != 0u, b1 = (lane & 2u) != 0u, b0 = (lane & 1u) != 0u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = (b2 ? x[c + 4] : x[c]) + dpp_f<kDppRowHalfMirror>(b2 ? x[c] : x[c + 4]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) x[c] = (b1 ? x[c + 2] : x[c]) + dpp_f<kDppXor2>(b1 ? x[c] : x[c + 2]);
+        x[0] = (b0 ? x[1] : x[0]) + dpp_f<kDppXor1>(b0 ? x[0] : x[1]);
+        return x[0] + dpp_f<kDppRowMirror>(dpp_f<kDppRowHalfMirror>(x[0]));   // (lane l and l ^ 8)
+    }
+
     // one(tile's codes, its number, whether every row sees all of it) for the wave's tiles, every parts-th; none(number) for
-    // those that no row sees. `lds`: the queries' pieces go there first.
-    template <class One, class None>
+    // those that no row sees. `lds`: the queries' pieces go there first (OWN: the wave's own room and rows).
+    template <bool OWN = false, class One, class None>
     __device__ __forceinline__ void walk(const Attn4Args & a, uint32_t h, uint32_t part, uint32_t parts, h8 * lds, uint32_t wave, uint32_t lane,
                                          One one, None none) {
         constexpr size_t tb = kv4_tile_bytes(TYPE);
@@ -115,7 +169,7 @@ struct Weights4 : Attn4<D, NT, 1, TYPE> {
             load(k0, kp + nth(0u) * tb, pair, lane);
             load(k1, kp + nth(1u) * tb, pair, lane);
         }
-        load_queries(a.scale, lane, lds, wave);
+        load_queries<OWN>(a.scale, lane, lds, wave);
         __syncthreads();
         for (uint32_t x = 0; x < cnt; x += 2u) {                   // two tiles ahead
             one(k0, nth(x), true);
@@ -203,61 +257,50 @@ __global__ __launch_bounds__(256, weights_waves(D, NT)) void k_attn4_weights(Att
     using W = Weights4<D, NT, TYPE>;
     __shared__ __align__(16) uint8_t room[W::kQ];
     const uint32_t h = blockIdx.x, split = blockIdx.y, rg = blockIdx.z, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u;
     W w;
     w.load_runs(a, h, rg * 16u * NT, lane);
-    // each row's maximum and the inverse of its sum over the splits, the four lanes of a row taking them in turn
-    float M[NT], il[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const float2 * pairs = (const float2 *)a.part + weights4_pair(p, a.n_head_kv, 0u, h, rg, 16u * n + (lane & 15u));
-        const size_t step = weights4_pair(p, a.n_head_kv, 1u, 0u, 0u, 0u);
-        float2 x[kWeightsSplits / 4];                              // (all on their way at once)
-#pragma unroll
-        for (uint32_t j = 0; j < kWeightsSplits / 4; ++j)
-            x[j] = g + 4u * j < a.S ? pairs[(g + 4u * j) * step] : make_float2(-__builtin_inff(), 0.0f);
-        float m = -__builtin_inff(), l = 0.0f;
-#pragma unroll
-        for (uint32_t j = 0; j < kWeightsSplits / 4; ++j) m = fmaxf(m, x[j].x);
-#pragma unroll
-        for (uint32_t j = 0; j < kWeightsSplits / 4; ++j) l += x[j].y * (x[j].x == m ? 1.0f : __builtin_amdgcn_exp2f(x[j].x - m));
-        M[n] = rows_max(m);
-        l = rows_sum(l * (m == M[n] ? 1.0f : __builtin_amdgcn_exp2f(m - M[n])));
-        const bool empty = l == 0.0f || rg * 16u * NT + 16u * n + (lane & 15u) >= a.T * a.G;
-        il[n] = empty ? 0.0f : 1.0f / l;
-        M[n] = empty ? __builtin_inff() : M[n];                    // (weights of 0, whatever the scores are)
-    }
+    w.load_sums(a, p, h, rg, lane);
     float * sums = (float *)((uint8_t *)a.part + p.sums) + ((size_t)h * p.n_rg + rg) * p.n_pad;
     w.walk(a, h, split * kWaves + wave, a.S * kWaves, (h8 *)room, wave, lane,
            [&](const typename W::Codes & k, uint32_t i, bool whole) {
-               f4 s[NT][2];
-               uint32_t ql = lane;
-               asm volatile("" : "+v"(ql));
-               w.scores(k, (h8 *)room + ql, s);
-               float x[8] = {};
-#pragma unroll
-               for (int n = 0; n < NT; ++n) {
-                   const uint32_t in = whole ? 0xFFu : w.seen(n, i, g);
-#pragma unroll
-                   for (int c = 0; c < 8; ++c) {
-                       const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][c >> 2][c & 3], w.csc[n], -M[n]));
-                       const float z = __builtin_fmaf(e, il[n], x[c]);
-                       x[c] = whole || ((in >> c) & 1u) ? z : x[c];
-                   }
-               }
-               // over the 16 lanes of a row of the wave: halves handed over between lanes 7 - x and x, 2 and 1 apart; then all eight
-               const bool b2 = (lane & 4u) != 0u, b1 = (lane & 2u) != 0u, b0 = (lane & 1u) != 0u;
-#pragma unroll
-               for (int c = 0; c < 4; ++c) x[c] = (b2 ? x[c + 4] : x[c]) + dpp_f<kDppRowHalfMirror>(b2 ? x[c] : x[c + 4]);
-#pragma unroll
-               for (int c = 0; c < 2; ++c) x[c] = (b1 ? x[c + 2] : x[c]) + dpp_f<kDppXor2>(b1 ? x[c] : x[c + 2]);
-               x[0] = (b0 ? x[1] : x[0]) + dpp_f<kDppXor1>(b0 ? x[0] : x[1]);
-               x[0] += dpp_f<kDppRowMirror>(dpp_f<kDppRowHalfMirror>(x[0]));   // (lane l and l ^ 8)
-               if ((lane & 8u) == 0u) sums[32u * i + 16u * ((lane >> 2) & 1u) + 4u * g + (lane & 3u)] = x[0];
+               const float x = w.sums(k, i, whole, (h8 *)room, lane);
+               if ((lane & 8u) == 0u) sums[32u * i + W::place(lane)] = x;
            },
            [&](uint32_t i) {
                if (lane < 32u) sums[32u * i + lane] = 0.0f;
            });
+}
+
+// The last two passes in one for rows that are one group of 16 (a decode token's) of few KV heads and cells (weights4_plan.hpp): a wave a KV
+// head, the waves' sums of a tile meet in LDS and are results.
+template <int D, uint32_t TYPE>
+__global__ __launch_bounds__(65536 / D) void k_attn4_weights_one(Attn4Args a, Weights4Plan p, const float * before, float decay) {
+    using W = Weights4<D, 1, TYPE>;
+    __shared__ __align__(16) uint8_t room[1024 / D][W::kQ];
+    __shared__ float part[2][1024 / D][32];
+    const uint32_t h = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u;
+    W w;
+    w.load_runs(a, h, 0u, lane);
+    w.load_sums(a, p, h, 0u, lane);
+    uint32_t buf = 0u;
+    auto out = [&](uint32_t i, bool any) {
+        const uint32_t c = 32u * i + lane;
+        if (h != 0u || lane >= 32u || c >= a.n_kv) return;
+        float x = 0.0f;
+        if (any)
+            for (uint32_t v = 0; v < a.n_head_kv; ++v) x += part[buf][v][lane];
+        a.out[c] = before == nullptr ? x : __builtin_fmaf(decay, before[c], x);
+    };
+    w.template walk<true>(a, h, blockIdx.x, gridDim.x, (h8 *)room[h], 0u, lane,
+           [&](const typename W::Codes & k, uint32_t i, bool whole) {
+               const float x = w.sums(k, i, whole, (h8 *)room[h], lane);
+               if ((lane & 8u) == 0u) part[buf][h][W::place(lane)] = x;
+               lds_barrier();                                      // (the waves see the same cells: they come here as often)
+               out(i, true);
+               buf ^= 1u;
+           },
+           [&](uint32_t i) { out(i, false); });
 }
 
 // Cells' sums over n row sets: 64 cells a workgroup, its four waves every fourth row set, joined in their order.
@@ -283,24 +326,32 @@ __global__ __launch_bounds__(256) void k_attn4_cells(const float * sums, uint32_
 }
 
 template <int D, int NT, uint32_t TYPE>
-static int launch_weights(const Attn4Args & a, const Weights4Plan & p, hipStream_t s) {
+static int launch_weights(const Attn4Args & a, const Weights4Plan & p, const float * before, float decay, hipStream_t s) {
     const dim3 grid(a.n_head_kv, a.S, (a.T * a.G + 16u * NT - 1u) / (16u * NT)), wg(64u * kWaves);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4_rowsums<D, NT, TYPE>), grid, wg, 0, s, a, p);
+    if constexpr (NT == 1 && D <= 256)
+        if (p.one != 0u) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4_weights_one<D, TYPE>), dim3(p.one), dim3(64u * a.n_head_kv), 0, s, a, p, before, decay);
+            return hipGetLastError() == hipSuccess ? 0 : -4;
+        }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4_weights<D, NT, TYPE>), grid, wg, 0, s, a, p);
+    const uint32_t n = a.n_head_kv * p.n_rg;
+    hipLaunchKernelGGL(k_attn4_cells, dim3((a.n_kv + 63u) / 64u), dim3(256), 0, s, (const float *)((uint8_t *)a.part + p.sums), n, p.n_pad, a.n_kv, before,
+                       decay, a.out);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
 template <uint32_t TYPE>
-static int launch_weights_t(const Attn4Args & a, const Weights4Plan & p, hipStream_t s) {
+static int launch_weights_t(const Attn4Args & a, const Weights4Plan & p, const float * before, float decay, hipStream_t s) {
     switch (a.D * 8u + p.NT) {
-        case 64 * 8 + 1: return launch_weights<64, 1, TYPE>(a, p, s);
-        case 64 * 8 + 2: return launch_weights<64, 2, TYPE>(a, p, s);
-        case 64 * 8 + 4: return launch_weights<64, 4, TYPE>(a, p, s);
-        case 128 * 8 + 1: return launch_weights<128, 1, TYPE>(a, p, s);
-        case 128 * 8 + 2: return launch_weights<128, 2, TYPE>(a, p, s);
-        case 128 * 8 + 4: return launch_weights<128, 4, TYPE>(a, p, s);
-        case 256 * 8 + 1: return launch_weights<256, 1, TYPE>(a, p, s);
-        case 512 * 8 + 1: return launch_weights<512, 1, TYPE>(a, p, s);
+        case 64 * 8 + 1: return launch_weights<64, 1, TYPE>(a, p, before, decay, s);
+        case 64 * 8 + 2: return launch_weights<64, 2, TYPE>(a, p, before, decay, s);
+        case 64 * 8 + 4: return launch_weights<64, 4, TYPE>(a, p, before, decay, s);
+        case 128 * 8 + 1: return launch_weights<128, 1, TYPE>(a, p, before, decay, s);
+        case 128 * 8 + 2: return launch_weights<128, 2, TYPE>(a, p, before, decay, s);
+        case 128 * 8 + 4: return launch_weights<128, 4, TYPE>(a, p, before, decay, s);
+        case 256 * 8 + 1: return launch_weights<256, 1, TYPE>(a, p, before, decay, s);
+        case 512 * 8 + 1: return launch_weights<512, 1, TYPE>(a, p, before, decay, s);
         default: return -2;
     }
 }
@@ -308,12 +359,6 @@ static int launch_weights_t(const Attn4Args & a, const Weights4Plan & p, hipStre
 }  // namespace tsr
 
 int tsr_launch_attn4_weights(const tsr::Attn4Args & a, const tsr::Weights4Plan & p, const float * before, float decay, hipStream_t s) {
-    if (a.n_kv != 0u) {
-        const int rc = a.type == tsr::kKvQ4_0 ? tsr::launch_weights_t<tsr::kKvQ4_0>(a, p, s) : tsr::launch_weights_t<tsr::kKvQ4_1>(a, p, s);
-        if (rc) return rc;
-        const uint32_t n = a.n_head_kv * p.n_rg;
-        hipLaunchKernelGGL(tsr::k_attn4_cells, dim3((a.n_kv + 63u) / 64u), dim3(256), 0, s, (const float *)((uint8_t *)a.part + p.sums), n, p.n_pad,
-                           a.n_kv, before, decay, a.out);
-    }
-    return hipGetLastError() == hipSuccess ? 0 : -4;
+    if (a.n_kv == 0u) return 0;
+    return a.type == tsr::kKvQ4_0 ? tsr::launch_weights_t<tsr::kKvQ4_0>(a, p, before, decay, s) : tsr::launch_weights_t<tsr::kKvQ4_1>(a, p, before, decay, s);
 }

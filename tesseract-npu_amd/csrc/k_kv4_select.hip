@@ -11,7 +11,9 @@
 // whose 16 columns several tokens fill that look at the same blocks. What leaves is a key a block, an unsigned number in
 // the order of the scores. k_kv4_pick_blocks then finds the cut (pick.hpp). Both are a few microseconds of waiting for memory
 // and for each other's steps, not work: reductions and scans run on DPP, keys are asked for before the runs that say which
-// of them count.
+// of them count. A token of 32 heads of 128 over 8 KV heads, 2048 blocks: scores 4.9 us, cut 6.8 (an empty kernel 1.7); 33 sequences' tokens
+// of 8 heads of 256 over 4, 94 blocks: 9.8 and 6.5. 512 tokens of 32 heads of 128 behind 120 blocks take 26.8 for the scores, bound by
+// the matrix instruction (13.7 at what an 8192^3 product reaches, 66 TFLOP/s); with 4x4x4 they took 53.
 #include "kernels.hpp"
 #include "pick.hpp"
 

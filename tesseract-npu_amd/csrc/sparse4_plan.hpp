@@ -28,6 +28,9 @@ inline Attn4BlocksPlan attn4_blocks_plan(uint32_t T, uint32_t D, uint32_t n_head
     const uint64_t G = n_head / n_head_kv, tiles = (uint64_t)n_sel * (block / 32u);
     p.C = G <= 4u && D >= 128u ? 4u : G <= 8u ? 2u : 1u;           // a workgroup's rows are one token's: as few columns as hold them
     const uint64_t rows = 16u / p.C, n = (uint64_t)T * n_head_kv * ((G + rows - 1u) / rows), fill = n_cu / n;
+    // Splits fill the card, but a list of up to 20 tiles is not worth a join. Scores, cut and attention in us: 8 tokens of 8 heads of 256 over 4
+    // over 32 tiles, S 1, 2, 4: 33.3, 30.8, 28.4; 32 such tokens S 1, 2: 38.9, 43.5; a token of 32 heads of 128 over 8 over 64
+    // tiles S 1, 8, 16: 34.0, 26.6, 26.9; one of a head of 512 S 1, 8: 87, 42.8.
     const uint64_t S = tiles <= 20u ? 1u : fill;
     p.S = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ S, (tiles + 3u) / 4u, 256u }));
     p.ws_bytes = p.S > 1u ? 4u * (size_t)p.S * T * n_head * (2u + D) : 0u;

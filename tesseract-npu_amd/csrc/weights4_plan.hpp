@@ -15,6 +15,7 @@ struct Weights4Plan {
     uint32_t n_rg;           // workgroups' row sets of a KV head
     uint32_t S;              // splits of the cells
     uint32_t n_pad;          // cells in whole tiles
+    uint32_t one;            // workgroups of the form with a wave a KV head (0: not that form)
     size_t sums;             // byte offset of the sums behind the (maximum, sum) pairs
     size_t ws_bytes;
 };
@@ -33,6 +34,10 @@ inline Weights4Plan weights4_plan(uint32_t T, uint32_t D, uint32_t n_head, uint3
     // 105, 98; 16 tokens behind 8192 22.2, 24.8, 36.0. Heads of 256 keep to one (64 tokens of 8 heads over 4, 32768 cells: 72.6, 91.1).
     const uint64_t R = T * G, groups = (R + 15u) / 16u, products = groups * n_head_kv * tiles * (D / 32u) / (4u * n_cu);
     p.NT = D > 128u || groups == 1u || products < 64u ? 1u : groups == 2u || products < 256u ? 2u : 4u;
+    // One group of rows of few heads: the heads' weights meet in a workgroup, a launch less, but a KV head's codes no longer come from the
+    // L2 that its first pass filled. 14 heads of 64 over 2, 512 and 32768 cells: 10.1 -> 7.7 and 13.1 -> 11.1 us; 8 of 256 over 4, 4096 cells:
+    // 17.6 -> 16.3; 32 of 128 over 8, 2048, 8192 and 32768 cells: 10.3 -> 9.9, 13.1 -> 12.1 to 14.4, 19.0 -> 19.9.
+    p.one = groups == 1u && n_head_kv * D <= 1024u && (uint64_t)n_head_kv * D * n_kv <= (1u << 22) ? (uint32_t)std::min<uint64_t>(tiles, 2u * n_cu) : 0u;
     p.n_pad = (uint32_t)(32u * tiles);
     // a launch's sums take at most 64 MiB, or are one token's
     const uint64_t rows = 16u * p.NT, most = std::max<uint64_t>(1u, ((uint64_t)64 << 20) / (4u * (uint64_t)p.n_pad * n_head_kv));   // row sets of a KV head

@@ -101,7 +101,7 @@ static int plans() {
                         const size_t last = tsr::weights4_pair(p, hkv, p.S - 1u, hkv - 1u, p.n_rg - 1u, 16u * p.NT - 1u);
                         if (!(p.NT == 1u || (p.NT == 2u && D <= 256u) || (p.NT == 4u && D <= 128u)) || p.S == 0u || p.S > tsr::kWeightsSplits || p.S > tiles ||
                             p.tokens == 0u || p.tokens > T || (uint64_t)p.n_rg * 16u * p.NT < (uint64_t)p.tokens * G || p.n_rg > 65535u ||
-                            p.n_pad != 32u * tiles || 8u * (last + 1u) != p.sums || p.ws_bytes != p.sums + 4u * n * p.n_pad || p.sums % 16u != 0u) {
+                            p.one > tiles || (p.one != 0u && (hkv * D > 1024u || p.n_rg != 1u || p.NT != 1u || p.tokens != T)) || p.n_pad != 32u * tiles || 8u * (last + 1u) != p.sums || p.ws_bytes != p.sums + 4u * n * p.n_pad || p.sums % 16u != 0u) {
                             printf("plan: T %u D %u heads %u G %u cells %u\n", T, D, hkv, G, kv);
                             return 1;
                         }
