@@ -13,7 +13,7 @@
 // and for each other's steps, not work: reductions and scans run on DPP, keys are asked for before the runs that say which
 // of them count. A token of 32 heads of 128 over 8 KV heads, 2048 blocks: scores 4.9 us, cut 6.8 (an empty kernel 1.7); 33 sequences' tokens
 // of 8 heads of 256 over 4, 94 blocks: 9.8 and 6.5. 512 tokens of 32 heads of 128 behind 120 blocks take 26.8 for the scores, bound by
-// the matrix instruction (13.7 at what an 8192^3 product reaches, 66 TFLOP/s); with 4x4x4 they took 53.
+// the matrix instruction (13.7 at what an 8192^3 product reaches, 66 TFLOP/s); with 4x4x4 they took 51 to 54.
 #include "kernels.hpp"
 #include "pick.hpp"
 
