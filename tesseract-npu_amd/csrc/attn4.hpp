@@ -851,7 +851,8 @@ struct Attn4 {
                 if (z == 0u && g == 0u && c == 0u) ml[wave * RT + RW * n + rl] = make_float2(m[n], l[n]);
 #pragma unroll
                 for (uint32_t j = 0; j < DC / 16; ++j) {
-                    const f4 x = o[n][z * (DC / 16) + j];
+                    f4 x = o[n][z * (DC / 16) + j];
+                    if constexpr (C > 1) asm("" : "+v"(x));        // (read here: merged behind the conditions the reads took scratch memory)
                     if (C == 1 || ((z * (DC / 16) + j) / 2u) % C == c)
                         *(float4 *)(lo + (wave * RT + RW * n + rl) * DC + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
                 }
