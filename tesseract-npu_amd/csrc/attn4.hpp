@@ -835,50 +835,6 @@ struct Attn4 {
                 }
         }
     }
-
-    // The waves' sums joined, behind finish(): rows r0 .. of at most R, row r's result to place(r); `split`: unnormalised, its
-    // maximum and sum to sums(r, m, l). room: kRoom bytes of LDS, ml: a pair for each of the waves' rows.
-    template <class Place, class Sums>
-    __device__ __forceinline__ void join(uint8_t * room, float2 * ml, uint32_t r0, uint32_t R, bool split, uint32_t wave, uint32_t lane,
-                                         Place place, Sums sums) const {
-        const uint32_t g = lane >> 4, c = lane & (C - 1u), rl = (lane & 15u) / C;
-        float * lo = (float *)room;
-#pragma unroll
-        for (uint32_t z = 0; z < D / DC; ++z) {
-            __syncthreads();                                       // (the queries, the values before have been read)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (z == 0u && g == 0u && c == 0u) ml[wave * RT + RW * n + rl] = make_float2(m[n], l[n]);
-#pragma unroll
-                for (uint32_t j = 0; j < DC / 16; ++j) {
-                    f4 x = o[n][z * (DC / 16) + j];
-                    if constexpr (C > 1) asm("" : "+v"(x));        // (read here: merged behind the conditions the reads took scratch memory)
-                    if (C == 1 || ((z * (DC / 16) + j) / 2u) % C == c)
-                        *(float4 *)(lo + (wave * RT + RW * n + rl) * DC + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
-                }
-            }
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < RT * (DC / 4); i += 64u * kWaves) {
-                const uint32_t r = i / (DC / 4), d = 4u * (i % (DC / 4));
-                if (r0 + r >= R) continue;
-                float2 u[kWaves];
-                float M = -__builtin_inff(), L = 0.0f;
-#pragma unroll
-                for (uint32_t x = 0; x < kWaves; ++x) { u[x] = ml[x * RT + r]; M = fmaxf(M, u[x].x); }
-                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (uint32_t x = 0; x < kWaves; ++x) {
-                    const float f = u[x].x == M ? 1.0f : __builtin_amdgcn_exp2f(u[x].x - M);
-                    const float4 v = *(const float4 *)(lo + (x * RT + r) * DC + d);
-                    L += u[x].y * f;
-                    y.x += v.x * f; y.y += v.y * f; y.z += v.z * f; y.w += v.w * f;
-                }
-                const float il = split ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
-                *(float4 *)(place(r0 + r) + z * DC + d) = make_float4(y.x * il, y.y * il, y.z * il, y.w * il);
-                if (split && z == 0u && d == 0u) sums(r0 + r, M, L);
-            }
-        }
-    }
 };
 
 // Waves a SIMD that a kernel has registers for: the most that need no spills, but for heads of 512 over q4_1 with two columns a

@@ -18,14 +18,16 @@ __global__ __launch_bounds__(256, waves_of(D, NT, C, TYPE)) void k_attn4(Attn4Ar
     using A = Attn4<D, NT, C, TYPE>;
     constexpr uint32_t RT = A::RW * NT;                            // rows of the workgroup
     const uint32_t h = blockIdx.x, split = blockIdx.y, rg = gridDim.z - 1u - blockIdx.z;   // causal: the long rows first
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x & 63u, g = lane >> 4;
+    const uint32_t c = lane & (C - 1u), rl = (lane & 15u) / C;
     const uint32_t r0 = rg * RT, R = a.T * a.G, nh = a.G * a.n_head_kv;
     const size_t nr = (size_t)a.T * nh;
+    constexpr uint32_t DC = A::DC;
     __shared__ __align__(16) uint8_t room[A::kRoom];
-    __shared__ float2 ml[kWaves * RT];
+    h8 * lq = (h8 *)room;
     A w;
     w.load_runs(a, h, r0, lane);
-    w.run(a, h, split * kWaves + wave, a.S * kWaves, (h8 *)room, wave, lane);
+    w.run(a, h, split * kWaves + wave, a.S * kWaves, lq, wave, lane);
     w.finish();
     // where row r's result goes: the output, or its place in the split's partial rows
     auto place = [&](uint32_t r) {
@@ -37,7 +39,44 @@ __global__ __launch_bounds__(256, waves_of(D, NT, C, TYPE)) void k_attn4(Attn4Ar
         const uint32_t t = token(a, r);
         *(float2 *)(a.part + attn4_part_sum(nr, D, a.S, split, (size_t)t * nh + h * a.G + r - t * a.G)) = make_float2(m, l);
     };
-    w.join(room, ml, r0, R, a.S > 1u, wave, lane, place, sums);
+    // the waves' sums joined (here and not in a function, whose reads of w.o end up in private memory or otherwise before the loop's
+    // waits: a token of 8 heads of 256 behind 65536 cells 22.6 us, 24.5 so)
+    __shared__ float2 ml[kWaves * RT];
+    float * lo = (float *)room;
+#pragma unroll
+    for (uint32_t z = 0; z < D / DC; ++z) {
+        __syncthreads();                                       // (the queries, the values before have been read)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (z == 0u && g == 0u && c == 0u) ml[wave * RT + A::RW * n + rl] = make_float2(w.m[n], w.l[n]);
+#pragma unroll
+            for (uint32_t j = 0; j < DC / 16; ++j) {
+                const f4 x = w.o[n][z * (DC / 16) + j];
+                if (C == 1 || ((z * (DC / 16) + j) / 2u) % C == c)
+                    *(float4 *)(lo + (wave * RT + A::RW * n + rl) * DC + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
+            }
+        }
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < RT * (DC / 4); e += 64u * kWaves) {
+            const uint32_t r = e / (DC / 4), d = 4u * (e % (DC / 4));
+            if (r0 + r >= R) continue;
+            float2 u[kWaves];
+            float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+            for (uint32_t x = 0; x < kWaves; ++x) { u[x] = ml[x * RT + r]; M = fmaxf(M, u[x].x); }
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t x = 0; x < kWaves; ++x) {
+                const float f = u[x].x == M ? 1.0f : __builtin_amdgcn_exp2f(u[x].x - M);
+                const float4 v = *(const float4 *)(lo + (x * RT + r) * DC + d);
+                L += u[x].y * f;
+                y.x += v.x * f; y.y += v.y * f; y.z += v.z * f; y.w += v.w * f;
+            }
+            const float il = a.S > 1u ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+            *(float4 *)(place(r0 + r) + z * DC + d) = make_float4(y.x * il, y.y * il, y.z * il, y.w * il);
+            if (a.S > 1u && z == 0u && d == 0u) sums(r0 + r, M, L);
+        }
+    }
 }
 
 // The splits of a row joined: a workgroup a row. 256 / (D / 4) groups of threads take splits in turn, then meet in LDS; the

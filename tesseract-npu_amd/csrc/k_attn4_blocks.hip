@@ -40,7 +40,41 @@ __global__ __launch_bounds__(256, waves_of(D, 1, C, TYPE)) void k_attn4_blocks(A
     w.finish();
     auto place = [&](uint32_t r) { return a.S > 1u ? a.part + attn4_part_row(nr, D, split, row0 + r) : out + (size_t)r * D; };
     auto sums = [&](uint32_t r, float m, float l) { *(float2 *)(a.part + attn4_part_sum(nr, D, a.S, split, row0 + r)) = make_float2(m, l); };
-    w.join(room, ml, r0, a.G, a.S > 1u, wave, lane, place, sums);
+    // the waves' sums joined, as k_attn4.hip has it
+    constexpr uint32_t RT = A::RT, DC = A::DC;
+    const uint32_t g = lane >> 4, c = lane & (C - 1u), rl = (lane & 15u) / C;
+    float * lo = (float *)room;
+#pragma unroll
+    for (uint32_t z = 0; z < D / DC; ++z) {
+        __syncthreads();                                       // (the queries, the values before have been read)
+        if (z == 0u && g == 0u && c == 0u) ml[wave * RT + rl] = make_float2(w.m[0], w.l[0]);
+#pragma unroll
+        for (uint32_t j = 0; j < DC / 16; ++j) {
+            const f4 x = w.o[0][z * (DC / 16) + j];
+            if (C == 1 || ((z * (DC / 16) + j) / 2u) % C == c)
+                *(float4 *)(lo + (wave * RT + rl) * DC + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < RT * (DC / 4); e += 64u * kWaves) {
+            const uint32_t r = e / (DC / 4), d = 4u * (e % (DC / 4));
+            if (r0 + r >= a.G) continue;
+            float2 u[kWaves];
+            float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+            for (uint32_t x = 0; x < kWaves; ++x) { u[x] = ml[x * RT + r]; M = fmaxf(M, u[x].x); }
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t x = 0; x < kWaves; ++x) {
+                const float f = u[x].x == M ? 1.0f : __builtin_amdgcn_exp2f(u[x].x - M);
+                const float4 v = *(const float4 *)(lo + (x * RT + r) * DC + d);
+                L += u[x].y * f;
+                y.x += v.x * f; y.y += v.y * f; y.z += v.z * f; y.w += v.w * f;
+            }
+            const float il = a.S > 1u ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+            *(float4 *)(place(r0 + r) + z * DC + d) = make_float4(y.x * il, y.y * il, y.z * il, y.w * il);
+            if (a.S > 1u && z == 0u && d == 0u) sums(r0 + r, M, L);
+        }
+    }
 }
 
 template <int D, int C, uint32_t TYPE>
