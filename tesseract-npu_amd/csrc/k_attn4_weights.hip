@@ -70,6 +70,10 @@ struct Weights4 : Attn4<D, NT, 1, TYPE> {
     template <bool OWN>
     __device__ __forceinline__ void load_queries(float scale, uint32_t lane, h8 * lds, uint32_t wave) {
         A::template load_queries<MIN ? 135 : 140, OWN>(scale, lane, lds, wave);   // (135: the sum of a block fits f16)
+        // The unit of a row of zeros under a small scale leaves f32's range, and infinities, which the maxima start from and cells that are
+        // not seen get, would meet a 0. Sums of codes stay below 2^45, whose exp2 in a unit of 2^-126 or less is 1.
+#pragma unroll
+        for (int n = 0; n < NT; ++n) this->csc[n] = fmaxf(this->csc[n], 0x1p-126f);
         if constexpr (MIN)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
