@@ -299,6 +299,9 @@ class LlamaDecoder:
         if self.track is not None and cell < self.n_cells:
             for L in self.layers:
                 H.BufferPart(L["weights"], 4 * cell, 4 * (self.n_cells - cell)).fill(0)
+        if self.sparse is not None and cell > self.n_cells:        # (cells that are passed over are seen as they are)
+            for L in self.layers:
+                self._all_bounds(L, cell)
         self.n_cells = min(self.n_cells, cell)
 
     def _all_bounds(self, L: dict, n: int) -> None:
@@ -370,8 +373,8 @@ class LlamaDecoder:
         ins[3 * U:3 * U + T] = toks
         if self.kv4:
             ins[4 * U:8 * U].reshape(U, 4)[:T, 1] = pos - self.dropped + 1
-        if self.sparse is not None:
-            ins[8 * U:] = cell0, cell0 + T
+        if self.sparse is not None:        # (with the block in front, which a generated token may have filled)
+            ins[8 * U:] = max(cell0 - 1, 0), cell0 + T
         if ins.nbytes <= 16384:                                   # queued behind the ubatch before, no wait
             d.write_async(pf["in"], ins)
         else:
@@ -406,7 +409,7 @@ class LlamaDecoder:
                 d.flash_attn_kv4(qkv, T, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, cell0 + T, att,
                                  nq, runs=pf["runs"])
                 if self.sparse is not None:
-                    d.kv4_bounds(L["kc"], c.head_dim, self.sparse.block, cell0 + T, L["bounds"], cells=pf["new"], n_new=T)
+                    d.kv4_bounds(L["kc"], c.head_dim, self.sparse.block, cell0 + T, L["bounds"], cells=pf["new"], n_new=T + 1)
                 if self.track is not None:
                     r = min(T, self.TRACKED_ROWS)
                     d.attn_weights_kv4(qkv.ptr + (T - r) * w3 * f4, r, w3, L["kc"], c.head_dim, c.n_head, c.n_head_kv, self.scale,
