@@ -282,7 +282,8 @@ class LlamaDecoder:
         return self.params.ptr + 8
 
     def prefill_history(self, weights: SyntheticWeights, n: int) -> None:
-        """Cells 0 .. n-1 of every cache hold QACT'd rows of weights.kv_history (SET_ROWS_KV)."""
+        """Cells 0 .. n-1 of every cache hold QACT'd rows of weights.kv_history (SET_ROWS_KV): another context."""
+        self._written_from(0)
         idx = self.dev.upload(np.arange(n, dtype=np.int64))
         for il, L in enumerate(self.layers):
             for which, kv in ((0, L["kc"]), (1, L["vc"])):

@@ -59,3 +59,23 @@ def test_a_step_ahead(dev):
     check_bounds(m, 540)
     m.check()
     m.free()
+
+
+def test_a_history_of_another_context(dev):
+    """Cells that a history fills have got no attention, nor have those behind them."""
+    cfg = LL.tiny_config("tiny-evict")
+    w = LL.SyntheticWeights(cfg)
+    m = LL.LlamaDecoder(dev, cfg, w, 300, kv_type=H.KV_Q4_0, track=1.0)
+    m.prefill(np.arange(100, dtype=np.int32), 0)
+    for i in range(4):
+        m.step_graph(None, 100 + i)
+    m.prefill_history(w, 60)
+    assert m.n_cells == 60
+    for L in m.layers:
+        assert (L["weights"].read(np.float32, (300,)) == 0).all()
+    m.step_graph(3, 60)
+    for L in m.layers:
+        got = L["weights"].read(np.float32, (300,))
+        assert abs(float(got.astype(np.float64).sum()) - cfg.n_head) <= 61 * cfg.n_head * 2.0 ** -20 and (got[61:] == 0).all()
+    m.check()
+    m.free()
