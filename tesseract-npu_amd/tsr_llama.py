@@ -341,11 +341,11 @@ class LlamaDecoder:
         toks = np.ascontiguousarray(tokens, np.int32).reshape(-1)
         if toks.size == 0:
             raise ValueError("prefill of no tokens")
-        if pos0 == 0:                      # another context
-            self.dropped = 0
-        if pos0 < self.dropped or pos0 - self.dropped + toks.size > self.kv_size:
+        dropped = self.dropped if pos0 != 0 else 0                # (position 0 is another context)
+        if pos0 < dropped or pos0 - dropped + toks.size > self.kv_size:
             raise ValueError(f"positions {pos0} .. {pos0 + toks.size - 1} outside the cache of {self.kv_size} cells")
-        self._written_from(pos0 - self.dropped)
+        self.dropped = dropped
+        self._written_from(pos0 - dropped)
         for u0 in range(0, toks.size, ubatch):
             self._prefill_ubatch(toks[u0:u0 + ubatch], pos0 + u0)
         c, d = self.cfg, self.dev

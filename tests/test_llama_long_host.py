@@ -1,0 +1,61 @@
+"""LlamaDecoder's positions, cells and options of long contexts on the CPU, over a pretended device. No GPU calls."""
+import numpy as np
+import pytest
+
+import tsr_llama as LL
+
+
+class Piece:
+    ptr, nbytes = 0, 1 << 40
+
+    def free(self):
+        pass
+
+
+class Device:
+    """Takes every call and does nothing."""
+
+    def alloc(self, n):
+        return Piece()
+
+    def __getattr__(self, name):
+        return lambda *args, **kw: None
+
+
+def decoder(kv_size=500, n_cells=0):
+    m = object.__new__(LL.LlamaDecoder)
+    m.dev, m.cfg, m.kv_size, m.kv4, m.fused = Device(), LL.tiny_config(), kv_size, True, True
+    m.layers, m.track, m.n_cells, m._pf = [], 1.0, n_cells, {"x": Piece()}
+    m.out_norm = m.wout = m.logits = m.next = m.tok = None
+    m.placed = []
+
+    def ubatch(toks, pos0):
+        m.placed.append((pos0 - m.dropped, toks.size))
+        m.n_cells = pos0 - m.dropped + toks.size
+
+    m._prefill_ubatch = ubatch
+    return m
+
+
+def tokens(n):
+    return np.zeros(n, np.int32)
+
+
+def test_a_refused_prompt_changes_nothing():
+    m = decoder(n_cells=403)
+    m.evict(300)
+    for n, pos0 in ((501, 0), (201, 403)):
+        with pytest.raises(ValueError):
+            m.prefill(tokens(n), pos0)
+        assert (m.dropped, m.n_cells) == (103, 300) and not m.placed
+    m.prefill(tokens(7), 403)
+    assert m.placed == [(300, 7)]
+
+
+def test_a_prompt_of_position_0_is_another_context():
+    m = decoder(n_cells=403)
+    m.evict(300)
+    m.prefill(tokens(500), 0)
+    assert m.dropped == 0 and m.placed == [(0, 500)]
+    m.prefill(tokens(10), 200)                                      # positions are cells again
+    assert m.placed[-1] == (200, 10)
