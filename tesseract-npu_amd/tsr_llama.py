@@ -184,7 +184,7 @@ class LlamaDecoder:
     weights are multiplied by at every token (1: nothing is forgotten), None: no weights."""
 
     scaling = rope_ff = sparse = track = None
-    dropped = n_cells = 0                  # evicted cells; cells in use
+    dropped = n_cells = kept = 0           # evicted cells; cells in use; of them those that the last eviction kept
     TRACKED_ROWS = 64                      # of a prompt's ubatch: its last tokens' weights
 
     def __init__(self, dev: H.Device, cfg: LlamaConfig, weights: SyntheticWeights, kv_size: int, fused: bool = True,
@@ -292,8 +292,20 @@ class LlamaDecoder:
                 rows.free()
             if self.sparse is not None:
                 self._all_bounds(L, n)
-        self.n_cells, self.dropped = n, 0
+        self.n_cells, self.dropped, self.kept = n, 0, 0
         self.dev.sync()
+
+    def _place(self, pos: int, n: int, anew: bool) -> None:
+        """Cells for n tokens from position pos on (anew: of another context). Those that an eviction kept stay: a step back ends where it
+        was."""
+        dropped, kept = (0, 0) if anew else (self.dropped, self.kept)
+        cell = pos - dropped
+        if cell < 0 or cell + n > self.kv_size:
+            raise ValueError(f"positions {pos} .. {pos + n - 1} outside the cache of {self.kv_size} cells")
+        if cell < kept:
+            raise ValueError(f"position {pos} before an eviction, whose {kept} cells hold others")
+        self.dropped, self.kept = dropped, kept
+        self._written_from(cell)
 
     def _written_from(self, cell: int) -> None:
         """Cells from here on are written anew: what the tokens that were there got of attention is not theirs."""
@@ -341,11 +353,7 @@ class LlamaDecoder:
         toks = np.ascontiguousarray(tokens, np.int32).reshape(-1)
         if toks.size == 0:
             raise ValueError("prefill of no tokens")
-        dropped = self.dropped if pos0 != 0 else 0                # (position 0 is another context)
-        if pos0 < dropped or pos0 - dropped + toks.size > self.kv_size:
-            raise ValueError(f"positions {pos0} .. {pos0 + toks.size - 1} outside the cache of {self.kv_size} cells")
-        self.dropped = dropped
-        self._written_from(pos0 - dropped)
+        self._place(pos0, toks.size, pos0 == 0)
         for u0 in range(0, toks.size, ubatch):
             self._prefill_ubatch(toks[u0:u0 + ubatch], pos0 + u0)
         c, d = self.cfg, self.dev
@@ -450,9 +458,7 @@ class LlamaDecoder:
         d.kv_set_rows(L["vc"], 1, qkv.ptr + (c.n_q + c.E) * 4, T, w3, cell, self.bad, stream=stream)
 
     def _mask(self, pos: int, n_kv: int | None):
-        if not 0 <= pos - self.dropped < self.kv_size:
-            raise ValueError(f"position {pos} outside the cache of {self.kv_size} cells")
-        self._written_from(pos - self.dropped)
+        self._place(pos, 1, False)
         if n_kv is None:
             n_kv = min(self.kv_size, (pos + 1 + 255) // 256 * 256)
         return msum_decode(pos, n_kv), np.array([[pos, pos + 1]], np.uint32)
@@ -573,7 +579,8 @@ class LlamaDecoder:
 
     def evict(self, n_keep: int, first: int = 4, last: int = 64) -> None:
         """Thin every layer's caches out to n_keep of their cells: the first, the last and those that attention gave most weight
-        (track). Positions go on; the next token's cell is n_keep. Waits for the device."""
+        (track). Positions go on; the next token's cell is n_keep, and no position before it is taken again, but 0: another
+        context. Waits for the device."""
         if self.track is None:
             raise ValueError("no weights of cells: track was not asked for")
         n, d, c = self.n_cells, self.dev, self.cfg
@@ -593,8 +600,8 @@ class LlamaDecoder:
         d.sync()
         idx.free()
         kept.free()
-        self.dropped += n - n_keep
-        self.n_cells = n_keep
+        if n > n_keep:
+            self.dropped, self.n_cells, self.kept = self.dropped + n - n_keep, n_keep, n_keep
 
     def step(self, token: int | None, pos: int, n_kv: int | None = None) -> None:
         """One eager decode token at position pos (cell pos): every op a separate call, FLASH_ATTN_EXT

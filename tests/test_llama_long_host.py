@@ -59,3 +59,29 @@ def test_a_prompt_of_position_0_is_another_context():
     assert m.dropped == 0 and m.placed == [(0, 500)]
     m.prefill(tokens(10), 200)                                      # positions are cells again
     assert m.placed[-1] == (200, 10)
+
+
+def test_kept_cells_are_not_written_again():
+    """Their positions are no longer the decoder's to tell: a step back ends where the eviction was."""
+    m = decoder(n_cells=403)
+    m.evict(300)
+    for pos in (-1, 1, 102, 103, 250, 402):
+        with pytest.raises(ValueError):
+            m._mask(pos, None)
+        with pytest.raises(ValueError):
+            m.prefill(tokens(2), pos)
+        assert (m.dropped, m.n_cells) == (103, 300) and not m.placed
+    m._mask(403, None)
+    m.prefill(tokens(60), 403)
+    m._mask(410, None)                                              # a step back behind the kept cells
+    m.evict(200)
+    assert m.dropped == 103 + 107 and m.n_cells == 200
+    with pytest.raises(ValueError):
+        m._mask(409, None)
+    m._mask(410, None)
+
+
+def test_an_eviction_of_nothing_moves_nothing():
+    m = decoder(n_cells=403)
+    m.evict(403)
+    m._mask(50, None)
