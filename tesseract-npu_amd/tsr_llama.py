@@ -295,10 +295,10 @@ class LlamaDecoder:
         self.n_cells, self.dropped, self.kept = n, 0, 0
         self.dev.sync()
 
-    def _place(self, pos: int, n: int, anew: bool) -> None:
-        """Cells for n tokens from position pos on (anew: of another context). Those that an eviction kept stay: a step back ends where it
-        was."""
-        dropped, kept = (0, 0) if anew else (self.dropped, self.kept)
+    def _place(self, pos: int, n: int) -> None:
+        """Cells for n tokens from position pos on; position 0 is another context. Those that an eviction kept stay: a step back ends
+        where it was."""
+        dropped, kept = (self.dropped, self.kept) if pos != 0 else (0, 0)
         cell = pos - dropped
         if cell < 0 or cell + n > self.kv_size:
             raise ValueError(f"positions {pos} .. {pos + n - 1} outside the cache of {self.kv_size} cells")
@@ -353,7 +353,7 @@ class LlamaDecoder:
         toks = np.ascontiguousarray(tokens, np.int32).reshape(-1)
         if toks.size == 0:
             raise ValueError("prefill of no tokens")
-        self._place(pos0, toks.size, pos0 == 0)
+        self._place(pos0, toks.size)
         for u0 in range(0, toks.size, ubatch):
             self._prefill_ubatch(toks[u0:u0 + ubatch], pos0 + u0)
         c, d = self.cfg, self.dev
@@ -458,7 +458,7 @@ class LlamaDecoder:
         d.kv_set_rows(L["vc"], 1, qkv.ptr + (c.n_q + c.E) * 4, T, w3, cell, self.bad, stream=stream)
 
     def _mask(self, pos: int, n_kv: int | None):
-        self._place(pos, 1, False)
+        self._place(pos, 1)
         if n_kv is None:
             n_kv = min(self.kv_size, (pos + 1 + 255) // 256 * 256)
         return msum_decode(pos, n_kv), np.array([[pos, pos + 1]], np.uint32)

@@ -61,6 +61,14 @@ def test_a_prompt_of_position_0_is_another_context():
     assert m.placed[-1] == (200, 10)
 
 
+def test_a_token_of_position_0_is_another_context():
+    m = decoder(n_cells=403)
+    m.evict(300)
+    m._mask(0, None)
+    assert (m.dropped, m.n_cells) == (0, 0)
+    m._mask(1, None)
+
+
 def test_kept_cells_are_not_written_again():
     """Their positions are no longer the decoder's to tell: a step back ends where the eviction was."""
     m = decoder(n_cells=403)
