@@ -63,7 +63,7 @@ class RopeScale:
     attn_factor: float = 1.0
     beta_fast: float = 32.0
     beta_slow: float = 1.0
-    freq_factors: tuple[float, ...] | None = None
+    freq_factors: tuple[float, ...] | None = None   # one for each pair of a head's values
 
 
 @dataclass(frozen=True)
@@ -197,6 +197,8 @@ class LlamaDecoder:
         self.sparse, self.track = sparse, track
         if cfg.rope_scale is not None:
             r = cfg.rope_scale
+            if r.freq_factors is not None and len(r.freq_factors) != cfg.head_dim // 2:   # (the kernels read as many)
+                raise ValueError(f"{len(r.freq_factors)} frequency factors for heads of {cfg.head_dim // 2} pairs")
             self.scaling = H.RopeScaling(cfg.rope_base, 1.0 / r.factor, r.ext_factor, r.attn_factor, r.beta_fast, r.beta_slow,
                                          r.n_ctx_orig)
             if r.freq_factors is not None:

@@ -93,3 +93,11 @@ def test_an_eviction_of_nothing_moves_nothing():
     m = decoder(n_cells=403)
     m.evict(403)
     m._mask(50, None)
+
+
+@pytest.mark.parametrize("n", [0, 1, 31, 33, 64])
+def test_frequency_factors_are_a_pair_s(n):
+    """One for each pair of a head's values; the kernels read as many."""
+    cfg = LL.tiny_config(rope_scale=LL.RopeScale(4.0, freq_factors=(1.0,) * n))
+    with pytest.raises(ValueError):
+        LL.LlamaDecoder(None, cfg, None, 100)
