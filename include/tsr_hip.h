@@ -440,7 +440,8 @@ size_t tsr_hip_flash_attn_kv4_blocks_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t 
  * sums' order is fixed: the same call gives the same bits.
  *   kc             a 4-bit K cache, E = n_head_kv * D
  *   runs_dev       as tsr_hip_flash_attn_kv4
- *   ws_dev         tsr_hip_attn_weights_kv4_ws(...) bytes, with tsr_hip_flash_attn_kv4's rules (never of 0 bytes for n_kv > 0) */
+ *   ws_dev         tsr_hip_attn_weights_kv4_ws(...) bytes, with tsr_hip_flash_attn_kv4's rules (never of 0 bytes for n_kv > 0);
+ *                  what does for n_kv cells does for fewer */
 int tsr_hip_attn_weights_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const tsr_hip_kv * kc, uint32_t D,
                              uint32_t n_head, uint32_t n_head_kv, float scale, uint32_t n_kv, const uint32_t * runs_dev,
                              const float * before_dev, float decay, float * out_dev, void * ws_dev, size_t ws_bytes, void * stream);

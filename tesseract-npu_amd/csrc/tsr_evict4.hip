@@ -30,7 +30,7 @@ static int workspace(tsr_hip_ctx * ctx, size_t need, void * ws_dev, hipStream_t 
 
 size_t tsr_hip_attn_weights_kv4_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t n_kv) {
     if (ctx == nullptr || T == 0u || T > 65535u || !heads_ok(D, n_head, n_head_kv) || n_kv == 0u || n_kv > 0x7FFFFFFFu) return 0u;
-    return tsr::weights4_plan(T, D, n_head, n_head_kv, n_kv, (uint32_t)ctx->n_cu).ws_bytes;
+    return tsr::weights4_ws(T, D, n_head, n_head_kv, n_kv, (uint32_t)ctx->n_cu);
 }
 
 int tsr_hip_attn_weights_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const tsr_hip_kv * kc, uint32_t D,
@@ -47,7 +47,8 @@ int tsr_hip_attn_weights_kv4(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T,
         return TSR_HIP_E_ARG;
     if (n_kv == 0u) return TSR_HIP_OK;
     const tsr::Weights4Plan p = tsr::weights4_plan(T, D, n_head, n_head_kv, n_kv, (uint32_t)ctx->n_cu);
-    if (ws_dev != nullptr && (ws_bytes < p.ws_bytes || ((uintptr_t)ws_dev & 15u) != 0u)) return TSR_HIP_E_ARG;
+    if (ws_dev != nullptr && (ws_bytes < tsr::weights4_ws(T, D, n_head, n_head_kv, n_kv, (uint32_t)ctx->n_cu) || ((uintptr_t)ws_dev & 15u) != 0u))
+        return TSR_HIP_E_ARG;
     tsr::Attn4Args a{};
     a.q_stride = q_stride;
     a.k = kc->dev;
