@@ -410,7 +410,8 @@ int tsr_hip_kv4_bounds(tsr_hip_ctx * ctx, const tsr_hip_kv * kc, uint32_t D, uin
  *   q_dev          as tsr_hip_flash_attn_kv4; 16-byte aligned, the stride a multiple of 4
  *   bounds_dev     as tsr_hip_kv4_bounds, bounds_blocks >= ceil(n_kv / block) blocks a head (that entry point's nb)
  *   ws_dev         tsr_hip_kv4_select_ws(...) bytes, with tsr_hip_flash_attn_kv4's rules (never of 0 bytes); the
- *                  workspace of this call may be that of the attention behind it
+ *                  workspace of this call may be that of the attention behind it; what does for T tokens and n_kv cells does for
+ *                  fewer
  * D, heads, T <= 65535 as tsr_hip_flash_attn_kv4; 1 <= n_sel <= 65536. */
 int tsr_hip_kv4_select(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint64_t q_stride, const uint32_t * bounds_dev,
                        uint32_t bounds_blocks, uint32_t D, uint32_t n_head, uint32_t n_head_kv, uint32_t block, uint32_t n_kv,

@@ -7,14 +7,17 @@
 
 namespace tsr {
 
-// Block selection: the tokens of a launch, so that their keys (one of 8 bytes a KV head and block) take at most 64 MiB (or are
-// one token's) and its grid's second axis fits.
+// Block selection: a key of 8 bytes a KV head and block. The tokens of a launch, so that their keys take at most 64 MiB (or are one
+// token's) and its grid's second axis fits, and the workspace, which never falls with more tokens or blocks.
+constexpr uint64_t kSelectKeys = (uint64_t)64 << 20;
+constexpr uint32_t kSelectTokens = 32768u;
+constexpr uint64_t kv4_token_keys(uint32_t n_head_kv, uint64_t n_blocks) { return 8u * std::max<uint64_t>(1u, n_blocks) * n_head_kv; }
 inline uint32_t kv4_select_tokens(uint32_t T, uint32_t n_head_kv, uint64_t n_blocks) {
-    const uint64_t one = 8u * std::max<uint64_t>(1u, n_blocks) * n_head_kv;
-    return (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ T, ((uint64_t)64 << 20) / one, 32768u }));
+    return (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>({ T, kSelectKeys / kv4_token_keys(n_head_kv, n_blocks), kSelectTokens }));
 }
 inline size_t kv4_select_ws(uint32_t T, uint32_t n_head_kv, uint64_t n_blocks) {
-    return (size_t)kv4_select_tokens(T, n_head_kv, n_blocks) * n_head_kv * (size_t)std::max<uint64_t>(1u, n_blocks) * 8u;
+    const uint64_t one = kv4_token_keys(n_head_kv, n_blocks);
+    return (size_t)std::min(std::min(T, kSelectTokens) * one, std::max(kSelectKeys, one));
 }
 
 // Attention over listed blocks: columns of the matrix instruction a row (attn4.hpp) and splits of a token's tiles.

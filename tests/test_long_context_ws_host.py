@@ -3,3 +3,7 @@
 
 def test_weights(native):
     assert "workspaces" in native("weights_ws_check")
+
+
+def test_selection(native):
+    assert "workspaces" in native("select_ws_check")
