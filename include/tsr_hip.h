@@ -404,8 +404,8 @@ int tsr_hip_kv4_bounds(tsr_hip_ctx * ctx, const tsr_hip_kv * kc, uint32_t D, uin
  * candidates are the blocks with a cell that it sees: of runs_dev's two runs a token as tsr_hip_flash_attn_kv4 takes
  * them (NULL: all n_kv cells). Where they are more than n_sel, the n_first lowest and the n_last highest are taken (a context's
  * start, its newest cells; n_first + n_last <= n_sel) and of the others those with the largest scores: max over the KV
- * head's query heads of sum over channels of max(q lo, q hi), at least the score of each of the block's cells; in f64, so
- * that sums' rounding decides between no two blocks but equal ones, of which the lowest is taken. Queries are finite: of a KV head
+ * head's query heads of sum over channels of max(q lo, q hi), at least the score of each of the block's cells; in f64, the
+ * same sums for the same bounds met, and of equal ones the lowest is taken. Queries are finite: of a KV head
  * with one that is not the blocks' scores may be no numbers, which are below every other.
  *   q_dev          as tsr_hip_flash_attn_kv4; 16-byte aligned, the stride a multiple of 4
  *   bounds_dev     as tsr_hip_kv4_bounds, bounds_blocks >= ceil(n_kv / block) blocks a head (that entry point's nb)

@@ -2,12 +2,12 @@
 // scores.
 //
 // The score of a block is max over the KV head's query heads of sum over channels of max(q lo, q hi).
-// It decides between blocks that may lie close together, so that it is f64, made as q (hi + lo) + |q| (hi - lo), twice the score:
-// products of f32 and sums of bf16 are exact or off by 2^-53 there, far below what tells two blocks apart. Equal scores go to
-// the lowest block.
+// It decides between blocks that may lie close together, so that it is f64, made as max(q, 0) hi + min(q, 0) lo: products are
+// exact, sums off by 2^-53 of their terms, far below what tells two blocks apart, and the bound that q does not meet adds 0, so
+// that blocks whose scores are equal by the formula are so here. Equal scores go to the lowest block.
 //
 // k_kv4_scores is a product of bounds and queries on the f64 matrix instruction 4x4x4 (four of them at once: 16 blocks by
-// four query heads, each channel once with q and once with |q|), 18 cycles an instruction; k_kv4_scores_many on 16x16x4, 64 cycles,
+// four query heads, each channel once with hi and once with lo), 18 cycles an instruction; k_kv4_scores_many on 16x16x4, 64 cycles,
 // whose 16 columns several tokens fill that look at the same blocks. What leaves is a key a block, an unsigned number in
 // the order of the scores. k_kv4_pick_blocks then finds the cut (pick.hpp). Both are a few microseconds of waiting for memory
 // and for each other's steps, not work: reductions and scans run on DPP, keys are asked for before the runs that say which
@@ -34,11 +34,14 @@ __device__ __forceinline__ BlockRange blocks_of(uint32_t lo, uint32_t hi, uint32
     return lo < hi ? BlockRange{ lo / block, (hi + block - 1u) / block } : BlockRange{ 0u, 0u };
 }
 
-// hi + lo and hi - lo of a word of bounds.
-struct Bounds2 { double mid, half; };
-__device__ __forceinline__ Bounds2 bounds2(uint32_t w) {
-    const double lo = (double)bf(w << 16), hi = (double)bf(w & 0xFFFF0000u);
-    return Bounds2{ hi + lo, hi - lo };
+// The bounds of a word.
+struct Bounds2 { double hi, lo; };
+__device__ __forceinline__ Bounds2 bounds2(uint32_t w) { return Bounds2{ (double)bf(w & 0xFFFF0000u), (double)bf(w << 16) }; }
+// The parts of q that meet hi and lo, by its sign.
+struct Query2 { double up, down; };
+__device__ __forceinline__ Query2 query2(float q) {
+    const uint32_t u = fb(q), m = (uint32_t)((int32_t)u >> 31);
+    return Query2{ (double)bf(u & ~m), (double)bf(u & m) };
 }
 
 // Few tokens: workgroup (KV heads fastest, part of the blocks; token), a wave 16 blocks at a time and the token's query heads, NG
@@ -102,9 +105,9 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores(Kv4SelectArgs a
 #pragma unroll
                         for (int n = 0; n < NG; ++n) {
                             const float y[4] = { q[n][m].x, q[n][m].y, q[n][m].z, q[n][m].w };
-                            const double v = (double)y[i];
-                            acc[n][0] = __builtin_amdgcn_mfma_f64_4x4x4f64(z.mid, v, acc[n][0], 0, 0, 0);
-                            acc[n][1] = __builtin_amdgcn_mfma_f64_4x4x4f64(z.half, __builtin_fabs(v), acc[n][1], 0, 0, 0);
+                            const Query2 v = query2(y[i]);
+                            acc[n][0] = __builtin_amdgcn_mfma_f64_4x4x4f64(z.hi, v.up, acc[n][0], 0, 0, 0);
+                            acc[n][1] = __builtin_amdgcn_mfma_f64_4x4x4f64(z.lo, v.down, acc[n][1], 0, 0, 0);
                         }
                     }
                 }
@@ -179,9 +182,9 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_kv4_scores_many(Kv4SelectA
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const Bounds2 z = bounds2(x[i]);
-                    const double v = (double)y[i];
-                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(z.mid, v, acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(z.half, __builtin_fabs(v), acc, 0, 0, 0);
+                    const Query2 v = query2(y[i]);
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(z.hi, v.up, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(z.lo, v.down, acc, 0, 0, 0);
                 }
             }
         }
