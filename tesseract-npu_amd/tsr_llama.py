@@ -180,12 +180,13 @@ def msum_causal(pos0: int, T: int, n_kv: int) -> np.ndarray:
 
 class LlamaDecoder:
     """The model on one device: weights uploaded once, one q8_0 K and V cache per layer of kv_size
-    cells, and the activation buffers of one decode token. sparse, track: over 4-bit caches alone; track is what earlier
-    weights are multiplied by at every token (1: nothing is forgotten), None: no weights."""
+    cells, and the activation buffers of one decode token. sparse, track: over 4-bit caches alone; track, 0 .. 1, is what earlier
+    weights are multiplied by at every token (1: nothing is forgotten), None: no weights. Of a prompt's ubatch the last
+    TRACKED_ROWS tokens give weight, none of them aged by the others: what a prompt leaves depends on its ubatches."""
 
     scaling = rope_ff = sparse = track = None
     dropped = n_cells = kept = 0           # evicted cells; cells in use; of them those that the last eviction kept
-    TRACKED_ROWS = 64                      # of a prompt's ubatch: its last tokens' weights
+    TRACKED_ROWS = 64                      # of a prompt's ubatch: its last tokens give weight
 
     def __init__(self, dev: H.Device, cfg: LlamaConfig, weights: SyntheticWeights, kv_size: int, fused: bool = True,
                  qkv_in_attn: bool = True, kv_type: int = H.KV_Q8_0, sparse: SparseAttention | None = None,
@@ -424,7 +425,7 @@ class LlamaDecoder:
                 if self.track is not None:
                     r = min(T, self.TRACKED_ROWS)
                     d.attn_weights_kv4(qkv.ptr + (T - r) * w3 * f4, r, w3, L["kc"], c.head_dim, c.n_head, c.n_head_kv, self.scale,
-                                       cell0 + T, L["weights"], before=L["weights"], decay=self.track,
+                                       cell0 + T, L["weights"], before=L["weights"], decay=self.track ** T,
                                        runs=pf["runs"].ptr + (T - r) * 16)
             else:
                 d.flash_attn(qkv, T, w3, L["kc"], L["vc"], c.head_dim, c.n_head, c.n_head_kv, self.scale, msum, att, nq,

@@ -7,6 +7,7 @@ import kv4_ref as R
 import sparse4_ref as P
 import tsr_hip as H
 import tsr_llama as LL
+import weights4_ref as W
 from test_gpu_llama_kv4 import images
 
 pytestmark = pytest.mark.gpu
@@ -77,5 +78,24 @@ def test_a_history_of_another_context(dev):
     for L in m.layers:
         got = L["weights"].read(np.float32, (300,))
         assert abs(float(got.astype(np.float64).sum()) - cfg.n_head) <= 61 * cfg.n_head * 2.0 ** -20 and (got[61:] == 0).all()
+    m.check()
+    m.free()
+
+
+def test_weights_age_by_the_token(dev):
+    """A ubatch's tokens are as many as make its weights' age: earlier weights are multiplied once for each."""
+    cfg = LL.tiny_config("tiny-evict")
+    D, nh, nkv = cfg.head_dim, cfg.n_head, cfg.n_head_kv
+    m = LL.LlamaDecoder(dev, cfg, LL.SyntheticWeights(cfg), 300, kv_type=H.KV_Q4_1, track=0.9)
+    L = m.layers[-1]
+    m.prefill(np.arange(60, dtype=np.int32), 0)
+    before = L["weights"].read(np.float32, (300,))
+    m.prefill(np.arange(8, dtype=np.int32), 60)
+    q = m._pf["qkv"].read(np.float32, (8, cfg.n_q + 2 * cfg.E))[:, :cfg.n_q]
+    runs = np.zeros((8, 4), np.int64)
+    runs[:, 1] = 61 + np.arange(8)
+    want, tol = W.weights(np.ascontiguousarray(q), images(m, L)[0], H.KV_Q4_1, D, nh, nkv, np.float64(np.float32(m.scale)), 68, runs,
+                          before[:68], 0.9 ** 8)
+    R.check(L["weights"].read(np.float32, (300,))[:68], want, tol, "prompt")
     m.check()
     m.free()
