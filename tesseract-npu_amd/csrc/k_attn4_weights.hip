@@ -16,6 +16,7 @@
 // Its time and theirs add up here. K in two f16 pieces with its scales, shared by a workgroup's waves through LDS, needs none of the
 // four and three products for two: 110 us, and 121 for q4_0, which takes 98 so.
 #include "attn4.hpp"
+#include "long_grid.hpp"
 #include "weights4_plan.hpp"
 
 namespace tsr {
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(65536 / D) void k_attn4_weights_one(Attn4Args a, We
 __global__ __launch_bounds__(256) void k_attn4_cells(const float * sums, uint32_t n, uint32_t n_pad, uint32_t n_kv, const float * before, float decay,
                                                      float * out) {
     __shared__ float part[4][64];
-    const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u, c = blockIdx.x * 64u + lane;
+    const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u, c = long_block() * 64u + lane;
     float x = 0.0f;
     if (c < n_kv)
         for (uint32_t i = wave; i < n; i += 32u) {                 // (eight on their way at once)
@@ -340,7 +341,7 @@ static int launch_weights(const Attn4Args & a, const Weights4Plan & p, const flo
         }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_attn4_weights<D, NT, TYPE>), grid, wg, 0, s, a, p);
     const uint32_t n = a.n_head_kv * p.n_rg;
-    hipLaunchKernelGGL(k_attn4_cells, dim3((a.n_kv + 63u) / 64u), dim3(256), 0, s, (const float *)((uint8_t *)a.part + p.sums), n, p.n_pad, a.n_kv, before,
+    hipLaunchKernelGGL(k_attn4_cells, long_grid(((uint64_t)a.n_kv + 63u) / 64u), dim3(256), 0, s, (const float *)((uint8_t *)a.part + p.sums), n, p.n_pad, a.n_kv, before,
                        decay, a.out);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }

@@ -15,6 +15,7 @@
 // of 8 heads of 256 over 4, 94 blocks: 9.8 and 6.5. 512 tokens of 32 heads of 128 behind 120 blocks take 26.8 for the scores, bound by
 // the matrix instruction (13.7 at what an 8192^3 product reaches, 66 TFLOP/s); with 4x4x4 they took 51 to 54.
 #include "kernels.hpp"
+#include "long_grid.hpp"
 #include "pick.hpp"
 
 namespace tsr {
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(64 * pick_waves(WAVES)) void k_kv4_pick_blocks(Kv4S
 template <int D>
 static void launch_scores(const Kv4SelectArgs & a, hipStream_t s) {
     const uint32_t all = (a.n_blocks + 16u * kScoreWaves - 1u) / (16u * kScoreWaves), tpt = a.G <= 16u ? 16u / a.G : 1u;
-    const uint32_t lists = a.T * a.n_head_kv, parts = a.T == 1u ? all : min(all, max(1u, 1024u / lists));
+    const uint32_t lists = a.T * a.n_head_kv, parts = min(all, a.T == 1u ? kAxisGroups / a.n_head_kv : max(1u, 1024u / lists));
     const dim3 grid(a.n_head_kv * parts, a.T), wg(64u * kScoreWaves);
     if (a.T >= 64u) hipLaunchKernelGGL(k_kv4_scores_many<D>, dim3(a.n_head_kv * all, (a.T + tpt - 1u) / tpt), wg, 0, s, a);
     else if (a.G <= 4u) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_kv4_scores<D, 1>), grid, wg, 0, s, a, parts);

@@ -9,6 +9,7 @@
 // cells (with the cells that stay, where a source is none) and from there over them.
 #include "kernels.hpp"
 #include "kv4.hpp"
+#include "long_grid.hpp"
 #include "tsr_dev.hpp"
 
 namespace tsr {
@@ -32,7 +33,8 @@ __global__ __launch_bounds__(256) void k_kv4_gather(KvGatherArgs a) {
     constexpr uint32_t tb = kv4_tile_bytes(TYPE);
     __shared__ int64_t from[64];                                   // a cell's codes in its source plane; -1: none
     __shared__ uint32_t scale[64];                                 // its scales behind them (block 0)
-    const uint32_t i0 = 64u * blockIdx.x, planes = a.E / 64u, p0 = kGatherPlanes * blockIdx.y;
+    const uint32_t i0 = 64u * long_block(), planes = a.E / 64u, p0 = kGatherPlanes * blockIdx.y;
+    if (i0 >= a.n) return;
     if (threadIdx.x < 64u) {
         const int64_t c = gather_from(a, i0 + threadIdx.x);
         const uint32_t cell = (uint32_t)c;
@@ -106,7 +108,8 @@ __global__ __launch_bounds__(256) void k_kv4_gather(KvGatherArgs a) {
 template <uint32_t WHICH>
 __global__ __launch_bounds__(256) void k_kv_gather(KvGatherArgs a) {
     __shared__ int64_t from[16];
-    const uint32_t u = blockIdx.x, v0 = 256u * blockIdx.y, nbk = a.E / 32u, l = threadIdx.x;
+    const uint32_t u = long_block(), v0 = 256u * blockIdx.y, nbk = a.E / 32u, l = threadIdx.x;
+    if (16ull * u >= a.n) return;
     if (l < 16u) from[l] = gather_from(a, 16u * u + l);
     __syncthreads();
     auto quants = [&](int64_t c) { return a.src + a.src_off + (size_t)(c >> 4) * 16u * a.E; };
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(256) void k_kv_gather(KvGatherArgs a) {
 
 // rows of `bytes` (a multiple of 16), from_step and to_step apart
 __global__ __launch_bounds__(256) void k_kv_rows_copy(uint8_t * to, size_t to_step, const uint8_t * from, size_t from_step, size_t bytes) {
-    const size_t i = 16u * ((size_t)blockIdx.x * 256u + threadIdx.x);
+    const size_t i = 16u * ((size_t)long_block() * 256u + threadIdx.x);
     if (i < bytes) *(uint4 *)(to + blockIdx.y * to_step + i) = *(const uint4 *)(from + blockIdx.y * from_step + i);
 }
 
@@ -153,11 +156,11 @@ __global__ __launch_bounds__(256) void k_kv_rows_copy(uint8_t * to, size_t to_st
 int tsr_launch_kv_gather(const tsr::KvGatherArgs & a, uint32_t type, uint32_t which, hipStream_t s) {
     using namespace tsr;
     if (type == kKvQ8_0) {
-        const dim3 grid((a.n + 15u) / 16u, (a.E + 255u) / 256u);
+        const dim3 grid = long_grid(((uint64_t)a.n + 15u) / 16u, (a.E + 255u) / 256u);
         if (which == 0u) hipLaunchKernelGGL(k_kv_gather<0>, grid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL(k_kv_gather<1>, grid, dim3(256), 0, s, a);
     } else {
-        const dim3 grid((a.n + 63u) / 64u, (a.E / 64u + kGatherPlanes - 1u) / kGatherPlanes);
+        const dim3 grid = long_grid(((uint64_t)a.n + 63u) / 64u, (a.E / 64u + kGatherPlanes - 1u) / kGatherPlanes);
         if (type == kKvQ4_0 && which == 0u) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_kv4_gather<kKvQ4_0, 0>), grid, dim3(256), 0, s, a);
         else if (type == kKvQ4_0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_kv4_gather<kKvQ4_0, 1>), grid, dim3(256), 0, s, a);
         else if (which == 0u) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_kv4_gather<kKvQ4_1, 0>), grid, dim3(256), 0, s, a);
@@ -167,6 +170,6 @@ int tsr_launch_kv_gather(const tsr::KvGatherArgs & a, uint32_t type, uint32_t wh
 }
 
 int tsr_launch_kv_rows_copy(uint8_t * to, size_t to_step, const uint8_t * from, size_t from_step, size_t bytes, uint32_t rows, hipStream_t s) {
-    hipLaunchKernelGGL(tsr::k_kv_rows_copy, dim3((uint32_t)((bytes + 4095u) / 4096u), rows), dim3(256), 0, s, to, to_step, from, from_step, bytes);
+    hipLaunchKernelGGL(tsr::k_kv_rows_copy, tsr::long_grid((bytes + 4095u) / 4096u, rows), dim3(256), 0, s, to, to_step, from, from_step, bytes);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
