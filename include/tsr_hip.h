@@ -419,8 +419,9 @@ int tsr_hip_kv4_select(tsr_hip_ctx * ctx, const float * q_dev, uint32_t T, uint6
                        void * ws_dev, size_t ws_bytes, void * stream);
 size_t tsr_hip_kv4_select_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t n_head_kv, uint32_t block, uint32_t n_kv);
 
-/* The attention: tsr_hip_flash_attn_kv4 of each token and KV head over the cells of its listed blocks that its runs allow.
- * Arguments, precision, empty rows and the workspace (tsr_hip_flash_attn_kv4_blocks_ws) as there; no mask.
+/* The attention: tsr_hip_flash_attn_kv4 of each token and KV head over the cells of its listed blocks that its runs allow. Every
+ * token reads its own cells, where that call shares them: 512 tokens of one sequence over 32 blocks of 64 each gain from some 10000
+ * cells on, 64 behind 7680 too. Arguments, precision, empty rows and the workspace (tsr_hip_flash_attn_kv4_blocks_ws) as there; no mask.
  *   blocks_dev     [T][n_head_kv][n_sel] int32, 4-byte aligned, read when the kernels run: as tsr_hip_kv4_select gives
  *                  them, or others in any order; an entry that is negative or of no cell below n_kv is passed over, a block that is
  *                  listed twice counts twice. */
@@ -437,7 +438,7 @@ size_t tsr_hip_flash_attn_kv4_blocks_ws(tsr_hip_ctx * ctx, uint32_t T, uint32_t 
 
 /* out_dev[c] = decay * before_dev[c] + sum over tokens t and query heads of softmax(scale q K^T)[c], c < n_kv (f32): the weights that
  * tsr_hip_flash_attn_kv4 of the same arguments gives cell c (0 of rows that do not see it, and of rows that see nothing). Scores
- * and precision as there; no mask. before_dev NULL or decay 0: no addend, before_dev is not read; before_dev may be out_dev. The
+ * and precision as there, but that q4_1's m meet the sums of a block's q in two f16 pieces, 22 bits; no mask. before_dev NULL or decay 0: no addend, before_dev is not read; before_dev may be out_dev. The
  * sums' order is fixed: the same call gives the same bits.
  *   kc             a 4-bit K cache, E = n_head_kv * D
  *   runs_dev       as tsr_hip_flash_attn_kv4

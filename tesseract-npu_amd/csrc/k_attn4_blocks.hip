@@ -2,8 +2,8 @@
 // what a wave does): a token's query heads of one KV head share a list and are the rows of its workgroups, whose waves take
 // the lists' tiles in turn, those that the rows see whole first (gathered 64 entries at a time), the list asked for ahead of all else.
 //
-// Bound: a token's latency (32 heads of 128 over 8 KV heads, 32 blocks of 64 in 16 splits: 6.8 us and the join 4, its 9.4 MB in 2). Many
-// tokens: vector instructions, since the codes of a list are unpacked for its few rows alone (512 such tokens 160 us of a call's 193;
+// Bound: a token's latency (32 heads of 128 over 8 KV heads, 32 blocks of 64 in 16 splits: 7.2 us and the join 3.9, its 9.4 MB in 2). Many
+// tokens: vector instructions, since the codes of a list are unpacked for its few rows alone (512 such tokens 160 us of a call's 194;
 // the products would take 14). 33 sequences' tokens of two heads of 256 a list: 22 us, one tile ahead a wave.
 #include "attn4.hpp"
 

@@ -10,9 +10,9 @@
 // or, for one group of rows of few heads, both at once: k_attn4_weights_one.
 // A workgroup's waves have the same rows (up to four groups of 16: nothing but scores to hold) and take tiles in turn.
 //
-// Bound: a decode token's three launches (32 heads of 128 over 8 KV heads behind 8192 cells: 13.1 us, 5.9 + 7.2 + 2.5 by themselves, the
+// Bound: a decode token's three launches (32 heads of 128 over 8 KV heads behind 8192 cells: 13.0 us, 5.7 + 6.8 + 2.5 by themselves, the
 // codes' 9 MB in 2); for many rows the f32 operations on the scores, 4 for every product of 16 x 16 x 32 and then 4 and an exponential
-// a score: 64 such tokens behind 32768 cells of q4_1 take 108.6 us, 61 + 60, of which the matrix instruction is busy for 14 each.
+// a score: 64 such tokens behind 32768 cells of q4_1 take 108 to 111 us, 61 + 60, of which the matrix instruction is busy for 14 each.
 // Its time and theirs add up here. K in two f16 pieces with its scales, shared by a workgroup's waves through LDS, needs none of the
 // four and three products for two: 110 us, and 121 for q4_0, which takes 98 so.
 #include "attn4.hpp"

@@ -11,8 +11,8 @@
 // whose 16 columns several tokens fill that look at the same blocks. What leaves is a key a block, an unsigned number in
 // the order of the scores. k_kv4_pick_blocks then finds the cut (pick.hpp). Both are a few microseconds of waiting for memory
 // and for each other's steps, not work: reductions and scans run on DPP, keys are asked for before the runs that say which
-// of them count. A token of 32 heads of 128 over 8 KV heads, 2048 blocks: scores 4.9 us, cut 6.8 (an empty kernel 1.7); 33 sequences' tokens
-// of 8 heads of 256 over 4, 94 blocks: 9.8 and 6.5. 512 tokens of 32 heads of 128 behind 120 blocks take 26.8 for the scores, bound by
+// of them count. A token of 32 heads of 128 over 8 KV heads, 2048 blocks: scores 4.8 us, cut 6.9 (an empty kernel 1.7); 33 sequences' tokens
+// of 8 heads of 256 over 4, 94 blocks: 10.1 and 6.4. 512 tokens of 32 heads of 128 behind 120 blocks take 27.0 for the scores, bound by
 // the matrix instruction (13.7 at what an 8192^3 product reaches, 66 TFLOP/s); with 4x4x4 they took 51 to 54.
 #include "kernels.hpp"
 #include "long_grid.hpp"
@@ -282,6 +282,11 @@ static void launch_scores(const Kv4SelectArgs & a, hipStream_t s) {
     const uint32_t all = (a.n_blocks + 16u * kScoreWaves - 1u) / (16u * kScoreWaves), tpt = a.G <= 16u ? 16u / a.G : 1u;
     const uint32_t lists = a.T * a.n_head_kv, parts = min(all, a.T == 1u ? kAxisGroups / a.n_head_kv : max(1u, 1024u / lists));
     const dim3 grid(a.n_head_kv * parts, a.T), wg(64u * kScoreWaves);
+    // The host does not know whether tokens share their blocks. Scores and cut in us, 4x4x4 / 16x16x4, tokens of one sequence; of
+    // sequences side by side: 32 heads of 128 over 8, 1024 blocks: 32 tokens 38.1 / 19.6; 11.4 / 11.2, 64 tokens 68.7 / 33.1; 11.7 / 15.9; 120
+    // blocks: 32 tokens 9.5 / 9.1; 7.6 / 8.4, 64 tokens 13.3 / 9.2; 7.4 / 7.7; 8 heads of 256 over 4, 94 blocks: 32 tokens 9.5 / 11.9; 7.0 / 10.1,
+    // 64 tokens 13.2 / 11.9; 9.5 / 10.3. Workgroups of 4x4x4 in all, 256, 1024, 4096: 33 tokens behind 1024 blocks 67.9, 49.4, 44.4;
+    // 12.1, 12.0, 16.8; 63 tokens 70.2, 68.5, 68.2; 12.4, 13.6, 19.9.
     if (a.T >= 64u) hipLaunchKernelGGL(k_kv4_scores_many<D>, dim3(a.n_head_kv * all, (a.T + tpt - 1u) / tpt), wg, 0, s, a);
     else if (a.G <= 4u) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_kv4_scores<D, 1>), grid, wg, 0, s, a, parts);
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_kv4_scores<D, 2>), grid, wg, 0, s, a, parts);

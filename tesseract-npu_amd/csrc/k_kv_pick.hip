@@ -2,7 +2,8 @@
 // weights (pick.hpp), in the order of their cells.
 //
 // One workgroup of 16 waves finds the cut and writes the list; up to 65536 weights stay in its registers. Bound: what one compute unit
-// loads and counts: 16384 of 65536 cells take 31 us (its 64 weights a lane some 2000 instructions), 777 of 1500 5 us.
+// loads and counts: 16384 of 65536 cells take 31 us (its 64 weights a lane some 2000 instructions), 777 of 1500 5 us; a quarter of
+// 8192, 16384 and 32768 8, 11 and 19, of 131072, which are read again at every pass, 128.
 #include "kernels.hpp"
 #include "pick.hpp"
 
